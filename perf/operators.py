@@ -189,8 +189,8 @@ def _inputs(case, seed):
 def prepare(case, seed):
     s, kind, n = _inputs(case, seed), case["kind"], case["lanes"]
     if own:
-        from qwen35 import KvCache4
         s["eng"] = engine()
+        from qwen35 import KvCache4
         s["lanes"] = np.arange(n, dtype=np.int32)
         bf16 = functools.partial(torch.empty, dtype=torch.bfloat16, device=DEV)
         if kind in ("heads", "append"):
