@@ -234,6 +234,98 @@ int q35_op_attn_decode(q35_engine* e, q35_state* s, int layer, const int32_t* la
                        int T, const uint16_t* proj_dev, const uint16_t* q_norm_dev, const uint16_t* k_norm_dev,
                        uint16_t* out_dev, int form);
 int q35_op_lm_head_argmax(q35_engine* e, const uint16_t* x_dev, int M, int32_t* tok_dev, float* logits_dev);
+/* A K/V cache in 4 bits for any attention layer, and the operators around it: the heads' norms and
+ * rotation, the append, and the attention that reads it, with a sliding window and sinks. The
+ * reference has no counterpart (its cache is bf16); a slot takes head_dim * 17/32 bytes for K and
+ * as many for V, less than 4/15 of bf16's.
+ * Format: 32 consecutive dims of a head at one slot share a scale byte b, standing for
+ * 2^(b - 127): the smallest power of two with max|x| <= 6 * 2^(b - 127), kept within b = 8 .. 252
+ * (smaller groups become zeros, larger ones saturate at 6 * 2^125); a code is sign << 3 | index
+ * into (0, 0.5, 1, 1.5, 2, 3, 4, 6), the nearest one, ties to the even index. A group with an infinity
+ * or a NaN gets b = 255 and reads back as NaN throughout.
+ * All these calls are enqueued on the engine stream without waiting (q35_sync waits) and allocate
+ * nothing; lanes, positions and descriptors are host memory, read before the call returns. Calls of one
+ * engine run in their order; the caller's buffers must be ready before the call and stay until it has
+ * run. The calling thread's current HIP device does not matter. */
+typedef struct q35_kv4 q35_kv4;
+/* A cache of `layers` x `lanes` x `cap` slots of kv_heads heads; head_dim is 64, 128 or 256, cap at
+ * most the engine's max_ctx. Each (layer, lane) holds slots [0, length); lengths start at 0. A cache
+ * whose engine is destroyed already is freed with e NULL. */
+int q35_kv4_alloc(q35_engine* e, int layers, int lanes, int cap, int kv_heads, int head_dim, q35_kv4** out);
+int q35_kv4_free(q35_engine* e, q35_kv4* c);
+/* Length of n lanes (i when lanes is NULL), in every layer: 0 starts a lane over, less than the length drops
+ * its last slots (rejected drafts); slots past the old length read as whatever they last held (zeros
+ * at first). */
+int q35_kv4_set_len(q35_engine* e, q35_kv4* c, const int32_t* lanes, const int32_t* len, int n);
+int q35_kv4_len(q35_engine* e, q35_kv4* c, int layer, int lane, int32_t* out);
+/* Slots [slot0, slot0 + n_slots) of lanes [lane0, lane0 + n_lanes) from / to device buffers in row order: codes
+ * [n_lanes][kv_heads][n_slots][head_dim / 2], two codes a byte, the lower dim in the low nibble;
+ * scales [n_lanes][kv_heads][n_slots][head_dim / 32]. A write starts at most at a lane's length
+ * and raises it to slot0 + n_slots; a read stays below it. */
+int q35_kv4_write(q35_engine* e, q35_kv4* c, int layer, int lane0, int n_lanes, int slot0, int n_slots,
+                  const uint8_t* k_codes, const uint8_t* k_scales, const uint8_t* v_codes, const uint8_t* v_scales);
+int q35_kv4_read(q35_engine* e, q35_kv4* c, int layer, int lane0, int n_lanes, int slot0, int n_slots, uint8_t* k_codes,
+                 uint8_t* k_scales, uint8_t* v_codes, uint8_t* v_scales);
+
+/* Rows of heads in a device buffer of bf16: element (row r, head h, dim d) at ptr[r * row_stride +
+ * h * head_stride + d], so a projection's rows are read where they lie. ptr 16-byte aligned, strides
+ * multiples of 8 elements; an output's rows and heads must not overlap. */
+typedef struct q35_view {
+    const uint16_t* ptr;
+    int64_t row_stride, head_stride;
+} q35_view;
+/* q and k of a layer's rows (row i * T + t: sequence i's row at position pos[i] + t), and for an append v.
+ * q and k: y = x * rsqrt(mean(x^2) + eps) * (1 + norm) per head (norm [head_dim] bf16), then dims
+ * [0, rot_dim) rotated in pairs (d, d + rot_dim / 2) by position * theta^(-2 d / rot_dim); the sum, the
+ * root and the angles in float64, the rest in float32, one rounding to bf16 at the end. */
+typedef struct q35_heads {
+    int q_heads, rot_dim;
+    double theta, eps;
+    const uint16_t *q_norm, *k_norm;
+    q35_view q, k, v;                /* q: ptr NULL leaves q out */
+    q35_view q_out, k_out, v_out;    /* may be the input views themselves */
+} q35_heads;
+/* q_out and k_out = normed and rotated q and k (v, v_out: NULL). */
+int q35_op_qk_norm_rope(q35_engine* e, const q35_heads* h, int kv_heads, int head_dim, const int32_t* pos, int n, int T);
+/* The same pass with the append: q_out as above; the float32 k and the bf16 v go into slots pos[i] + t of lane
+ * lanes[i] (i when NULL) of the layer in 4 bits. pos[i] is at most the lane's length, which becomes
+ * pos[i] + T; no lane twice. k_out / v_out (nullable): the values that the new codes stand for. */
+int q35_op_kv4_append(q35_engine* e, q35_kv4* c, int layer, const int32_t* lanes, const int32_t* pos, int n, int T,
+                      const q35_heads* h);
+/* Attention over the cache: row i * T + t of q (normed and rotated, q_heads a multiple of kv_heads, query
+ * head h on kv head h / (q_heads / kv_heads)) sees slots (p - window, p] and [0, sinks) of lane
+ * lanes[i], p = pos[i] + t; window 0: [0, p]. The lane must hold pos[i] + T slots, the rows' own included;
+ * a lane may occur more than once. out = softmax(scale * q K^T) V, times sigmoid(gate) if gate is given, in
+ * float32 with the weights rounded to bf16 for the product with V, and one rounding to bf16. A NaN in
+ * a slot reaches the rows that see it and no others. */
+int q35_op_attn_kv4(q35_engine* e, q35_kv4* c, int layer, const int32_t* lanes, const int32_t* pos, int n, int T,
+                    int q_heads, const q35_view* q, const q35_view* gate, float scale, int window, int sinks,
+                    const q35_view* out);
+
+/* Sampled verification of drafted tokens from given random numbers (the reference verifies greedily,
+ * engine/mtp_accept.h:248). Lane i has k <= 8 drafts, k + 1 rows of target logits, with p_j =
+ * softmax(logits_j / temperature), and the drafter's k rows with q_j likewise; draft_logits NULL: a
+ * drafter certain of its drafts, q_j = 1 there (greedy drafts). Draft j stays while u_j q_j(d_j) < p_j(d_j). The
+ * token after the a accepted ones comes from max(p_a - q_a, 0) if draft a was refused (from p_a if
+ * nothing is left of it), else from p_a: the lowest id whose running sum exceeds u_k times the total. So
+ * every token has the target's distribution. A negative draft ends a lane's drafts; an id of vocab or
+ * more is refused. temperature 0: a draft stays while it is its row's argmax (lowest id on ties), the token is
+ * row a's argmax, draft_logits and u unused (u may not be NULL). A row with a NaN, a +inf or only -inf
+ * logits has no distribution: its draft is refused and its token is -1; a draft row without one refuses its
+ * draft, and the token comes from p_a. accepted [n] = a, tokens [n][k + 1] = the accepted drafts, the
+ * token, then -1; both device memory. All sums and probabilities are float64. n * (k + 1) <= max_rows.
+ * Enqueued on the engine stream without waiting; its workspace is the engine's. */
+typedef struct q35_drafts {
+    const void* logits;              /* device [n * (k + 1)][ld] */
+    int64_t ld;
+    const void* draft_logits;        /* device [n * k][draft_ld], or NULL */
+    int64_t draft_ld;
+    int dtype;                       /* of both: 0 float32, 1 bfloat16 */
+    const int32_t* drafts;           /* device [n][k] */
+    const float* u;                  /* device [n][k + 1], in [0, 1) */
+    double temperature;              /* 0, or at least 0.001 */
+} q35_drafts;
+int q35_op_draft_verify(q35_engine* e, const q35_drafts* d, int n, int k, int vocab, int32_t* accepted, int32_t* tokens);
 int q35_sync(q35_engine* e);
 /* Live per-kernel timing: with option "kprof" = family (1 projection/MLP GEMMs, 2 lm_head
  * GEMM, 3 GDN recurrence, 4 attention core, 0 off), each launch of that family is bracketed

@@ -19,7 +19,9 @@
 
 #include "../../include/q35.h"
 #include "q35_common.h"
+#include "q35_host.h"
 #include "q35_kernels.h"
+#include "q35_kv4.h"
 #include "q35_safetensors.h"
 
 using namespace q35;
@@ -27,22 +29,6 @@ using namespace q35;
 namespace {
 
 thread_local std::string g_err;
-
-struct Q35Error : std::runtime_error {
-    int code;
-    Q35Error(int c, const std::string& m) : std::runtime_error(m), code(c) {}
-};
-
-#define HCK(x)                                                                              \
-    do {                                                                                    \
-        hipError_t _e = (x);                                                                \
-        if (_e != hipSuccess)                                                               \
-            throw Q35Error(Q35_ERR_HIP, std::string(#x) + ": " + hipGetErrorString(_e));   \
-    } while (0)
-#define REQ(cond, code, msg)                                  \
-    do {                                                      \
-        if (!(cond)) throw Q35Error((code), (msg));           \
-    } while (0)
 
 uint64_t hmix(uint64_t x) {
     uint64_t z = x + 0x9E3779B97F4A7C15ull;
@@ -135,6 +121,8 @@ struct q35_engine {
     uint16_t *x, *h, *delta, *nrm, *proj, *gu, *aout, *cat;
     float *o, *q, *sc, *stats, *part, *pval, *inv_freq;
     float* kpart;
+    float* kv4_part = nullptr;       // the 4-bit cache's attention: partial results of split rows
+    double* verify_ws = nullptr;     // draft verification: the rows' chunk statistics
     uint16_t* prod;
     int *pidx, *tok_dev, *rlane, *rpos, *rslot, *rcur, *rwcur, *rpend, *ridx_src, *ridx_dst, *din = nullptr;
     int sc_ld = 0, max_chunks = 0;
@@ -412,6 +400,8 @@ void alloc_scratch(q35_engine* e) {
     e->pidx = dalloc<int>(R * (size_t)(kVocab / 16));
     e->kpart = dalloc<float>(R * 16 * kHidden);
     e->topv_dev = dalloc<float>(R);
+    e->kv4_part = dalloc<float>(kv4_part_floats());
+    e->verify_ws = dalloc<double>(verify_ws_doubles((int)R));
     e->gchunk = dalloc<float>(gdn_chunk_ws_floats(R));
     e->gcdec = dalloc<float>((size_t)((R + 63) / 64) * kHv);
     e->prod = dalloc<uint16_t>(R * kFF);
@@ -855,7 +845,13 @@ bool shape_ok(const Placement& p, const std::string& name, const std::vector<int
     return sh.size() == 1 && sh[0] == p.rows;
 }
 
-int guard(const std::function<void()>& f) {
+}  // namespace
+
+// The calling thread's error text, for the other translation units of the library (the MTP
+// policy entry points) that return a status without going through guard().
+void q35_set_error(const char* msg) { g_err = msg; }
+
+int q35::guard(const std::function<void()>& f) {
     try {
         f();
         return Q35_OK;
@@ -867,11 +863,8 @@ int guard(const std::function<void()>& f) {
         return Q35_ERR_STATE;
     }
 }
-}  // namespace
 
-// The calling thread's error text, for the other translation units of the library (the MTP
-// policy entry points) that return a status without going through guard().
-void q35_set_error(const char* msg) { g_err = msg; }
+q35::EngineView q35::engine_view(q35_engine* e) { return {e->device, e->R, e->max_ctx, e->st, e->kv4_part, e->verify_ws}; }
 
 // ====================================================================== C ABI
 extern "C" {
@@ -909,7 +902,7 @@ int q35_destroy(q35_engine* e) {
         e->graphs.clear();
         void* ds[] = {e->blob, e->x, e->h, e->delta, e->nrm, e->proj, e->gu, e->aout, e->cat, e->o, e->q,
                       e->sc, e->stats, e->part, e->pval, e->pidx, e->prod, e->din, e->inv_freq,
-                      e->logits_dev, e->kpart, e->gchunk, e->gcdec, e->topv_dev};
+                      e->logits_dev, e->kpart, e->gchunk, e->gcdec, e->topv_dev, e->kv4_part, e->verify_ws};
         for (void* p : ds) if (p) hipFree(p);
         void* hs[] = {e->hin, e->h_out};
         for (void* p : hs) if (p) hipHostFree(p);

@@ -1,0 +1,408 @@
+// Verification of drafted tokens against the target's probabilities, from given random numbers.
+//
+// A lane has k drafts d_0 .. d_{k-1}, k + 1 rows of target logits (row j before draft j, row k after
+// the last) and, unless its drafter is certain of its drafts, k rows of the drafter's logits. With
+// p_j = softmax(l_j / T) and q_j = softmax(l'_j / T) (1 at the draft for a certain drafter):
+//   draft j stays while u_j q_j(d_j) < p_j(d_j); the first that does not ends the lane at row a = j,
+//   and its token comes from the weights max(p_a - q_a, 0); without one, from p_a, a = the drafts' number;
+//   the token is the first whose running sum of weights exceeds u_k times their total.
+// Every token then has the target's distribution, whatever the drafter.
+//
+// The token is a border between two sums of up to 10^6 terms, so everything here is float64: with
+// float32's exp and sums one token in forty at a 248,320-word vocabulary would be another one. A float64
+// exp2 of its own (13 fused multiply-adds) costs what the logits' loads cost: both run together.
+// The logits are read once (verify_stats); what follows touches one row of a lane again, or two.
+#include "q35_common.h"
+#include "q35_kv4.h"
+
+namespace q35 {
+
+// 2^x for x <= 0 by the Taylor series of 2^f, |f| <= 1/2 (the first term left out is below 2^-56);
+// 0 under 2^-1000.
+__device__ __forceinline__ double exp2_neg(double x) {
+    const double k = rint(x), f = (x - k) * 0.69314718055994530942;
+    double p = 1.0 / 6227020800.0;
+    p = __builtin_fma(p, f, 1.0 / 479001600.0);
+    p = __builtin_fma(p, f, 1.0 / 39916800.0);
+    p = __builtin_fma(p, f, 1.0 / 3628800.0);
+    p = __builtin_fma(p, f, 1.0 / 362880.0);
+    p = __builtin_fma(p, f, 1.0 / 40320.0);
+    p = __builtin_fma(p, f, 1.0 / 5040.0);
+    p = __builtin_fma(p, f, 1.0 / 720.0);
+    p = __builtin_fma(p, f, 1.0 / 120.0);
+    p = __builtin_fma(p, f, 1.0 / 24.0);
+    p = __builtin_fma(p, f, 1.0 / 6.0);
+    p = __builtin_fma(p, f, 0.5);
+    p = __builtin_fma(p, f, 1.0);
+    p = __builtin_fma(p, f, 1.0);
+    const int e = (int)fmax(k, -1001.0);
+    const double s = __longlong_as_double((long long)(1023 + e) << 52);
+    return x < -1000.0 ? 0.0 : p * s;
+}
+
+constexpr int kMaxChunk = 8192;
+struct Stat { double m, s; };        // a chunk's largest logit, and the sum of 2^((l - m) c); greedy: its index
+
+__device__ __forceinline__ double wsum(double v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+// Four (f32) or eight (bf16) logits from i on; -inf past the vocabulary. Rows may start at any element.
+template <bool BF16>
+__device__ __forceinline__ void load_logits(const void* row, int i, int vocab, float* v) {
+    constexpr int N = BF16 ? 8 : 4;
+    if (i + N <= vocab) {
+        uint32_t w[4];
+        __builtin_memcpy(w, (const char*)row + (size_t)i * (BF16 ? 2 : 4), 16);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (BF16) {
+                v[2 * j] = __uint_as_float(w[j] << 16);
+                v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+            } else {
+                v[j] = __uint_as_float(w[j]);
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+        v[j] = i + j >= vocab ? -INFINITY : BF16 ? bf2f(((const uint16_t*)row)[i + j]) : ((const float*)row)[i + j];
+}
+template <bool BF16>
+__device__ __forceinline__ float logit(const void* row, int i) {
+    return BF16 ? bf2f(((const uint16_t*)row)[i]) : ((const float*)row)[i];
+}
+
+// Target row j of a lane (j <= k), or draft row j - k - 1, and the place of its stats.
+template <bool BF16>
+__device__ __forceinline__ const void* row_of(const VerifyArgs& a, int lane, int j) {
+    const char* p = j <= a.k ? (const char*)a.logits : (const char*)a.draft_logits;
+    const long long r = j <= a.k ? ((long long)lane * (a.k + 1) + j) * a.ld : ((long long)lane * a.k + j - a.k - 1) * a.ldd;
+    return p + r * (BF16 ? 2 : 4);
+}
+__device__ __forceinline__ int rows_of(const VerifyArgs& a) { return a.draft_logits ? 2 * a.k + 1 : a.k + 1; }
+__device__ __forceinline__ Stat* stats_of(const VerifyArgs& a, int lane, int j) {
+    return (Stat*)a.stats + ((size_t)lane * rows_of(a) + j) * a.chunks;
+}
+
+// A block per (chunk, row): the chunk in registers, its maximum, then its sum of exponentials.
+template <bool BF16, int LOADS>
+__global__ void __launch_bounds__(256) verify_stats(VerifyArgs a) {
+    constexpr int N = BF16 ? 8 : 4;
+    __shared__ float mx[4];
+    __shared__ double sm[4];
+    __shared__ int at[4];
+    const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int c = blockIdx.x % a.chunks, rr = blockIdx.x / a.chunks, j = rr % rows_of(a), ln = rr / rows_of(a);
+    const void* row = row_of<BF16>(a, ln, j);
+    const int i0 = c * a.chunk;
+    float v[LOADS][N];
+#pragma unroll
+    for (int b = 0; b < LOADS; ++b) load_logits<BF16>(row, i0 + (b * 256 + (int)threadIdx.x) * N, a.vocab, v[b]);
+    float m = -INFINITY;
+    bool nan = false;
+#pragma unroll
+    for (int b = 0; b < LOADS; ++b)
+#pragma unroll
+        for (int e = 0; e < N; ++e) { m = fmaxf(m, v[b][e]); nan |= v[b][e] != v[b][e]; }
+    m = wave_max(m);
+    if (__any(nan)) m = __uint_as_float(0x7fc00000u);
+    if (lane == 0) mx[wv] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+    nan = mx[0] != mx[0] || mx[1] != mx[1] || mx[2] != mx[2] || mx[3] != mx[3];
+    Stat* out = stats_of(a, ln, j) + c;
+    if (a.inv_temp == 0.0) {             // greedy: the lowest index of the maximum
+        int best = 0x7fffffff;
+#pragma unroll
+        for (int b = LOADS - 1; b >= 0; --b)
+#pragma unroll
+            for (int e = N - 1; e >= 0; --e)
+                if (v[b][e] == m) best = i0 + (b * 256 + (int)threadIdx.x) * N + e;
+#pragma unroll
+        for (int o = 32; o; o >>= 1) best = min(best, __shfl_xor(best, o));
+        if (lane == 0) at[wv] = best;
+        __syncthreads();
+        if (threadIdx.x == 0) *out = {nan ? (double)__uint_as_float(0x7fc00000u) : (double)m, (double)min(min(at[0], at[1]), min(at[2], at[3]))};
+        return;
+    }
+    double s = 0.0;
+    if (!nan && m > -INFINITY && m < INFINITY) {
+        const double f = a.inv_temp * 1.4426950408889634074, md = m;
+#pragma unroll
+        for (int b = 0; b < LOADS; ++b)
+#pragma unroll
+            for (int e = 0; e < N; ++e) s += exp2_neg(((double)v[b][e] - md) * f);
+    }
+    s = wsum(s);
+    if (lane == 0) sm[wv] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) *out = {nan ? (double)__uint_as_float(0x7fc00000u) : (double)m, (sm[0] + sm[1]) + (sm[2] + sm[3])};
+}
+
+// A row's maximum and sum from its chunks', by one wave; greedy: the maximum and its lowest index.
+__device__ __forceinline__ Stat row_stat(const VerifyArgs& a, const Stat* st, double f) {
+    const int lane = threadIdx.x & 63;
+    double m = -INFINITY;
+    bool nan = false;
+    for (int c = lane; c < a.chunks; c += 64) { m = fmax(m, st[c].m); nan |= st[c].m != st[c].m; }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) m = fmax(m, __shfl_xor(m, o));
+    if (__any(nan)) m = __longlong_as_double(0x7ff8000000000000ll);
+    double s = 0.0;
+    if (f == 0.0) {
+        s = 2147483647.0;
+        for (int c = lane; c < a.chunks; c += 64) if (st[c].m == m) s = fmin(s, st[c].s);
+#pragma unroll
+        for (int o = 32; o; o >>= 1) s = fmin(s, __shfl_xor(s, o));
+    } else {
+        for (int c = lane; c < a.chunks; c += 64) if (st[c].s > 0.0) s += st[c].s * exp2_neg((st[c].m - m) * f);
+        s = wsum(s);
+    }
+    return {m, s};
+}
+// A row with a NaN, an infinity above or nothing but -inf has no distribution.
+__device__ __forceinline__ bool has_dist(const Stat& s) { return s.m > -INFINITY && s.m < INFINITY; }
+
+// What becomes of a lane: its accepted drafts, and where its token comes from.
+enum { kFromTarget = 0, kNotDraft = 1, kRest = 2, kNoToken = 3, kArgmax = 4 };
+struct Fate { int accepted, kind, draft; };
+
+// All waves make the lane's row statistics into rs (row order of row_of); then every thread decides alike.
+template <bool BF16>
+__device__ __forceinline__ Fate decide(const VerifyArgs& a, int ln, double f, Stat* rs) {
+    const int wv = threadIdx.x >> 6, nw = blockDim.x >> 6;
+    for (int j = wv; j < rows_of(a); j += nw) {
+        const Stat s = row_stat(a, stats_of(a, ln, j), f);
+        if ((threadIdx.x & 63) == 0) rs[j] = s;
+    }
+    __syncthreads();
+    const int* d = a.drafts + (size_t)ln * a.k;
+    const float* u = a.u + (size_t)ln * (a.k + 1);
+    for (int j = 0; j < a.k; ++j) {
+        const int t = d[j];
+        if (t < 0) return {j, !has_dist(rs[j]) ? kNoToken : f == 0.0 ? kArgmax : kFromTarget, -1};
+        const bool in = t < a.vocab, dist = has_dist(rs[j]);
+        if (f == 0.0) {
+            if (dist && (double)t == rs[j].s) continue;
+            return {j, dist ? kArgmax : kNoToken, t};
+        }
+        const double p = in && dist ? exp2_neg(((double)logit<BF16>(row_of<BF16>(a, ln, j), t) - rs[j].m) * f) / rs[j].s : 0.0;
+        if (!a.draft_logits) {
+            if ((double)u[j] < p) continue;
+            return {j, dist ? in ? kNotDraft : kFromTarget : kNoToken, t};
+        }
+        const Stat& qs = rs[a.k + 1 + j];
+        const bool qd = has_dist(qs);
+        const double q = in && qd ? exp2_neg(((double)logit<BF16>(row_of<BF16>(a, ln, a.k + 1 + j), t) - qs.m) * f) / qs.s : 0.0;
+        if (qd && (double)u[j] * q < p) continue;
+        return {j, dist ? qd ? kRest : kFromTarget : kNoToken, t};
+    }
+    return {a.k, !has_dist(rs[a.k]) ? kNoToken : f == 0.0 ? kArgmax : kFromTarget, -1};
+}
+
+// The weight of token i of the lane's row: p up to a factor, without the draft, or max(p - q, 0).
+template <bool BF16>
+struct Weights {
+    const void *pr, *qr;
+    double f, pm, qm, pz, qz;        // pz, qz: 1 / sum (kRest)
+    int kind, draft, vocab;
+    __device__ __forceinline__ Weights(const VerifyArgs& a, int ln, const Fate& ft, double f_, const Stat* rs)
+        : f(f_), kind(ft.kind), draft(ft.draft), vocab(a.vocab) {
+        pr = row_of<BF16>(a, ln, ft.accepted);
+        pm = rs[ft.accepted].m;
+        pz = 1.0 / rs[ft.accepted].s;
+        if (kind == kRest) {
+            qr = row_of<BF16>(a, ln, a.k + 1 + ft.accepted);
+            qm = rs[a.k + 1 + ft.accepted].m;
+            qz = 1.0 / rs[a.k + 1 + ft.accepted].s;
+        }
+    }
+    // of N tokens from i on; 0 past the vocabulary
+    template <int N>
+    __device__ __forceinline__ void at(int i, double* w) const {
+        constexpr int L = BF16 ? 8 : 4;
+        float v[N];
+#pragma unroll
+        for (int b = 0; b < N; b += L) load_logits<BF16>(pr, i + b, vocab, v + b);
+#pragma unroll
+        for (int e = 0; e < N; ++e) w[e] = exp2_neg(((double)v[e] - pm) * f);
+        if (kind == kRest) {
+#pragma unroll
+            for (int b = 0; b < N; b += L) load_logits<BF16>(qr, i + b, vocab, v + b);
+#pragma unroll
+            for (int e = 0; e < N; ++e) w[e] = fmax(w[e] * pz - exp2_neg(((double)v[e] - qm) * f) * qz, 0.0);
+        } else if (kind == kNotDraft) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) if (i + e == draft) w[e] = 0.0;
+        }
+    }
+};
+
+// The chunks' sums of max(p - q, 0), for the lanes that draw from it: a block per (chunk, lane).
+template <bool BF16>
+__global__ void __launch_bounds__(256) verify_rest(VerifyArgs a, double* rest) {
+    __shared__ Stat rs[2 * kVerifyDrafts + 1];
+    __shared__ double sm[4];
+    const int c = blockIdx.x % a.chunks, ln = blockIdx.x / a.chunks;
+    const double f = a.inv_temp * 1.4426950408889634074;
+    const Fate ft = decide<BF16>(a, ln, f, rs);
+    if (ft.kind != kRest) return;
+    const Weights<BF16> wt(a, ln, ft, f, rs);
+    double s = 0.0;
+    for (int i = c * a.chunk + (int)threadIdx.x * 8; i < min((c + 1) * a.chunk, a.vocab); i += 2048) {
+        double w[8];
+        wt.template at<8>(i, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += w[e];
+    }
+    s = wsum(s);
+    if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) rest[(size_t)ln * a.chunks + c] = (sm[0] + sm[1]) + (sm[2] + sm[3]);
+}
+
+// A block per lane: the decision, the chunk that holds the border, the token in it.
+constexpr int kMaxChunks = 512;
+template <bool BF16>
+__global__ void __launch_bounds__(1024) verify_token(VerifyArgs a, const double* rest) {
+    __shared__ Stat rs[2 * kVerifyDrafts + 1];
+    __shared__ double cw[kMaxChunks], part[16];
+    __shared__ int where[16], pick;
+    __shared__ double base, border;
+    const int ln = blockIdx.x, wv = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const double f = a.inv_temp * 1.4426950408889634074;
+    Fate ft = decide<BF16>(a, ln, f, rs);
+    int token = -1;
+    if (ft.kind == kArgmax) token = (int)rs[ft.accepted].s;
+    if (ft.kind < kNoToken) {
+        Weights<BF16> wt(a, ln, ft, f, rs);
+        for (int pass = 0; pass < 2; ++pass) {
+            const Stat* st = stats_of(a, ln, ft.accepted);
+            for (int c = threadIdx.x; c < a.chunks; c += 1024)
+                cw[c] = wt.kind == kRest ? rest[(size_t)ln * a.chunks + c]
+                        : st[c].s > 0.0 ? st[c].s * exp2_neg((st[c].m - wt.pm) * f) : 0.0;
+            __syncthreads();
+            if (wt.kind == kNotDraft) {      // the draft's chunk, summed without it
+                const int c = ft.draft / a.chunk, i = c * a.chunk + (int)threadIdx.x * 8;
+                double w[8], s = 0.0;
+                if ((int)threadIdx.x * 8 < a.chunk) {
+                    wt.template at<8>(i, w);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) s += w[e];
+                }
+                s = wsum(s);
+                if (lane == 0) part[wv] = s;
+                __syncthreads();
+                if (threadIdx.x == 0) {
+                    s = 0.0;
+                    for (int w2 = 0; w2 < 16; ++w2) s += part[w2];
+                    cw[c] = s;
+                }
+                __syncthreads();
+            }
+            if (threadIdx.x == 0) {
+                double tot = 0.0;
+                for (int c = 0; c < a.chunks; ++c) tot += cw[c];
+                const double b = (double)a.u[(size_t)ln * (a.k + 1) + a.k] * tot;
+                int got = -1;
+                double run = 0.0, at = 0.0;
+                for (int c = 0; c < a.chunks; ++c) {
+                    if (cw[c] > 0.0) { got = c; at = run; }
+                    run += cw[c];
+                    if (run > b) break;
+                }
+                pick = got;
+                base = at;
+                border = b;
+            }
+            __syncthreads();
+            if (pick >= 0) break;
+            wt.kind = kFromTarget;           // nothing is left of p - q (or of p without the draft): p itself
+            __syncthreads();
+        }
+        if (pick >= 0) {
+            const int i = pick * a.chunk + (int)threadIdx.x * 8;
+            double w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = 0.0;
+            if ((int)threadIdx.x * 8 < a.chunk) wt.template at<8>(i, w);
+            double mine = 0.0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mine += w[e];
+            double run = mine;               // inclusive sums of the wave's lanes
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const double up = __shfl_up(run, o);
+                if (lane >= o) run += up;
+            }
+            __syncthreads();
+            if (lane == 63) part[wv] = run;
+            __syncthreads();
+            run = base + (run - mine);
+            for (int w2 = 0; w2 < wv; ++w2) run += part[w2];
+            int first = 0x7fffffff, last = -1;       // the first past the border, and the last with any weight
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                run += w[e];
+                if (w[e] > 0.0) {
+                    last = i + e;
+                    if (run > border && first == 0x7fffffff) first = i + e;
+                }
+            }
+#pragma unroll
+            for (int o = 32; o; o >>= 1) { first = min(first, __shfl_xor(first, o)); last = max(last, __shfl_xor(last, o)); }
+            if (lane == 0) { where[wv] = first; part[wv] = last; }
+            __syncthreads();
+            first = 0x7fffffff;
+            last = -1;
+            for (int w2 = 0; w2 < 16; ++w2) { first = min(first, where[w2]); last = max(last, (int)part[w2]); }
+            token = first < a.vocab ? first : last;
+        }
+    }
+    if (threadIdx.x == 0) a.accepted[ln] = ft.accepted;
+    if ((int)threadIdx.x <= a.k)
+        a.tokens[(size_t)ln * (a.k + 1) + threadIdx.x] =
+            (int)threadIdx.x < ft.accepted ? a.drafts[(size_t)ln * a.k + threadIdx.x] : (int)threadIdx.x == ft.accepted ? token : -1;
+}
+
+// Chunks of 8192 logits, fewer while the rows are too few to fill the card with them (2048 is the
+// least); vocab <= 2^20 keeps a row at kMaxChunks or less.
+static int chunk_of(long long rows, int vocab) {
+    int chunk = kMaxChunk;
+    while (chunk > 2048 && rows * ((vocab + chunk - 1) / chunk) < 1024) chunk /= 2;
+    return chunk;
+}
+size_t verify_ws_doubles(int max_rows) {
+    // 2 max_rows rows of up to 128 chunks of 8192, or fewer rows of smaller chunks: under 1024 chunks
+    // at twice their size, so at most 2048 and one more a row
+    const size_t rows = 2 * (size_t)max_rows;
+    return 2 * (rows * 128 + 2048 + rows) + (rows * 128 + 2048 + rows);
+}
+
+template <bool BF16>
+static hipError_t launch_v(VerifyArgs& a, hipStream_t st) {
+    const int per = a.draft_logits ? 2 * a.k + 1 : a.k + 1;
+    a.chunk = chunk_of((long long)a.n * per, a.vocab);
+    a.chunks = (a.vocab + a.chunk - 1) / a.chunk;
+    double* rest = a.stats + 2 * (size_t)a.n * per * a.chunks;
+    const dim3 grid((unsigned)a.chunks * a.n * per);
+    constexpr int N = BF16 ? 8 : 4;
+    if (a.chunk == 8192) hipLaunchKernelGGL((verify_stats<BF16, 32 / N>), grid, dim3(256), 0, st, a);
+    else if (a.chunk == 4096) hipLaunchKernelGGL((verify_stats<BF16, 16 / N>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((verify_stats<BF16, 8 / N>), grid, dim3(256), 0, st, a);
+    hipError_t rc = hipGetLastError();
+    if (rc != hipSuccess) return rc;
+    if (a.draft_logits && a.inv_temp != 0.0) {
+        hipLaunchKernelGGL(verify_rest<BF16>, dim3((unsigned)a.chunks * a.n), dim3(256), 0, st, a, rest);
+        if ((rc = hipGetLastError()) != hipSuccess) return rc;
+    }
+    hipLaunchKernelGGL(verify_token<BF16>, dim3(a.n), dim3(1024), 0, st, a, (const double*)rest);
+    return hipGetLastError();
+}
+hipError_t launch_verify(VerifyArgs& a, hipStream_t st) { return a.bf16 ? launch_v<true>(a, st) : launch_v<false>(a, st); }
+
+}  // namespace q35

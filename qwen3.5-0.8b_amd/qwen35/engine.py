@@ -29,6 +29,21 @@ class _Config(C.Structure):
                 ("use_graph", C.c_int)]
 
 
+class _View(C.Structure):
+    _fields_ = [("ptr", C.c_void_p), ("row_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class _Heads(C.Structure):
+    _fields_ = [("q_heads", C.c_int), ("rot_dim", C.c_int), ("theta", C.c_double), ("eps", C.c_double),
+                ("q_norm", C.c_void_p), ("k_norm", C.c_void_p)] + [
+                    (n, _View) for n in ("q", "k", "v", "q_out", "k_out", "v_out")]
+
+
+class _Drafts(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("ld", C.c_int64), ("draft_logits", C.c_void_p), ("draft_ld", C.c_int64),
+                ("dtype", C.c_int), ("drafts", C.c_void_p), ("u", C.c_void_p), ("temperature", C.c_double)]
+
+
 _SIGS = {
     "q35_last_error": ([], C.c_char_p),
     "q35_create": ([C.POINTER(_Config), C.POINTER(C.c_void_p)], C.c_int),
@@ -80,6 +95,19 @@ _SIGS = {
     "q35_op_attn_decode": ([C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int]
                            + [C.c_void_p] * 4 + [C.c_int], C.c_int),
     "q35_op_lm_head_argmax": ([C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p], C.c_int),
+    "q35_kv4_alloc": ([C.c_void_p] + [C.c_int] * 5 + [C.POINTER(C.c_void_p)], C.c_int),
+    "q35_kv4_free": ([C.c_void_p, C.c_void_p], C.c_int),
+    "q35_kv4_set_len": ([C.c_void_p] * 4 + [C.c_int], C.c_int),
+    "q35_kv4_len": ([C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.POINTER(C.c_int32)], C.c_int),
+    "q35_kv4_write": ([C.c_void_p, C.c_void_p] + [C.c_int] * 5 + [C.c_void_p] * 4, C.c_int),
+    "q35_kv4_read": ([C.c_void_p, C.c_void_p] + [C.c_int] * 5 + [C.c_void_p] * 4, C.c_int),
+    "q35_op_qk_norm_rope": ([C.c_void_p, C.POINTER(_Heads), C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_int], C.c_int),
+    "q35_op_kv4_append": ([C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
+                           C.POINTER(_Heads)], C.c_int),
+    "q35_op_attn_kv4": ([C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int,
+                         C.POINTER(_View), C.POINTER(_View), C.c_float, C.c_int, C.c_int, C.POINTER(_View)], C.c_int),
+    "q35_op_draft_verify": ([C.c_void_p, C.POINTER(_Drafts), C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p],
+                            C.c_int),
     "q35_sync": ([C.c_void_p], C.c_int),
     "q35_kprof_read": ([C.c_void_p, C.POINTER(C.c_float), C.POINTER(C.c_int)], C.c_int),
     "q35_set_option": ([C.c_void_p, C.c_char_p, C.c_int], C.c_int),
@@ -116,6 +144,19 @@ def _i32(a) -> np.ndarray:
 
 def _p(a: np.ndarray):
     return a.ctypes.data_as(C.c_void_p)
+
+
+def _lp(lanes: np.ndarray | None, pos: np.ndarray):
+    """Lanes of a call with one position each (None: lane i)."""
+    if lanes is None:
+        return None
+    if lanes.size != pos.size:
+        raise ValueError(f"{lanes.size} lanes and {pos.size} positions")
+    return _p(lanes)
+
+
+def _heads(q_heads, rot_dim, theta, eps, q_norm, k_norm, *views) -> _Heads:
+    return _Heads(q_heads, rot_dim, theta, eps, q_norm, k_norm, *[_View(*v) if v is not None else _View() for v in views])
 
 
 def safetensors_scan(data: bytes | np.ndarray) -> tuple[int, int]:
@@ -235,6 +276,44 @@ class Engine:
     def op_lm_head_argmax(self, x_ptr: int, M: int, tok_ptr: int, logits_ptr: int = 0):
         _ck(load_library().q35_op_lm_head_argmax(self.h, C.c_void_p(x_ptr), M, C.c_void_p(tok_ptr),
                                                  C.c_void_p(logits_ptr) if logits_ptr else None))
+
+    # the 4-bit cache's operators (asynchronous on the engine stream: sync() waits). A view is (pointer, elements
+    # from row to row, elements from head to head) of bf16 rows in a device buffer.
+    def op_qk_norm_rope(self, pos, T: int, q_heads: int, kv_heads: int, head_dim: int, *, rot_dim: int, theta: float,
+                        eps: float, q_norm: int, k_norm: int, k, k_out, q=None, q_out=None):
+        """Norms of q and k per head and their rotation in one pass (q35_op_qk_norm_rope): row i * T + t at
+        position pos[i] + t."""
+        p = _i32(pos)
+        h = _heads(q_heads, rot_dim, theta, eps, q_norm, k_norm, q, k, None, q_out, k_out, None)
+        _ck(load_library().q35_op_qk_norm_rope(self.h, C.byref(h), kv_heads, head_dim, _p(p), p.size, T))
+
+    def op_kv4_append(self, cache: "KvCache4", layer: int, lanes, pos, T: int, q_heads: int, *, rot_dim: int,
+                      theta: float, eps: float, q_norm: int, k_norm: int, k, v, q=None, q_out=None, k_out=None,
+                      v_out=None):
+        """The same pass with k and v appended to `cache` in 4 bits (q35_op_kv4_append); lanes None: lane i."""
+        p, la = _i32(pos), None if lanes is None else _i32(lanes)
+        h = _heads(q_heads, rot_dim, theta, eps, q_norm, k_norm, q, k, v, q_out, k_out, v_out)
+        _ck(load_library().q35_op_kv4_append(self.h, cache.h, layer, _lp(la, p), _p(p), p.size, T, C.byref(h)))
+
+    def op_attn_kv4(self, cache: "KvCache4", layer: int, lanes, pos, T: int, q_heads: int, q, out, *,
+                    scale: float | None = None, window: int = 0, sinks: int = 0, gate=None):
+        """Attention of T rows per sequence over `cache` (q35_op_attn_kv4): a row at p sees slots (p - window, p] and
+        [0, sinks), all up to p with window 0; scale None: head_dim ** -0.5; gate: the output times its sigmoid."""
+        p, la = _i32(pos), None if lanes is None else _i32(lanes)
+        qv, gv, ov = _View(*q), _View(*gate) if gate is not None else None, _View(*out)
+        _ck(load_library().q35_op_attn_kv4(self.h, cache.h, layer, _lp(la, p), _p(p), p.size, T, q_heads, C.byref(qv),
+                                           C.byref(gv) if gv is not None else None,
+                                           cache.head_dim ** -0.5 if scale is None else scale, window, sinks,
+                                           C.byref(ov)))
+
+    def op_draft_verify(self, n: int, k: int, vocab: int, logits: int, drafts: int, u: int, accepted: int, tokens: int, *,
+                        temperature: float = 1.0, draft_logits: int = 0, bf16: bool = False, ld: int = 0,
+                        draft_ld: int = 0):
+        """Sampled verification of n lanes' k drafts from the random numbers u [n][k + 1] (q35_op_draft_verify); the
+        logits' row strides are vocab unless given."""
+        d = _Drafts(logits, ld or vocab, draft_logits or None, draft_ld or vocab, int(bf16), drafts, u, temperature)
+        _ck(load_library().q35_op_draft_verify(self.h, C.byref(d), n, k, vocab, C.c_void_p(accepted),
+                                               C.c_void_p(tokens)))
 
     def timer_begin(self):
         _ck(load_library().q35_timer_begin(self.h))
@@ -454,6 +533,55 @@ class State:
         _ck(load_library().q35_mtp_adaptive_step(self.eng.h, self.h, _p(ln) if ln is not None else None, n, _p(c),
                                                  C.cast(pol, C.c_void_p), stop, _p(emit), _p(ne), _p(dep), _p(st)))
         return [list(emit[i, :ne[i]]) for i in range(n)], dep
+
+
+class KvCache4:
+    """A K/V cache in 4 bits of `layers` attention layers (q35_kv4_*, include/q35.h): lanes x cap slots of
+    kv_heads heads; each (layer, lane) holds slots [0, length)."""
+
+    def __init__(self, eng: Engine, lanes: int, cap: int, layers: int = 1, kv_heads: int = 2, head_dim: int = 256):
+        self.eng = eng
+        self.layers, self.lanes, self.cap, self.kv_heads, self.head_dim = layers, lanes, cap, kv_heads, head_dim
+        self.h = None
+        h = C.c_void_p()
+        _ck(load_library().q35_kv4_alloc(eng.h, layers, lanes, cap, kv_heads, head_dim, C.byref(h)))
+        self.h = h
+
+    def length(self, layer: int, lane: int) -> int:
+        v = C.c_int32()
+        _ck(load_library().q35_kv4_len(self.eng.h, self.h, layer, lane, C.byref(v)))
+        return v.value
+
+    def set_len(self, lanes, lengths):
+        """Lengths of these lanes in every layer: 0 starts a lane over, fewer slots drop its last ones."""
+        n, la = _i32(lengths), None if lanes is None else _i32(lanes)
+        _ck(load_library().q35_kv4_set_len(self.eng.h, self.h, _lp(la, n), _p(n), n.size))
+
+    def write(self, layer: int, lane0: int, n_lanes: int, slot0: int, n_slots: int, k_codes: int, k_scales: int,
+              v_codes: int, v_scales: int):
+        """Slots from device buffers of codes [n_lanes][kv_heads][n_slots][head_dim / 2] and scale bytes
+        [..][head_dim / 32] (device pointers)."""
+        self._copy("q35_kv4_write", layer, lane0, n_lanes, slot0, n_slots, k_codes, k_scales, v_codes, v_scales)
+
+    def read(self, layer: int, lane0: int, n_lanes: int, slot0: int, n_slots: int, k_codes: int, k_scales: int,
+             v_codes: int, v_scales: int):
+        """Slots to device buffers, in write's layout."""
+        self._copy("q35_kv4_read", layer, lane0, n_lanes, slot0, n_slots, k_codes, k_scales, v_codes, v_scales)
+
+    def _copy(self, call, layer, lane0, n_lanes, slot0, n_slots, *ptrs):
+        _ck(getattr(load_library(), call)(self.eng.h, self.h, layer, lane0, n_lanes, slot0, n_slots,
+                                          *[C.c_void_p(p) for p in ptrs]))
+
+    def close(self):
+        if self.h:
+            load_library().q35_kv4_free(self.eng.h, self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 class Forward:
