@@ -116,7 +116,7 @@ HeadArgs head_args(const q35_heads& s, int kv_heads, int D, int n, int T, bool c
     a.q_norm = s.q_norm; a.k_norm = s.k_norm;
     a.q_heads = s.q_heads; a.kv_heads = kv_heads; a.D = D; a.rot = s.rot_dim; a.T = T;
     a.eps = s.eps;
-    a.log2_theta = s.rot_dim ? std::log2(s.theta) : 0.0;
+    a.rate = s.rot_dim ? -2.0 * std::log2(s.theta) / s.rot_dim : 0.0;
     return a;
 }
 

@@ -53,7 +53,7 @@ struct HeadArgs {
     HeadView q, k, v, q_out, k_out, v_out;   // v, q_out, k_out, v_out: p null where not wanted
     const uint16_t *q_norm, *k_norm;
     int q_heads, kv_heads, D, rot, T;
-    double eps, log2_theta;
+    double eps, rate;            // rate: -2 log2(theta) / rot, the angles' exponents' step
     uint8_t* cache;              // layer base, or null
     size_t lane_bytes, region;   // bytes of a lane (its kv_heads regions), of a region
     int pos[kSeqArgs];
@@ -71,9 +71,10 @@ struct Kv4Attn {
     int window, sinks;           // window 0: every slot up to the row's own
     float scale;
     float* part;                 // split workspace (kv4_part_floats())
-    int pos[kSeqArgs];
-    uint16_t lane[kSeqArgs];
-    uint16_t first[kSeqArgs + 1];  // first split of each sequence (set by the launcher)
+    int n, splits;               // sequences and their splits together (the launcher sets these and first)
+    alignas(16) int pos[kSeqArgs];
+    alignas(16) uint16_t lane[kSeqArgs];
+    alignas(16) uint16_t first[kSeqArgs];   // first split of each sequence; 0xffff past the last
 };
 size_t kv4_part_floats();
 hipError_t launch_attn_kv4(Kv4Attn& a, int n, hipStream_t st);

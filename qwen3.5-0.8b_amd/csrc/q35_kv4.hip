@@ -20,6 +20,11 @@ __device__ __forceinline__ uint32_t two_values(uint32_t w, float scale) {
 }
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
 
+__device__ __forceinline__ f32x4 wide(uint2 w) {          // four bf16
+    return f32x4{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
+                 __uint_as_float(w.y & 0xffff0000u)};
+}
+
 // ------------------------------------------------------------------ norms, rotation, append
 // sin and cos of a quarter turn's worth around 0 by their Taylor series in float64 (|r| <= pi / 4:
 // the first terms left out are below 2^-54).
@@ -43,11 +48,29 @@ __device__ __forceinline__ void sincos_small(double r, double& s, double& c) {
     s = __builtin_fma(r * z, a, r);
     c = __builtin_fma(z, b, 1.0);
 }
-// cos and sin of pos * theta^(-2 i / rot). In turns the whole part drops out exactly, so a far
-// position keeps its angle: float32 angles are off by up to 4e-3 at position 1e5.
-__device__ __forceinline__ float2 turn(int pos, int i, int rot, double log2_theta) {
+// 2^x for x <= 0 by the Taylor series of 2^f, |f| <= 1/2 (the first term left out is below 2^-56).
+__device__ __forceinline__ double exp2_d(double x) {
+    const double k = rint(x), f = (x - k) * 0.69314718055994530942;
+    double p = 1.0 / 6227020800.0;
+    p = __builtin_fma(p, f, 1.0 / 479001600.0);
+    p = __builtin_fma(p, f, 1.0 / 39916800.0);
+    p = __builtin_fma(p, f, 1.0 / 3628800.0);
+    p = __builtin_fma(p, f, 1.0 / 362880.0);
+    p = __builtin_fma(p, f, 1.0 / 40320.0);
+    p = __builtin_fma(p, f, 1.0 / 5040.0);
+    p = __builtin_fma(p, f, 1.0 / 720.0);
+    p = __builtin_fma(p, f, 1.0 / 120.0);
+    p = __builtin_fma(p, f, 1.0 / 24.0);
+    p = __builtin_fma(p, f, 1.0 / 6.0);
+    p = __builtin_fma(p, f, 0.5);
+    p = __builtin_fma(p, f, 1.0);
+    return __builtin_ldexp(__builtin_fma(p, f, 1.0), (int)k);
+}
+// cos and sin of pos * theta^(-2 i / rot) = pos * 2^(i * rate). In turns the whole part drops out exactly,
+// so a far position keeps its angle: float32 angles are off by up to 4e-3 at position 1e5.
+__device__ __forceinline__ float2 turn(int pos, int i, double rate) {
     constexpr double kInv2Pi = 0.15915494309189533577;
-    double u = (double)pos * (exp2(-2.0 * i / rot * log2_theta) * kInv2Pi);
+    double u = (double)pos * (exp2_d(i * rate) * kInv2Pi);
     u -= rint(u);
     const double q = rint(4.0 * u);
     double s, c;
@@ -57,108 +80,171 @@ __device__ __forceinline__ float2 turn(int pos, int i, int rot, double log2_thet
     return k & 2 ? make_float2((float)-cc, (float)-ss) : make_float2((float)cc, (float)ss);
 }
 
-__device__ __forceinline__ float4 load4(const uint16_t* p) {
-    const uint2 w = *(const uint2*)p;
-    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
-                       __uint_as_float(w.y & 0xffff0000u));
+// Sum over a head's 16 lanes in float64, by DPP moves.
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double v) {
+    const unsigned long long w = __builtin_bit_cast(unsigned long long, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)w, CTRL, 0xf, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(w >> 32), CTRL, 0xf, 0xf, false);
+    return __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo);
+}
+__device__ __forceinline__ double head_sum(double v) {
+    v += dpp_d<0x128>(v);
+    v += dpp_d<0x124>(v);
+    v += dpp_d<0x4E>(v);
+    v += dpp_d<0xB1>(v);
+    return v;
+}
+constexpr int kAngles = 512;         // of a block's rows: 4 x 128
+// 1 / sqrt(x) from the instruction's approximation by two Newton steps (float64 to its last bits)
+__device__ __forceinline__ double rsqrt_d(double x) {
+    double y = __builtin_amdgcn_rsq(x);
+    y = y * __builtin_fma(-0.5 * x * y, y, 1.5);
+    return y * __builtin_fma(-0.5 * x * y, y, 1.5);
 }
 
-// One wave per row and unit of 256 dims (256 / D heads of q, of k or of v), four dims a lane. What it
-// writes is decided by borders (a code's midpoints, a scale's step), so every float32 operation is one
-// rounding in the stated order, and the sum of squares, the root and the angles are float64.
+// A block takes `per_block` rows (or, of few rows with many heads, a part of one row's heads); a wave four heads
+// of a row at a time -- q's, k's and v's in one list -- 16 lanes a head, a lane dims 64 c + 4 l .. + 3 of
+// each 64 (so a head's sum needs four steps between lanes for D products, and loads and stores are whole
+// 128-byte runs). The rows' angles are made once for the block, with the first heads' loads in flight.
+// What the kernel writes is decided by borders (a code's midpoints, a scale's step), so every float32
+// operation is one rounding in the stated order, and the sum of squares, the root and the angles are
+// float64.
 template <int D>
-__global__ void __launch_bounds__(256) heads_kernel(HeadArgs a, int rows, int units) {
-    constexpr int kPer = 256 / D;            // heads of a unit
-    constexpr int kLanes = D / 4;            // lanes of a head
-    __shared__ float xs[4][256];
-    __shared__ float2 cs[4][128];
-    const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const long long w = (long long)blockIdx.x * 4 + wv;
-    const int r = (int)(w / units);
-    if (r >= rows) return;                   // whole waves; no block barrier below
-    int u = (int)(w % units);
-    const int qu = a.q.p ? (a.q_heads + kPer - 1) / kPer : 0, ku = (a.kv_heads + kPer - 1) / kPer;
-    const int kind = u < qu ? 0 : u < qu + ku ? 1 : 2;
-    u -= kind == 0 ? 0 : kind == 1 ? qu : qu + ku;
-    const int heads = kind == 0 ? a.q_heads : a.kv_heads;
-    const int h = u * kPer + lane / kLanes, d0 = lane % kLanes * 4;
-    const bool on = h < heads;
-    const int seq = r / a.T, t = r - seq * a.T, pos = a.pos[seq] + t;
-    const HeadView in = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-    const HeadView out = kind == 0 ? a.q_out : kind == 1 ? a.k_out : a.v_out;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (on) x = load4(in.p + r * in.row + h * in.head + d0);
-    if (kind < 2) {
-        double ss = ((double)(x.x * x.x) + (double)(x.y * x.y)) + ((double)(x.z * x.z) + (double)(x.w * x.w));
+__global__ void __launch_bounds__(256) heads_kernel(HeadArgs a, int rows, int per_block, int parts, int units) {
+    constexpr int C = D / 64;
+    __shared__ float xs[4][4][D];
+    __shared__ float2 cs[kAngles];
+    const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63, j = lane >> 4, l = lane & 15;
+    const int r0 = blockIdx.x / parts * per_block, u0 = blockIdx.x % parts * units;
+    const int nq = a.q.p ? a.q_heads : 0, all = nq + a.kv_heads * (a.v.p ? 2 : 1), half = a.rot / 2;
+    const int nu = min(units, (all + 3) / 4 - u0), items = min(per_block, rows - r0) * nu;
+    struct Item { int r, kind, h; };         // kind: 0 q, 1 k, 2 v, 3 none
+    const auto item = [&](int i) {
+        const int rr = i / nu;
+        const int x = (u0 + i - rr * nu) * 4 + j;
+        Item t;
+        t.r = r0 + rr;
+        t.kind = i >= items || x >= all ? 3 : x < nq ? 0 : x < nq + a.kv_heads ? 1 : 2;
+        t.h = t.kind == 0 ? x : t.kind == 1 ? x - nq : x - nq - a.kv_heads;
+        return t;
+    };
+    const auto fetch = [&](const Item& t, uint2* w) {
+        const uint16_t* p = t.kind == 0 ? a.q.p + t.r * a.q.row + t.h * a.q.head
+                          : t.kind == 1 ? a.k.p + t.r * a.k.row + t.h * a.k.head : a.v.p + t.r * a.v.row + t.h * a.v.head;
 #pragma unroll
-        for (int o = kLanes / 2; o; o >>= 1) ss += __shfl_xor(ss, o);
-        const float rs = (float)(1.0 / sqrt(ss / D + a.eps));
-        const float4 nw = load4((kind == 0 ? a.q_norm : a.k_norm) + d0);
-        x.x = x.x * rs * (1.0f + nw.x);
-        x.y = x.y * rs * (1.0f + nw.y);
-        x.z = x.z * rs * (1.0f + nw.z);
-        x.w = x.w * rs * (1.0f + nw.w);
-        const int half = a.rot / 2;
-        for (int i = lane; i < half; i += 64) cs[wv][i] = turn(pos, i, a.rot, a.log2_theta);
-        *(float4*)&xs[wv][lane * 4] = x;
-        wave_sync();
-        const float* hx = &xs[wv][lane / kLanes * D];
-        float y[4] = {x.x, x.y, x.z, x.w};
+        for (int c = 0; c < C; ++c) w[c] = t.kind < 3 ? *(const uint2*)(p + 64 * c + 4 * l) : make_uint2(0, 0);
+    };
+    Item now = item(wv);
+    uint2 raw[C];
+    fetch(now, raw);
+    for (int i = tid; i < min(per_block, rows - r0) * half; i += 256) {
+        const int rr = i / half, r = r0 + rr;
+        cs[i] = turn(a.pos[r / a.T] + r % a.T, i - rr * half, a.rate);
+    }
+    lds_barrier();
+    for (int i = wv; i < items; i += 4) {            // whole waves; no block barrier in the loop
+        const Item t = now;
+        f32x4 x[C];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int d = d0 + e;
-            if (d < half) {
-                const float2 c = cs[wv][d];
-                y[e] = y[e] * c.x - hx[d + half] * c.y;
-            } else if (d < a.rot) {
-                const float2 c = cs[wv][d - half];
-                y[e] = y[e] * c.x + hx[d - half] * c.y;
+        for (int c = 0; c < C; ++c) x[c] = wide(raw[c]);
+        now = item(i + 4);
+        fetch(now, raw);
+        const int seq = t.r / a.T, pos = a.pos[seq] + t.r - seq * a.T;
+        const uint16_t* nw = t.kind == 0 ? a.q_norm : a.k_norm;
+        double ss = 0.0;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) ss = __builtin_fma((double)x[c][e], (double)x[c][e], ss);
+        const float rs = (float)rsqrt_d(head_sum(ss) * (1.0 / D) + a.eps);
+        if (t.kind < 2) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) x[c] = x[c] * rs * (1.0f + wide(*(const uint2*)(nw + 64 * c + 4 * l)));
+        }
+        if (half) {
+            float* hx = xs[wv][j];
+            const float2* cr = cs + (t.r - r0) * half;
+            wave_sync();
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+                if (64 * c < a.rot) *(f32x4*)&hx[64 * c + 4 * l] = x[c];
+            wave_sync();
+            if (t.kind < 2) {
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const int d = 64 * c + 4 * l;
+                    if (d >= a.rot) continue;
+                    if ((half & 3) == 0) {           // a lane's four dims lie on one side of the pairs
+                        const bool low = d < half;
+                        const int k = low ? d : d - half;
+                        const f32x4 o = *(const f32x4*)&hx[low ? d + half : k];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 cc = cr[k + e];
+                            const float p = x[c][e] * cc.x, q = o[e] * cc.y;
+                            x[c][e] = low ? p - q : p + q;
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if (d + e < half) {
+                                const float2 cc = cr[d + e];
+                                x[c][e] = x[c][e] * cc.x - hx[d + e + half] * cc.y;
+                            } else if (d + e < a.rot) {
+                                const float2 cc = cr[d + e - half];
+                                x[c][e] = x[c][e] * cc.x + hx[d + e - half] * cc.y;
+                            }
+                        }
+                    }
+                }
             }
         }
-        x = make_float4(y[0], y[1], y[2], y[3]);
-    }
-    if (kind == 0 || !a.cache) {
-        if (on && out.p) {
-            uint2 o;
-            o.x = f2bf2(x.x, x.y);
-            o.y = f2bf2(x.z, x.w);
-            *(uint2*)(const_cast<uint16_t*>(out.p) + r * out.row + h * out.head + d0) = o;
+        if (t.kind == 3) continue;                   // lanes without a head; their wave goes on
+        const HeadView& out = t.kind == 0 ? a.q_out : t.kind == 1 ? a.k_out : a.v_out;
+        uint16_t* op = const_cast<uint16_t*>(out.p) + t.r * out.row + t.h * out.head;
+        if (t.kind == 0 || !a.cache) {
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+                *(uint2*)(op + 64 * c + 4 * l) = make_uint2(f2bf2(x[c][0], x[c][1]), f2bf2(x[c][2], x[c][3]));
+            continue;
         }
-        return;
-    }
-    // the group's largest magnitude as bits (eight lanes): an infinity or a NaN is the largest of all
-    uint32_t top = 0;
+        uint8_t* tile = a.cache + a.lane[seq] * a.lane_bytes + t.h * a.region + (size_t)(pos >> 5) * kv4_tile_bytes(D);
+        const int tk = pos & 31;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint((&x.x)[e]) & 0x7fffffffu);
+        for (int c = 0; c < C; ++c) {
+            // the group's largest magnitude as bits (8 lanes): an infinity or a NaN is the largest of all
+            uint32_t top = 0;
 #pragma unroll
-    for (int o = 4; o; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
-    // top = 1.m 2^E: 6 * 2^(E - 2) covers it up to m = 0.5, else one step more. Kept within 2^-119 ..
-    // 2^125, so that no value of a group overflows bf16 or loses bits below its normal range.
-    uint32_t b = max((int)(top >> 23) - 2 + ((top & 0x7fffffu) > 0x400000u), 8);
-    b = top >= 0x7f800000u ? 255u : min(b, 252u);
-    const float sc = scale_of(b);
-    uint32_t code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, x.x, x.y, sc, 0);
-    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x.z, x.w, sc, 1);
-    if (!on) return;
-    if (out.p) {
-        uint2 o;
-        o.x = two_values<0>(code, sc);
-        o.y = two_values<1>(code, sc);
-        *(uint2*)(const_cast<uint16_t*>(out.p) + r * out.row + h * out.head + d0) = o;
+            for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(x[c][e]) & 0x7fffffffu);
+            top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x141, 0xf, 0xf, false));   // lane 7 - i of 8
+            top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xf, 0xf, false));
+            top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xf, 0xf, false));
+            // top = 1.m 2^E: 6 * 2^(E - 2) covers it up to m = 0.5, else one step more. Kept within
+            // 2^-119 .. 2^125, so that no value overflows bf16 or loses bits below its normal range.
+            uint32_t b = max((int)(top >> 23) - 2 + ((top & 0x7fffffu) > 0x400000u), 8);
+            b = top >= 0x7f800000u ? 255u : min(b, 252u);
+            const float sc = scale_of(b);
+            uint32_t code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, x[c][0], x[c][1], sc, 0);
+            code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[c][2], x[c][3], sc, 1);
+            const int d = 64 * c + 4 * l;
+            if (out.p) *(uint2*)(op + d) = make_uint2(two_values<0>(code, sc), two_values<1>(code, sc));
+            *(uint16_t*)(tile + (t.kind == 1 ? kv4_k_code(D, tk, d) : kv4_v_code(D, tk, d))) = (uint16_t)code;
+            if ((l & 7) == 0) tile[t.kind == 1 ? kv4_k_scale(D, tk, d >> 5) : kv4_v_scale(D, tk, d >> 5)] = (uint8_t)b;
+        }
     }
-    uint8_t* tile = a.cache + a.lane[seq] * a.lane_bytes + h * a.region + (size_t)(pos >> 5) * kv4_tile_bytes(D);
-    const int tk = pos & 31;
-    *(uint16_t*)(tile + (kind == 1 ? kv4_k_code(D, tk, d0) : kv4_v_code(D, tk, d0))) = (uint16_t)code;
-    if ((lane & 7) == 0) tile[kind == 1 ? kv4_k_scale(D, tk, d0 >> 5) : kv4_v_scale(D, tk, d0 >> 5)] = (uint8_t)b;
 }
 
 hipError_t launch_heads(const HeadArgs& a, int n, hipStream_t st) {
-    const int per = 256 / a.D, qu = a.q.p ? (a.q_heads + per - 1) / per : 0, ku = (a.kv_heads + per - 1) / per;
-    const int units = qu + ku * (a.v.p ? 2 : 1), rows = n * a.T;
-    const long long blocks = ((long long)rows * units + 3) / 4;
+    const int units = ((a.q.p ? a.q_heads : 0) + a.kv_heads * (a.v.p ? 2 : 1) + 3) / 4, rows = n * a.T;
+    // rows of a block: one while they are too few to give every CU four blocks, else up to four; of very few
+    // rows with many heads, four units (one a wave) in a block
+    const int per_block = rows >= 4096 ? 4 : rows >= 2048 ? 2 : 1;
+    const int some = rows < 256 ? std::min(units, 4) : units, parts = (units + some - 1) / some;
+    const long long blocks = (long long)((rows + per_block - 1) / per_block) * parts;
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
     auto k = a.D == 256 ? heads_kernel<256> : a.D == 128 ? heads_kernel<128> : heads_kernel<64>;
-    hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(256), 0, st, a, rows, units);
+    hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(256), 0, st, a, rows, per_block, parts, some);
     return hipGetLastError();
 }
 
@@ -394,34 +480,69 @@ __host__ __device__ inline TileList tile_list(int p0, int p1, int window, int si
 
 constexpr int kSplitRows = 16;       // rows of one partial result
 constexpr int kMaxSplits = 2048;     // partial results of one launch (workspace)
+constexpr int kSeqSplits = 256;      // splits of one sequence
 size_t kv4_part_floats() { return (size_t)kMaxSplits * kSplitRows * (256 + 4); }
 
-// Sequence of item z by bisection of first[].
-__device__ __forceinline__ int find_seq(const uint16_t* first, int n, int z) {
-    int lo = 0, hi = n - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (first[mid] <= z) lo = mid;
-        else hi = mid - 1;
+// What a block needs of its sequence. The arrays are kernel arguments, cold in every cache at a launch:
+// a wave loads all of them at once (four entries a lane) and finds the sequence by counting the entries of
+// first[] up to z, instead of bisecting them with a round trip to memory per step.
+struct Seq { int i, pos, lane, split, splits; };
+__device__ __forceinline__ int entry(uint32_t a, uint32_t b, uint32_t c, uint32_t d, int i) {
+    const uint32_t v = (i & 3) == 0 ? a : (i & 3) == 1 ? b : (i & 3) == 2 ? c : d;
+    return __builtin_amdgcn_readlane((int)v, i >> 2);
+}
+__device__ __forceinline__ Seq find_seq(const Kv4Attn& a, int z) {
+    const int lane = threadIdx.x & 63;
+    const uint2 f = ((const uint2*)a.first)[lane], l = ((const uint2*)a.lane)[lane];
+    const uint4 p = ((const uint4*)a.pos)[lane];
+    const uint32_t f0 = f.x & 0xffffu, f1 = f.x >> 16, f2 = f.y & 0xffffu, f3 = f.y >> 16, zz = (uint32_t)z;
+    const int i = __popcll(__ballot(f0 <= zz)) + __popcll(__ballot(f1 <= zz)) + __popcll(__ballot(f2 <= zz)) +
+                  __popcll(__ballot(f3 <= zz)) - 1;
+    Seq s;
+    s.i = i;
+    s.pos = entry(p.x, p.y, p.z, p.w, i);
+    s.lane = entry(l.x & 0xffffu, l.x >> 16, l.y & 0xffffu, l.y >> 16, i);
+    const int at = entry(f0, f1, f2, f3, i), end = i + 1 < a.n ? entry(f0, f1, f2, f3, i + 1) : a.splits;
+    s.split = z - at;
+    s.splits = end - at;
+    return s;
+}
+
+// The end of a row's four dims: normalised, gated, rounded.
+__device__ __forceinline__ void store_row4(const Kv4Attn& a, f32x4 o, float sum, int seq, int h, int rho, int d) {
+    const int group = a.q_heads / a.kv_heads, t = rho / group, hq = h * group + rho - t * group;
+    const long long row = (long long)seq * a.T + t;
+    o /= sum;
+    if (a.gate.p) {
+        const f32x4 gt = wide(*(const uint2*)(a.gate.p + row * a.gate.row + hq * a.gate.head + d));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] *= sigmoid_f(gt[i]);
     }
-    return lo;
+    *(uint2*)(const_cast<uint16_t*>(a.out.p) + row * a.out.row + hq * a.out.head + d) =
+        make_uint2(f2bf2(o[0], o[1]), f2bf2(o[2], o[3]));
+}
+// Partial result of (split z, kv head h, row rho): D sums, then the maximum and the sum of the weights.
+template <int D, int NQ>
+__device__ __forceinline__ const float* part_of(const Kv4Attn& a, int row_tiles, int z, int h, int rho) {
+    return a.part + ((((size_t)z * a.kv_heads + h) * row_tiles + rho / (NQ * 16)) * NQ * kSplitRows + rho % (NQ * 16)) * (D + 4);
 }
 
 // Decode and verify rows: a block per (sequence, split of its tiles, kv head, NQ x 16 rows), its four
 // waves on every fourth tile with the next one's loads in flight, their states joined through LDS.
 template <int D, int NQ>
-__global__ void __launch_bounds__(256) attn_kv4_kernel(Kv4Attn a, int n, int row_tiles) {
+__global__ void __launch_bounds__(256) attn_kv4_kernel(Kv4Attn a, int row_tiles) {
     __shared__ float os[4][16][D + 4];
     __shared__ float ms[4][16], ls[4][16];
     __shared__ uint32_t bs[4][16];
     const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63, nn = lane & 15, g = lane >> 4;
     const int rt = blockIdx.x % row_tiles, h = blockIdx.x / row_tiles % a.kv_heads, z = blockIdx.x / (row_tiles * a.kv_heads);
-    const int seq = find_seq(a.first, n, z), split = z - a.first[seq], splits = a.first[seq + 1] - a.first[seq];
-    const int group = a.q_heads / a.kv_heads, rows = a.T * group, rho0 = rt * NQ * 16, pos = a.pos[seq];
+    const Seq sq = find_seq(a, z);
+    const int seq = sq.i, split = sq.split, splits = sq.splits, pos = sq.pos;
+    const int group = a.q_heads / a.kv_heads, rows = a.T * group, rho0 = rt * NQ * 16;
     const int rho1 = min(rho0 + NQ * 16, rows) - 1;
     const TileList tl = tile_list(pos + rho0 / group, pos + rho1 / group, a.window, a.sinks);
     const int t0 = (int)((long long)tl.count * split / splits), t1 = (int)((long long)tl.count * (split + 1) / splits);
-    const uint8_t* region = a.cache + a.lane[seq] * a.lane_bytes + h * a.region;
+    const uint8_t* region = a.cache + sq.lane * a.lane_bytes + h * a.region;
 
     q35_bf16x8 qf[NQ][D / 32];
     Sight sight[NQ];
@@ -486,19 +607,8 @@ __global__ void __launch_bounds__(256) attn_kv4_kernel(Kv4Attn a, int n, int row
                 o += f * *(const f32x4*)&os[w][n0][d];
             }
             if (((bs[0][n0] | bs[1][n0] | bs[2][n0] | bs[3][n0]) >> (d / 32)) & 1) o *= __uint_as_float(0x7fc00000u);
-            const int t = rho / group, hq = h * group + rho - t * group;
-            const long long row = (long long)seq * a.T + t;
             if (splits == 1) {
-                o /= sum;
-                if (a.gate.p) {
-                    const float4 gt = load4(a.gate.p + row * a.gate.row + hq * a.gate.head + d);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o[i] *= sigmoid_f((&gt.x)[i]);
-                }
-                uint2 w;
-                w.x = f2bf2(o[0], o[1]);
-                w.y = f2bf2(o[2], o[3]);
-                *(uint2*)(const_cast<uint16_t*>(a.out.p) + row * a.out.row + hq * a.out.head + d) = w;
+                store_row4(a, o, sum, seq, h, rho, d);
             } else {
                 float* p = a.part + ((size_t)blockIdx.x * NQ + c) * kSplitRows * (D + 4) + n0 * (D + 4);
                 *(f32x4*)(p + d) = o;
@@ -508,70 +618,124 @@ __global__ void __launch_bounds__(256) attn_kv4_kernel(Kv4Attn a, int n, int row
     }
 }
 
-// Joins the splits of the sequences that have more than one: a block per (sequence, kv head, row), a
-// thread per four dims, the splits in order.
+// Joins the splits of sequences that have few (up to 8): a thread per four dims of a row, all its
+// loads at once.
+constexpr int kFewSplits = 8;
 template <int D, int NQ>
-__global__ void __launch_bounds__(64) attn_kv4_join(Kv4Attn a, int row_tiles) {
-    const int group = a.q_heads / a.kv_heads, rows = a.T * group;
-    const int rho = blockIdx.x % rows, h = blockIdx.x / rows % a.kv_heads, seq = blockIdx.x / (rows * a.kv_heads);
-    const int splits = a.first[seq + 1] - a.first[seq], d = threadIdx.x * 4;
-    if (splits == 1 || d >= D) return;
-    const int rt = rho / (NQ * 16), c = rho % (NQ * 16) / 16, n0 = rho % 16;
-    const size_t step = (size_t)row_tiles * a.kv_heads * NQ * kSplitRows * (D + 4);
-    const float* p = a.part + (((size_t)a.first[seq] * a.kv_heads + h) * row_tiles + rt) * NQ * kSplitRows * (D + 4) +
-                     ((size_t)c * kSplitRows + n0) * (D + 4);
-    float m = -INFINITY;
-    for (int s = 0; s < splits; ++s) m = fmaxf(m, p[s * step + D]);
+__global__ void __launch_bounds__(256) attn_kv4_join_few(Kv4Attn a, int row_tiles) {
+    const int rows = a.T * (a.q_heads / a.kv_heads);
+    const long long e = ((long long)blockIdx.x * 256 + threadIdx.x) / (D / 4);
+    const int d = threadIdx.x % (D / 4) * 4;
+    const int rho = (int)(e % rows), h = (int)(e / rows % a.kv_heads);
+    const long long seq = e / ((long long)rows * a.kv_heads);
+    if (seq >= a.n) return;
+    const int first = a.first[seq], splits = (seq + 1 < a.n ? a.first[seq + 1] : a.splits) - first;
+    if (splits == 1) return;
+    const float* p = part_of<D, NQ>(a, row_tiles, first, h, rho);
+    const size_t step = (size_t)a.kv_heads * row_tiles * NQ * kSplitRows * (D + 4);
+    f32x4 o[kFewSplits];
+    float2 ml[kFewSplits];
+#pragma unroll
+    for (int s = 0; s < kFewSplits; ++s) {
+        const bool in = s < splits;
+        o[s] = in ? *(const f32x4*)(p + s * step + d) : f32x4{0.f, 0.f, 0.f, 0.f};
+        ml[s] = in ? *(const float2*)(p + s * step + D) : make_float2(-INFINITY, 0.f);
+    }
+    float m = ml[0].x;
+#pragma unroll
+    for (int s = 1; s < kFewSplits; ++s) m = fmaxf(m, ml[s].x);
     const float mz = m == -INFINITY ? 0.f : m;
     float sum = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < splits; ++s) {
-        const float f = __builtin_amdgcn_exp2f(p[s * step + D] - mz);
-        sum += f * p[s * step + D + 1];
-        o += f * *(const f32x4*)(p + s * step + d);
-    }
-    o /= sum;
-    const int t = rho / group, hq = h * group + rho - t * group;
-    const long long row = (long long)seq * a.T + t;
-    if (a.gate.p) {
-        const float4 gt = load4(a.gate.p + row * a.gate.row + hq * a.gate.head + d);
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] *= sigmoid_f((&gt.x)[i]);
+    for (int s = 0; s < kFewSplits; ++s) {
+        const float f = __builtin_amdgcn_exp2f(ml[s].x - mz);
+        sum += f * ml[s].y;
+        x += f * o[s];
     }
-    uint2 w;
-    w.x = f2bf2(o[0], o[1]);
-    w.y = f2bf2(o[2], o[3]);
-    *(uint2*)(const_cast<uint16_t*>(a.out.p) + row * a.out.row + hq * a.out.head + d) = w;
+    store_row4(a, x, sum, (int)seq, h, rho, d);
+}
+
+// The same for any number of splits: a block per (sequence, kv head, row, 64 dims). The splits' factors are
+// made once into LDS; 16 threads take a split's dims, 16 splits at a time, and their sums meet in LDS:
+// always in the same order.
+template <int D, int NQ>
+__global__ void __launch_bounds__(256) attn_kv4_join(Kv4Attn a, int row_tiles) {
+    __shared__ float fs[kSeqSplits];
+    __shared__ float red[8];
+    __shared__ f32x4 os[256];
+    const int rows = a.T * (a.q_heads / a.kv_heads), tid = threadIdx.x, d = blockIdx.x % (D / 64) * 64 + tid % 16 * 4;
+    const int e = blockIdx.x / (D / 64), rho = e % rows, h = e / rows % a.kv_heads, seq = e / (rows * a.kv_heads);
+    const int first = a.first[seq], splits = (seq + 1 < a.n ? a.first[seq + 1] : a.splits) - first;
+    if (splits == 1) return;
+    const float* p = part_of<D, NQ>(a, row_tiles, first, h, rho);
+    const size_t step = (size_t)a.kv_heads * row_tiles * NQ * kSplitRows * (D + 4);
+    f32x4 v[kSeqSplits / 16];
+#pragma unroll
+    for (int i = 0; i < kSeqSplits / 16; ++i) {
+        const int s = i * 16 + tid / 16;
+        v[i] = s < splits ? *(const f32x4*)(p + s * step + d) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (tid < splits) ml = *(const float2*)(p + tid * step + D);
+    const float wm = wave_max(ml.x);
+    if ((tid & 63) == 0) red[tid >> 6] = wm;
+    __syncthreads();
+    const float m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float f = __builtin_amdgcn_exp2f(ml.x - (m == -INFINITY ? 0.f : m));
+    fs[tid] = f;
+    const float ws = wave_sum(f * ml.y);
+    if ((tid & 63) == 0) red[4 + (tid >> 6)] = ws;
+    __syncthreads();
+    const float sum = (red[4] + red[5]) + (red[6] + red[7]);
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kSeqSplits / 16; ++i) o += fs[i * 16 + tid / 16] * v[i];
+    os[tid] = o;
+    __syncthreads();
+    if (tid >= 16) return;
+#pragma unroll
+    for (int i = 1; i < 16; ++i) o += os[i * 16 + tid];
+    store_row4(a, o, sum, seq, h, rho, d);
 }
 
 template <int D>
 static hipError_t launch_attn(Kv4Attn& a, int n, hipStream_t st) {
     const int group = a.q_heads / a.kv_heads, rows = a.T * group, nq = rows > 16 ? 2 : 1;
     const int row_tiles = (rows + nq * 16 - 1) / (nq * 16), items = a.kv_heads * row_tiles;
-    // splits: enough blocks to fill the card twice over, each of its four waves with a tile at least
+    // splits: enough blocks for two a CU, each of its four waves with two tiles at least
     long long tiles = 0;
     for (int i = 0; i < n; ++i) tiles += tile_list(a.pos[i], a.pos[i] + a.T - 1, a.window, a.sinks).count;
     const long long want = std::max<long long>(1, 512 / items);
-    const int per = (int)std::max<long long>(4, (tiles + want - 1) / want);
+    const int per = (int)std::max<long long>(8, (tiles + want - 1) / want);
     int z = 0;
-    bool joined = false;
+    int most = 1;
     for (int i = 0; i < n; ++i) {
         a.first[i] = (uint16_t)z;
         const int count = tile_list(a.pos[i], a.pos[i] + a.T - 1, a.window, a.sinks).count;
         const int room = (int)((kMaxSplits / ((long long)items * nq) - z) - (n - 1 - i));
-        const int s = std::max(1, std::min(room, (count + per - 1) / per));
-        joined |= s > 1;
+        const int s = std::max(1, std::min({room, kSeqSplits, (count + per - 1) / per}));
+        most = std::max(most, s);
         z += s;
     }
-    a.first[n] = (uint16_t)z;
+    for (int i = n; i < kSeqArgs; ++i) a.first[i] = 0xffff;
+    a.n = n;
+    a.splits = z;
     const unsigned blocks = (unsigned)z * items;
-    if (nq == 1) hipLaunchKernelGGL((attn_kv4_kernel<D, 1>), dim3(blocks), dim3(256), 0, st, a, n, row_tiles);
-    else hipLaunchKernelGGL((attn_kv4_kernel<D, 2>), dim3(blocks), dim3(256), 0, st, a, n, row_tiles);
+    if (nq == 1) hipLaunchKernelGGL((attn_kv4_kernel<D, 1>), dim3(blocks), dim3(256), 0, st, a, row_tiles);
+    else hipLaunchKernelGGL((attn_kv4_kernel<D, 2>), dim3(blocks), dim3(256), 0, st, a, row_tiles);
     hipError_t rc = hipGetLastError();
-    if (rc != hipSuccess || !joined) return rc;
-    const unsigned jb = (unsigned)n * a.kv_heads * rows;
-    if (nq == 1) hipLaunchKernelGGL((attn_kv4_join<D, 1>), dim3(jb), dim3(64), 0, st, a, row_tiles);
-    else hipLaunchKernelGGL((attn_kv4_join<D, 2>), dim3(jb), dim3(64), 0, st, a, row_tiles);
+    if (rc != hipSuccess || most == 1) return rc;
+    const long long heads = (long long)n * a.kv_heads * rows;
+    if (most <= kFewSplits) {
+        const unsigned jb = (unsigned)((heads * (D / 4) + 255) / 256);
+        if (nq == 1) hipLaunchKernelGGL((attn_kv4_join_few<D, 1>), dim3(jb), dim3(256), 0, st, a, row_tiles);
+        else hipLaunchKernelGGL((attn_kv4_join_few<D, 2>), dim3(jb), dim3(256), 0, st, a, row_tiles);
+    } else {
+        const unsigned jb = (unsigned)(heads * (D / 64));
+        if (nq == 1) hipLaunchKernelGGL((attn_kv4_join<D, 1>), dim3(jb), dim3(256), 0, st, a, row_tiles);
+        else hipLaunchKernelGGL((attn_kv4_join<D, 2>), dim3(jb), dim3(256), 0, st, a, row_tiles);
+    }
     return hipGetLastError();
 }
 hipError_t launch_attn_kv4(Kv4Attn& a, int n, hipStream_t st) {

@@ -17,27 +17,30 @@
 
 namespace q35 {
 
-// 2^x for x <= 0 by the Taylor series of 2^f, |f| <= 1/2 (the first term left out is below 2^-56);
-// 0 under 2^-1000.
-__device__ __forceinline__ double exp2_neg(double x) {
-    const double k = rint(x), f = (x - k) * 0.69314718055994530942;
-    double p = 1.0 / 6227020800.0;
-    p = __builtin_fma(p, f, 1.0 / 479001600.0);
-    p = __builtin_fma(p, f, 1.0 / 39916800.0);
-    p = __builtin_fma(p, f, 1.0 / 3628800.0);
-    p = __builtin_fma(p, f, 1.0 / 362880.0);
-    p = __builtin_fma(p, f, 1.0 / 40320.0);
-    p = __builtin_fma(p, f, 1.0 / 5040.0);
-    p = __builtin_fma(p, f, 1.0 / 720.0);
-    p = __builtin_fma(p, f, 1.0 / 120.0);
-    p = __builtin_fma(p, f, 1.0 / 24.0);
-    p = __builtin_fma(p, f, 1.0 / 6.0);
-    p = __builtin_fma(p, f, 0.5);
-    p = __builtin_fma(p, f, 1.0);
-    p = __builtin_fma(p, f, 1.0);
-    const int e = (int)fmax(k, -1001.0);
-    const double s = __longlong_as_double((long long)(1023 + e) << 52);
-    return x < -1000.0 ? 0.0 : p * s;
+// e^((l - m) / T) = 2^(d c), d = l - m <= 0, c = log2(e) / T. d c + 1.5 * 2^52 rounds to a whole number whose low
+// bits are the exponent; what is left, |f| <= 1/2, is d c minus it, in one rounding; 2^f is the
+// polynomial that interpolates it at the ten Chebyshev points (relative error under 2e-14, far under what
+// a border between a million terms notices). 0 under 2^-1074, so also for l = -inf.
+struct Scale { double c, low; };     // low: -1100 / c
+__device__ __forceinline__ Scale scale_from(double inv_temp) {
+    const double c = inv_temp * 1.4426950408889634074;
+    return {c, -1100.0 / c};
+}
+__device__ __forceinline__ double power(double d, const Scale& sc) {
+    d = fmax(d, sc.low);
+    const double t = __builtin_fma(d, sc.c, 6755399441055744.0), k = t - 6755399441055744.0;
+    const double f = __builtin_fma(d, sc.c, -k);
+    double p = 1.0205907319260632e-07;
+    p = __builtin_fma(p, f, 1.3259645343488558e-06);
+    p = __builtin_fma(p, f, 1.5252672910770481e-05);
+    p = __builtin_fma(p, f, 0.00015403433750730278);
+    p = __builtin_fma(p, f, 0.0013333558200829426);
+    p = __builtin_fma(p, f, 0.009618129193935192);
+    p = __builtin_fma(p, f, 0.05550410866465135);
+    p = __builtin_fma(p, f, 0.24022650695640335);
+    p = __builtin_fma(p, f, 0.6931471805599462);
+    p = __builtin_fma(p, f, 1.0000000000000135);
+    return __builtin_ldexp(p, (int)(uint32_t)__builtin_bit_cast(unsigned long long, t));
 }
 
 constexpr int kMaxChunk = 8192;
@@ -102,18 +105,16 @@ __global__ void __launch_bounds__(256) verify_stats(VerifyArgs a) {
     float v[LOADS][N];
 #pragma unroll
     for (int b = 0; b < LOADS; ++b) load_logits<BF16>(row, i0 + (b * 256 + (int)threadIdx.x) * N, a.vocab, v[b]);
-    float m = -INFINITY;
-    bool nan = false;
+    float m = -INFINITY;                 // (a NaN anywhere makes it one)
 #pragma unroll
     for (int b = 0; b < LOADS; ++b)
 #pragma unroll
-        for (int e = 0; e < N; ++e) { m = fmaxf(m, v[b][e]); nan |= v[b][e] != v[b][e]; }
-    m = wave_max(m);
-    if (__any(nan)) m = __uint_as_float(0x7fc00000u);
+        for (int e = 0; e < N; ++e) m = __builtin_elementwise_maximum(m, v[b][e]);
+    const bool nan = __any(m != m);
+    m = nan ? __uint_as_float(0x7fc00000u) : wave_max(m);
     if (lane == 0) mx[wv] = m;
     __syncthreads();
-    m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-    nan = mx[0] != mx[0] || mx[1] != mx[1] || mx[2] != mx[2] || mx[3] != mx[3];
+    m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(mx[0], mx[1]), __builtin_elementwise_maximum(mx[2], mx[3]));
     Stat* out = stats_of(a, ln, j) + c;
     if (a.inv_temp == 0.0) {             // greedy: the lowest index of the maximum
         int best = 0x7fffffff;
@@ -126,40 +127,51 @@ __global__ void __launch_bounds__(256) verify_stats(VerifyArgs a) {
         for (int o = 32; o; o >>= 1) best = min(best, __shfl_xor(best, o));
         if (lane == 0) at[wv] = best;
         __syncthreads();
-        if (threadIdx.x == 0) *out = {nan ? (double)__uint_as_float(0x7fc00000u) : (double)m, (double)min(min(at[0], at[1]), min(at[2], at[3]))};
+        if (threadIdx.x == 0) *out = {(double)m, (double)min(min(at[0], at[1]), min(at[2], at[3]))};
         return;
     }
     double s = 0.0;
-    if (!nan && m > -INFINITY && m < INFINITY) {
-        const double f = a.inv_temp * 1.4426950408889634074, md = m;
+    if (m > -INFINITY && m < INFINITY) {
+        const Scale sc = scale_from(a.inv_temp);
+        const double md = m;
 #pragma unroll
         for (int b = 0; b < LOADS; ++b)
 #pragma unroll
-            for (int e = 0; e < N; ++e) s += exp2_neg(((double)v[b][e] - md) * f);
+            for (int e = 0; e < N; ++e) s += power((double)v[b][e] - md, sc);
     }
     s = wsum(s);
     if (lane == 0) sm[wv] = s;
     __syncthreads();
-    if (threadIdx.x == 0) *out = {nan ? (double)__uint_as_float(0x7fc00000u) : (double)m, (sm[0] + sm[1]) + (sm[2] + sm[3])};
+    if (threadIdx.x == 0) *out = {(double)m, (sm[0] + sm[1]) + (sm[2] + sm[3])};
 }
 
 // A row's maximum and sum from its chunks', by one wave; greedy: the maximum and its lowest index.
-__device__ __forceinline__ Stat row_stat(const VerifyArgs& a, const Stat* st, double f) {
+constexpr int kMaxChunks = 512;
+__device__ __forceinline__ Stat row_stat(const VerifyArgs& a, const Stat* st, const Scale& sc) {
     const int lane = threadIdx.x & 63;
+    Stat v[kMaxChunks / 64];
+#pragma unroll
+    for (int i = 0; i < kMaxChunks / 64; ++i) {
+        v[i] = {-INFINITY, 0.0};
+        if (i * 64 + lane < a.chunks) v[i] = st[i * 64 + lane];
+    }
     double m = -INFINITY;
     bool nan = false;
-    for (int c = lane; c < a.chunks; c += 64) { m = fmax(m, st[c].m); nan |= st[c].m != st[c].m; }
+#pragma unroll
+    for (int i = 0; i < kMaxChunks / 64; ++i) { m = fmax(m, v[i].m); nan |= v[i].m != v[i].m; }
 #pragma unroll
     for (int o = 32; o; o >>= 1) m = fmax(m, __shfl_xor(m, o));
     if (__any(nan)) m = __longlong_as_double(0x7ff8000000000000ll);
     double s = 0.0;
-    if (f == 0.0) {
+    if (a.inv_temp == 0.0) {
         s = 2147483647.0;
-        for (int c = lane; c < a.chunks; c += 64) if (st[c].m == m) s = fmin(s, st[c].s);
+#pragma unroll
+        for (int i = 0; i < kMaxChunks / 64; ++i) if (v[i].m == m) s = fmin(s, v[i].s);
 #pragma unroll
         for (int o = 32; o; o >>= 1) s = fmin(s, __shfl_xor(s, o));
     } else {
-        for (int c = lane; c < a.chunks; c += 64) if (st[c].s > 0.0) s += st[c].s * exp2_neg((st[c].m - m) * f);
+#pragma unroll
+        for (int i = 0; i < kMaxChunks / 64; ++i) if (v[i].s > 0.0) s += v[i].s * power(v[i].m - m, sc);
         s = wsum(s);
     }
     return {m, s};
@@ -171,47 +183,63 @@ __device__ __forceinline__ bool has_dist(const Stat& s) { return s.m > -INFINITY
 enum { kFromTarget = 0, kNotDraft = 1, kRest = 2, kNoToken = 3, kArgmax = 4 };
 struct Fate { int accepted, kind, draft; };
 
-// All waves make the lane's row statistics into rs (row order of row_of); then every thread decides alike.
+// All waves make the lane's row statistics into rs (row order of row_of), k threads the drafts' probabilities
+// into pq; then every thread decides alike.
+struct Draft { int id; double p, q; };
 template <bool BF16>
-__device__ __forceinline__ Fate decide(const VerifyArgs& a, int ln, double f, Stat* rs) {
-    const int wv = threadIdx.x >> 6, nw = blockDim.x >> 6;
+__device__ __forceinline__ Fate decide(const VerifyArgs& a, int ln, const Scale& sc, Stat* rs, Draft* pq) {
+    const int wv = threadIdx.x >> 6, nw = blockDim.x >> 6, tid = threadIdx.x;
+    const bool greedy = a.inv_temp == 0.0;
+    Draft d = {-1, 0.0, 1.0};
+    float lp = -INFINITY, lq = -INFINITY;
+    if (tid < a.k) {
+        d.id = a.drafts[(size_t)ln * a.k + tid];
+        if (d.id >= 0 && d.id < a.vocab && !greedy) {
+            lp = logit<BF16>(row_of<BF16>(a, ln, tid), d.id);
+            if (a.draft_logits) lq = logit<BF16>(row_of<BF16>(a, ln, a.k + 1 + tid), d.id);
+        }
+    }
     for (int j = wv; j < rows_of(a); j += nw) {
-        const Stat s = row_stat(a, stats_of(a, ln, j), f);
-        if ((threadIdx.x & 63) == 0) rs[j] = s;
+        const Stat s = row_stat(a, stats_of(a, ln, j), sc);
+        if ((tid & 63) == 0) rs[j] = s;
     }
     __syncthreads();
-    const int* d = a.drafts + (size_t)ln * a.k;
+    if (tid < a.k) {
+        const Stat ps = rs[tid];
+        d.p = has_dist(ps) ? power((double)lp - ps.m, sc) / ps.s : 0.0;
+        if (a.draft_logits) {
+            const Stat qs = rs[a.k + 1 + tid];
+            d.q = has_dist(qs) ? power((double)lq - qs.m, sc) / qs.s : 0.0;
+        }
+        pq[tid] = d;
+    }
+    __syncthreads();
     const float* u = a.u + (size_t)ln * (a.k + 1);
     for (int j = 0; j < a.k; ++j) {
-        const int t = d[j];
-        if (t < 0) return {j, !has_dist(rs[j]) ? kNoToken : f == 0.0 ? kArgmax : kFromTarget, -1};
-        const bool in = t < a.vocab, dist = has_dist(rs[j]);
-        if (f == 0.0) {
+        const int t = pq[j].id;
+        const bool dist = has_dist(rs[j]);
+        if (t < 0) return {j, !dist ? kNoToken : greedy ? kArgmax : kFromTarget, -1};
+        if (greedy) {
             if (dist && (double)t == rs[j].s) continue;
             return {j, dist ? kArgmax : kNoToken, t};
         }
-        const double p = in && dist ? exp2_neg(((double)logit<BF16>(row_of<BF16>(a, ln, j), t) - rs[j].m) * f) / rs[j].s : 0.0;
-        if (!a.draft_logits) {
-            if ((double)u[j] < p) continue;
-            return {j, dist ? in ? kNotDraft : kFromTarget : kNoToken, t};
-        }
-        const Stat& qs = rs[a.k + 1 + j];
-        const bool qd = has_dist(qs);
-        const double q = in && qd ? exp2_neg(((double)logit<BF16>(row_of<BF16>(a, ln, a.k + 1 + j), t) - qs.m) * f) / qs.s : 0.0;
-        if (qd && (double)u[j] * q < p) continue;
-        return {j, dist ? qd ? kRest : kFromTarget : kNoToken, t};
+        const bool qd = !a.draft_logits || has_dist(rs[a.k + 1 + j]);
+        if (qd && (double)u[j] * pq[j].q < pq[j].p) continue;
+        const int from = a.draft_logits ? kRest : kNotDraft;
+        return {j, !dist ? kNoToken : qd && (a.draft_logits || t < a.vocab) ? from : kFromTarget, t};
     }
-    return {a.k, !has_dist(rs[a.k]) ? kNoToken : f == 0.0 ? kArgmax : kFromTarget, -1};
+    return {a.k, !has_dist(rs[a.k]) ? kNoToken : greedy ? kArgmax : kFromTarget, -1};
 }
 
 // The weight of token i of the lane's row: p up to a factor, without the draft, or max(p - q, 0).
 template <bool BF16>
 struct Weights {
     const void *pr, *qr;
-    double f, pm, qm, pz, qz;        // pz, qz: 1 / sum (kRest)
+    Scale sc;
+    double pm, qm, pz, qz;           // maxima, 1 / sums (kRest)
     int kind, draft, vocab;
-    __device__ __forceinline__ Weights(const VerifyArgs& a, int ln, const Fate& ft, double f_, const Stat* rs)
-        : f(f_), kind(ft.kind), draft(ft.draft), vocab(a.vocab) {
+    __device__ __forceinline__ Weights(const VerifyArgs& a, int ln, const Fate& ft, const Scale& sc_, const Stat* rs)
+        : sc(sc_), kind(ft.kind), draft(ft.draft), vocab(a.vocab) {
         pr = row_of<BF16>(a, ln, ft.accepted);
         pm = rs[ft.accepted].m;
         pz = 1.0 / rs[ft.accepted].s;
@@ -229,12 +257,12 @@ struct Weights {
 #pragma unroll
         for (int b = 0; b < N; b += L) load_logits<BF16>(pr, i + b, vocab, v + b);
 #pragma unroll
-        for (int e = 0; e < N; ++e) w[e] = exp2_neg(((double)v[e] - pm) * f);
+        for (int e = 0; e < N; ++e) w[e] = power((double)v[e] - pm, sc);
         if (kind == kRest) {
 #pragma unroll
             for (int b = 0; b < N; b += L) load_logits<BF16>(qr, i + b, vocab, v + b);
 #pragma unroll
-            for (int e = 0; e < N; ++e) w[e] = fmax(w[e] * pz - exp2_neg(((double)v[e] - qm) * f) * qz, 0.0);
+            for (int e = 0; e < N; ++e) w[e] = fmax(w[e] * pz - power((double)v[e] - qm, sc) * qz, 0.0);
         } else if (kind == kNotDraft) {
 #pragma unroll
             for (int e = 0; e < N; ++e) if (i + e == draft) w[e] = 0.0;
@@ -246,12 +274,13 @@ struct Weights {
 template <bool BF16>
 __global__ void __launch_bounds__(256) verify_rest(VerifyArgs a, double* rest) {
     __shared__ Stat rs[2 * kVerifyDrafts + 1];
+    __shared__ Draft pq[kVerifyDrafts];
     __shared__ double sm[4];
     const int c = blockIdx.x % a.chunks, ln = blockIdx.x / a.chunks;
-    const double f = a.inv_temp * 1.4426950408889634074;
-    const Fate ft = decide<BF16>(a, ln, f, rs);
+    const Scale sc = scale_from(a.inv_temp);
+    const Fate ft = decide<BF16>(a, ln, sc, rs, pq);
     if (ft.kind != kRest) return;
-    const Weights<BF16> wt(a, ln, ft, f, rs);
+    const Weights<BF16> wt(a, ln, ft, sc, rs);
     double s = 0.0;
     for (int i = c * a.chunk + (int)threadIdx.x * 8; i < min((c + 1) * a.chunk, a.vocab); i += 2048) {
         double w[8];
@@ -265,85 +294,88 @@ __global__ void __launch_bounds__(256) verify_rest(VerifyArgs a, double* rest) {
     if (threadIdx.x == 0) rest[(size_t)ln * a.chunks + c] = (sm[0] + sm[1]) + (sm[2] + sm[3]);
 }
 
+// Inclusive sum over the block's 1024 threads, by place; part: 16 doubles.
+__device__ __forceinline__ double block_scan(double v, double* part) {
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double up = __shfl_up(v, o);
+        if (lane >= o) v += up;
+    }
+    __syncthreads();
+    if (lane == 63) part[wv] = v;
+    __syncthreads();
+    for (int w = 0; w < wv; ++w) v += part[w];
+    return v;
+}
+// The lowest `first` and the highest `last` of the block's threads.
+__device__ __forceinline__ int2 block_ends(int first, int last, int2* ends) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) { first = min(first, __shfl_xor(first, o)); last = max(last, __shfl_xor(last, o)); }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) ends[threadIdx.x >> 6] = make_int2(first, last);
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 16; ++w) { first = min(first, ends[w].x); last = max(last, ends[w].y); }
+    return make_int2(first, last);
+}
+
 // A block per lane: the decision, the chunk that holds the border, the token in it.
-constexpr int kMaxChunks = 512;
 template <bool BF16>
 __global__ void __launch_bounds__(1024) verify_token(VerifyArgs a, const double* rest) {
     __shared__ Stat rs[2 * kVerifyDrafts + 1];
-    __shared__ double cw[kMaxChunks], part[16];
-    __shared__ int where[16], pick;
-    __shared__ double base, border;
-    const int ln = blockIdx.x, wv = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const double f = a.inv_temp * 1.4426950408889634074;
-    Fate ft = decide<BF16>(a, ln, f, rs);
+    __shared__ Draft pq[kVerifyDrafts];
+    __shared__ double part[16], total, base;
+    __shared__ int2 ends[16];
+    const int ln = blockIdx.x, tid = threadIdx.x;
+    const Scale sc = scale_from(a.inv_temp);
+    const Fate ft = decide<BF16>(a, ln, sc, rs, pq);
     int token = -1;
     if (ft.kind == kArgmax) token = (int)rs[ft.accepted].s;
     if (ft.kind < kNoToken) {
-        Weights<BF16> wt(a, ln, ft, f, rs);
-        for (int pass = 0; pass < 2; ++pass) {
-            const Stat* st = stats_of(a, ln, ft.accepted);
-            for (int c = threadIdx.x; c < a.chunks; c += 1024)
-                cw[c] = wt.kind == kRest ? rest[(size_t)ln * a.chunks + c]
-                        : st[c].s > 0.0 ? st[c].s * exp2_neg((st[c].m - wt.pm) * f) : 0.0;
-            __syncthreads();
+        Weights<BF16> wt(a, ln, ft, sc, rs);
+        int pick = -1;
+        double border = 0.0;
+        for (int pass = 0; pass < 2 && pick < 0; ++pass) {
+            double cw = 0.0;                 // this thread's chunk
+            if (tid < a.chunks) {
+                const Stat st = stats_of(a, ln, ft.accepted)[tid];
+                cw = wt.kind == kRest ? rest[(size_t)ln * a.chunks + tid]
+                     : st.s > 0.0 ? st.s * power(st.m - wt.pm, sc) : 0.0;
+            }
             if (wt.kind == kNotDraft) {      // the draft's chunk, summed without it
-                const int c = ft.draft / a.chunk, i = c * a.chunk + (int)threadIdx.x * 8;
+                const int c = ft.draft / a.chunk;
                 double w[8], s = 0.0;
-                if ((int)threadIdx.x * 8 < a.chunk) {
-                    wt.template at<8>(i, w);
+                if (tid * 8 < a.chunk) {
+                    wt.template at<8>(c * a.chunk + tid * 8, w);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) s += w[e];
                 }
-                s = wsum(s);
-                if (lane == 0) part[wv] = s;
+                s = block_scan(s, part);
+                if (tid == 1023) total = s;
                 __syncthreads();
-                if (threadIdx.x == 0) {
-                    s = 0.0;
-                    for (int w2 = 0; w2 < 16; ++w2) s += part[w2];
-                    cw[c] = s;
-                }
+                if (tid == c) cw = total;
                 __syncthreads();
             }
-            if (threadIdx.x == 0) {
-                double tot = 0.0;
-                for (int c = 0; c < a.chunks; ++c) tot += cw[c];
-                const double b = (double)a.u[(size_t)ln * (a.k + 1) + a.k] * tot;
-                int got = -1;
-                double run = 0.0, at = 0.0;
-                for (int c = 0; c < a.chunks; ++c) {
-                    if (cw[c] > 0.0) { got = c; at = run; }
-                    run += cw[c];
-                    if (run > b) break;
-                }
-                pick = got;
-                base = at;
-                border = b;
-            }
+            const double run = block_scan(cw, part);
+            if (tid == 1023) total = run;
             __syncthreads();
-            if (pick >= 0) break;
-            wt.kind = kFromTarget;           // nothing is left of p - q (or of p without the draft): p itself
-            __syncthreads();
+            border = (double)a.u[(size_t)ln * (a.k + 1) + a.k] * total;
+            const int2 at = block_ends(cw > 0.0 && run > border ? tid : 0x7fffffff, cw > 0.0 ? tid : -1, ends);
+            pick = at.x < a.chunks ? at.x : at.y;
+            if (tid == pick) base = run - cw;
+            wt.kind = pick < 0 ? (int)kFromTarget : wt.kind;   // nothing is left of p - q (or of p without the draft): p itself
         }
         if (pick >= 0) {
-            const int i = pick * a.chunk + (int)threadIdx.x * 8;
-            double w[8];
+            const int i = pick * a.chunk + tid * 8;
+            double w[8], mine = 0.0;
 #pragma unroll
             for (int e = 0; e < 8; ++e) w[e] = 0.0;
-            if ((int)threadIdx.x * 8 < a.chunk) wt.template at<8>(i, w);
-            double mine = 0.0;
+            if (tid * 8 < a.chunk) wt.template at<8>(i, w);
 #pragma unroll
             for (int e = 0; e < 8; ++e) mine += w[e];
-            double run = mine;               // inclusive sums of the wave's lanes
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const double up = __shfl_up(run, o);
-                if (lane >= o) run += up;
-            }
-            __syncthreads();
-            if (lane == 63) part[wv] = run;
-            __syncthreads();
+            double run = block_scan(mine, part);
             run = base + (run - mine);
-            for (int w2 = 0; w2 < wv; ++w2) run += part[w2];
             int first = 0x7fffffff, last = -1;       // the first past the border, and the last with any weight
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -353,20 +385,12 @@ __global__ void __launch_bounds__(1024) verify_token(VerifyArgs a, const double*
                     if (run > border && first == 0x7fffffff) first = i + e;
                 }
             }
-#pragma unroll
-            for (int o = 32; o; o >>= 1) { first = min(first, __shfl_xor(first, o)); last = max(last, __shfl_xor(last, o)); }
-            if (lane == 0) { where[wv] = first; part[wv] = last; }
-            __syncthreads();
-            first = 0x7fffffff;
-            last = -1;
-            for (int w2 = 0; w2 < 16; ++w2) { first = min(first, where[w2]); last = max(last, (int)part[w2]); }
-            token = first < a.vocab ? first : last;
+            const int2 at = block_ends(first, last, ends);
+            token = at.x < a.vocab ? at.x : at.y;
         }
     }
-    if (threadIdx.x == 0) a.accepted[ln] = ft.accepted;
-    if ((int)threadIdx.x <= a.k)
-        a.tokens[(size_t)ln * (a.k + 1) + threadIdx.x] =
-            (int)threadIdx.x < ft.accepted ? a.drafts[(size_t)ln * a.k + threadIdx.x] : (int)threadIdx.x == ft.accepted ? token : -1;
+    if (tid == 0) a.accepted[ln] = ft.accepted;
+    if (tid <= a.k) a.tokens[(size_t)ln * (a.k + 1) + tid] = tid < ft.accepted ? pq[tid].id : tid == ft.accepted ? token : -1;
 }
 
 // Chunks of 8192 logits, fewer while the rows are too few to fill the card with them (2048 is the

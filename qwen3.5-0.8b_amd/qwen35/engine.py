@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from pathlib import Path
 
 import numpy as np
@@ -29,19 +30,12 @@ class _Config(C.Structure):
                 ("use_graph", C.c_int)]
 
 
-class _View(C.Structure):
-    _fields_ = [("ptr", C.c_void_p), ("row_stride", C.c_int64), ("head_stride", C.c_int64)]
-
-
-class _Heads(C.Structure):
-    _fields_ = [("q_heads", C.c_int), ("rot_dim", C.c_int), ("theta", C.c_double), ("eps", C.c_double),
-                ("q_norm", C.c_void_p), ("k_norm", C.c_void_p)] + [
-                    (n, _View) for n in ("q", "k", "v", "q_out", "k_out", "v_out")]
-
-
-class _Drafts(C.Structure):
-    _fields_ = [("logits", C.c_void_p), ("ld", C.c_int64), ("draft_logits", C.c_void_p), ("draft_ld", C.c_int64),
-                ("dtype", C.c_int), ("drafts", C.c_void_p), ("u", C.c_void_p), ("temperature", C.c_double)]
+# q35_view, q35_heads and q35_drafts (include/q35.h), packed as bytes: a ctypes.Structure's fields cost a
+# call of a few microseconds more than its kernel takes.
+_VIEW = struct.Struct("@Pqq")
+_HEADS = struct.Struct("@iiddPP" + 6 * "Pqq")
+_DRAFTS = struct.Struct("@PqPqiPPd")
+_NO_VIEW = (0, 0, 0)
 
 
 _SIGS = {
@@ -101,13 +95,12 @@ _SIGS = {
     "q35_kv4_len": ([C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.POINTER(C.c_int32)], C.c_int),
     "q35_kv4_write": ([C.c_void_p, C.c_void_p] + [C.c_int] * 5 + [C.c_void_p] * 4, C.c_int),
     "q35_kv4_read": ([C.c_void_p, C.c_void_p] + [C.c_int] * 5 + [C.c_void_p] * 4, C.c_int),
-    "q35_op_qk_norm_rope": ([C.c_void_p, C.POINTER(_Heads), C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_int], C.c_int),
-    "q35_op_kv4_append": ([C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
-                           C.POINTER(_Heads)], C.c_int),
+    "q35_op_qk_norm_rope": ([C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_int], C.c_int),
+    "q35_op_kv4_append": ([C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p],
+                          C.c_int),
     "q35_op_attn_kv4": ([C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int,
-                         C.POINTER(_View), C.POINTER(_View), C.c_float, C.c_int, C.c_int, C.POINTER(_View)], C.c_int),
-    "q35_op_draft_verify": ([C.c_void_p, C.POINTER(_Drafts), C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p],
-                            C.c_int),
+                         C.c_void_p, C.c_void_p, C.c_float, C.c_int, C.c_int, C.c_void_p], C.c_int),
+    "q35_op_draft_verify": ([C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p], C.c_int),
     "q35_sync": ([C.c_void_p], C.c_int),
     "q35_kprof_read": ([C.c_void_p, C.POINTER(C.c_float), C.POINTER(C.c_int)], C.c_int),
     "q35_set_option": ([C.c_void_p, C.c_char_p, C.c_int], C.c_int),
@@ -146,17 +139,22 @@ def _p(a: np.ndarray):
     return a.ctypes.data_as(C.c_void_p)
 
 
+def _addr(a: np.ndarray) -> int:
+    return a.__array_interface__["data"][0]
+
+
 def _lp(lanes: np.ndarray | None, pos: np.ndarray):
     """Lanes of a call with one position each (None: lane i)."""
     if lanes is None:
         return None
     if lanes.size != pos.size:
         raise ValueError(f"{lanes.size} lanes and {pos.size} positions")
-    return _p(lanes)
+    return _addr(lanes)
 
 
-def _heads(q_heads, rot_dim, theta, eps, q_norm, k_norm, *views) -> _Heads:
-    return _Heads(q_heads, rot_dim, theta, eps, q_norm, k_norm, *[_View(*v) if v is not None else _View() for v in views])
+def _heads(q_heads, rot_dim, theta, eps, q_norm, k_norm, q, k, v, q_out, k_out, v_out) -> bytes:
+    return _HEADS.pack(q_heads, rot_dim, theta, eps, q_norm, k_norm, *(q or _NO_VIEW), *k, *(v or _NO_VIEW),
+                       *(q_out or _NO_VIEW), *(k_out or _NO_VIEW), *(v_out or _NO_VIEW))
 
 
 def safetensors_scan(data: bytes | np.ndarray) -> tuple[int, int]:
@@ -285,7 +283,7 @@ class Engine:
         position pos[i] + t."""
         p = _i32(pos)
         h = _heads(q_heads, rot_dim, theta, eps, q_norm, k_norm, q, k, None, q_out, k_out, None)
-        _ck(load_library().q35_op_qk_norm_rope(self.h, C.byref(h), kv_heads, head_dim, _p(p), p.size, T))
+        _ck(load_library().q35_op_qk_norm_rope(self.h, h, kv_heads, head_dim, _addr(p), p.size, T))
 
     def op_kv4_append(self, cache: "KvCache4", layer: int, lanes, pos, T: int, q_heads: int, *, rot_dim: int,
                       theta: float, eps: float, q_norm: int, k_norm: int, k, v, q=None, q_out=None, k_out=None,
@@ -293,27 +291,25 @@ class Engine:
         """The same pass with k and v appended to `cache` in 4 bits (q35_op_kv4_append); lanes None: lane i."""
         p, la = _i32(pos), None if lanes is None else _i32(lanes)
         h = _heads(q_heads, rot_dim, theta, eps, q_norm, k_norm, q, k, v, q_out, k_out, v_out)
-        _ck(load_library().q35_op_kv4_append(self.h, cache.h, layer, _lp(la, p), _p(p), p.size, T, C.byref(h)))
+        _ck(load_library().q35_op_kv4_append(self.h, cache.h, layer, _lp(la, p), _addr(p), p.size, T, h))
 
     def op_attn_kv4(self, cache: "KvCache4", layer: int, lanes, pos, T: int, q_heads: int, q, out, *,
                     scale: float | None = None, window: int = 0, sinks: int = 0, gate=None):
         """Attention of T rows per sequence over `cache` (q35_op_attn_kv4): a row at p sees slots (p - window, p] and
         [0, sinks), all up to p with window 0; scale None: head_dim ** -0.5; gate: the output times its sigmoid."""
         p, la = _i32(pos), None if lanes is None else _i32(lanes)
-        qv, gv, ov = _View(*q), _View(*gate) if gate is not None else None, _View(*out)
-        _ck(load_library().q35_op_attn_kv4(self.h, cache.h, layer, _lp(la, p), _p(p), p.size, T, q_heads, C.byref(qv),
-                                           C.byref(gv) if gv is not None else None,
+        _ck(load_library().q35_op_attn_kv4(self.h, cache.h, layer, _lp(la, p), _addr(p), p.size, T, q_heads,
+                                           _VIEW.pack(*q), None if gate is None else _VIEW.pack(*gate),
                                            cache.head_dim ** -0.5 if scale is None else scale, window, sinks,
-                                           C.byref(ov)))
+                                           _VIEW.pack(*out)))
 
     def op_draft_verify(self, n: int, k: int, vocab: int, logits: int, drafts: int, u: int, accepted: int, tokens: int, *,
                         temperature: float = 1.0, draft_logits: int = 0, bf16: bool = False, ld: int = 0,
                         draft_ld: int = 0):
         """Sampled verification of n lanes' k drafts from the random numbers u [n][k + 1] (q35_op_draft_verify); the
         logits' row strides are vocab unless given."""
-        d = _Drafts(logits, ld or vocab, draft_logits or None, draft_ld or vocab, int(bf16), drafts, u, temperature)
-        _ck(load_library().q35_op_draft_verify(self.h, C.byref(d), n, k, vocab, C.c_void_p(accepted),
-                                               C.c_void_p(tokens)))
+        d = _DRAFTS.pack(logits, ld or vocab, draft_logits, draft_ld or vocab, int(bf16), drafts, u, temperature)
+        _ck(load_library().q35_op_draft_verify(self.h, d, n, k, vocab, accepted, tokens))
 
     def timer_begin(self):
         _ck(load_library().q35_timer_begin(self.h))
@@ -555,7 +551,7 @@ class KvCache4:
     def set_len(self, lanes, lengths):
         """Lengths of these lanes in every layer: 0 starts a lane over, fewer slots drop its last ones."""
         n, la = _i32(lengths), None if lanes is None else _i32(lanes)
-        _ck(load_library().q35_kv4_set_len(self.eng.h, self.h, _lp(la, n), _p(n), n.size))
+        _ck(load_library().q35_kv4_set_len(self.eng.h, self.h, _lp(la, n), _addr(n), n.size))
 
     def write(self, layer: int, lane0: int, n_lanes: int, slot0: int, n_slots: int, k_codes: int, k_scales: int,
               v_codes: int, v_scales: int):

@@ -67,18 +67,18 @@ def bed(lib):
 
 
 def heads(**kw):
-    from qwen35.engine import _Heads, _View
+    from qwen35.engine import _HEADS
     h = dict(q_heads=4, rot_dim=32, theta=1e7, eps=1e-6, q_norm=4096, k_norm=4096)
     v = dict(q=(1 << 16, 512, 64), k=(2 << 16, 512, 64), v=(3 << 16, 512, 64), q_out=(4 << 16, 256, 64), k_out=(0, 0, 0),
              v_out=(0, 0, 0))
     for n, x in kw.items():
         (v if n in v else h)[n] = x
-    return _Heads(**h, **{n: _View(*x) for n, x in v.items()})
+    return _HEADS.pack(*[x or 0 for x in h.values()], *[y for x in v.values() for y in x])
 
 
 def append(bed, lanes, pos, T=1, layer=0, **kw):
     la, p, h = np.array(lanes, np.int32), np.array(pos, np.int32), heads(**kw)
-    return bed.L.q35_op_kv4_append(bed.e, bed.c, layer, la.ctypes.data, p.ctypes.data, p.size, T, C.byref(h))
+    return bed.L.q35_op_kv4_append(bed.e, bed.c, layer, la.ctypes.data, p.ctypes.data, p.size, T, h)
 
 
 def test_append(bed):
@@ -121,19 +121,18 @@ def test_sequences_past_one_launch(lib):
     e, c = C.c_void_p(lib.stub_engine()), C.c_void_p()
     assert lib.q35_kv4_alloc(e, 1, 600, 8, 1, 64, C.byref(c)) == 0
     p, h = np.zeros(600, np.int32), heads()
-    assert lib.q35_op_kv4_append(e, c, 0, None, p.ctypes.data, 600, 2, C.byref(h)) == 0
+    assert lib.q35_op_kv4_append(e, c, 0, None, p.ctypes.data, 600, 2, h) == 0
     assert lib.stub_launches(e) == 3
     assert lib.q35_kv4_free(e, c) == 0
 
 
 def test_norm_rope(bed):
-    from qwen35.engine import _View
     p = np.array([0, 2 ** 31 - 4], np.int32)
     none = dict(v=(0, 0, 0), k_out=(5 << 16, 128, 64))
 
     def call(T=1, kv=2, dim=64, n=2, **kw):
         h = heads(**{**none, **kw})
-        return bed.L.q35_op_qk_norm_rope(bed.e, C.byref(h), kv, dim, p.ctypes.data, n, T)
+        return bed.L.q35_op_qk_norm_rope(bed.e, h, kv, dim, p.ctypes.data, n, T)
 
     assert call() == 0 and call(T=3) == 0
     bed.refused(ARG, call(T=4), "position out of range")
@@ -147,15 +146,14 @@ def test_norm_rope(bed):
 
 
 def test_attention(bed):
-    from qwen35.engine import _View
+    from qwen35.engine import _VIEW
     assert bed.set_len([0, 1, 2], [10, 0, 100]) == 0
     q0, out0 = (1 << 16, 512, 64), (2 << 16, 256, 64)
 
     def call(lanes, pos, T=1, layer=0, hq=4, q=q0, out=out0, gate=None, scale=0.125, window=0, sinks=0):
         la, p = np.array(lanes, np.int32), np.array(pos, np.int32)
-        g = _View(*gate) if gate else None
-        return bed.L.q35_op_attn_kv4(bed.e, bed.c, layer, la.ctypes.data, p.ctypes.data, p.size, T, hq, C.byref(_View(*q)),
-                                     C.byref(g) if g else None, scale, window, sinks, C.byref(_View(*out)))
+        return bed.L.q35_op_attn_kv4(bed.e, bed.c, layer, la.ctypes.data, p.ctypes.data, p.size, T, hq, _VIEW.pack(*q),
+                                     _VIEW.pack(*gate) if gate else None, scale, window, sinks, _VIEW.pack(*out))
 
     assert call([0, 0, 2], [9, 0, 99]) == 0                  # a lane may occur twice
     assert call([0], [7], T=3, window=1, sinks=5) == 0
@@ -173,8 +171,8 @@ def test_attention(bed):
         bed.refused(code, call(*args, **kw), text)
     assert bed.L.stub_launches(bed.e) == n
     other = C.c_void_p(bed.L.stub_engine())
-    assert bed.L.q35_op_attn_kv4(other, bed.c, 0, None, np.zeros(1, np.int32).ctypes.data, 1, 1, 4, C.byref(_View(*q0)), None,
-                                 1.0, 0, 0, C.byref(_View(*out0))) == ARG
+    assert bed.L.q35_op_attn_kv4(other, bed.c, 0, None, np.zeros(1, np.int32).ctypes.data, 1, 1, 4, _VIEW.pack(*q0), None,
+                                 1.0, 0, 0, _VIEW.pack(*out0)) == ARG
 
 
 def test_cache_shapes_lengths_copies(bed):
@@ -208,12 +206,12 @@ def test_cache_shapes_lengths_copies(bed):
 
 
 def test_verify(bed):
-    from qwen35.engine import _Drafts
+    from qwen35.engine import _DRAFTS
 
     def call(n=4, k=2, vocab=100, acc=16, tok=16, **kw):
-        d = _Drafts(**{**dict(logits=16, ld=100, draft_logits=None, draft_ld=100, dtype=0, drafts=16, u=16, temperature=1.0),
-                       **kw})
-        return bed.L.q35_op_draft_verify(bed.e, C.byref(d), n, k, vocab, acc, tok)
+        d = dict(logits=16, ld=100, draft_logits=0, draft_ld=100, dtype=0, drafts=16, u=16, temperature=1.0)
+        d.update(kw)
+        return bed.L.q35_op_draft_verify(bed.e, _DRAFTS.pack(*[x or 0 for x in d.values()]), n, k, vocab, acc, tok)
 
     assert call() == 0 and call(n=21) == 0 and call(temperature=0.0) == 0 and call(draft_logits=16, dtype=1) == 0
     n = bed.L.stub_launches(bed.e)
