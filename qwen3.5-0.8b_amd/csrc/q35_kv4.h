@@ -56,12 +56,13 @@ struct HeadArgs {
     double eps, rate;            // rate: -2 log2(theta) / rot, the angles' exponents' step
     uint8_t* cache;              // layer base, or null
     size_t lane_bytes, region;   // bytes of a lane (its kv_heads regions), of a region
+    uint32_t q_inv, kv_inv;      // 2^32 / heads + 1 (set by the launcher)
     int pos[kSeqArgs];
     uint16_t lane[kSeqArgs];
 };
 // q and k: RMS norm per head and rotation; with a.cache, k and v through 4 bits into the cache. n <= kSeqArgs
 // sequences of T rows.
-hipError_t launch_heads(const HeadArgs& a, int n, hipStream_t st);
+hipError_t launch_heads(HeadArgs& a, int n, hipStream_t st);
 
 struct Kv4Attn {
     const uint8_t* cache;        // layer base

@@ -95,7 +95,7 @@ __device__ __forceinline__ double head_sum(double v) {
     v += dpp_d<0xB1>(v);
     return v;
 }
-constexpr int kAngles = 512;         // of a block's rows: 4 x 128
+constexpr int kAngles = 512;         // of a block's rows: kBlockRows x 128
 // 1 / sqrt(x) from the instruction's approximation by two Newton steps (float64 to its last bits)
 __device__ __forceinline__ double rsqrt_d(double x) {
     double y = __builtin_amdgcn_rsq(x);
@@ -103,114 +103,120 @@ __device__ __forceinline__ double rsqrt_d(double x) {
     return y * __builtin_fma(-0.5 * x * y, y, 1.5);
 }
 
-// A block takes `per_block` rows (or, of few rows with many heads, a part of one row's heads); a wave four heads
-// of a row at a time -- q's, k's and v's in one list -- 16 lanes a head, a lane dims 64 c + 4 l .. + 3 of
-// each 64 (so a head's sum needs four steps between lanes for D products, and loads and stores are whole
-// 128-byte runs). The rows' angles are made once for the block, with the first heads' loads in flight.
-// What the kernel writes is decided by borders (a code's midpoints, a scale's step), so every float32
-// operation is one rounding in the stated order, and the sum of squares, the root and the angles are
-// float64.
-template <int D>
-__global__ void __launch_bounds__(256) heads_kernel(HeadArgs a, int rows, int per_block, int parts, int units) {
+// A block takes `per_block` rows (of few rows with many heads: a part of one row's heads). Its work is the list of
+// the rows' (row, head)s of q, then of k, then of v; a wave takes four of one kind at a time, 16 lanes a
+// head, a lane dims 64 c + 4 l .. + 3 of each 64: a head's sum needs four steps between lanes for D
+// products, and loads and stores are whole 128-byte runs. The rows' angles are made once for the block, with
+// the first heads' loads in flight. What the kernel writes is decided by borders (a code's midpoints, a
+// scale's step), so every float32 operation is one rounding in the stated order, and the sum of
+// squares, the root and the angles are float64. QUADS: rot / 2 is a multiple of 4, so a lane's four dims lie
+// on one side of the pairs.
+constexpr int kBlockRows = 4;
+template <int D, bool QUADS>
+__global__ void __launch_bounds__(256) heads_kernel(HeadArgs a, int rows, int per_block, int parts, int some) {
     constexpr int C = D / 64;
     __shared__ float xs[4][4][D];
     __shared__ float2 cs[kAngles];
+    __shared__ int2 at[kBlockRows];          // a row's position and lane
     const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63, j = lane >> 4, l = lane & 15;
-    const int r0 = blockIdx.x / parts * per_block, u0 = blockIdx.x % parts * units;
-    const int nq = a.q.p ? a.q_heads : 0, all = nq + a.kv_heads * (a.v.p ? 2 : 1), half = a.rot / 2;
-    const int nu = min(units, (all + 3) / 4 - u0), items = min(per_block, rows - r0) * nu;
-    struct Item { int r, kind, h; };         // kind: 0 q, 1 k, 2 v, 3 none
+    const int r0 = blockIdx.x / parts * per_block, nr = min(per_block, rows - r0), half = a.rot / 2;
+    // wave items of each kind, and this block's part of them
+    const int iq = a.q.p ? (nr * a.q_heads + 3) / 4 : 0, ik = (nr * a.kv_heads + 3) / 4;
+    const int i0 = blockIdx.x % parts * some, i1 = min(i0 + some, iq + (a.v.p ? 2 : 1) * ik);
+    struct Item { int kind, rr, h; bool on; };
     const auto item = [&](int i) {
-        const int rr = i / nu;
-        const int x = (u0 + i - rr * nu) * 4 + j;
         Item t;
-        t.r = r0 + rr;
-        t.kind = i >= items || x >= all ? 3 : x < nq ? 0 : x < nq + a.kv_heads ? 1 : 2;
-        t.h = t.kind == 0 ? x : t.kind == 1 ? x - nq : x - nq - a.kv_heads;
+        t.kind = i < iq ? 0 : i < iq + ik ? 1 : 2;
+        const int heads = t.kind == 0 ? a.q_heads : a.kv_heads, x = (t.kind == 0 ? i : t.kind == 1 ? i - iq : i - iq - ik) * 4 + j;
+        t.rr = heads == 1 ? x : (int)__umulhi((uint32_t)x, t.kind == 0 ? a.q_inv : a.kv_inv);
+        t.h = x - t.rr * heads;
+        t.on = i < i1 && t.rr < nr;
         return t;
     };
     const auto fetch = [&](const Item& t, uint2* w) {
-        const uint16_t* p = t.kind == 0 ? a.q.p + t.r * a.q.row + t.h * a.q.head
-                          : t.kind == 1 ? a.k.p + t.r * a.k.row + t.h * a.k.head : a.v.p + t.r * a.v.row + t.h * a.v.head;
+        const HeadView& in = t.kind == 0 ? a.q : t.kind == 1 ? a.k : a.v;
+        const uint16_t* p = in.p + (r0 + t.rr) * in.row + t.h * in.head + 4 * l;
 #pragma unroll
-        for (int c = 0; c < C; ++c) w[c] = t.kind < 3 ? *(const uint2*)(p + 64 * c + 4 * l) : make_uint2(0, 0);
+        for (int c = 0; c < C; ++c) w[c] = t.on ? *(const uint2*)(p + 64 * c) : make_uint2(0, 0);
     };
-    Item now = item(wv);
+    Item now = item(__builtin_amdgcn_readfirstlane(i0 + wv));
     uint2 raw[C];
     fetch(now, raw);
-    for (int i = tid; i < min(per_block, rows - r0) * half; i += 256) {
+    for (int i = tid; i < nr * half; i += 256) {
         const int rr = i / half, r = r0 + rr;
         cs[i] = turn(a.pos[r / a.T] + r % a.T, i - rr * half, a.rate);
     }
+    if (tid < nr) {
+        const int r = r0 + tid, seq = r / a.T;
+        at[tid] = make_int2(a.pos[seq] + r - seq * a.T, a.lane[seq]);
+    }
     lds_barrier();
-    for (int i = wv; i < items; i += 4) {            // whole waves; no block barrier in the loop
+    for (int i = __builtin_amdgcn_readfirstlane(i0 + wv); i < i1; i += 4) {      // whole waves; no block barrier in the loop
         const Item t = now;
+        const int kind = t.kind;
         f32x4 x[C];
 #pragma unroll
         for (int c = 0; c < C; ++c) x[c] = wide(raw[c]);
         now = item(i + 4);
         fetch(now, raw);
-        const int seq = t.r / a.T, pos = a.pos[seq] + t.r - seq * a.T;
-        const uint16_t* nw = t.kind == 0 ? a.q_norm : a.k_norm;
-        double ss = 0.0;
+        if (kind < 2) {
+            const uint16_t* nw = (kind == 0 ? a.q_norm : a.k_norm) + 4 * l;
+            uint2 w[C];
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) ss = __builtin_fma((double)x[c][e], (double)x[c][e], ss);
-        const float rs = (float)rsqrt_d(head_sum(ss) * (1.0 / D) + a.eps);
-        if (t.kind < 2) {
-#pragma unroll
-            for (int c = 0; c < C; ++c) x[c] = x[c] * rs * (1.0f + wide(*(const uint2*)(nw + 64 * c + 4 * l)));
-        }
-        if (half) {
-            float* hx = xs[wv][j];
-            const float2* cr = cs + (t.r - r0) * half;
-            wave_sync();
+            for (int c = 0; c < C; ++c) w[c] = *(const uint2*)(nw + 64 * c);
+            double ss = 0.0;
 #pragma unroll
             for (int c = 0; c < C; ++c)
-                if (64 * c < a.rot) *(f32x4*)&hx[64 * c + 4 * l] = x[c];
-            wave_sync();
-            if (t.kind < 2) {
 #pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const int d = 64 * c + 4 * l;
-                    if (d >= a.rot) continue;
-                    if ((half & 3) == 0) {           // a lane's four dims lie on one side of the pairs
+                for (int e = 0; e < 4; ++e) ss = __builtin_fma((double)x[c][e], (double)x[c][e], ss);
+            const float rs = (float)rsqrt_d(head_sum(ss) * (1.0 / D) + a.eps);
+            float* hx = xs[wv][j];
+            wave_sync();
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                x[c] = x[c] * rs * (1.0f + wide(w[c]));
+                if (64 * c < a.rot) *(f32x4*)&hx[64 * c + 4 * l] = x[c];
+            }
+            wave_sync();
+            const float2* cr = cs + (t.on ? t.rr : 0) * half;
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const int d = 64 * c + 4 * l;
+                if (64 * c >= a.rot) break;
+                if (QUADS) {
+                    if (d < a.rot) {
                         const bool low = d < half;
                         const int k = low ? d : d - half;
                         const f32x4 o = *(const f32x4*)&hx[low ? d + half : k];
+                        const f32x4 c0 = *(const f32x4*)&cr[k], c1 = *(const f32x4*)&cr[k + 2];
+                        const f32x4 p = x[c] * f32x4{c0[0], c0[2], c1[0], c1[2]}, q = o * f32x4{c0[1], c0[3], c1[1], c1[3]};
+                        x[c] = low ? p - q : p + q;
+                    }
+                } else {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float2 cc = cr[k + e];
-                            const float p = x[c][e] * cc.x, q = o[e] * cc.y;
-                            x[c][e] = low ? p - q : p + q;
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            if (d + e < half) {
-                                const float2 cc = cr[d + e];
-                                x[c][e] = x[c][e] * cc.x - hx[d + e + half] * cc.y;
-                            } else if (d + e < a.rot) {
-                                const float2 cc = cr[d + e - half];
-                                x[c][e] = x[c][e] * cc.x + hx[d + e - half] * cc.y;
-                            }
+                    for (int e = 0; e < 4; ++e) {
+                        if (d + e < half) {
+                            const float2 cc = cr[d + e];
+                            x[c][e] = x[c][e] * cc.x - hx[d + e + half] * cc.y;
+                        } else if (d + e < a.rot) {
+                            const float2 cc = cr[d + e - half];
+                            x[c][e] = x[c][e] * cc.x + hx[d + e - half] * cc.y;
                         }
                     }
                 }
             }
         }
-        if (t.kind == 3) continue;                   // lanes without a head; their wave goes on
-        const HeadView& out = t.kind == 0 ? a.q_out : t.kind == 1 ? a.k_out : a.v_out;
-        uint16_t* op = const_cast<uint16_t*>(out.p) + t.r * out.row + t.h * out.head;
-        if (t.kind == 0 || !a.cache) {
+        const HeadView& out = kind == 0 ? a.q_out : kind == 1 ? a.k_out : a.v_out;
+        uint16_t* op = const_cast<uint16_t*>(out.p) + (r0 + t.rr) * out.row + t.h * out.head + 4 * l;
+        if (kind == 0 || !a.cache) {
 #pragma unroll
             for (int c = 0; c < C; ++c)
-                *(uint2*)(op + 64 * c + 4 * l) = make_uint2(f2bf2(x[c][0], x[c][1]), f2bf2(x[c][2], x[c][3]));
+                if (t.on) *(uint2*)(op + 64 * c) = make_uint2(f2bf2(x[c][0], x[c][1]), f2bf2(x[c][2], x[c][3]));
             continue;
         }
-        uint8_t* tile = a.cache + a.lane[seq] * a.lane_bytes + t.h * a.region + (size_t)(pos >> 5) * kv4_tile_bytes(D);
-        const int tk = pos & 31;
+        const int2 where = at[t.on ? t.rr : 0];
+        uint8_t* tile = a.cache + where.y * a.lane_bytes + t.h * a.region + (size_t)(where.x >> 5) * kv4_tile_bytes(D);
+        const int tk = where.x & 31;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             // the group's largest magnitude as bits (8 lanes): an infinity or a NaN is the largest of all
@@ -228,22 +234,29 @@ __global__ void __launch_bounds__(256) heads_kernel(HeadArgs a, int rows, int pe
             uint32_t code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, x[c][0], x[c][1], sc, 0);
             code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[c][2], x[c][3], sc, 1);
             const int d = 64 * c + 4 * l;
-            if (out.p) *(uint2*)(op + d) = make_uint2(two_values<0>(code, sc), two_values<1>(code, sc));
-            *(uint16_t*)(tile + (t.kind == 1 ? kv4_k_code(D, tk, d) : kv4_v_code(D, tk, d))) = (uint16_t)code;
-            if ((l & 7) == 0) tile[t.kind == 1 ? kv4_k_scale(D, tk, d >> 5) : kv4_v_scale(D, tk, d >> 5)] = (uint8_t)b;
+            if (!t.on) continue;
+            if (out.p) *(uint2*)(op + 64 * c) = make_uint2(two_values<0>(code, sc), two_values<1>(code, sc));
+            *(uint16_t*)(tile + (kind == 1 ? kv4_k_code(D, tk, d) : kv4_v_code(D, tk, d))) = (uint16_t)code;
+            if ((l & 7) == 0) tile[kind == 1 ? kv4_k_scale(D, tk, d >> 5) : kv4_v_scale(D, tk, d >> 5)] = (uint8_t)b;
         }
     }
 }
 
-hipError_t launch_heads(const HeadArgs& a, int n, hipStream_t st) {
-    const int units = ((a.q.p ? a.q_heads : 0) + a.kv_heads * (a.v.p ? 2 : 1) + 3) / 4, rows = n * a.T;
+hipError_t launch_heads(HeadArgs& a, int n, hipStream_t st) {
+    const int rows = n * a.T, kinds = a.v.p ? 2 : 1;
     // rows of a block: one while they are too few to give every CU four blocks, else up to four; of very few
-    // rows with many heads, four units (one a wave) in a block
-    const int per_block = rows >= 4096 ? 4 : rows >= 2048 ? 2 : 1;
-    const int some = rows < 256 ? std::min(units, 4) : units, parts = (units + some - 1) / some;
+    // rows with many heads, four wave items (one a wave) in a block
+    const int per_block = rows >= 4096 ? kBlockRows : rows >= 2048 ? 2 : 1;
+    const int items = ((a.q.p ? per_block * a.q_heads + 3 : 0) / 4) + kinds * ((per_block * a.kv_heads + 3) / 4);
+    const int some = rows < 256 ? std::min(items, 4) : items, parts = (items + some - 1) / some;
     const long long blocks = (long long)((rows + per_block - 1) / per_block) * parts;
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
-    auto k = a.D == 256 ? heads_kernel<256> : a.D == 128 ? heads_kernel<128> : heads_kernel<64>;
+    a.q_inv = a.q_heads > 1 ? (uint32_t)(0x100000000ull / a.q_heads + 1) : 0;
+    a.kv_inv = a.kv_heads > 1 ? (uint32_t)(0x100000000ull / a.kv_heads + 1) : 0;
+    const bool quads = a.rot % 8 == 0;
+    auto k = a.D == 256 ? (quads ? heads_kernel<256, true> : heads_kernel<256, false>)
+           : a.D == 128 ? (quads ? heads_kernel<128, true> : heads_kernel<128, false>)
+                        : (quads ? heads_kernel<64, true> : heads_kernel<64, false>);
     hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(256), 0, st, a, rows, per_block, parts, some);
     return hipGetLastError();
 }
@@ -298,20 +311,27 @@ struct Tile {
     uint32_t ks;
     uint2 vs;
 };
-template <int D>
-__device__ __forceinline__ Tile<D> load_tile(const uint8_t* region, int tile) {
+// ONCE: the tile is read by one block only (nontemporal loads)
+template <int D, bool ONCE>
+__device__ __forceinline__ void load_k(Tile<D>& t, const uint8_t* p) {
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
-    const uint8_t* p = region + (size_t)tile * kv4_tile_bytes(D);
-    Tile<D> t;
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) t.k[i] = __builtin_nontemporal_load((const u32x4*)(p + i * 1024 + lane * 16));
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i)
-        t.v[i] = __builtin_nontemporal_load((const u32x4*)(p + 16 * D + i * 1024 + lane * 16));
+    for (int i = 0; i < D / 64; ++i) {
+        const u32x4* w = (const u32x4*)(p + i * 1024 + lane * 16);
+        t.k[i] = ONCE ? __builtin_nontemporal_load(w) : *w;
+    }
     if (D == 256) t.ks = *(const uint32_t*)(p + 32 * D + lane * 4);
     else t.ks = *(const uint16_t*)(p + 32 * D + (D == 64 ? (g >> 1) * 16 + m : lane) * 2);
+}
+template <int D, bool ONCE>
+__device__ __forceinline__ void load_v(Tile<D>& t, const uint8_t* p) {
+    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+        const u32x4* w = (const u32x4*)(p + 16 * D + i * 1024 + lane * 16);
+        t.v[i] = ONCE ? __builtin_nontemporal_load(w) : *w;
+    }
     t.vs = *(const uint2*)(p + 33 * D + m * D / 512 * 32 + g * 8);
-    return t;
 }
 template <int D>
 __device__ __forceinline__ float k_scale(const Tile<D>& t, int half, int s) {
@@ -359,10 +379,12 @@ struct Rows {
     f32x4 o[NQ][D / 16];         // O^T: dims (4 g + r) D / 16 + i of row n in o[.][i][r]
 };
 
-template <int D, int NQ>
-__device__ __forceinline__ void tile_step(const Tile<D>& t, const uint8_t* tile_p, int slot0, bool edge,
-                                          const q35_bf16x8 (*qf)[D / 32], const Sight* sight, float scale2,
-                                          Rows<D, NQ>& st) {
+// q: the rows' Q^T operands, [NQ][D / 32], in registers (NQ = 1) or, 16 rows more, in LDS with 64 lanes each
+// (the four waves of a block have the same rows). REFILL: t's registers take the tile at next_p as soon as its K, then
+// its V, is used up (32 registers less than a second tile; the loads have the other half's work to arrive).
+template <int D, int NQ, bool REFILL, class Q>
+__device__ __forceinline__ void tile_step(Tile<D>& t, const uint8_t* tile_p, const uint8_t* next_p, int slot0, bool edge, const Q& q,
+                                          const Sight* sight, float scale2, Rows<D, NQ>& st) {
     const int lane = threadIdx.x & 63, g = lane >> 4;
     f32x4 s[NQ][2];
 #pragma unroll
@@ -374,9 +396,10 @@ __device__ __forceinline__ void tile_step(const Tile<D>& t, const uint8_t* tile_
             const q35_bf16x8 kf = k_frag<D>(t, half, k);
 #pragma unroll
             for (int c = 0; c < NQ; ++c)
-                s[c][half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[c][k], s[c][half], 0, 0, 0);
+                s[c][half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q(c, k), s[c][half], 0, 0, 0);
         }
     }
+    if (REFILL) load_k<D, false>(t, next_p);
 #pragma unroll
     for (int c = 0; c < NQ; ++c) { s[c][0] *= scale2; s[c][1] *= scale2; }     // before the mask: scale may be 0 or negative
     uint2 vsb = t.vs;
@@ -462,6 +485,7 @@ __device__ __forceinline__ void tile_step(const Tile<D>& t, const uint8_t* tile_
     pv(std::integral_constant<int, 10>{});
     pv(std::integral_constant<int, 12>{});
     pv(std::integral_constant<int, 14>{});
+    if (REFILL) load_v<D, false>(t, next_p);
 }
 
 // The tiles that rows at positions p0 .. p1 read: those of the sinks, then those from the first row's
@@ -527,92 +551,125 @@ __device__ __forceinline__ const float* part_of(const Kv4Attn& a, int row_tiles,
     return a.part + ((((size_t)z * a.kv_heads + h) * row_tiles + rho / (NQ * 16)) * NQ * kSplitRows + rho % (NQ * 16)) * (D + 4);
 }
 
-// Decode and verify rows: a block per (sequence, split of its tiles, kv head, NQ x 16 rows), its four
-// waves on every fourth tile with the next one's loads in flight, their states joined through LDS.
-template <int D, int NQ>
-__global__ void __launch_bounds__(256) attn_kv4_kernel(Kv4Attn a, int row_tiles) {
-    __shared__ float os[4][16][D + 4];
+// A block per (sequence, split of its tiles, kv head, NQ x 16 rows): its four waves take every fourth tile
+// with the next one's loads in flight, and their states are joined through LDS. PAIRS (prompts): the
+// block takes the row tiles i and last - i, one after the other, so that every block has the same work
+// under the causal mask, all its tiles included (splits == 1).
+template <int D, int NQ, bool PAIRS>
+__global__ void __launch_bounds__(256, D == 256 ? 2 : 1) attn_kv4_kernel(Kv4Attn a, int row_tiles) {
+    __shared__ __attribute__((aligned(16))) float os[4][16][D + 4];
     __shared__ float ms[4][16], ls[4][16];
     __shared__ uint32_t bs[4][16];
-    const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63, nn = lane & 15, g = lane >> 4;
-    const int rt = blockIdx.x % row_tiles, h = blockIdx.x / row_tiles % a.kv_heads, z = blockIdx.x / (row_tiles * a.kv_heads);
+    static_assert(NQ == 1 || sizeof(os) >= NQ * (D / 32) * 1024, "the Q operands lie where the waves' sums go at the end");
+    constexpr bool kOnce = !PAIRS && NQ == 1, kRefill = NQ == 2 && D == 256;
+    const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63, nn = lane & 15, g = lane >> 4;
+    const int tiles = PAIRS ? (row_tiles + 1) / 2 : row_tiles;
+    const int h = blockIdx.x / tiles % a.kv_heads, z = blockIdx.x / (tiles * a.kv_heads), rt0 = blockIdx.x % tiles;
     const Seq sq = find_seq(a, z);
-    const int seq = sq.i, split = sq.split, splits = sq.splits, pos = sq.pos;
-    const int group = a.q_heads / a.kv_heads, rows = a.T * group, rho0 = rt * NQ * 16;
-    const int rho1 = min(rho0 + NQ * 16, rows) - 1;
-    const TileList tl = tile_list(pos + rho0 / group, pos + rho1 / group, a.window, a.sinks);
-    const int t0 = (int)((long long)tl.count * split / splits), t1 = (int)((long long)tl.count * (split + 1) / splits);
+    const int seq = sq.i, splits = sq.splits, pos = sq.pos, group = a.q_heads / a.kv_heads, rows = a.T * group;
     const uint8_t* region = a.cache + sq.lane * a.lane_bytes + h * a.region;
-
-    q35_bf16x8 qf[NQ][D / 32];
-    Sight sight[NQ];
-    Rows<D, NQ> st;
-#pragma unroll
-    for (int c = 0; c < NQ; ++c) {
-        const int rho = min(rho0 + c * 16 + nn, rows - 1), t = rho / group;
-        const uint16_t* q = a.q.p + ((long long)seq * a.T + t) * a.q.row + (h * group + rho - t * group) * a.q.head;
-#pragma unroll
-        for (int k = 0; k < D / 32; ++k) qf[c][k] = *(const q35_bf16x8*)(q + g * (D / 4) + 8 * k);
-        sight[c] = {pos + t, a.window > 0 ? pos + t - a.window + 1 : 0, a.sinks};
-        st.m[c] = -INFINITY;
-        st.l[c] = 0.f;
-        st.bad[c] = 0;
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) st.o[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    // tiles whose every slot every row of the block sees: from the last row's window to the first row's slot
-    const int full0 = a.window > 0 ? max(pos + rho1 / group - a.window + 1, 0) : 0, full1 = pos + rho0 / group;
     const float scale2 = a.scale * 1.44269504088896f;
-    auto at = [&](int i) { return i < tl.sink ? i : i - tl.sink + tl.main; };
-    if (t0 + wv < t1) {
-        Tile<D> cur = load_tile<D>(region, at(t0 + wv));
+    for (int pass = 0; pass < (PAIRS ? 2 : 1); ++pass) {
+        const int rt = pass ? rt0 : PAIRS ? row_tiles - 1 - rt0 : rt0, rho0 = rt * NQ * 16;
+        if (pass && rt == row_tiles - 1 - rt0) break;        // the middle one
+        const int rho1 = min(rho0 + NQ * 16, rows) - 1;
+        const TileList tl = tile_list(pos + rho0 / group, pos + rho1 / group, a.window, a.sinks);
+        const int t0 = (int)((long long)tl.count * sq.split / splits), t1 = (int)((long long)tl.count * (sq.split + 1) / splits);
+        const auto q_at = [&](int rho, int gg, int k) {
+            rho = min(rho, rows - 1);
+            const int t = rho / group;
+            return *(const q35_bf16x8*)(a.q.p + ((long long)seq * a.T + t) * a.q.row + (h * group + rho - t * group) * a.q.head +
+                                        gg * (D / 4) + 8 * k);
+        };
+        auto at = [&](int i) { return i < tl.sink ? i : i - tl.sink + tl.main; };
+        Tile<D> cur;
+        const auto tile_at = [&](int i) { return region + (size_t)at(i) * kv4_tile_bytes(D); };
+        if (t0 + wv < t1) {
+            load_k<D, kOnce>(cur, tile_at(t0 + wv));
+            load_v<D, kOnce>(cur, tile_at(t0 + wv));
+        }
+        q35_bf16x8 qf[NQ == 1 ? D / 32 : 1];
+        q35_bf16x8* ql = (q35_bf16x8*)&os[0][0][0];
+        if constexpr (NQ == 1) {
+#pragma unroll
+            for (int k = 0; k < D / 32; ++k) qf[k] = q_at(rho0 + nn, g, k);
+        } else {
+            if (pass) __syncthreads();
+            for (int i = tid; i < NQ * (D / 32) * 64; i += 256) {
+                const int ln = i & 63, k = i / 64 % (D / 32), c = i / (64 * (D / 32));
+                ql[i] = q_at(rho0 + c * 16 + (ln & 15), ln >> 4, k);
+            }
+            lds_barrier();
+        }
+        int qlane = lane;
+        const auto q = [&](int c, int k) { return NQ == 1 ? qf[k] : ql[(c * (D / 32) + k) * 64 + qlane]; };
+        Sight sight[NQ];
+        Rows<D, NQ> st;
+#pragma unroll
+        for (int c = 0; c < NQ; ++c) {
+            const int p = pos + min(rho0 + c * 16 + nn, rows - 1) / group;
+            sight[c] = {p, a.window > 0 ? p - a.window + 1 : 0, a.sinks};
+            st.m[c] = -INFINITY;
+            st.l[c] = 0.f;
+            st.bad[c] = 0;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) st.o[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        // tiles whose every slot every row of the block sees: from the last row's window to the first row's slot
+        const int full0 = a.window > 0 ? max(pos + rho1 / group - a.window + 1, 0) : 0, full1 = pos + rho0 / group;
         for (int i = t0 + wv; i < t1; i += 4) {
             const int tile = at(i);
-            const Tile<D> next = load_tile<D>(region, at(min(i + 4, t1 - 1)));
+            if (NQ > 1) asm volatile("" : "+v"(qlane));     // or the compiler reads Q ahead of the loop, and spills it
+            const uint8_t* next_p = tile_at(min(i + 4, t1 - 1));
+            Tile<D> next;
+            if (!kRefill) {
+                load_k<D, kOnce>(next, next_p);
+                load_v<D, kOnce>(next, next_p);
+            }
             const bool edge = tile * 32 < full0 || tile * 32 + 31 > full1;
-            tile_step<D, NQ>(cur, region + (size_t)tile * kv4_tile_bytes(D), tile * 32, edge, qf, sight, scale2, st);
-            cur = next;
+            tile_step<D, NQ, kRefill>(cur, tile_at(i), next_p, tile * 32, edge, q, sight, scale2, st);
+            if (!kRefill) cur = next;
         }
-    }
 #pragma unroll
-    for (int c = 0; c < NQ; ++c) {
-        if (rho0 + c * 16 >= rows) break;
-        if (c) __syncthreads();
-        float l = st.l[c];
-        l += xor16(l);
-        l += xor32(l);
-        uint32_t bad = st.bad[c];
-        bad |= (uint32_t)__shfl_xor((int)bad, 16);
-        bad |= (uint32_t)__shfl_xor((int)bad, 32);
-        if (g == 0) { ms[wv][nn] = st.m[c]; ls[wv][nn] = l; bs[wv][nn] = bad; }
+        for (int c = 0; c < NQ; ++c) {
+            if (rho0 + c * 16 >= rows) break;
+            if (NQ > 1 || pass || c) __syncthreads();        // os was read: Q, or the 16 rows before these
+            float l = st.l[c];
+            l += xor16(l);
+            l += xor32(l);
+            uint32_t bad = st.bad[c];
+            bad |= (uint32_t)__shfl_xor((int)bad, 16);
+            bad |= (uint32_t)__shfl_xor((int)bad, 32);
+            if (g == 0) { ms[wv][nn] = st.m[c]; ls[wv][nn] = l; bs[wv][nn] = bad; }
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+            for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int i = 0; i < D / 16; i += 4) {
-                const f32x4 o = {st.o[c][i][r], st.o[c][i + 1][r], st.o[c][i + 2][r], st.o[c][i + 3][r]};
-                *(f32x4*)&os[wv][nn][(4 * g + r) * (D / 16) + i] = o;
-            }
-        __syncthreads();
-        for (int e = threadIdx.x; e < 16 * (D / 4); e += 256) {
-            const int n0 = e / (D / 4), d = e % (D / 4) * 4, rho = rho0 + c * 16 + n0;
-            if (rho >= rows) break;
-            const float m = fmaxf(fmaxf(ms[0][n0], ms[1][n0]), fmaxf(ms[2][n0], ms[3][n0]));
-            const float mz = m == -INFINITY ? 0.f : m;
-            float sum = 0.f;
-            f32x4 o = {0.f, 0.f, 0.f, 0.f};
+                for (int i = 0; i < D / 16; i += 4) {
+                    const f32x4 o = {st.o[c][i][r], st.o[c][i + 1][r], st.o[c][i + 2][r], st.o[c][i + 3][r]};
+                    *(f32x4*)&os[wv][nn][(4 * g + r) * (D / 16) + i] = o;
+                }
+            __syncthreads();
+            for (int e = tid; e < 16 * (D / 4); e += 256) {
+                const int n0 = e / (D / 4), d = e % (D / 4) * 4, rho = rho0 + c * 16 + n0;
+                if (rho >= rows) break;
+                const float m = fmaxf(fmaxf(ms[0][n0], ms[1][n0]), fmaxf(ms[2][n0], ms[3][n0]));
+                const float mz = m == -INFINITY ? 0.f : m;
+                float sum = 0.f;
+                f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float f = __builtin_amdgcn_exp2f(ms[w][n0] - mz);
-                sum += f * ls[w][n0];
-                o += f * *(const f32x4*)&os[w][n0][d];
-            }
-            if (((bs[0][n0] | bs[1][n0] | bs[2][n0] | bs[3][n0]) >> (d / 32)) & 1) o *= __uint_as_float(0x7fc00000u);
-            if (splits == 1) {
-                store_row4(a, o, sum, seq, h, rho, d);
-            } else {
-                float* p = a.part + ((size_t)blockIdx.x * NQ + c) * kSplitRows * (D + 4) + n0 * (D + 4);
-                *(f32x4*)(p + d) = o;
-                if (d == 0) { p[D] = m; p[D + 1] = sum; }
+                for (int w = 0; w < 4; ++w) {
+                    const float f = __builtin_amdgcn_exp2f(ms[w][n0] - mz);
+                    sum += f * ls[w][n0];
+                    o += f * *(const f32x4*)&os[w][n0][d];
+                }
+                if (((bs[0][n0] | bs[1][n0] | bs[2][n0] | bs[3][n0]) >> (d / 32)) & 1) o *= __uint_as_float(0x7fc00000u);
+                if (splits == 1) {
+                    store_row4(a, o, sum, seq, h, rho, d);
+                } else {
+                    float* p = a.part + ((size_t)blockIdx.x * NQ + c) * kSplitRows * (D + 4) + n0 * (D + 4);
+                    *(f32x4*)(p + d) = o;
+                    if (d == 0) { p[D] = m; p[D + 1] = sum; }
+                }
             }
         }
     }
@@ -721,9 +778,18 @@ static hipError_t launch_attn(Kv4Attn& a, int n, hipStream_t st) {
     for (int i = n; i < kSeqArgs; ++i) a.first[i] = 0xffff;
     a.n = n;
     a.splits = z;
+    // prompts: row tiles in pairs of the same work once the pairs alone give every CU two blocks
+    const long long pairs = (long long)n * a.kv_heads * ((row_tiles + 1) / 2);
+    if (std::max<long long>({(long long)z * items, pairs, (long long)n * a.kv_heads * rows * (D / 4)}) > 0x7fffffffLL)
+        return hipErrorInvalidValue;
+    if (row_tiles > 1 && most == 1 && pairs >= 512) {
+        if (nq == 1) hipLaunchKernelGGL((attn_kv4_kernel<D, 1, true>), dim3((unsigned)pairs), dim3(256), 0, st, a, row_tiles);
+        else hipLaunchKernelGGL((attn_kv4_kernel<D, 2, true>), dim3((unsigned)pairs), dim3(256), 0, st, a, row_tiles);
+        return hipGetLastError();
+    }
     const unsigned blocks = (unsigned)z * items;
-    if (nq == 1) hipLaunchKernelGGL((attn_kv4_kernel<D, 1>), dim3(blocks), dim3(256), 0, st, a, row_tiles);
-    else hipLaunchKernelGGL((attn_kv4_kernel<D, 2>), dim3(blocks), dim3(256), 0, st, a, row_tiles);
+    if (nq == 1) hipLaunchKernelGGL((attn_kv4_kernel<D, 1, false>), dim3(blocks), dim3(256), 0, st, a, row_tiles);
+    else hipLaunchKernelGGL((attn_kv4_kernel<D, 2, false>), dim3(blocks), dim3(256), 0, st, a, row_tiles);
     hipError_t rc = hipGetLastError();
     if (rc != hipSuccess || most == 1) return rc;
     const long long heads = (long long)n * a.kv_heads * rows;

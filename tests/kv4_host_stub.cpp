@@ -28,7 +28,7 @@ static hipError_t count() {
     ++g_now->launches;
     return hipSuccess;
 }
-hipError_t launch_heads(const HeadArgs&, int, hipStream_t) { return count(); }
+hipError_t launch_heads(HeadArgs&, int, hipStream_t) { return count(); }
 hipError_t launch_attn_kv4(Kv4Attn&, int, hipStream_t) { return count(); }
 hipError_t launch_kv4_copy(const Kv4Copy&, bool, hipStream_t) { return count(); }
 hipError_t launch_verify(VerifyArgs&, hipStream_t) { return count(); }
