@@ -9,6 +9,7 @@ namespace q35 {
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // The pair of values in byte SEL of w, times the power of two in `scale`'s exponent: exact; NaN
@@ -309,29 +310,44 @@ template <int D>
 struct Tile {
     u32x4 k[D / 64], v[D / 64];
     uint32_t ks;
-    uint2 vs;
+    u32x2 vs;
 };
+// A lane's places in a tile; with the tile's address in scalar registers (scalar_ptr) a load needs no other
+// vector register for its address.
+struct Lanes { uint32_t blob, ks, vs; };
+template <int D>
+__device__ __forceinline__ Lanes lane_offsets() {
+    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+    return {(uint32_t)lane * 16, (uint32_t)(D == 256 ? lane * 4 : D == 64 ? ((g >> 1) * 16 + m) * 2 : lane * 2),
+            (uint32_t)(m * D / 512 * 32 + g * 8)};
+}
+typedef const __attribute__((address_space(1))) char* gptr;
+__device__ __forceinline__ gptr scalar_ptr(const uint8_t* p) {
+    const unsigned long long u = (unsigned long long)p;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u), hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
+    return (gptr)(((unsigned long long)hi << 32) | lo);
+}
+template <class T, bool ONCE = false>
+__device__ __forceinline__ T load_at(gptr p, uint32_t off) {
+    const auto* w = (const __attribute__((address_space(1))) T*)(p + off);
+    if constexpr (ONCE) return __builtin_nontemporal_load(w);
+    else return *w;
+}
 // ONCE: the tile is read by one block only (nontemporal loads)
 template <int D, bool ONCE>
-__device__ __forceinline__ void load_k(Tile<D>& t, const uint8_t* p) {
-    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+__device__ __forceinline__ void load_k(Tile<D>& t, const uint8_t* tile, const Lanes& o) {
+    const gptr p = scalar_ptr(tile);
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) {
-        const u32x4* w = (const u32x4*)(p + i * 1024 + lane * 16);
-        t.k[i] = ONCE ? __builtin_nontemporal_load(w) : *w;
-    }
-    if (D == 256) t.ks = *(const uint32_t*)(p + 32 * D + lane * 4);
-    else t.ks = *(const uint16_t*)(p + 32 * D + (D == 64 ? (g >> 1) * 16 + m : lane) * 2);
+    for (int i = 0; i < D / 64; ++i) t.k[i] = load_at<u32x4, ONCE>(p, o.blob + i * 1024);
+    const gptr ps = scalar_ptr(tile + 32 * D);
+    t.ks = D == 256 ? load_at<uint32_t>(ps, o.ks) : load_at<uint16_t>(ps, o.ks);
 }
 template <int D, bool ONCE>
-__device__ __forceinline__ void load_v(Tile<D>& t, const uint8_t* p) {
-    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+__device__ __forceinline__ void load_v(Tile<D>& t, const uint8_t* tile, const Lanes& o) {
+    const gptr p = scalar_ptr(tile + 16 * D);
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) {
-        const u32x4* w = (const u32x4*)(p + 16 * D + i * 1024 + lane * 16);
-        t.v[i] = ONCE ? __builtin_nontemporal_load(w) : *w;
-    }
-    t.vs = *(const uint2*)(p + 33 * D + m * D / 512 * 32 + g * 8);
+    for (int i = 0; i < D / 64; ++i) t.v[i] = load_at<u32x4, ONCE>(p, o.blob + i * 1024);
+    t.vs = load_at<u32x2>(scalar_ptr(tile + 33 * D), o.vs);
 }
 template <int D>
 __device__ __forceinline__ float k_scale(const Tile<D>& t, int half, int s) {
@@ -369,12 +385,13 @@ __device__ __forceinline__ void v_frags(const Tile<D>& t, const float* vs, q35_b
 
 // Which slots a row sees: (pos - window, pos] and [0, sinks); window 0: [0, pos].
 struct Sight { int pos, low, sinks; };
-__device__ __forceinline__ bool sees(const Sight& s, int slot) { return slot <= s.pos && (slot >= s.low || slot < s.sinks); }
+__device__ __forceinline__ bool sees(const Sight& s, int slot) { return (slot <= s.pos) & ((slot >= s.low) | (slot < s.sinks)); }
 
 // The running state of NQ x 16 rows over the tiles of one wave.
 template <int D, int NQ>
 struct Rows {
-    float m[NQ], l[NQ];          // of row n: its maximum (log2 units), the lane group's share of its sum
+    float m[NQ];                 // of row n: the reference of its exponents (log2 units)
+    f32x4 l[NQ];                 // its sum of weights, four times
     uint32_t bad[NQ];            // groups of 32 dims whose V held a NaN at a slot the row sees
     f32x4 o[NQ][D / 16];         // O^T: dims (4 g + r) D / 16 + i of row n in o[.][i][r]
 };
@@ -382,27 +399,33 @@ struct Rows {
 // q: the rows' Q^T operands, [NQ][D / 32], in registers (NQ = 1) or, 16 rows more, in LDS with 64 lanes each
 // (the four waves of a block have the same rows). REFILL: t's registers take the tile at next_p as soon as its K, then
 // its V, is used up (32 registers less than a second tile; the loads have the other half's work to arrive).
+// edge: some row may not see some slot.
 template <int D, int NQ, bool REFILL, class Q>
-__device__ __forceinline__ void tile_step(Tile<D>& t, const uint8_t* tile_p, const uint8_t* next_p, int slot0, bool edge, const Q& q,
-                                          const Sight* sight, float scale2, Rows<D, NQ>& st) {
+__device__ __forceinline__ void tile_step(Tile<D>& t, const uint8_t* tile_p, const uint8_t* next_p, const Lanes& lo, int slot0,
+                                          bool edge, const Q& q, const Sight* sight, float scale2, Rows<D, NQ>& st) {
     const int lane = threadIdx.x & 63, g = lane >> 4;
     f32x4 s[NQ][2];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
+    for (int c = 0; c < NQ; ++c) s[c][0] = s[c][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    q35_bf16x8 qn[NQ];
 #pragma unroll
-        for (int c = 0; c < NQ; ++c) s[c][half] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < NQ; ++c) qn[c] = q(c, 0);
 #pragma unroll
-        for (int k = 0; k < D / 32; ++k) {
+    for (int k = 0; k < D / 32; ++k) {
+        q35_bf16x8 qk[NQ];
+#pragma unroll
+        for (int c = 0; c < NQ; ++c) { qk[c] = qn[c]; if (k + 1 < D / 32) qn[c] = q(c, k + 1); }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
             const q35_bf16x8 kf = k_frag<D>(t, half, k);
 #pragma unroll
             for (int c = 0; c < NQ; ++c)
-                s[c][half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q(c, k), s[c][half], 0, 0, 0);
+                s[c][half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qk[c], s[c][half], 0, 0, 0);
         }
+        if (REFILL) __builtin_amdgcn_sched_barrier(0);     // fragments made far ahead would not fit the registers
     }
-    if (REFILL) load_k<D, false>(t, next_p);
-#pragma unroll
-    for (int c = 0; c < NQ; ++c) { s[c][0] *= scale2; s[c][1] *= scale2; }     // before the mask: scale may be 0 or negative
-    uint2 vsb = t.vs;
+    if (REFILL) load_k<D, false>(t, next_p, lo);
+    u32x2 vsb = t.vs;
     // A slot some row may not see: its score is dropped, and a NaN group of V there must not meet the
     // zero weight. Such a group is read as finite and noted for the rows that do see it.
     if (edge) {
@@ -435,29 +458,29 @@ __device__ __forceinline__ void tile_step(Tile<D>& t, const uint8_t* tile_p, con
     q35_bf16x8 pf[NQ];
 #pragma unroll
     for (int c = 0; c < NQ; ++c) {
-        float top = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, s[c][j >> 2][j & 3]);
-        top = fmaxf(top, xor16(top));
-        top = fmaxf(top, xor32(top));
-        const float mn = fmaxf(st.m[c], top);
-        const float ms = mn == -INFINITY ? 0.f : mn;      // nothing seen so far: e^(-inf) stays 0
-        if (__any(mn > st.m[c])) {
-            const float al = __builtin_amdgcn_exp2f(st.m[c] - ms);
+        float top = fmaxf(fmaxf(s[c][0][0], s[c][0][1]), fmaxf(s[c][0][2], s[c][0][3]));
+        top = fmaxf(top, fmaxf(fmaxf(s[c][1][0], s[c][1][1]), fmaxf(s[c][1][2], s[c][1][3])));
+        // the reference of the row's exponents follows its maximum only when that is past it by 2^8: weights
+        // stay under 2^8 (as exact as under 1), and almost every tile goes without the four lanes' common
+        // maximum and the rescale of O
+        if (__any(top * scale2 > st.m[c] + 8.f)) {
+            top = fmaxf(top, xor16(top));
+            top = fmaxf(top, xor32(top)) * scale2;
+            const float mn = fmaxf(st.m[c], top), al = __builtin_amdgcn_exp2f(st.m[c] - (mn == -INFINITY ? 0.f : mn));
             st.l[c] *= al;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) st.o[c][i] *= al;
             st.m[c] = mn;
         }
+        const float ms = st.m[c] == -INFINITY ? 0.f : st.m[c];      // nothing seen so far: e^(-inf) stays 0
         float p[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            p[j] = __builtin_amdgcn_exp2f(s[c][j >> 2][j & 3] - ms);
-            st.l[c] += p[j];
-        }
-        // weights of 2^-9 relative rounding for the bf16 product; their sum stays float32
+        for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][j >> 2][j & 3], scale2, -ms));
+        // weights rounded to bf16 (2^-9) for the product; their sum is that of the rounded ones, a product with ones
         const u32x4 pw = {f2bf2(p[0], p[1]), f2bf2(p[2], p[3]), f2bf2(p[4], p[5]), f2bf2(p[6], p[7])};
         pf[c] = __builtin_bit_cast(q35_bf16x8, pw);
+        st.l[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_bf16x8, u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}),
+                                                          pf[c], st.l[c], 0, 0, 0);
     }
     float vs[8];
 #pragma unroll
@@ -475,6 +498,7 @@ __device__ __forceinline__ void tile_step(Tile<D>& t, const uint8_t* tile_p, con
                 st.o[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, pf[c], st.o[c][d], 0, 0, 0);
                 st.o[c][d + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, pf[c], st.o[c][d + 1], 0, 0, 0);
             }
+            if (REFILL) __builtin_amdgcn_sched_barrier(0);
         }
     };
     pv(std::integral_constant<int, 0>{});
@@ -485,7 +509,7 @@ __device__ __forceinline__ void tile_step(Tile<D>& t, const uint8_t* tile_p, con
     pv(std::integral_constant<int, 10>{});
     pv(std::integral_constant<int, 12>{});
     pv(std::integral_constant<int, 14>{});
-    if (REFILL) load_v<D, false>(t, next_p);
+    if (REFILL) load_v<D, false>(t, next_p, lo);
 }
 
 // The tiles that rows at positions p0 .. p1 read: those of the sinks, then those from the first row's
@@ -532,19 +556,34 @@ __device__ __forceinline__ Seq find_seq(const Kv4Attn& a, int z) {
     return s;
 }
 
-// The end of a row's four dims: normalised, gated, rounded.
-__device__ __forceinline__ void store_row4(const Kv4Attn& a, f32x4 o, float sum, int seq, int h, int rho, int d) {
-    const int group = a.q_heads / a.kv_heads, t = rho / group, hq = h * group + rho - t * group;
-    const long long row = (long long)seq * a.T + t;
-    o /= sum;
-    if (a.gate.p) {
-        const f32x4 gt = wide(*(const uint2*)(a.gate.p + row * a.gate.row + hq * a.gate.head + d));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] *= sigmoid_f(gt[i]);
+// Where a row's dims go: normalised, gated, rounded. N dims (1, 2 or 4) from d on.
+struct Out {
+    const uint16_t* gate;
+    uint16_t* out;
+    __device__ __forceinline__ Out(const Kv4Attn& a, long long seq, int h, int rho) {
+        const int group = a.q_heads / a.kv_heads, t = rho / group, hq = h * group + rho - t * group;
+        const long long row = seq * a.T + t;
+        gate = a.gate.p + row * a.gate.row + hq * a.gate.head;
+        out = const_cast<uint16_t*>(a.out.p) + row * a.out.row + hq * a.out.head;
     }
-    *(uint2*)(const_cast<uint16_t*>(a.out.p) + row * a.out.row + hq * a.out.head + d) =
-        make_uint2(f2bf2(o[0], o[1]), f2bf2(o[2], o[3]));
-}
+    template <int N>
+    __device__ __forceinline__ void store(const Kv4Attn& a, float* x, float sum, int d) const {
+        const float inv = __builtin_amdgcn_rcpf(sum);
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] *= inv;
+        if (a.gate.p) {              // sigmoid by the instructions' 2^x and 1/x (a float32 ulp each)
+            uint16_t gt[N];
+            __builtin_memcpy(gt, gate + d, 2 * N);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                x[i] *= __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(bf2f(gt[i]) * -1.44269504088896f));
+        }
+        uint16_t w[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = f2bf(x[i]);
+        __builtin_memcpy(out + d, w, 2 * N);
+    }
+};
 // Partial result of (split z, kv head h, row rho): D sums, then the maximum and the sum of the weights.
 template <int D, int NQ>
 __device__ __forceinline__ const float* part_of(const Kv4Attn& a, int row_tiles, int z, int h, int rho) {
@@ -557,7 +596,8 @@ __device__ __forceinline__ const float* part_of(const Kv4Attn& a, int row_tiles,
 // under the causal mask, all its tiles included (splits == 1).
 template <int D, int NQ, bool PAIRS>
 __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) attn_kv4_kernel(Kv4Attn a, int row_tiles) {
-    __shared__ __attribute__((aligned(16))) float os[4][16][D + 4];
+    constexpr int kQuarter = D / 64;         // of the D / 16 accumulators of 16 rows
+    __shared__ f32x4 os[4][4][kQuarter][64];
     __shared__ float ms[4][16], ls[4][16];
     __shared__ uint32_t bs[4][16];
     static_assert(NQ == 1 || sizeof(os) >= NQ * (D / 32) * 1024, "the Q operands lie where the waves' sums go at the end");
@@ -568,7 +608,10 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) attn_kv4_kernel(Kv4Attn
     const Seq sq = find_seq(a, z);
     const int seq = sq.i, splits = sq.splits, pos = sq.pos, group = a.q_heads / a.kv_heads, rows = a.T * group;
     const uint8_t* region = a.cache + sq.lane * a.lane_bytes + h * a.region;
-    const float scale2 = a.scale * 1.44269504088896f;
+    // positive, so that the largest product has the largest exponent and a dropped one's -inf stays it: a negative
+    // scale's sign goes to q, 0 becomes the smallest normal number
+    const float scale2 = fmaxf(fabsf(a.scale) * 1.44269504088896f, 1.17549435e-38f);
+    const Lanes lo = lane_offsets<D>();
     for (int pass = 0; pass < (PAIRS ? 2 : 1); ++pass) {
         const int rt = pass ? rt0 : PAIRS ? row_tiles - 1 - rt0 : rt0, rho0 = rt * NQ * 16;
         if (pass && rt == row_tiles - 1 - rt0) break;        // the middle one
@@ -578,18 +621,20 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) attn_kv4_kernel(Kv4Attn
         const auto q_at = [&](int rho, int gg, int k) {
             rho = min(rho, rows - 1);
             const int t = rho / group;
-            return *(const q35_bf16x8*)(a.q.p + ((long long)seq * a.T + t) * a.q.row + (h * group + rho - t * group) * a.q.head +
-                                        gg * (D / 4) + 8 * k);
+            u32x4 w = *(const u32x4*)(a.q.p + ((long long)seq * a.T + t) * a.q.row + (h * group + rho - t * group) * a.q.head +
+                                      gg * (D / 4) + 8 * k);
+            if (a.scale < 0.f) w ^= 0x80008000u;
+            return __builtin_bit_cast(q35_bf16x8, w);
         };
         auto at = [&](int i) { return i < tl.sink ? i : i - tl.sink + tl.main; };
         Tile<D> cur;
         const auto tile_at = [&](int i) { return region + (size_t)at(i) * kv4_tile_bytes(D); };
         if (t0 + wv < t1) {
-            load_k<D, kOnce>(cur, tile_at(t0 + wv));
-            load_v<D, kOnce>(cur, tile_at(t0 + wv));
+            load_k<D, kOnce>(cur, tile_at(t0 + wv), lo);
+            load_v<D, kOnce>(cur, tile_at(t0 + wv), lo);
         }
         q35_bf16x8 qf[NQ == 1 ? D / 32 : 1];
-        q35_bf16x8* ql = (q35_bf16x8*)&os[0][0][0];
+        q35_bf16x8* ql = (q35_bf16x8*)&os[0][0][0][0];
         if constexpr (NQ == 1) {
 #pragma unroll
             for (int k = 0; k < D / 32; ++k) qf[k] = q_at(rho0 + nn, g, k);
@@ -610,64 +655,84 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) attn_kv4_kernel(Kv4Attn
             const int p = pos + min(rho0 + c * 16 + nn, rows - 1) / group;
             sight[c] = {p, a.window > 0 ? p - a.window + 1 : 0, a.sinks};
             st.m[c] = -INFINITY;
-            st.l[c] = 0.f;
+            st.l[c] = f32x4{0.f, 0.f, 0.f, 0.f};
             st.bad[c] = 0;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) st.o[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
         // tiles whose every slot every row of the block sees: from the last row's window to the first row's slot
         const int full0 = a.window > 0 ? max(pos + rho1 / group - a.window + 1, 0) : 0, full1 = pos + rho0 / group;
-        for (int i = t0 + wv; i < t1; i += 4) {
+        for (int i = __builtin_amdgcn_readfirstlane(t0 + wv); i < t1; i += 4) {
             const int tile = at(i);
             if (NQ > 1) asm volatile("" : "+v"(qlane));     // or the compiler reads Q ahead of the loop, and spills it
             const uint8_t* next_p = tile_at(min(i + 4, t1 - 1));
             Tile<D> next;
             if (!kRefill) {
-                load_k<D, kOnce>(next, next_p);
-                load_v<D, kOnce>(next, next_p);
+                load_k<D, kOnce>(next, next_p, lo);
+                load_v<D, kOnce>(next, next_p, lo);
             }
             const bool edge = tile * 32 < full0 || tile * 32 + 31 > full1;
-            tile_step<D, NQ, kRefill>(cur, tile_at(i), next_p, tile * 32, edge, q, sight, scale2, st);
+            tile_step<D, NQ, kRefill>(cur, tile_at(i), next_p, lo, tile * 32, edge, q, sight, scale2, st);
             if (!kRefill) cur = next;
         }
+        // The four waves' states: wave w ends a quarter of the row's dims, which the others pass it through
+        // LDS; a lane keeps its row, and its accumulators go as they are.
 #pragma unroll
         for (int c = 0; c < NQ; ++c) {
             if (rho0 + c * 16 >= rows) break;
             if (NQ > 1 || pass || c) __syncthreads();        // os was read: Q, or the 16 rows before these
-            float l = st.l[c];
-            l += xor16(l);
-            l += xor32(l);
             uint32_t bad = st.bad[c];
             bad |= (uint32_t)__shfl_xor((int)bad, 16);
             bad |= (uint32_t)__shfl_xor((int)bad, 32);
-            if (g == 0) { ms[wv][nn] = st.m[c]; ls[wv][nn] = l; bs[wv][nn] = bad; }
+            if (g == 0) { ms[wv][nn] = st.m[c]; ls[wv][nn] = st.l[c][0]; bs[wv][nn] = bad; }
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+            for (int w = 0; w < 4; ++w)
 #pragma unroll
-                for (int i = 0; i < D / 16; i += 4) {
-                    const f32x4 o = {st.o[c][i][r], st.o[c][i + 1][r], st.o[c][i + 2][r], st.o[c][i + 3][r]};
-                    *(f32x4*)&os[wv][nn][(4 * g + r) * (D / 16) + i] = o;
-                }
+                for (int i = 0; i < kQuarter; ++i)
+                    if (w != wv) os[w][wv][i][lane] = st.o[c][w * kQuarter + i];
             __syncthreads();
-            for (int e = tid; e < 16 * (D / 4); e += 256) {
-                const int n0 = e / (D / 4), d = e % (D / 4) * 4, rho = rho0 + c * 16 + n0;
-                if (rho >= rows) break;
-                const float m = fmaxf(fmaxf(ms[0][n0], ms[1][n0]), fmaxf(ms[2][n0], ms[3][n0]));
-                const float mz = m == -INFINITY ? 0.f : m;
-                float sum = 0.f;
-                f32x4 o = {0.f, 0.f, 0.f, 0.f};
+            float m = st.m[c], sum = 0.f, f[4];
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const float f = __builtin_amdgcn_exp2f(ms[w][n0] - mz);
-                    sum += f * ls[w][n0];
-                    o += f * *(const f32x4*)&os[w][n0][d];
+            for (int w = 0; w < 4; ++w) m = fmaxf(m, ms[w][nn]);
+            bad = 0;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                f[w] = __builtin_amdgcn_exp2f(ms[w][nn] - (m == -INFINITY ? 0.f : m));
+                sum += f[w] * ls[w][nn];
+                bad |= bs[w][nn];
+            }
+            f32x4 o[kQuarter];
+#pragma unroll
+            for (int i = 0; i < kQuarter; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < 4; ++w)              // in the same order in every wave
+#pragma unroll
+                for (int i = 0; i < kQuarter; ++i) {
+                    f32x4 x;
+                    if (w == wv) {
+                        x = st.o[c][i];
+#pragma unroll
+                        for (int k = 1; k < 4; ++k) x = wv == k ? st.o[c][k * kQuarter + i] : x;
+                    } else {
+                        x = os[wv][w][i][lane];
+                    }
+                    o[i] += f[w] * x;
                 }
-                if (((bs[0][n0] | bs[1][n0] | bs[2][n0] | bs[3][n0]) >> (d / 32)) & 1) o *= __uint_as_float(0x7fc00000u);
+            const int rho = rho0 + c * 16 + nn;
+            if (rho >= rows) continue;
+            const Out to(a, seq, h, rho);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int d = (4 * g + r) * (D / 16) + wv * kQuarter;
+                float x[kQuarter];
+#pragma unroll
+                for (int i = 0; i < kQuarter; ++i) x[i] = (bad >> (d / 32)) & 1 ? __uint_as_float(0x7fc00000u) : o[i][r];
                 if (splits == 1) {
-                    store_row4(a, o, sum, seq, h, rho, d);
+                    to.store<kQuarter>(a, x, sum, d);
                 } else {
-                    float* p = a.part + ((size_t)blockIdx.x * NQ + c) * kSplitRows * (D + 4) + n0 * (D + 4);
-                    *(f32x4*)(p + d) = o;
+                    float* p = a.part + ((size_t)blockIdx.x * NQ + c) * kSplitRows * (D + 4) + nn * (D + 4);
+#pragma unroll
+                    for (int i = 0; i < kQuarter; ++i) p[d + i] = x[i];
                     if (d == 0) { p[D] = m; p[D + 1] = sum; }
                 }
             }
@@ -710,7 +775,7 @@ __global__ void __launch_bounds__(256) attn_kv4_join_few(Kv4Attn a, int row_tile
         sum += f * ml[s].y;
         x += f * o[s];
     }
-    store_row4(a, x, sum, (int)seq, h, rho, d);
+    Out(a, seq, h, rho).store<4>(a, (float*)&x, sum, d);
 }
 
 // The same for any number of splits: a block per (sequence, kv head, row, 64 dims). The splits' factors are
@@ -753,7 +818,7 @@ __global__ void __launch_bounds__(256) attn_kv4_join(Kv4Attn a, int row_tiles) {
     if (tid >= 16) return;
 #pragma unroll
     for (int i = 1; i < 16; ++i) o += os[i * 16 + tid];
-    store_row4(a, o, sum, seq, h, rho, d);
+    Out(a, seq, h, rho).store<4>(a, (float*)&o, sum, d);
 }
 
 template <int D>
