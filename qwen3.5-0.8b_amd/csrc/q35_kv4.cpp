@@ -322,6 +322,8 @@ int q35_op_draft_verify(q35_engine* e, const q35_drafts* d, int n, int k, int vo
         a.logits = d->logits; a.draft_logits = d->temperature == 0.0 ? nullptr : d->draft_logits;
         a.ld = d->ld; a.ldd = d->draft_ld; a.bf16 = d->dtype; a.n = n; a.k = k; a.vocab = vocab;
         a.inv_temp = d->temperature == 0.0 ? 0.0 : 1.0 / d->temperature;
+        a.scale.c = a.inv_temp * 1.4426950408889634074;
+        a.scale.low = a.inv_temp == 0.0 ? 0.0 : -1100.0 / a.scale.c;
         a.drafts = d->drafts; a.u = d->u; a.accepted = accepted; a.tokens = tokens; a.stats = ev.verify_ws;
         OnDevice on(ev.device);
         HCK(launch_verify(a, ev.st));

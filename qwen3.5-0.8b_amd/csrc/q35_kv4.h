@@ -91,11 +91,13 @@ struct Kv4Copy {
 hipError_t launch_kv4_copy(const Kv4Copy& a, bool write, hipStream_t st);
 
 // Verification of drafts (q35_verify.hip).
+struct VerifyScale { double c, low; };   // log2(e) / temperature; -1100 / c
 struct VerifyArgs {
     const void *logits, *draft_logits;   // [n][k + 1][ld], [n][k][ldd] (null: drafts are certain); f32 or bf16
     long long ld, ldd;
     int bf16, n, k, vocab;
     double inv_temp;                     // 0: greedy
+    VerifyScale scale;
     const int* drafts;                   // [n][k]; the first negative one ends a lane's drafts
     const float* u;                      // [n][k + 1]
     int *accepted, *tokens;              // [n], [n][k + 1]

@@ -21,11 +21,7 @@ namespace q35 {
 // bits are the exponent; what is left, |f| <= 1/2, is d c minus it, in one rounding; 2^f is the
 // polynomial that interpolates it at the ten Chebyshev points (relative error under 2e-14, far under what
 // a border between a million terms notices). 0 under 2^-1074, so also for l = -inf.
-struct Scale { double c, low; };     // low: -1100 / c
-__device__ __forceinline__ Scale scale_from(double inv_temp) {
-    const double c = inv_temp * 1.4426950408889634074;
-    return {c, -1100.0 / c};
-}
+typedef VerifyScale Scale;
 __device__ __forceinline__ double power(double d, const Scale& sc) {
     d = fmax(d, sc.low);
     const double t = __builtin_fma(d, sc.c, 6755399441055744.0), k = t - 6755399441055744.0;
@@ -46,30 +42,64 @@ __device__ __forceinline__ double power(double d, const Scale& sc) {
 constexpr int kMaxChunk = 8192;
 struct Stat { double m, s; };        // a chunk's largest logit, and the sum of 2^((l - m) c); greedy: its index
 
-__device__ __forceinline__ double wsum(double v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+// Reductions and running sums over a wave by DPP moves (a shuffle of a double is two trips to LDS, and the last
+// kernel is a chain of them): within rows of 16 by 1, 2, 4 and 8 lanes, then row 0 into 1 and 2 into 3, then
+// the lower half into the upper. Lane 63 ends with all lanes' result.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_or(double v, double none) {
+    const unsigned long long w = __builtin_bit_cast(unsigned long long, v), n = __builtin_bit_cast(unsigned long long, none);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp((int)(uint32_t)n, (int)(uint32_t)w, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp((int)(uint32_t)(n >> 32), (int)(uint32_t)(w >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_or(int v, int none) { return __builtin_amdgcn_update_dpp(none, v, CTRL, ROWS, 0xf, false); }
+template <class T, class F>
+__device__ __forceinline__ T wave_scan(T v, T none, F f) {
+    v = f(v, dpp_or<0x111, 0xf>(v, none));       // row_shr:1
+    v = f(v, dpp_or<0x112, 0xf>(v, none));
+    v = f(v, dpp_or<0x114, 0xf>(v, none));
+    v = f(v, dpp_or<0x118, 0xf>(v, none));
+    v = f(v, dpp_or<0x142, 0xa>(v, none));       // row_bcast:15
+    return f(v, dpp_or<0x143, 0xc>(v, none));    // row_bcast:31
+}
+__device__ __forceinline__ double last_lane(double v) {
+    const unsigned long long w = __builtin_bit_cast(unsigned long long, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)w, 63), hi = __builtin_amdgcn_readlane((int)(uint32_t)(w >> 32), 63);
+    return __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo);
+}
+__device__ __forceinline__ double running(double v) { return wave_scan(v, 0.0, [](double x, double y) { return x + y; }); }
+__device__ __forceinline__ double wsum(double v) { return last_lane(running(v)); }
+__device__ __forceinline__ double wmax(double v) {
+    return last_lane(wave_scan(v, -(double)INFINITY, [](double x, double y) { return fmax(x, y); }));
+}
+__device__ __forceinline__ int wmin_i(int v) {
+    return __builtin_amdgcn_readlane(wave_scan(v, 0x7fffffff, [](int x, int y) { return min(x, y); }), 63);
+}
+__device__ __forceinline__ int wmax_i(int v) {
+    return __builtin_amdgcn_readlane(wave_scan(v, -0x7fffffff, [](int x, int y) { return max(x, y); }), 63);
 }
 
-// Four (f32) or eight (bf16) logits from i on; -inf past the vocabulary. Rows may start at any element.
+// Four (f32) or eight (bf16) logits from i on. Rows may start at any element.
+template <bool BF16>
+__device__ __forceinline__ void load_whole(const void* row, int i, float* v) {
+    uint32_t w[4];
+    __builtin_memcpy(w, (const char*)row + (size_t)i * (BF16 ? 2 : 4), 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (BF16) {
+            v[2 * j] = __uint_as_float(w[j] << 16);
+            v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+        } else {
+            v[j] = __uint_as_float(w[j]);
+        }
+    }
+}
+// The same with -inf past the vocabulary.
 template <bool BF16>
 __device__ __forceinline__ void load_logits(const void* row, int i, int vocab, float* v) {
     constexpr int N = BF16 ? 8 : 4;
-    if (i + N <= vocab) {
-        uint32_t w[4];
-        __builtin_memcpy(w, (const char*)row + (size_t)i * (BF16 ? 2 : 4), 16);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (BF16) {
-                v[2 * j] = __uint_as_float(w[j] << 16);
-                v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-            } else {
-                v[j] = __uint_as_float(w[j]);
-            }
-        }
-        return;
-    }
+    if (i + N <= vocab) return load_whole<BF16>(row, i, v);
 #pragma unroll
     for (int j = 0; j < N; ++j)
         v[j] = i + j >= vocab ? -INFINITY : BF16 ? bf2f(((const uint16_t*)row)[i + j]) : ((const float*)row)[i + j];
@@ -104,7 +134,11 @@ __global__ void __launch_bounds__(256) verify_stats(VerifyArgs a) {
     const int i0 = c * a.chunk;
     float v[LOADS][N];
 #pragma unroll
-    for (int b = 0; b < LOADS; ++b) load_logits<BF16>(row, i0 + (b * 256 + (int)threadIdx.x) * N, a.vocab, v[b]);
+    for (int b = 0; b < LOADS; ++b) {        // (a chunk within the vocabulary: no check a load)
+        const int i = i0 + (b * 256 + (int)threadIdx.x) * N;
+        if (i0 + a.chunk <= a.vocab) load_whole<BF16>(row, i, v[b]);
+        else load_logits<BF16>(row, i, a.vocab, v[b]);
+    }
     float m = -INFINITY;                 // (a NaN anywhere makes it one)
 #pragma unroll
     for (int b = 0; b < LOADS; ++b)
@@ -123,8 +157,7 @@ __global__ void __launch_bounds__(256) verify_stats(VerifyArgs a) {
 #pragma unroll
             for (int e = N - 1; e >= 0; --e)
                 if (v[b][e] == m) best = i0 + (b * 256 + (int)threadIdx.x) * N + e;
-#pragma unroll
-        for (int o = 32; o; o >>= 1) best = min(best, __shfl_xor(best, o));
+        best = wmin_i(best);
         if (lane == 0) at[wv] = best;
         __syncthreads();
         if (threadIdx.x == 0) *out = {(double)m, (double)min(min(at[0], at[1]), min(at[2], at[3]))};
@@ -132,7 +165,7 @@ __global__ void __launch_bounds__(256) verify_stats(VerifyArgs a) {
     }
     double s = 0.0;
     if (m > -INFINITY && m < INFINITY) {
-        const Scale sc = scale_from(a.inv_temp);
+        const Scale sc = a.scale;
         const double md = m;
 #pragma unroll
         for (int b = 0; b < LOADS; ++b)
@@ -159,16 +192,14 @@ __device__ __forceinline__ Stat row_stat(const VerifyArgs& a, const Stat* st, co
     bool nan = false;
 #pragma unroll
     for (int i = 0; i < kMaxChunks / 64; ++i) { m = fmax(m, v[i].m); nan |= v[i].m != v[i].m; }
-#pragma unroll
-    for (int o = 32; o; o >>= 1) m = fmax(m, __shfl_xor(m, o));
+    m = wmax(m);
     if (__any(nan)) m = __longlong_as_double(0x7ff8000000000000ll);
     double s = 0.0;
     if (a.inv_temp == 0.0) {
         s = 2147483647.0;
 #pragma unroll
         for (int i = 0; i < kMaxChunks / 64; ++i) if (v[i].m == m) s = fmin(s, v[i].s);
-#pragma unroll
-        for (int o = 32; o; o >>= 1) s = fmin(s, __shfl_xor(s, o));
+        s = -wmax(-s);
     } else {
 #pragma unroll
         for (int i = 0; i < kMaxChunks / 64; ++i) if (v[i].s > 0.0) s += v[i].s * power(v[i].m - m, sc);
@@ -277,7 +308,7 @@ __global__ void __launch_bounds__(256) verify_rest(VerifyArgs a, double* rest) {
     __shared__ Draft pq[kVerifyDrafts];
     __shared__ double sm[4];
     const int c = blockIdx.x % a.chunks, ln = blockIdx.x / a.chunks;
-    const Scale sc = scale_from(a.inv_temp);
+    const Scale sc = a.scale;
     const Fate ft = decide<BF16>(a, ln, sc, rs, pq);
     if (ft.kind != kRest) return;
     const Weights<BF16> wt(a, ln, ft, sc, rs);
@@ -297,21 +328,19 @@ __global__ void __launch_bounds__(256) verify_rest(VerifyArgs a, double* rest) {
 // Inclusive sum over the block's 1024 threads, by place; part: 16 doubles.
 __device__ __forceinline__ double block_scan(double v, double* part) {
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double up = __shfl_up(v, o);
-        if (lane >= o) v += up;
-    }
+    v = running(v);
     __syncthreads();
     if (lane == 63) part[wv] = v;
     __syncthreads();
-    for (int w = 0; w < wv; ++w) v += part[w];
-    return v;
+    double before = 0.0;
+#pragma unroll
+    for (int w = 0; w < 15; ++w) before += w < wv ? part[w] : 0.0;
+    return before + v;
 }
 // The lowest `first` and the highest `last` of the block's threads.
 __device__ __forceinline__ int2 block_ends(int first, int last, int2* ends) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) { first = min(first, __shfl_xor(first, o)); last = max(last, __shfl_xor(last, o)); }
+    first = wmin_i(first);
+    last = wmax_i(last);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) ends[threadIdx.x >> 6] = make_int2(first, last);
     __syncthreads();
@@ -328,7 +357,7 @@ __global__ void __launch_bounds__(1024) verify_token(VerifyArgs a, const double*
     __shared__ double part[16], total, base;
     __shared__ int2 ends[16];
     const int ln = blockIdx.x, tid = threadIdx.x;
-    const Scale sc = scale_from(a.inv_temp);
+    const Scale sc = a.scale;
     const Fate ft = decide<BF16>(a, ln, sc, rs, pq);
     int token = -1;
     if (ft.kind == kArgmax) token = (int)rs[ft.accepted].s;
