@@ -11,6 +11,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((__vector_size__(8 * sizeof(float)))) float f32x8;
 
 // The pair of values in byte SEL of w, times the power of two in `scale`'s exponent: exact; NaN
 // where that exponent is 255 (all 256 bytes x 245 scales and 255 compared on MI355X).
@@ -397,10 +398,10 @@ struct Rows {
 };
 
 // q: the rows' Q^T operands, [NQ][D / 32], in registers (NQ = 1) or, 16 rows more, in LDS with 64 lanes each
-// (the four waves of a block have the same rows). REFILL: t's registers take the tile at next_p as soon as its K, then
-// its V, is used up (32 registers less than a second tile; the loads have the other half's work to arrive).
+// (the four waves of a block have the same rows). t's registers take the tile at next_p as soon as its K, then its
+// V, is used up. TIGHT: 32 rows of 256 dims leave no register for fragments made far ahead.
 // edge: some row may not see some slot.
-template <int D, int NQ, bool REFILL, class Q>
+template <int D, int NQ, bool ONCE, bool TIGHT, class Q>
 __device__ __forceinline__ void tile_step(Tile<D>& t, const uint8_t* tile_p, const uint8_t* next_p, const Lanes& lo, int slot0,
                                           bool edge, const Q& q, const Sight* sight, float scale2, Rows<D, NQ>& st) {
     const int lane = threadIdx.x & 63, g = lane >> 4;
@@ -422,9 +423,9 @@ __device__ __forceinline__ void tile_step(Tile<D>& t, const uint8_t* tile_p, con
             for (int c = 0; c < NQ; ++c)
                 s[c][half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qk[c], s[c][half], 0, 0, 0);
         }
-        if (REFILL) __builtin_amdgcn_sched_barrier(0);     // fragments made far ahead would not fit the registers
+        if (TIGHT) __builtin_amdgcn_sched_barrier(0);
     }
-    if (REFILL) load_k<D, false>(t, next_p, lo);
+    load_k<D, ONCE>(t, next_p, lo);
     u32x2 vsb = t.vs;
     // A slot some row may not see: its score is dropped, and a NaN group of V there must not meet the
     // zero weight. Such a group is read as finite and noted for the rows that do see it.
@@ -477,8 +478,8 @@ __device__ __forceinline__ void tile_step(Tile<D>& t, const uint8_t* tile_p, con
 #pragma unroll
         for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][j >> 2][j & 3], scale2, -ms));
         // weights rounded to bf16 (2^-9) for the product; their sum is that of the rounded ones, a product with ones
-        const u32x4 pw = {f2bf2(p[0], p[1]), f2bf2(p[2], p[3]), f2bf2(p[4], p[5]), f2bf2(p[6], p[7])};
-        pf[c] = __builtin_bit_cast(q35_bf16x8, pw);
+        const f32x8 pw = {p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]};
+        pf[c] = __builtin_convertvector(pw, q35_bf16x8);     // not f2bf2: the compiler must see what an MFMA is about to read
         st.l[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_bf16x8, u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}),
                                                           pf[c], st.l[c], 0, 0, 0);
     }
@@ -498,7 +499,7 @@ __device__ __forceinline__ void tile_step(Tile<D>& t, const uint8_t* tile_p, con
                 st.o[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, pf[c], st.o[c][d], 0, 0, 0);
                 st.o[c][d + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, pf[c], st.o[c][d + 1], 0, 0, 0);
             }
-            if (REFILL) __builtin_amdgcn_sched_barrier(0);
+            if (TIGHT) __builtin_amdgcn_sched_barrier(0);
         }
     };
     pv(std::integral_constant<int, 0>{});
@@ -509,7 +510,7 @@ __device__ __forceinline__ void tile_step(Tile<D>& t, const uint8_t* tile_p, con
     pv(std::integral_constant<int, 10>{});
     pv(std::integral_constant<int, 12>{});
     pv(std::integral_constant<int, 14>{});
-    if (REFILL) load_v<D, false>(t, next_p, lo);
+    load_v<D, ONCE>(t, next_p, lo);
 }
 
 // The tiles that rows at positions p0 .. p1 read: those of the sinks, then those from the first row's
@@ -591,7 +592,7 @@ __device__ __forceinline__ const float* part_of(const Kv4Attn& a, int row_tiles,
 }
 
 // A block per (sequence, split of its tiles, kv head, NQ x 16 rows): its four waves take every fourth tile
-// with the next one's loads in flight, and their states are joined through LDS. PAIRS (prompts): the
+// with the next ones' loads in flight, and their states are joined through LDS. PAIRS (prompts): the
 // block takes the row tiles i and last - i, one after the other, so that every block has the same work
 // under the causal mask, all its tiles included (splits == 1).
 template <int D, int NQ, bool PAIRS>
@@ -601,7 +602,11 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) attn_kv4_kernel(Kv4Attn
     __shared__ float ms[4][16], ls[4][16];
     __shared__ uint32_t bs[4][16];
     static_assert(NQ == 1 || sizeof(os) >= NQ * (D / 32) * 1024, "the Q operands lie where the waves' sums go at the end");
-    constexpr bool kOnce = !PAIRS && NQ == 1, kRefill = NQ == 2 && D == 256;
+    constexpr bool kOnce = !PAIRS && NQ == 1, kTight = NQ == 2 && D == 256;
+    // tiles in registers: one of 256 dims (a second one's registers cost more than its loads in flight bring: 128
+    // lanes x 3 rows x 2000 slots 25.7 instead of 23.8 us), two smaller ones (64 lanes of 128 dims under a
+    // window 12.9 instead of 14.9 us)
+    constexpr int kAhead = D == 256 ? 1 : 2;
     const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63, nn = lane & 15, g = lane >> 4;
     const int tiles = PAIRS ? (row_tiles + 1) / 2 : row_tiles;
     const int h = blockIdx.x / tiles % a.kv_heads, z = blockIdx.x / (tiles * a.kv_heads), rt0 = blockIdx.x % tiles;
@@ -627,11 +632,14 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) attn_kv4_kernel(Kv4Attn
             return __builtin_bit_cast(q35_bf16x8, w);
         };
         auto at = [&](int i) { return i < tl.sink ? i : i - tl.sink + tl.main; };
-        Tile<D> cur;
+        Tile<D> buf[kAhead];
         const auto tile_at = [&](int i) { return region + (size_t)at(i) * kv4_tile_bytes(D); };
         if (t0 + wv < t1) {
-            load_k<D, kOnce>(cur, tile_at(t0 + wv), lo);
-            load_v<D, kOnce>(cur, tile_at(t0 + wv), lo);
+#pragma unroll
+            for (int b = 0; b < kAhead; ++b) {
+                load_k<D, kOnce>(buf[b], tile_at(min(t0 + wv + 4 * b, t1 - 1)), lo);
+                load_v<D, kOnce>(buf[b], tile_at(min(t0 + wv + 4 * b, t1 - 1)), lo);
+            }
         }
         q35_bf16x8 qf[NQ == 1 ? D / 32 : 1];
         q35_bf16x8* ql = (q35_bf16x8*)&os[0][0][0][0];
@@ -662,18 +670,17 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) attn_kv4_kernel(Kv4Attn
         }
         // tiles whose every slot every row of the block sees: from the last row's window to the first row's slot
         const int full0 = a.window > 0 ? max(pos + rho1 / group - a.window + 1, 0) : 0, full1 = pos + rho0 / group;
-        for (int i = __builtin_amdgcn_readfirstlane(t0 + wv); i < t1; i += 4) {
-            const int tile = at(i);
-            if (NQ > 1) asm volatile("" : "+v"(qlane));     // or the compiler reads Q ahead of the loop, and spills it
-            const uint8_t* next_p = tile_at(min(i + 4, t1 - 1));
-            Tile<D> next;
-            if (!kRefill) {
-                load_k<D, kOnce>(next, next_p, lo);
-                load_v<D, kOnce>(next, next_p, lo);
+        for (int i0 = __builtin_amdgcn_readfirstlane(t0 + wv); i0 < t1; i0 += 4 * kAhead) {
+#pragma unroll
+            for (int b = 0; b < kAhead; ++b) {
+                const int i = i0 + 4 * b;
+                if (i >= t1) break;
+                if (NQ > 1) asm volatile("" : "+v"(qlane));     // or the compiler reads Q ahead of the loop, and spills it
+                const int tile = at(i);
+                const bool edge = tile * 32 < full0 || tile * 32 + 31 > full1;
+                tile_step<D, NQ, kOnce, kTight>(buf[b], tile_at(i), tile_at(min(i + 4 * kAhead, t1 - 1)), lo, tile * 32, edge, q,
+                                                sight, scale2, st);
             }
-            const bool edge = tile * 32 < full0 || tile * 32 + 31 > full1;
-            tile_step<D, NQ, kRefill>(cur, tile_at(i), next_p, lo, tile * 32, edge, q, sight, scale2, st);
-            if (!kRefill) cur = next;
         }
         // The four waves' states: wave w ends a quarter of the row's dims, which the others pass it through
         // LDS; a lane keeps its row, and its accumulators go as they are.
@@ -825,10 +832,12 @@ template <int D>
 static hipError_t launch_attn(Kv4Attn& a, int n, hipStream_t st) {
     const int group = a.q_heads / a.kv_heads, rows = a.T * group, nq = rows > 16 ? 2 : 1;
     const int row_tiles = (rows + nq * 16 - 1) / (nq * 16), items = a.kv_heads * row_tiles;
-    // splits: enough blocks for two a CU, each of its four waves with two tiles at least
+    // splits: a block a CU (two a CU: 64 lanes under a window 15.6 instead of 12.9 us with the join, 100 lanes x 4096
+    // slots 50.6 instead of 45.7), each of its four waves with two tiles at least (four: 1 lane x 32768 slots
+    // 14.7 instead of 13.6)
     long long tiles = 0;
     for (int i = 0; i < n; ++i) tiles += tile_list(a.pos[i], a.pos[i] + a.T - 1, a.window, a.sinks).count;
-    const long long want = std::max<long long>(1, 512 / items);
+    const long long want = std::max<long long>(1, 256 / items);
     const int per = (int)std::max<long long>(8, (tiles + want - 1) / want);
     int z = 0;
     int most = 1;
