@@ -154,6 +154,15 @@ int q35_mtp_round_stop(q35_engine* e, q35_state* s, const int32_t* lanes, int n,
 int q35_mtp_verify(q35_engine* e, q35_state* s, const int32_t* lanes, int n, const int32_t* cur, int k,
                    const int32_t* drafts, int32_t stop, int32_t* emit, int32_t* n_emit, int64_t* stats);
 
+/* The verify half of a sampled round (no counterpart in the reference, whose rounds are greedy): the body, rollback
+ * and arguments of q35_mtp_verify, but the drafts are kept and the bonus drawn at `temperature` from the
+ * random numbers u [n][k + 1] (host, in [0, 1)) by q35_op_draft_verify's rule with drafts that the drafter is
+ * certain of, so every emitted token has the distribution softmax(logits / temperature); temperature 0 is
+ * q35_mtp_verify. An accepted draft equal to `stop` ends the accepted prefix and is emitted pending. */
+int q35_mtp_verify_sample(q35_engine* e, q35_state* s, const int32_t* lanes, int n, const int32_t* cur, int k,
+                          const int32_t* drafts, double temperature, const float* u, int32_t stop, int32_t* emit,
+                          int32_t* n_emit, int64_t* stats);
+
 /* Adaptive speculation depth (mtpadapt::Tracker, engine/mtp_adaptive.h:1-254): one policy per
  * request decides the depth of its next round -- 2, 1, or 0 (plain steps for the rest of the
  * request) -- from the tokens its own rounds emitted: the window estimate is emitted tokens per

@@ -123,6 +123,7 @@ struct q35_engine {
     float* kpart;
     float* kv4_part = nullptr;       // the 4-bit cache's attention: partial results of split rows
     double* verify_ws = nullptr;     // draft verification: the rows' chunk statistics
+    int *verify_io = nullptr, *h_verify_io = nullptr;   // sampled rounds: [drafts | u | accepted | tokens], R each
     uint16_t* prod;
     int *pidx, *tok_dev, *rlane, *rpos, *rslot, *rcur, *rwcur, *rpend, *ridx_src, *ridx_dst, *din = nullptr;
     int sc_ld = 0, max_chunks = 0;
@@ -402,6 +403,8 @@ void alloc_scratch(q35_engine* e) {
     e->topv_dev = dalloc<float>(R);
     e->kv4_part = dalloc<float>(kv4_part_floats());
     e->verify_ws = dalloc<double>(verify_ws_doubles((int)R));
+    e->verify_io = dalloc<int>(4 * R);
+    e->h_verify_io = halloc<int>(4 * R);
     e->gchunk = dalloc<float>(gdn_chunk_ws_floats(R));
     e->gcdec = dalloc<float>((size_t)((R + 63) / 64) * kHv);
     e->prod = dalloc<uint16_t>(R * kFF);
@@ -902,9 +905,9 @@ int q35_destroy(q35_engine* e) {
         e->graphs.clear();
         void* ds[] = {e->blob, e->x, e->h, e->delta, e->nrm, e->proj, e->gu, e->aout, e->cat, e->o, e->q,
                       e->sc, e->stats, e->part, e->pval, e->pidx, e->prod, e->din, e->inv_freq,
-                      e->logits_dev, e->kpart, e->gchunk, e->gcdec, e->topv_dev, e->kv4_part, e->verify_ws};
+                      e->logits_dev, e->kpart, e->gchunk, e->gcdec, e->topv_dev, e->kv4_part, e->verify_ws, e->verify_io};
         for (void* p : ds) if (p) hipFree(p);
-        void* hs[] = {e->hin, e->h_out};
+        void* hs[] = {e->hin, e->h_out, e->h_verify_io};
         for (void* p : hs) if (p) hipHostFree(p);
         noalloc_release(e->device, e);
         hipEventDestroy(e->ev0);
@@ -1585,9 +1588,12 @@ int q35_mtp_round(q35_engine* e, q35_state* s, const int32_t* lanes, int n, cons
 // 150-177; mtpaccept::accept_round, engine/mtp_accept.h:248): per lane, the (k+1)-row body
 // over [cur, d1..dk] with per-row GDN factors, accept of the longest prefix the target rows
 // confirm (the stop cut applied), then the state, window and MTP cache kept for rows 0..a.
+// sampling (nullable): instead of the greedy accept, drafts kept and the bonus drawn at its temperature from
+// its random numbers u [n][k + 1] (q35_op_draft_verify's rule, the drafter taken as certain of its drafts).
+struct Sampling { double temperature; const float* u; };
 static void mtp_verify_accept(q35_engine* e, q35_state* s, const std::vector<int>& ls, const std::vector<int>& P,
                    const int32_t* cur, int k, const std::vector<std::vector<int>>& drafts, int32_t stop,
-                   int32_t* emit, int32_t* n_emit, int64_t* stats) {
+                   int32_t* emit, int32_t* n_emit, int64_t* stats, const Sampling* sampling = nullptr) {
     const int n = (int)ls.size();
     // verify body over [cur, d1..dk] per lane with per-row GDN checkpoints
     HCK(hipStreamSynchronize(e->st));
@@ -1599,17 +1605,39 @@ static void mtp_verify_accept(q35_engine* e, q35_state* s, const std::vector<int
             e->h_lane[r] = ls[i]; e->h_pos[r] = P[i] + t; e->h_slot[r] = P[i] + t;
         }
     body(e, s, R, T, true);
-    lm_head(e, 0, R, false, !body_final_normed(e, R, T, true) ? e->final_norm : nullptr);
-    HCK(hipMemcpyAsync(e->h_out, e->tok_dev, R * sizeof(int), hipMemcpyDeviceToHost, e->st));
+    lm_head(e, 0, R, sampling != nullptr, !body_final_normed(e, R, T, true) ? e->final_norm : nullptr);
+    int *io = e->h_verify_io, *acc = io + 2 * (size_t)e->R, *tok = io + 3 * (size_t)e->R;
+    if (sampling) {
+        for (int i = 0; i < n; ++i) std::copy(drafts[i].begin(), drafts[i].end(), io + i * k);
+        std::memcpy(io + e->R, sampling->u, (size_t)R * sizeof(float));
+        HCK(hipMemcpyAsync(e->verify_io, io, 2 * (size_t)e->R * sizeof(int), hipMemcpyHostToDevice, e->st));
+        VerifyArgs v{};
+        v.logits = e->logits_dev; v.ld = kVocab; v.n = n; v.k = k; v.vocab = kVocab;
+        v.drafts = e->verify_io; v.u = (const float*)(e->verify_io + e->R);
+        v.accepted = e->verify_io + 2 * (size_t)e->R; v.tokens = e->verify_io + 3 * (size_t)e->R;
+        v.stats = e->verify_ws;
+        v.set_temperature(sampling->temperature);
+        HCK(launch_verify(v, e->st));
+        HCK(hipMemcpyAsync(acc, v.accepted, 2 * (size_t)e->R * sizeof(int), hipMemcpyDeviceToHost, e->st));
+    } else {
+        HCK(hipMemcpyAsync(e->h_out, e->tok_dev, R * sizeof(int), hipMemcpyDeviceToHost, e->st));
+    }
     HCK(hipStreamSynchronize(e->st));
+    if (sampling)
+        for (int i = 0; i < n; ++i)
+            REQ(tok[i * T + acc[i]] >= 0, Q35_ERR_STATE, "a verify row's logits have no distribution");
     std::vector<int> rows(n);
     for (int i = 0; i < n; ++i) {
         const int* tgt = e->h_out + i * T;
         int a = 0;
-        while (a < k && drafts[i][a] == tgt[a] && drafts[i][a] != stop) ++a;
+        if (sampling)
+            while (a < acc[i] && drafts[i][a] != stop) ++a;
+        else
+            while (a < k && drafts[i][a] == tgt[a] && drafts[i][a] != stop) ++a;
         int m = 0;
         for (int j = 0; j < a; ++j) emit[i * (k + 1) + m++] = drafts[i][j];
-        emit[i * (k + 1) + m++] = tgt[a];
+        // the token after the kept ones: with the stop cut in a sampled round, the kept stop draft itself
+        emit[i * (k + 1) + m++] = !sampling ? tgt[a] : a < acc[i] ? drafts[i][a] : tok[i * T + a];
         n_emit[i] = m;
         const int l = ls[i];
         s->prefix[l] = P[i] + a + 1;
@@ -1656,29 +1684,48 @@ int q35_mtp_round_stop(q35_engine* e, q35_state* s, const int32_t* lanes, int n,
 
 // The verify half of a round on drafts the caller made (mtpaccept::accept_round's candidates,
 // engine/mtp_accept.h:248): draft step j of lane i in drafts[i * k + j].
+static void mtp_verify(q35_engine* e, q35_state* s, const int32_t* lanes, int n, const int32_t* cur, int k,
+                       const int32_t* drafts, int32_t stop, int32_t* emit, int32_t* n_emit, int64_t* stats,
+                       const Sampling* sampling) {
+    REQ(e && s && cur && drafts && emit && n_emit, Q35_ERR_ARG, "null argument");
+    REQ(k >= 1 && k <= s->mtp_k, Q35_ERR_STATE, "k exceeds the state's MTP slots");
+    REQ(n > 0 && n * (k + 1) <= e->R, Q35_ERR_CAP, "rows exceed max_rows");
+    ++e->meta_epoch;
+    std::vector<int> ls(n), P(n);
+    std::vector<std::vector<int>> dr(n, std::vector<int>(k));
+    for (int i = 0; i < n; ++i) {
+        ls[i] = lanes ? lanes[i] : i;
+        check_lane(s, ls[i]);
+        check_tok(cur[i]);
+        for (int j = 0; j < i; ++j) REQ(ls[j] != ls[i], Q35_ERR_ARG, "duplicate lane in one round");
+        P[i] = s->prefix[ls[i]];
+        REQ(P[i] + k + 1 <= s->cap, Q35_ERR_CAP, "lane cache is full");
+        REQ(s->mtp_len[ls[i]] + k <= s->mtp_cap, Q35_ERR_CAP, "MTP cache is full");
+        for (int j = 0; j < k; ++j) {
+            check_tok(drafts[i * k + j]);
+            dr[i][j] = drafts[i * k + j];
+        }
+    }
+    mtp_verify_accept(e, s, ls, P, cur, k, dr, stop, emit, n_emit, stats, sampling);
+}
+
 int q35_mtp_verify(q35_engine* e, q35_state* s, const int32_t* lanes, int n, const int32_t* cur, int k,
                    const int32_t* drafts, int32_t stop, int32_t* emit, int32_t* n_emit, int64_t* stats) {
+    return guard([&] { mtp_verify(e, s, lanes, n, cur, k, drafts, stop, emit, n_emit, stats, nullptr); });
+}
+
+int q35_mtp_verify_sample(q35_engine* e, q35_state* s, const int32_t* lanes, int n, const int32_t* cur, int k,
+                          const int32_t* drafts, double temperature, const float* u, int32_t stop, int32_t* emit,
+                          int32_t* n_emit, int64_t* stats) {
     return guard([&] {
-        REQ(e && s && cur && drafts && emit && n_emit, Q35_ERR_ARG, "null argument");
+        REQ(e && s && u, Q35_ERR_ARG, "null argument");
+        REQ(verify_temperature_ok(temperature), Q35_ERR_ARG, "temperature is 0 or at least 0.001");
         REQ(k >= 1 && k <= s->mtp_k, Q35_ERR_STATE, "k exceeds the state's MTP slots");
-        REQ(n > 0 && n * (k + 1) <= e->R, Q35_ERR_CAP, "rows exceed max_rows");
-        ++e->meta_epoch;
-        std::vector<int> ls(n), P(n);
-        std::vector<std::vector<int>> dr(n, std::vector<int>(k));
-        for (int i = 0; i < n; ++i) {
-            ls[i] = lanes ? lanes[i] : i;
-            check_lane(s, ls[i]);
-            check_tok(cur[i]);
-            for (int j = 0; j < i; ++j) REQ(ls[j] != ls[i], Q35_ERR_ARG, "duplicate lane in one round");
-            P[i] = s->prefix[ls[i]];
-            REQ(P[i] + k + 1 <= s->cap, Q35_ERR_CAP, "lane cache is full");
-            REQ(s->mtp_len[ls[i]] + k <= s->mtp_cap, Q35_ERR_CAP, "MTP cache is full");
-            for (int j = 0; j < k; ++j) {
-                check_tok(drafts[i * k + j]);
-                dr[i][j] = drafts[i * k + j];
-            }
-        }
-        mtp_verify_accept(e, s, ls, P, cur, k, dr, stop, emit, n_emit, stats);
+        REQ(n > 0 && n <= e->R, Q35_ERR_CAP, "rows exceed max_rows");
+        for (long long i = 0; i < (long long)n * (k + 1); ++i)
+            REQ(u[i] >= 0.f && u[i] < 1.f, Q35_ERR_ARG, "random numbers lie in [0, 1)");
+        const Sampling smp{temperature, u};
+        mtp_verify(e, s, lanes, n, cur, k, drafts, stop, emit, n_emit, stats, &smp);
     });
 }
 

@@ -316,14 +316,11 @@ int q35_op_draft_verify(q35_engine* e, const q35_drafts* d, int n, int k, int vo
         REQ(d->dtype == 0 || d->dtype == 1, Q35_ERR_ARG, "dtype is 0 (float32) or 1 (bfloat16)");
         const uintptr_t el = d->dtype ? 2 : 4;
         REQ((uintptr_t)d->logits % el == 0 && (uintptr_t)d->draft_logits % el == 0, Q35_ERR_ARG, "misaligned logits");
-        REQ(d->temperature >= 0.0 && std::isfinite(d->temperature) &&
-                (d->temperature == 0.0 || d->temperature >= 1e-3), Q35_ERR_ARG, "temperature is 0 or at least 0.001");
+        REQ(verify_temperature_ok(d->temperature), Q35_ERR_ARG, "temperature is 0 or at least 0.001");
         VerifyArgs a{};
         a.logits = d->logits; a.draft_logits = d->temperature == 0.0 ? nullptr : d->draft_logits;
         a.ld = d->ld; a.ldd = d->draft_ld; a.bf16 = d->dtype; a.n = n; a.k = k; a.vocab = vocab;
-        a.inv_temp = d->temperature == 0.0 ? 0.0 : 1.0 / d->temperature;
-        a.scale.c = a.inv_temp * 1.4426950408889634074;
-        a.scale.low = a.inv_temp == 0.0 ? 0.0 : -1100.0 / a.scale.c;
+        a.set_temperature(d->temperature);
         a.drafts = d->drafts; a.u = d->u; a.accepted = accepted; a.tokens = tokens; a.stats = ev.verify_ws;
         OnDevice on(ev.device);
         HCK(launch_verify(a, ev.st));

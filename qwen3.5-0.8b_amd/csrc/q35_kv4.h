@@ -103,7 +103,13 @@ struct VerifyArgs {
     int *accepted, *tokens;              // [n], [n][k + 1]
     double* stats;                       // workspace
     int chunks, chunk;                   // a row's chunks and their elements (set by the launcher)
+    void set_temperature(double t) {
+        inv_temp = t == 0.0 ? 0.0 : 1.0 / t;
+        scale.c = inv_temp * 1.4426950408889634074;
+        scale.low = t == 0.0 ? 0.0 : -1100.0 / scale.c;
+    }
 };
+inline bool verify_temperature_ok(double t) { return t == 0.0 || (t >= 1e-3 && t <= 1e300); }
 constexpr int kVerifyDrafts = 8;
 size_t verify_ws_doubles(int max_rows);
 hipError_t launch_verify(VerifyArgs& a, hipStream_t st);

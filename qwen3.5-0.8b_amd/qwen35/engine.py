@@ -86,6 +86,8 @@ _SIGS = {
                            C.c_void_p], C.c_int),
     "q35_mtp_verify": ([C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_int32,
                         C.c_void_p, C.c_void_p, C.c_void_p], C.c_int),
+    "q35_mtp_verify_sample": ([C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_double,
+                               C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p], C.c_int),
     "q35_op_attn_decode": ([C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int]
                            + [C.c_void_p] * 4 + [C.c_int], C.c_int),
     "q35_op_lm_head_argmax": ([C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p], C.c_int),
@@ -498,6 +500,22 @@ class State:
         st = stats if stats is not None else np.zeros(4, np.int64)
         _ck(load_library().q35_mtp_verify(self.eng.h, self.h, _p(ln) if ln is not None else None, n, _p(c), k,
                                           _p(d), stop, _p(emit), _p(ne), _p(st)))
+        return [list(emit[i, :ne[i]]) for i in range(n)]
+
+    def mtp_verify_sample(self, cur, drafts, u, temperature: float, lanes=None, stats: np.ndarray | None = None,
+                          stop: int = -1):
+        """The verify half of a sampled round (q35_mtp_verify_sample): drafts [n][k] kept and the next token drawn at
+        `temperature` from the random numbers u [n][k + 1]; returns each lane's emitted tokens."""
+        c = _i32(cur)
+        d = np.ascontiguousarray(np.asarray(drafts, np.int32).reshape(c.size, -1))
+        n, k = d.shape
+        r = np.ascontiguousarray(np.asarray(u, np.float32).reshape(n, k + 1))
+        ln = _i32(lanes) if lanes is not None else None
+        emit = np.zeros((n, k + 1), np.int32)
+        ne = np.zeros(n, np.int32)
+        st = stats if stats is not None else np.zeros(4, np.int64)
+        _ck(load_library().q35_mtp_verify_sample(self.eng.h, self.h, _p(ln) if ln is not None else None, n, _p(c), k, _p(d),
+                                                 temperature, _p(r), stop, _p(emit), _p(ne), _p(st)))
         return [list(emit[i, :ne[i]]) for i in range(n)]
 
     def mtp_round(self, cur, k: int, lanes=None, stats: np.ndarray | None = None, stop: int = -1):
