@@ -397,3 +397,72 @@ def test_cache_reuse_and_two_caches(eng):
     c = KvCache4(e2, 1, 64)
     e2.close()
     c.close()
+
+
+@pytest.mark.parametrize("hq,kv,d,rot,window,sinks", [(8, 2, 256, 64, 0, 0), (8, 2, 256, 64, 24, 4), (12, 3, 128, 128, 40, 0),
+                                                      (4, 4, 64, 32, 16, 2)])
+def test_rounds_of_a_layer(eng, hq, kv, d, rot, window, sinks):
+    """Speculative rounds of one layer as a server runs them, nothing waited for within a round: prompts of several
+    lengths, then rounds of 3 rows a lane -- heads and append from the projection's rows where they lie,
+    attention with the rows' own gate, verification of drafts -- and the rejected rows dropped, so that
+    the next round's append lies on them. Every round's output against float64 on the cache read back."""
+    import torch
+    from qwen35 import KvCache4
+    rng, D, n, k, V = np.random.default_rng(d + window), Dev(), 4, 2, 5003
+    c = KvCache4(eng, n, 200, layers=2, kv_heads=kv, head_dim=d)
+    lens = np.array([1, 31, 64, 90], np.int32)
+    layer = 1
+
+    def layer_call(lanes, pos, T):
+        R = len(lanes) * T
+        h = Heads(rng, R, hq, kv, d)
+        x, qn, kn = D.up(h.x), D.up(h.qn), D.up(h.kn)
+        q, out = (torch.zeros(R, hq, d, dtype=torch.int16, device="cuda") for _ in range(2))
+        torch.cuda.synchronize()
+        p = x.data_ptr()
+        v, vv = h.views(p)
+        eng.op_kv4_append(c, layer, lanes, pos, T, hq, rot_dim=rot, theta=1e7, eps=1e-6, q_norm=qn.data_ptr(),
+                          k_norm=kn.data_ptr(), v=vv, q_out=(q.data_ptr(), hq * d, d), **v)
+        eng.op_attn_kv4(c, layer, lanes, pos, T, hq, (q.data_ptr(), hq * d, d), (out.data_ptr(), hq * d, d), window=window,
+                        sinks=sinks, gate=(p + 2 * d, h.width, 2 * d))
+        return h, x, qn, kn, q, out
+
+    def check(lanes, pos, T, h, q, out):
+        gate = ref.val(h.x)[:, :2 * hq * d].reshape(-1, hq, 2 * d)[..., d:]
+        for i, (l, p) in enumerate(zip(lanes, pos)):
+            kc, ks, vc, vs = read_cache(eng, c, layer, l, 1, 0, p + T)
+            K, Vv = ref.values(kc, ks)[0], ref.values(vc, vs)[0]
+            r = slice(i * T, (i + 1) * T)
+            o, pv, big = ref.attention(ref.val(D.bits(q)[r]), K, Vv, p, window, sinks, d ** -0.5)
+            want, e = ref.attention_bound(o, pv, big, p + T, d, gate[r])
+            assert np.all(np.abs(ref.val(D.bits(out)[r]) - want) <= e), (l, p)
+
+    for l in range(n):                       # prompts, a lane at a time
+        call = layer_call([l], [0], int(lens[l]))
+        eng.sync()
+        check([l], [0], int(lens[l]), call[0], call[4], call[5])
+    taken = set()
+    for r in range(4):
+        print(f"rounds {hq} {kv} {d} {window} {sinks}: round {r} at {lens.tolist()}", flush=True)
+        lanes = rng.permutation(n).astype(np.int32)
+        pos = lens[lanes]
+        call = layer_call(lanes, pos, k + 1)
+        lg = torch.from_numpy(rng.standard_normal((n, k + 1, V)).astype(np.float32)).cuda()
+        lg[:, :, 7] = 9.0                    # about half of the probability
+        dr = torch.where(torch.from_numpy(rng.random((n, k)) < 0.6).cuda(), 7, 8).int()
+        u = torch.from_numpy(rng.random((n, k + 1)).astype(np.float32)).cuda()
+        acc, tok = torch.zeros(n, dtype=torch.int32, device="cuda"), torch.zeros(n, k + 1, dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        eng.op_draft_verify(n, k, V, lg.data_ptr(), dr.data_ptr(), u.data_ptr(), acc.data_ptr(), tok.data_ptr())
+        eng.sync()
+        check(lanes, pos, k + 1, call[0], call[4], call[5])
+        a = acc.cpu().numpy()
+        for i in range(n):
+            aa, w, border, near = ref.verify(lg[i].double().cpu().numpy(), dr[i].cpu().numpy(), u[i].double().cpu().numpy(), 1.0)
+            assert near > 1e-9 and a[i] == aa and ref.token_ok(int(tok[i, aa]), w, border)
+        lens[lanes] = pos + a + 1
+        c.set_len(lanes, lens[lanes])
+        taken |= set(a.tolist())
+        assert [c.length(layer, l) for l in range(n)] == lens.tolist() and c.length(0, 1) == int(lens[1])
+    assert len(taken) > 1                    # some rounds dropped rows, some fewer
+    c.close()
