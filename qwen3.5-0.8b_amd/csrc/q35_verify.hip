@@ -178,31 +178,35 @@ __global__ void __launch_bounds__(256) verify_stats(VerifyArgs a) {
     if (threadIdx.x == 0) *out = {(double)m, (sm[0] + sm[1]) + (sm[2] + sm[3])};
 }
 
-// A row's maximum and sum from its chunks', by one wave; greedy: the maximum and its lowest index.
+// A row's maximum and sum from its chunks' (chunk i * 64 + lane in v[i]), by one wave; greedy: the maximum
+// and its lowest index.
 constexpr int kMaxChunks = 512;
-__device__ __forceinline__ Stat row_stat(const VerifyArgs& a, const Stat* st, const Scale& sc) {
-    const int lane = threadIdx.x & 63;
-    Stat v[kMaxChunks / 64];
+template <int N>
+__device__ __forceinline__ void load_stats(const VerifyArgs& a, const Stat* st, Stat* v) {
 #pragma unroll
-    for (int i = 0; i < kMaxChunks / 64; ++i) {
+    for (int i = 0; i < N; ++i) {
+        const int c = i * 64 + (threadIdx.x & 63);
         v[i] = {-INFINITY, 0.0};
-        if (i * 64 + lane < a.chunks) v[i] = st[i * 64 + lane];
+        if (c < a.chunks) v[i] = st[c];
     }
+}
+template <int N>
+__device__ __forceinline__ Stat row_stat(const VerifyArgs& a, const Stat* v, const Scale& sc) {
     double m = -INFINITY;
     bool nan = false;
 #pragma unroll
-    for (int i = 0; i < kMaxChunks / 64; ++i) { m = fmax(m, v[i].m); nan |= v[i].m != v[i].m; }
+    for (int i = 0; i < N; ++i) { m = fmax(m, v[i].m); nan |= v[i].m != v[i].m; }
     m = wmax(m);
     if (__any(nan)) m = __longlong_as_double(0x7ff8000000000000ll);
     double s = 0.0;
     if (a.inv_temp == 0.0) {
         s = 2147483647.0;
 #pragma unroll
-        for (int i = 0; i < kMaxChunks / 64; ++i) if (v[i].m == m) s = fmin(s, v[i].s);
+        for (int i = 0; i < N; ++i) if (v[i].m == m) s = fmin(s, v[i].s);
         s = -wmax(-s);
     } else {
 #pragma unroll
-        for (int i = 0; i < kMaxChunks / 64; ++i) if (v[i].s > 0.0) s += v[i].s * power(v[i].m - m, sc);
+        for (int i = 0; i < N; ++i) if (v[i].s > 0.0) s += v[i].s * power(v[i].m - m, sc);
         s = wsum(s);
     }
     return {m, s};
@@ -212,14 +216,17 @@ __device__ __forceinline__ bool has_dist(const Stat& s) { return s.m > -INFINITY
 
 // What becomes of a lane: its accepted drafts, and where its token comes from.
 enum { kFromTarget = 0, kNotDraft = 1, kRest = 2, kNoToken = 3, kArgmax = 4 };
-struct Fate { int accepted, kind, draft; };
+struct Fate {
+    int accepted, kind, draft;
+    Stat p, q;                       // of target row `accepted`; of its draft row (kRest)
+};
 
 // All waves make the lane's row statistics into rs (row order of row_of), k threads the drafts' probabilities
 // into pq; then every thread decides alike.
 struct Draft { int id; double p, q; };
-template <bool BF16>
-__device__ __forceinline__ Fate decide(const VerifyArgs& a, int ln, const Scale& sc, Stat* rs, Draft* pq) {
-    const int wv = threadIdx.x >> 6, nw = blockDim.x >> 6, tid = threadIdx.x;
+template <bool BF16, int WAVES>
+__device__ __forceinline__ Fate decide_kind(const VerifyArgs& a, int ln, const Scale& sc, Stat* rs, Draft* pq) {
+    const int wv = threadIdx.x >> 6, tid = threadIdx.x;
     const bool greedy = a.inv_temp == 0.0;
     Draft d = {-1, 0.0, 1.0};
     float lp = -INFINITY, lq = -INFINITY;
@@ -230,9 +237,25 @@ __device__ __forceinline__ Fate decide(const VerifyArgs& a, int ln, const Scale&
             if (a.draft_logits) lq = logit<BF16>(row_of<BF16>(a, ln, a.k + 1 + tid), d.id);
         }
     }
-    for (int j = wv; j < rows_of(a); j += nw) {
-        const Stat s = row_stat(a, stats_of(a, ln, j), sc);
-        if ((tid & 63) == 0) rs[j] = s;
+    if (a.chunks <= 64) {                    // a wave's rows in flight together
+        constexpr int kMine = (2 * kVerifyDrafts + 1 + WAVES - 1) / WAVES;
+        Stat v[kMine];
+#pragma unroll
+        for (int i = 0; i < kMine; ++i)
+            if (wv + i * WAVES < rows_of(a)) load_stats<1>(a, stats_of(a, ln, wv + i * WAVES), v + i);
+#pragma unroll
+        for (int i = 0; i < kMine; ++i)
+            if (wv + i * WAVES < rows_of(a)) {
+                const Stat s = row_stat<1>(a, v + i, sc);
+                if ((tid & 63) == 0) rs[wv + i * WAVES] = s;
+            }
+    } else {
+        for (int j = wv; j < rows_of(a); j += WAVES) {
+            Stat v[kMaxChunks / 64];
+            load_stats<kMaxChunks / 64>(a, stats_of(a, ln, j), v);
+            const Stat s = row_stat<kMaxChunks / 64>(a, v, sc);
+            if ((tid & 63) == 0) rs[j] = s;
+        }
     }
     __syncthreads();
     if (tid < a.k) {
@@ -249,17 +272,24 @@ __device__ __forceinline__ Fate decide(const VerifyArgs& a, int ln, const Scale&
     for (int j = 0; j < a.k; ++j) {
         const int t = pq[j].id;
         const bool dist = has_dist(rs[j]);
-        if (t < 0) return {j, !dist ? kNoToken : greedy ? kArgmax : kFromTarget, -1};
+        if (t < 0) return {j, !dist ? kNoToken : greedy ? kArgmax : kFromTarget, -1, {}, {}};
         if (greedy) {
             if (dist && (double)t == rs[j].s) continue;
-            return {j, dist ? kArgmax : kNoToken, t};
+            return {j, dist ? kArgmax : kNoToken, t, {}, {}};
         }
         const bool qd = !a.draft_logits || has_dist(rs[a.k + 1 + j]);
         if (qd && (double)u[j] * pq[j].q < pq[j].p) continue;
         const int from = a.draft_logits ? kRest : kNotDraft;
-        return {j, !dist ? kNoToken : qd && (a.draft_logits || t < a.vocab) ? from : kFromTarget, t};
+        return {j, !dist ? kNoToken : qd && (a.draft_logits || t < a.vocab) ? from : kFromTarget, t, {}, {}};
     }
-    return {a.k, !has_dist(rs[a.k]) ? kNoToken : greedy ? kArgmax : kFromTarget, -1};
+    return {a.k, !has_dist(rs[a.k]) ? kNoToken : greedy ? kArgmax : kFromTarget, -1, {}, {}};
+}
+template <bool BF16, int WAVES>
+__device__ __forceinline__ Fate decide(const VerifyArgs& a, int ln, const Scale& sc, Stat* rs, Draft* pq) {
+    Fate f = decide_kind<BF16, WAVES>(a, ln, sc, rs, pq);
+    f.p = rs[f.accepted];
+    if (f.kind == kRest) f.q = rs[a.k + 1 + f.accepted];
+    return f;
 }
 
 // The weight of token i of the lane's row: p up to a factor, without the draft, or max(p - q, 0).
@@ -269,15 +299,15 @@ struct Weights {
     Scale sc;
     double pm, qm, pz, qz;           // maxima, 1 / sums (kRest)
     int kind, draft, vocab;
-    __device__ __forceinline__ Weights(const VerifyArgs& a, int ln, const Fate& ft, const Scale& sc_, const Stat* rs)
+    __device__ __forceinline__ Weights(const VerifyArgs& a, int ln, const Fate& ft, const Scale& sc_)
         : sc(sc_), kind(ft.kind), draft(ft.draft), vocab(a.vocab) {
         pr = row_of<BF16>(a, ln, ft.accepted);
-        pm = rs[ft.accepted].m;
-        pz = 1.0 / rs[ft.accepted].s;
+        pm = ft.p.m;
+        pz = 1.0 / ft.p.s;
         if (kind == kRest) {
             qr = row_of<BF16>(a, ln, a.k + 1 + ft.accepted);
-            qm = rs[a.k + 1 + ft.accepted].m;
-            qz = 1.0 / rs[a.k + 1 + ft.accepted].s;
+            qm = ft.q.m;
+            qz = 1.0 / ft.q.s;
         }
     }
     // of N tokens from i on; 0 past the vocabulary
@@ -301,17 +331,19 @@ struct Weights {
     }
 };
 
-// The chunks' sums of max(p - q, 0), for the lanes that draw from it: a block per (chunk, lane).
+// With a drafter's probabilities: the lanes' decisions, kept for verify_token, and the chunks' sums of max(p - q, 0)
+// for those that draw from it. A block per (chunk, lane).
 template <bool BF16>
-__global__ void __launch_bounds__(256) verify_rest(VerifyArgs a, double* rest) {
+__global__ void __launch_bounds__(256) verify_rest(VerifyArgs a, double* rest, Fate* fates) {
     __shared__ Stat rs[2 * kVerifyDrafts + 1];
     __shared__ Draft pq[kVerifyDrafts];
     __shared__ double sm[4];
     const int c = blockIdx.x % a.chunks, ln = blockIdx.x / a.chunks;
     const Scale sc = a.scale;
-    const Fate ft = decide<BF16>(a, ln, sc, rs, pq);
+    const Fate ft = decide<BF16, 4>(a, ln, sc, rs, pq);
+    if (c == 0 && threadIdx.x == 0) fates[ln] = ft;
     if (ft.kind != kRest) return;
-    const Weights<BF16> wt(a, ln, ft, sc, rs);
+    const Weights<BF16> wt(a, ln, ft, sc);
     double s = 0.0;
     for (int i = c * a.chunk + (int)threadIdx.x * 8; i < min((c + 1) * a.chunk, a.vocab); i += 2048) {
         double w[8];
@@ -351,18 +383,18 @@ __device__ __forceinline__ int2 block_ends(int first, int last, int2* ends) {
 
 // A block per lane: the decision, the chunk that holds the border, the token in it.
 template <bool BF16>
-__global__ void __launch_bounds__(1024) verify_token(VerifyArgs a, const double* rest) {
+__global__ void __launch_bounds__(1024) verify_token(VerifyArgs a, const double* rest, const Fate* fates) {
     __shared__ Stat rs[2 * kVerifyDrafts + 1];
     __shared__ Draft pq[kVerifyDrafts];
     __shared__ double part[16], total, base;
     __shared__ int2 ends[16];
     const int ln = blockIdx.x, tid = threadIdx.x;
     const Scale sc = a.scale;
-    const Fate ft = decide<BF16>(a, ln, sc, rs, pq);
+    const Fate ft = a.draft_logits ? fates[ln] : decide<BF16, 16>(a, ln, sc, rs, pq);
     int token = -1;
-    if (ft.kind == kArgmax) token = (int)rs[ft.accepted].s;
+    if (ft.kind == kArgmax) token = (int)ft.p.s;
     if (ft.kind < kNoToken) {
-        Weights<BF16> wt(a, ln, ft, sc, rs);
+        Weights<BF16> wt(a, ln, ft, sc);
         int pick = -1;
         double border = 0.0;
         for (int pass = 0; pass < 2 && pick < 0; ++pass) {
@@ -419,7 +451,7 @@ __global__ void __launch_bounds__(1024) verify_token(VerifyArgs a, const double*
         }
     }
     if (tid == 0) a.accepted[ln] = ft.accepted;
-    if (tid <= a.k) a.tokens[(size_t)ln * (a.k + 1) + tid] = tid < ft.accepted ? pq[tid].id : tid == ft.accepted ? token : -1;
+    if (tid <= a.k) a.tokens[(size_t)ln * (a.k + 1) + tid] = tid < ft.accepted ? a.drafts[(size_t)ln * a.k + tid] : tid == ft.accepted ? token : -1;
 }
 
 // Chunks of 8192 logits, fewer while the rows are too few to fill the card with them (2048 is the
@@ -430,10 +462,11 @@ static int chunk_of(long long rows, int vocab) {
     return chunk;
 }
 size_t verify_ws_doubles(int max_rows) {
+    // (chunk sums of the rows, of the lanes, the lanes' decisions)
     // 2 max_rows rows of up to 128 chunks of 8192, or fewer rows of smaller chunks: under 1024 chunks
     // at twice their size, so at most 2048 and one more a row
     const size_t rows = 2 * (size_t)max_rows;
-    return 2 * (rows * 128 + 2048 + rows) + (rows * 128 + 2048 + rows);
+    return 2 * (rows * 128 + 2048 + rows) + (rows * 128 + 2048 + rows) + sizeof(Fate) / 8 * (size_t)max_rows;
 }
 
 template <bool BF16>
@@ -442,6 +475,7 @@ static hipError_t launch_v(VerifyArgs& a, hipStream_t st) {
     a.chunk = chunk_of((long long)a.n * per, a.vocab);
     a.chunks = (a.vocab + a.chunk - 1) / a.chunk;
     double* rest = a.stats + 2 * (size_t)a.n * per * a.chunks;
+    Fate* fates = (Fate*)(rest + (size_t)a.n * a.chunks);
     const dim3 grid((unsigned)a.chunks * a.n * per);
     constexpr int N = BF16 ? 8 : 4;
     if (a.chunk == 8192) hipLaunchKernelGGL((verify_stats<BF16, 32 / N>), grid, dim3(256), 0, st, a);
@@ -450,10 +484,10 @@ static hipError_t launch_v(VerifyArgs& a, hipStream_t st) {
     hipError_t rc = hipGetLastError();
     if (rc != hipSuccess) return rc;
     if (a.draft_logits && a.inv_temp != 0.0) {
-        hipLaunchKernelGGL(verify_rest<BF16>, dim3((unsigned)a.chunks * a.n), dim3(256), 0, st, a, rest);
+        hipLaunchKernelGGL(verify_rest<BF16>, dim3((unsigned)a.chunks * a.n), dim3(256), 0, st, a, rest, fates);
         if ((rc = hipGetLastError()) != hipSuccess) return rc;
     }
-    hipLaunchKernelGGL(verify_token<BF16>, dim3(a.n), dim3(1024), 0, st, a, (const double*)rest);
+    hipLaunchKernelGGL(verify_token<BF16>, dim3(a.n), dim3(1024), 0, st, a, (const double*)rest, (const Fate*)fates);
     return hipGetLastError();
 }
 hipError_t launch_verify(VerifyArgs& a, hipStream_t st) { return a.bf16 ? launch_v<true>(a, st) : launch_v<false>(a, st); }

@@ -141,8 +141,13 @@ def _p(a: np.ndarray):
     return a.ctypes.data_as(C.c_void_p)
 
 
-def _addr(a: np.ndarray) -> int:
-    return a.__array_interface__["data"][0]
+def _addr(a: np.ndarray):
+    """Pointer to an int32 array, for a call that keeps it alive (numpy's own ways to the address take four times
+    as long; they remain for arrays that are empty or not writable)."""
+    try:
+        return C.byref(C.c_int32.from_buffer(a))
+    except (TypeError, ValueError):
+        return _p(a)
 
 
 def _lp(lanes: np.ndarray | None, pos: np.ndarray):
