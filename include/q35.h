@@ -269,8 +269,8 @@ int q35_kv4_set_len(q35_engine* e, q35_kv4* c, const int32_t* lanes, const int32
 int q35_kv4_len(q35_engine* e, q35_kv4* c, int layer, int lane, int32_t* out);
 /* Slots [slot0, slot0 + n_slots) of lanes [lane0, lane0 + n_lanes) from / to device buffers in row order: codes
  * [n_lanes][kv_heads][n_slots][head_dim / 2], two codes a byte, the lower dim in the low nibble;
- * scales [n_lanes][kv_heads][n_slots][head_dim / 32]. A write starts at most at a lane's length
- * and raises it to slot0 + n_slots; a read stays below it. */
+ * scales [n_lanes][kv_heads][n_slots][head_dim / 32] (a scale byte above 252 is stored as 255, NaN). A write
+ * starts at most at a lane's length and raises it to slot0 + n_slots; a read stays below it. */
 int q35_kv4_write(q35_engine* e, q35_kv4* c, int layer, int lane0, int n_lanes, int slot0, int n_slots,
                   const uint8_t* k_codes, const uint8_t* k_scales, const uint8_t* v_codes, const uint8_t* v_scales);
 int q35_kv4_read(q35_engine* e, q35_kv4* c, int layer, int lane0, int n_lanes, int slot0, int n_slots, uint8_t* k_codes,

@@ -246,9 +246,9 @@ __global__ void __launch_bounds__(256) heads_kernel(HeadArgs a, int rows, int pe
 
 hipError_t launch_heads(HeadArgs& a, int n, hipStream_t st) {
     const int rows = n * a.T, kinds = a.v.p ? 2 : 1;
-    // rows of a block: one while they are too few to give every CU four blocks, else up to four; of very few
+    // rows of a block: one while they are too few to give every CU two blocks of two, else up to four; of very few
     // rows with many heads, four wave items (one a wave) in a block
-    const int per_block = rows >= 4096 ? kBlockRows : rows >= 2048 ? 2 : 1;
+    const int per_block = rows >= 4096 ? kBlockRows : rows >= 1024 ? 2 : 1;
     const int items = ((a.q.p ? per_block * a.q_heads + 3 : 0) / 4) + kinds * ((per_block * a.kv_heads + 3) / 4);
     const int some = rows < 256 ? std::min(items, 4) : items, parts = (items + some - 1) / some;
     const long long blocks = (long long)((rows + per_block - 1) / per_block) * parts;
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(256) kv4_copy_kernel(Kv4Copy a) {
         if (d % 32 == 0) {
             uint8_t* c = tile + (v ? kv4_v_scale(a.D, tk, d / 32) : kv4_k_scale(a.D, tk, d / 32));
             uint8_t* o = (v ? a.vs : a.ks) + row * (a.D / 32) + d / 32;
-            if (WRITE) *c = *o;
+            if (WRITE) *c = *o > 252 ? 255 : *o;     // (2^126 and up: past bf16)
             else *o = *c;
         }
     }

@@ -381,6 +381,32 @@ def test_attention_row_is_its_own(eng):
     f.c.close()
 
 
+def test_write_any_bytes(eng):
+    """Codes are stored as they are, scale bytes up to 252 too and larger ones as 255; attention over
+    the largest and the smallest scales behind the rows that see none of them stays finite."""
+    import torch
+    from qwen35 import KvCache4
+    rng = np.random.default_rng(14)
+    c = KvCache4(eng, 1, 300, kv_heads=1, head_dim=64)
+    kc, vc = (rng.integers(0, 256, (1, 1, 300, 32)).astype(np.uint8) for _ in range(2))
+    ks, vs = (np.full((1, 1, 300, 2), 126, np.uint8) for _ in range(2))
+    ks[0, 0, 40:296, 0], vs[0, 0, 40:296, 1] = np.arange(256), np.arange(256)[::-1]
+    t = [torch.from_numpy(a).cuda() for a in (kc, ks, vc, vs)]
+    torch.cuda.synchronize()
+    c.write(0, 0, 1, 0, 300, *[x.data_ptr() for x in t])
+    eng.sync()
+    back = read_cache(eng, c, 0, 0, 1, 0, 300)
+    ks[ks > 252], vs[vs > 252] = 255, 255
+    assert all(np.array_equal(a, b) for a, b in zip(back, (kc, ks, vc, vs)))
+    f = Filled.__new__(Filled)
+    f.c, f.K, f.V = c, ref.values(kc, ks), ref.values(vc, vs)
+    for pos, T, window in [([37], 3, 0), ([298], 2, 3), ([36], 4, 7)]:
+        got, q, g = run_attention(eng, f, [0], pos, T, 4, rng, window)
+        check_attention(f, [0], pos, T, got, q, g, window)
+        assert np.isfinite(ref.val(got)).all()
+    c.close()
+
+
 def test_cache_reuse_and_two_caches(eng):
     """set_len starts a lane over on old contents; two caches of other shapes share the engine's
     workspace in one stream; a closed engine's cache can still be closed."""
