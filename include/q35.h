@@ -304,9 +304,9 @@ int q35_op_kv4_append(q35_engine* e, q35_kv4* c, int layer, const int32_t* lanes
 /* Attention over the cache: row i * T + t of q (normed and rotated, q_heads a multiple of kv_heads, query
  * head h on kv head h / (q_heads / kv_heads)) sees slots (p - window, p] and [0, sinks) of lane
  * lanes[i], p = pos[i] + t; window 0: [0, p]. The lane must hold pos[i] + T slots, the rows' own included;
- * a lane may occur more than once. out = softmax(scale * q K^T) V, times sigmoid(gate) if gate is given, in
- * float32 with the weights rounded to bf16 for the product with V, and one rounding to bf16. A NaN in
- * a slot reaches the rows that see it and no others. */
+ * a lane may occur more than once; scale * log2(e) is finite in float32. out = softmax(scale * q K^T) V,
+ * times sigmoid(gate) if gate is given, in float32 with the weights rounded to bf16 for the product with V,
+ * and one rounding to bf16. A NaN in a slot reaches the rows that see it and no others. */
 int q35_op_attn_kv4(q35_engine* e, q35_kv4* c, int layer, const int32_t* lanes, const int32_t* pos, int n, int T,
                     int q_heads, const q35_view* q, const q35_view* gate, float scale, int window, int sinks,
                     const q35_view* out);

@@ -67,6 +67,7 @@ void check_out(const HeadView& v, int heads, int rows, int D, const char* what) 
 void check_seqs(q35_kv4* c, int layer, const int32_t* lanes, const int32_t* pos, int n, int T, bool append) {
     REQ(layer >= 0 && layer < c->layers, Q35_ERR_ARG, "layer out of range");
     REQ(n > 0 && T > 0 && pos, Q35_ERR_ARG, "bad sequence count, row count or positions");
+    REQ((long long)n * T <= INT32_MAX, Q35_ERR_ARG, "bad sequence or row count");
     std::vector<char> seen(append ? c->lanes : 0, 0);
     for (int i = 0; i < n; ++i) {
         const int l = lanes ? lanes[i] : i;
@@ -280,7 +281,7 @@ int q35_op_attn_kv4(q35_engine* e, q35_kv4* c, int layer, const int32_t* lanes, 
             "q_heads must be a multiple of the cache's kv_heads");
         REQ(window >= 0 && sinks >= 0, Q35_ERR_ARG, "window and sinks must not be negative");
         REQ(window > 0 || sinks == 0, Q35_ERR_ARG, "sinks go with a window");
-        REQ(std::isfinite(scale), Q35_ERR_ARG, "scale must be finite");
+        REQ(std::isfinite(scale * 1.44269504f), Q35_ERR_ARG, "scale must be finite, times log2(e) too");
         Kv4Attn a{};
         a.q = view(*q, "q");
         a.out = view(*out, "out");

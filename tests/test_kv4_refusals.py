@@ -233,3 +233,24 @@ def test_lane_and_position_counts_must_match():
     from qwen35.engine import _i32, _lp
     with pytest.raises(ValueError):
         _lp(_i32([0, 1]), _i32([0]))
+
+
+def test_attention_numbers_past_their_types(lib):
+    """Rows past 2^31 in all, and a scale that overflows where the kernel takes it to base 2."""
+    from qwen35.engine import _VIEW
+    e, c = C.c_void_p(lib.stub_engine()), C.c_void_p()
+    assert lib.q35_kv4_alloc(e, 1, 1, 4096, 1, 64, C.byref(c)) == 0
+    full = np.array([4096], np.int32)
+    assert lib.q35_kv4_set_len(e, c, None, full.ctypes.data, 1) == 0
+    z = np.zeros(1 << 20, np.int32)
+
+    def call(n, T, scale):
+        return lib.q35_op_attn_kv4(e, c, 0, z.ctypes.data, z.ctypes.data, n, T, 1, _VIEW.pack(1 << 16, 64, 64), None, scale, 0, 0,
+                                   _VIEW.pack(1 << 17, 64, 64))
+
+    assert call(1 << 20, 4096, 1.0) == ARG and "row count" in lib.q35_last_error().decode()
+    assert call(1 << 19, 4096, 1.0) == ARG
+    assert call(1, 4096, 3e38) == ARG and "scale" in lib.q35_last_error().decode()
+    assert lib.stub_launches(e) == 0
+    assert call(1, 4096, 2e38) == 0 and lib.stub_launches(e) == 1
+    assert lib.q35_kv4_free(e, c) == 0
