@@ -39,6 +39,23 @@ __device__ __forceinline__ double power(double d, const Scale& sc) {
     return __builtin_ldexp(p, (int)(uint32_t)__builtin_bit_cast(unsigned long long, t));
 }
 
+// The same added to s, for sums whose largest term is 1: t[i] = 2^(i / 64) (LDS), and 2^f for the rest, |f| <= 1/128, by
+// a fourth degree (interpolated likewise; under 5e-15). Exponents end at -990, so the power goes into the bits.
+__device__ __forceinline__ void add_power(double& s, double d, const Scale& sc, double low, const double* t) {
+    d = fmax(d, low);
+    const double w = __builtin_fma(d, sc.c, 105553116266496.0), k = w - 105553116266496.0;   // whole 64ths
+    const double f = __builtin_fma(d, sc.c, -k);
+    const int n = (int)(uint32_t)__builtin_bit_cast(unsigned long long, w);
+    unsigned long long b = __builtin_bit_cast(unsigned long long, t[n & 63]);
+    b += (unsigned long long)(((uint32_t)n & ~63u) << 14) << 32;
+    double p = 0.009618140859595685;
+    p = __builtin_fma(p, f, 0.05550421039186821);
+    p = __builtin_fma(p, f, 0.2402265069589214);
+    p = __builtin_fma(p, f, 0.6931471805583931);
+    p = __builtin_fma(p, f, 1.0);
+    s = __builtin_fma(__builtin_bit_cast(double, b), p, s);
+}
+
 constexpr int kMaxChunk = 8192;
 struct Stat { double m, s; };        // a chunk's largest logit, and the sum of 2^((l - m) c); greedy: its index
 
@@ -128,6 +145,7 @@ __global__ void __launch_bounds__(256) verify_stats(VerifyArgs a) {
     __shared__ float mx[4];
     __shared__ double sm[4];
     __shared__ int at[4];
+    __shared__ double t[64];
     const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int c = blockIdx.x % a.chunks, rr = blockIdx.x / a.chunks, j = rr % rows_of(a), ln = rr / rows_of(a);
     const void* row = row_of<BF16>(a, ln, j);
@@ -139,6 +157,7 @@ __global__ void __launch_bounds__(256) verify_stats(VerifyArgs a) {
         if (i0 + a.chunk <= a.vocab) load_whole<BF16>(row, i, v[b]);
         else load_logits<BF16>(row, i, a.vocab, v[b]);
     }
+    if (threadIdx.x < 64) t[threadIdx.x] = exp2(threadIdx.x * (1.0 / 64));
     float m = -INFINITY;                 // (a NaN anywhere makes it one)
 #pragma unroll
     for (int b = 0; b < LOADS; ++b)
@@ -166,11 +185,11 @@ __global__ void __launch_bounds__(256) verify_stats(VerifyArgs a) {
     double s = 0.0;
     if (m > -INFINITY && m < INFINITY) {
         const Scale sc = a.scale;
-        const double md = m;
+        const double md = m, low = sc.low * 0.9;
 #pragma unroll
         for (int b = 0; b < LOADS; ++b)
 #pragma unroll
-            for (int e = 0; e < N; ++e) s += power((double)v[b][e] - md, sc);
+            for (int e = 0; e < N; ++e) add_power(s, (double)v[b][e] - md, sc, low, t);
     }
     s = wsum(s);
     if (lane == 0) sm[wv] = s;
