@@ -592,24 +592,28 @@ __device__ __forceinline__ const float* part_of(const Kv4Attn& a, int row_tiles,
 }
 
 // A block per (sequence, split of its tiles, kv head, NQ x 16 rows): its four waves take every fourth tile
-// with the next ones' loads in flight, and their states are joined through LDS. PAIRS (prompts): the
-// block takes the row tiles i and last - i, one after the other, so that every block has the same work
-// under the causal mask, all its tiles included (splits == 1).
-template <int D, int NQ, bool PAIRS>
+// with the next ones' loads in flight, and their states are joined through LDS. Under the causal mask the last
+// row tiles are the longest: they come first, so that the short ones fill the CUs' ends (4096 rows of 8 heads of
+// 256 in one prompt 96 us; each block with a long and a short tile in turn 100). One sequence of at most
+// two blocks a CU has them all at once: the second of a CU is then short where the first is long (2048 rows 35 us,
+// without 38, ascending 47).
+template <int D, int NQ>
 __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) attn_kv4_kernel(Kv4Attn a, int row_tiles) {
     constexpr int kQuarter = D / 64;         // of the D / 16 accumulators of 16 rows
     __shared__ f32x4 os[4][4][kQuarter][64];
     __shared__ float ms[4][16], ls[4][16];
     __shared__ uint32_t bs[4][16];
     static_assert(NQ == 1 || sizeof(os) >= NQ * (D / 32) * 1024, "the Q operands lie where the waves' sums go at the end");
-    constexpr bool kOnce = !PAIRS && NQ == 1, kTight = NQ == 2 && D == 256;
+    constexpr bool kOnce = NQ == 1, kTight = NQ == 2 && D == 256;
     // tiles in registers: one of 256 dims (a second one's registers cost more than its loads in flight bring: 128
     // lanes x 3 rows x 2000 slots 25.7 instead of 23.8 us), two smaller ones (64 lanes of 128 dims under a
     // window 12.9 instead of 14.9 us)
     constexpr int kAhead = D == 256 ? 1 : 2;
     const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63, nn = lane & 15, g = lane >> 4;
-    const int tiles = PAIRS ? (row_tiles + 1) / 2 : row_tiles;
-    const int h = blockIdx.x / tiles % a.kv_heads, z = blockIdx.x / (tiles * a.kv_heads), rt0 = blockIdx.x % tiles;
+    const int per_split = row_tiles * a.kv_heads, z = blockIdx.x / per_split;
+    int ix = blockIdx.x % per_split;
+    if (per_split == gridDim.x && per_split <= 512 && ix >= 256) ix = per_split - 1 - (ix - 256);
+    const int h = ix % a.kv_heads, rt = row_tiles - 1 - ix / a.kv_heads;
     const Seq sq = find_seq(a, z);
     const int seq = sq.i, splits = sq.splits, pos = sq.pos, group = a.q_heads / a.kv_heads, rows = a.T * group;
     const uint8_t* region = a.cache + sq.lane * a.lane_bytes + h * a.region;
@@ -617,131 +621,126 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) attn_kv4_kernel(Kv4Attn
     // scale's sign goes to q, 0 becomes the smallest normal number
     const float scale2 = fmaxf(fabsf(a.scale) * 1.44269504088896f, 1.17549435e-38f);
     const Lanes lo = lane_offsets<D>();
-    for (int pass = 0; pass < (PAIRS ? 2 : 1); ++pass) {
-        const int rt = pass ? rt0 : PAIRS ? row_tiles - 1 - rt0 : rt0, rho0 = rt * NQ * 16;
-        if (pass && rt == row_tiles - 1 - rt0) break;        // the middle one
-        const int rho1 = min(rho0 + NQ * 16, rows) - 1;
-        const TileList tl = tile_list(pos + rho0 / group, pos + rho1 / group, a.window, a.sinks);
-        const int t0 = (int)((long long)tl.count * sq.split / splits), t1 = (int)((long long)tl.count * (sq.split + 1) / splits);
-        const auto q_at = [&](int rho, int gg, int k) {
-            rho = min(rho, rows - 1);
-            const int t = rho / group;
-            u32x4 w = *(const u32x4*)(a.q.p + ((long long)seq * a.T + t) * a.q.row + (h * group + rho - t * group) * a.q.head +
-                                      gg * (D / 4) + 8 * k);
-            if (a.scale < 0.f) w ^= 0x80008000u;
-            return __builtin_bit_cast(q35_bf16x8, w);
-        };
-        auto at = [&](int i) { return i < tl.sink ? i : i - tl.sink + tl.main; };
-        Tile<D> buf[kAhead];
-        const auto tile_at = [&](int i) { return region + (size_t)at(i) * kv4_tile_bytes(D); };
-        if (t0 + wv < t1) {
+    const int rho0 = rt * NQ * 16, rho1 = min(rho0 + NQ * 16, rows) - 1;
+    const TileList tl = tile_list(pos + rho0 / group, pos + rho1 / group, a.window, a.sinks);
+    const int t0 = (int)((long long)tl.count * sq.split / splits), t1 = (int)((long long)tl.count * (sq.split + 1) / splits);
+    const auto q_at = [&](int rho, int gg, int k) {
+        rho = min(rho, rows - 1);
+        const int t = rho / group;
+        u32x4 w = *(const u32x4*)(a.q.p + ((long long)seq * a.T + t) * a.q.row + (h * group + rho - t * group) * a.q.head +
+                                  gg * (D / 4) + 8 * k);
+        if (a.scale < 0.f) w ^= 0x80008000u;
+        return __builtin_bit_cast(q35_bf16x8, w);
+    };
+    auto at = [&](int i) { return i < tl.sink ? i : i - tl.sink + tl.main; };
+    Tile<D> buf[kAhead];
+    const auto tile_at = [&](int i) { return region + (size_t)at(i) * kv4_tile_bytes(D); };
+    if (t0 + wv < t1) {
 #pragma unroll
-            for (int b = 0; b < kAhead; ++b) {
-                load_k<D, kOnce>(buf[b], tile_at(min(t0 + wv + 4 * b, t1 - 1)), lo);
-                load_v<D, kOnce>(buf[b], tile_at(min(t0 + wv + 4 * b, t1 - 1)), lo);
-            }
+        for (int b = 0; b < kAhead; ++b) {
+            load_k<D, kOnce>(buf[b], tile_at(min(t0 + wv + 4 * b, t1 - 1)), lo);
+            load_v<D, kOnce>(buf[b], tile_at(min(t0 + wv + 4 * b, t1 - 1)), lo);
         }
-        q35_bf16x8 qf[NQ == 1 ? D / 32 : 1];
-        q35_bf16x8* ql = (q35_bf16x8*)&os[0][0][0][0];
-        if constexpr (NQ == 1) {
+    }
+    q35_bf16x8 qf[NQ == 1 ? D / 32 : 1];
+    q35_bf16x8* ql = (q35_bf16x8*)&os[0][0][0][0];
+    if constexpr (NQ == 1) {
 #pragma unroll
-            for (int k = 0; k < D / 32; ++k) qf[k] = q_at(rho0 + nn, g, k);
-        } else {
-            if (pass) __syncthreads();
-            for (int i = tid; i < NQ * (D / 32) * 64; i += 256) {
-                const int ln = i & 63, k = i / 64 % (D / 32), c = i / (64 * (D / 32));
-                ql[i] = q_at(rho0 + c * 16 + (ln & 15), ln >> 4, k);
-            }
-            lds_barrier();
+        for (int k = 0; k < D / 32; ++k) qf[k] = q_at(rho0 + nn, g, k);
+    } else {
+        for (int i = tid; i < NQ * (D / 32) * 64; i += 256) {
+            const int ln = i & 63, k = i / 64 % (D / 32), c = i / (64 * (D / 32));
+            ql[i] = q_at(rho0 + c * 16 + (ln & 15), ln >> 4, k);
         }
-        int qlane = lane;
-        const auto q = [&](int c, int k) { return NQ == 1 ? qf[k] : ql[(c * (D / 32) + k) * 64 + qlane]; };
-        Sight sight[NQ];
-        Rows<D, NQ> st;
+        lds_barrier();
+    }
+    int qlane = lane;
+    const auto q = [&](int c, int k) { return NQ == 1 ? qf[k] : ql[(c * (D / 32) + k) * 64 + qlane]; };
+    Sight sight[NQ];
+    Rows<D, NQ> st;
 #pragma unroll
-        for (int c = 0; c < NQ; ++c) {
-            const int p = pos + min(rho0 + c * 16 + nn, rows - 1) / group;
-            sight[c] = {p, a.window > 0 ? p - a.window + 1 : 0, a.sinks};
-            st.m[c] = -INFINITY;
-            st.l[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-            st.bad[c] = 0;
+    for (int c = 0; c < NQ; ++c) {
+        const int p = pos + min(rho0 + c * 16 + nn, rows - 1) / group;
+        sight[c] = {p, a.window > 0 ? p - a.window + 1 : 0, a.sinks};
+        st.m[c] = -INFINITY;
+        st.l[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+        st.bad[c] = 0;
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) st.o[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < D / 16; ++i) st.o[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    // tiles whose every slot every row of the block sees: from the last row's window to the first row's slot
+    const int full0 = a.window > 0 ? max(pos + rho1 / group - a.window + 1, 0) : 0, full1 = pos + rho0 / group;
+    for (int i0 = __builtin_amdgcn_readfirstlane(t0 + wv); i0 < t1; i0 += 4 * kAhead) {
+#pragma unroll
+        for (int b = 0; b < kAhead; ++b) {
+            const int i = i0 + 4 * b;
+            if (i >= t1) break;
+            if (NQ > 1) asm volatile("" : "+v"(qlane));     // or the compiler reads Q ahead of the loop, and spills it
+            const int tile = at(i);
+            const bool edge = tile * 32 < full0 || tile * 32 + 31 > full1;
+            tile_step<D, NQ, kOnce, kTight>(buf[b], tile_at(i), tile_at(min(i + 4 * kAhead, t1 - 1)), lo, tile * 32, edge, q,
+                                            sight, scale2, st);
         }
-        // tiles whose every slot every row of the block sees: from the last row's window to the first row's slot
-        const int full0 = a.window > 0 ? max(pos + rho1 / group - a.window + 1, 0) : 0, full1 = pos + rho0 / group;
-        for (int i0 = __builtin_amdgcn_readfirstlane(t0 + wv); i0 < t1; i0 += 4 * kAhead) {
+    }
+    // The four waves' states: wave w ends a quarter of the row's dims, which the others pass it through
+    // LDS; a lane keeps its row, and its accumulators go as they are.
 #pragma unroll
-            for (int b = 0; b < kAhead; ++b) {
-                const int i = i0 + 4 * b;
-                if (i >= t1) break;
-                if (NQ > 1) asm volatile("" : "+v"(qlane));     // or the compiler reads Q ahead of the loop, and spills it
-                const int tile = at(i);
-                const bool edge = tile * 32 < full0 || tile * 32 + 31 > full1;
-                tile_step<D, NQ, kOnce, kTight>(buf[b], tile_at(i), tile_at(min(i + 4 * kAhead, t1 - 1)), lo, tile * 32, edge, q,
-                                                sight, scale2, st);
-            }
+    for (int c = 0; c < NQ; ++c) {
+        if (rho0 + c * 16 >= rows) break;
+        if (NQ > 1 || c) __syncthreads();        // os was read: Q, or the 16 rows before these
+        uint32_t bad = st.bad[c];
+        bad |= (uint32_t)__shfl_xor((int)bad, 16);
+        bad |= (uint32_t)__shfl_xor((int)bad, 32);
+        if (g == 0) { ms[wv][nn] = st.m[c]; ls[wv][nn] = st.l[c][0]; bs[wv][nn] = bad; }
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+            for (int i = 0; i < kQuarter; ++i)
+                if (w != wv) os[w][wv][i][lane] = st.o[c][w * kQuarter + i];
+        __syncthreads();
+        float m = st.m[c], sum = 0.f, f[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) m = fmaxf(m, ms[w][nn]);
+        bad = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            f[w] = __builtin_amdgcn_exp2f(ms[w][nn] - (m == -INFINITY ? 0.f : m));
+            sum += f[w] * ls[w][nn];
+            bad |= bs[w][nn];
         }
-        // The four waves' states: wave w ends a quarter of the row's dims, which the others pass it through
-        // LDS; a lane keeps its row, and its accumulators go as they are.
+        f32x4 o[kQuarter];
 #pragma unroll
-        for (int c = 0; c < NQ; ++c) {
-            if (rho0 + c * 16 >= rows) break;
-            if (NQ > 1 || pass || c) __syncthreads();        // os was read: Q, or the 16 rows before these
-            uint32_t bad = st.bad[c];
-            bad |= (uint32_t)__shfl_xor((int)bad, 16);
-            bad |= (uint32_t)__shfl_xor((int)bad, 32);
-            if (g == 0) { ms[wv][nn] = st.m[c]; ls[wv][nn] = st.l[c][0]; bs[wv][nn] = bad; }
+        for (int i = 0; i < kQuarter; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < 4; ++w)
+        for (int w = 0; w < 4; ++w)              // in the same order in every wave
 #pragma unroll
-                for (int i = 0; i < kQuarter; ++i)
-                    if (w != wv) os[w][wv][i][lane] = st.o[c][w * kQuarter + i];
-            __syncthreads();
-            float m = st.m[c], sum = 0.f, f[4];
+            for (int i = 0; i < kQuarter; ++i) {
+                f32x4 x;
+                if (w == wv) {
+                    x = st.o[c][i];
 #pragma unroll
-            for (int w = 0; w < 4; ++w) m = fmaxf(m, ms[w][nn]);
-            bad = 0;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                f[w] = __builtin_amdgcn_exp2f(ms[w][nn] - (m == -INFINITY ? 0.f : m));
-                sum += f[w] * ls[w][nn];
-                bad |= bs[w][nn];
-            }
-            f32x4 o[kQuarter];
-#pragma unroll
-            for (int i = 0; i < kQuarter; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int w = 0; w < 4; ++w)              // in the same order in every wave
-#pragma unroll
-                for (int i = 0; i < kQuarter; ++i) {
-                    f32x4 x;
-                    if (w == wv) {
-                        x = st.o[c][i];
-#pragma unroll
-                        for (int k = 1; k < 4; ++k) x = wv == k ? st.o[c][k * kQuarter + i] : x;
-                    } else {
-                        x = os[wv][w][i][lane];
-                    }
-                    o[i] += f[w] * x;
-                }
-            const int rho = rho0 + c * 16 + nn;
-            if (rho >= rows) continue;
-            const Out to(a, seq, h, rho);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int d = (4 * g + r) * (D / 16) + wv * kQuarter;
-                float x[kQuarter];
-#pragma unroll
-                for (int i = 0; i < kQuarter; ++i) x[i] = (bad >> (d / 32)) & 1 ? __uint_as_float(0x7fc00000u) : o[i][r];
-                if (splits == 1) {
-                    to.store<kQuarter>(a, x, sum, d);
+                    for (int k = 1; k < 4; ++k) x = wv == k ? st.o[c][k * kQuarter + i] : x;
                 } else {
-                    float* p = a.part + ((size_t)blockIdx.x * NQ + c) * kSplitRows * (D + 4) + nn * (D + 4);
-#pragma unroll
-                    for (int i = 0; i < kQuarter; ++i) p[d + i] = x[i];
-                    if (d == 0) { p[D] = m; p[D + 1] = sum; }
+                    x = os[wv][w][i][lane];
                 }
+                o[i] += f[w] * x;
+            }
+        const int rho = rho0 + c * 16 + nn;
+        if (rho >= rows) continue;
+        const Out to(a, seq, h, rho);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int d = (4 * g + r) * (D / 16) + wv * kQuarter;
+            float x[kQuarter];
+#pragma unroll
+            for (int i = 0; i < kQuarter; ++i) x[i] = (bad >> (d / 32)) & 1 ? __uint_as_float(0x7fc00000u) : o[i][r];
+            if (splits == 1) {
+                to.store<kQuarter>(a, x, sum, d);
+            } else {
+                float* p = a.part + ((((size_t)z * a.kv_heads + h) * row_tiles + rt) * NQ + c) * kSplitRows * (D + 4) + nn * (D + 4);
+#pragma unroll
+                for (int i = 0; i < kQuarter; ++i) p[d + i] = x[i];
+                if (d == 0) { p[D] = m; p[D + 1] = sum; }
             }
         }
     }
@@ -852,18 +851,10 @@ static hipError_t launch_attn(Kv4Attn& a, int n, hipStream_t st) {
     for (int i = n; i < kSeqArgs; ++i) a.first[i] = 0xffff;
     a.n = n;
     a.splits = z;
-    // prompts: row tiles in pairs of the same work once the pairs alone give every CU two blocks
-    const long long pairs = (long long)n * a.kv_heads * ((row_tiles + 1) / 2);
-    if (std::max<long long>({(long long)z * items, pairs, (long long)n * a.kv_heads * rows * (D / 4)}) > 0x7fffffffLL)
-        return hipErrorInvalidValue;
-    if (row_tiles > 1 && most == 1 && pairs >= 512) {
-        if (nq == 1) hipLaunchKernelGGL((attn_kv4_kernel<D, 1, true>), dim3((unsigned)pairs), dim3(256), 0, st, a, row_tiles);
-        else hipLaunchKernelGGL((attn_kv4_kernel<D, 2, true>), dim3((unsigned)pairs), dim3(256), 0, st, a, row_tiles);
-        return hipGetLastError();
-    }
+    if (std::max<long long>((long long)z * items, (long long)n * a.kv_heads * rows * (D / 4)) > 0x7fffffffLL) return hipErrorInvalidValue;
     const unsigned blocks = (unsigned)z * items;
-    if (nq == 1) hipLaunchKernelGGL((attn_kv4_kernel<D, 1, false>), dim3(blocks), dim3(256), 0, st, a, row_tiles);
-    else hipLaunchKernelGGL((attn_kv4_kernel<D, 2, false>), dim3(blocks), dim3(256), 0, st, a, row_tiles);
+    if (nq == 1) hipLaunchKernelGGL((attn_kv4_kernel<D, 1>), dim3(blocks), dim3(256), 0, st, a, row_tiles);
+    else hipLaunchKernelGGL((attn_kv4_kernel<D, 2>), dim3(blocks), dim3(256), 0, st, a, row_tiles);
     hipError_t rc = hipGetLastError();
     if (rc != hipSuccess || most == 1) return rc;
     const long long heads = (long long)n * a.kv_heads * rows;
