@@ -113,6 +113,10 @@ __device__ __forceinline__ double rsqrt_d(double x) {
 // scale's step), so every float32 operation is one rounding in the stated order, and the sum of
 // squares, the root and the angles are float64. QUADS: rot / 2 is a multiple of 4, so a lane's four dims lie
 // on one side of the pairs.
+// Many rows: HBM and the instructions a head takes share the time (4096 rows of 8 + 2 heads of 256, 42 MB: 11.6 us;
+// 1999 rows of 32 + 2 x 8 heads of 128 with the append, 51 MB: 15.7 us, its codes in stores of 2 bytes a lane that the
+// cache's fragment order scatters); few rows: the chain of launch, loads and angles (1 row 3.7 us, 256 rows with
+// the append 5.4).
 constexpr int kBlockRows = 4;
 template <int D, bool QUADS>
 __global__ void __launch_bounds__(256) heads_kernel(HeadArgs a, int rows, int per_block, int parts, int some) {
@@ -246,8 +250,9 @@ __global__ void __launch_bounds__(256) heads_kernel(HeadArgs a, int rows, int pe
 
 hipError_t launch_heads(HeadArgs& a, int n, hipStream_t st) {
     const int rows = n * a.T, kinds = a.v.p ? 2 : 1;
-    // rows of a block: one while they are too few to give every CU two blocks of two, else up to four; of very few
-    // rows with many heads, four wave items (one a wave) in a block
+    // rows of a block: one while they are too few to give every CU two blocks of two, else up to four (1999 rows of 32 q
+    // heads by one 16.4 us, two 15.8, four 19.7; 4096 of 8 by one 17.1, two 14.2, four 12.1); of very few rows
+    // with many heads, four wave items (one a wave) in a block
     const int per_block = rows >= 4096 ? kBlockRows : rows >= 1024 ? 2 : 1;
     const int items = ((a.q.p ? per_block * a.q_heads + 3 : 0) / 4) + kinds * ((per_block * a.kv_heads + 3) / 4);
     const int some = rows < 256 ? std::min(items, 4) : items, parts = (items + some - 1) / some;
@@ -264,7 +269,8 @@ hipError_t launch_heads(HeadArgs& a, int n, hipStream_t st) {
 }
 
 // ------------------------------------------------------------------ rows in and out of the cache
-// A thread per 8 dims of a (lane, kv head, slot): 4 bytes of codes, and a scale byte in one of four.
+// A thread per 8 dims of a (lane, kv head, slot): 4 bytes of codes, and a scale byte in one of four. Copies between
+// the fragment order and rows, for snapshots and checks: no step's path has it, so it is left simple.
 template <bool WRITE>
 __global__ void __launch_bounds__(256) kv4_copy_kernel(Kv4Copy a) {
     const int per = a.D / 8;
@@ -307,6 +313,11 @@ hipError_t launch_kv4_copy(const Kv4Copy& a, bool write, hipStream_t st) {
 // t * group + g at position pos + t. S^T = K Q^T and O^T = V^T P^T on 16x16x32 bf16 MFMAs with the
 // slots (S^T) and the dims (O^T) in M and 16 rows in N: a lane's column is one row in both, so the row's
 // maximum, sum and rescale live in the lane, and S^T's accumulators are P^T's operand as they are.
+// Decode and verify rows are bound by the cache's bytes: 256 lanes x 4096 slots of 2 heads of 256 (574 MB) 88 us,
+// 6.5 TB/s; 128 lanes x 3 rows x up to 2000 slots (84 MB) 23 us and a join of 4, a block a CU or two for 40 tiles.
+// Prompts are bound by what the VALU issues beside the MFMAs, most of it making bf16 fragments of codes (192 of a
+// step's 293 instructions for 66 MFMAs of 32 rows): 4096 rows of 8 heads of 256 (69 GFLOP) 97 us, 8192 rows 323 (850
+// TFLOP/s; a library's 8192^3 product reaches 1191).
 template <int D>
 struct Tile {
     u32x4 k[D / 64], v[D / 64];
@@ -747,7 +758,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) attn_kv4_kernel(Kv4Attn
 }
 
 // Joins the splits of sequences that have few (up to 8): a thread per four dims of a row, all its
-// loads at once.
+// loads at once. A launch and one trip to memory: 128 lanes x 12 rows of 256 dims 4.3 us.
 constexpr int kFewSplits = 8;
 template <int D, int NQ>
 __global__ void __launch_bounds__(256) attn_kv4_join_few(Kv4Attn a, int row_tiles) {
@@ -786,7 +797,7 @@ __global__ void __launch_bounds__(256) attn_kv4_join_few(Kv4Attn a, int row_tile
 
 // The same for any number of splits: a block per (sequence, kv head, row, 64 dims). The splits' factors are
 // made once into LDS; 16 threads take a split's dims, 16 splits at a time, and their sums meet in LDS:
-// always in the same order.
+// always in the same order. Latency here too: 8 rows of 128 splits 4.6 us.
 template <int D, int NQ>
 __global__ void __launch_bounds__(256) attn_kv4_join(Kv4Attn a, int row_tiles) {
     __shared__ float fs[kSeqSplits];
