@@ -492,3 +492,17 @@ def test_rounds_of_a_layer(eng, hq, kv, d, rot, window, sinks):
         assert [c.length(layer, l) for l in range(n)] == lens.tolist() and c.length(0, 1) == int(lens[1])
     assert len(taken) > 1                    # some rounds dropped rows, some fewer
     c.close()
+
+
+@pytest.mark.parametrize("hq,kv,d,T", [(8, 2, 64, 1100), (8, 2, 256, 1024), (9, 3, 128, 1300), (32, 4, 64, 700)])
+def test_attention_long_prompt(eng, hq, kv, d, T):
+    """One prompt of more row tiles than CUs, up to two a CU and more: rows from all over it, and none left out."""
+    rng = np.random.default_rng(T)
+    f = Filled(eng, rng, 1, T + 37, kv, d)
+    for window, sinks in [(0, 0), (100, 5)]:
+        print(f"attention long prompt {hq} {kv} {d} {T} {window} {sinks}", flush=True)
+        got, q, g = run_attention(eng, f, [0], [37], T, hq, rng, window, sinks, True)
+        assert not (got == 0x1234).all(-1).any()
+        for t in np.unique(np.r_[0, 1, T - 1, np.arange(31, T, 97), rng.integers(0, T, 12)]):
+            check_attention(f, [0], [37 + t], 1, got[t:t + 1], q[t:t + 1], g[t:t + 1], window, sinks)
+    f.c.close()
