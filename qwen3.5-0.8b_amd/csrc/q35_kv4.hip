@@ -98,11 +98,13 @@ __device__ __forceinline__ double head_sum(double v) {
     return v;
 }
 constexpr int kAngles = 512;         // of a block's rows: kBlockRows x 128
-// 1 / sqrt(x) from the instruction's approximation by two Newton steps (float64 to its last bits)
+// 1 / sqrt(x) from the instruction's approximation by two Newton steps (float64 to its last bits); 0 of an infinity,
+// whose steps would be inf * 0
 __device__ __forceinline__ double rsqrt_d(double x) {
     double y = __builtin_amdgcn_rsq(x);
     y = y * __builtin_fma(-0.5 * x * y, y, 1.5);
-    return y * __builtin_fma(-0.5 * x * y, y, 1.5);
+    y = y * __builtin_fma(-0.5 * x * y, y, 1.5);
+    return x == INFINITY ? 0.0 : y;
 }
 
 // A block takes `per_block` rows (of few rows with many heads: a part of one row's heads). Its work is the list of

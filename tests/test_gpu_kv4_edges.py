@@ -1,0 +1,94 @@
+"""The 4-bit cache's operators at values, sizes and slots where a wrong step shows: infinities and the ends of the
+float32 range, scores far from zero, rows that hang on single slots of a long context, several rows of heads in a
+block, calls larger than one launch takes. References and tolerances are those of tests/test_gpu_kv4.py."""
+import numpy as np
+import pytest
+
+import kv4_ref as ref
+import test_gpu_kv4 as base
+from test_gpu_kv4 import Dev, read_cache
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def eng():
+    from qwen35 import Engine
+    e = Engine(max_rows=64, max_ctx=40000, seed=None)
+    yield e
+    e.close()
+
+
+# ------------------------------------------------------------------------------ norms and append
+class Plain:
+    """q, k, v rows of one kv head and `hq` q heads, dense, for heads of given values."""
+
+    def __init__(self, x, hq, d):
+        D, R = Dev(), x.shape[0]
+        import torch
+        self.x, self.hq, self.d, self.R = ref.bf16_bits(x), hq, d, R          # [R][hq + 2][d]: q heads, k, v
+        self.w = ref.bf16_bits(np.random.default_rng(d).standard_normal(d) * 0.1)
+        self.dx, self.dw = D.up(self.x), D.up(self.w)
+        self.q = torch.zeros(R, hq, d, dtype=torch.int16, device="cuda")
+        self.k, self.v = (torch.zeros(R, 1, d, dtype=torch.int16, device="cuda") for _ in range(2))
+        torch.cuda.synchronize()
+
+    def args(self, rot, eps):
+        p, ld, d, w = self.dx.data_ptr(), (self.hq + 2) * self.d, self.d, self.dw.data_ptr()
+        return dict(rot_dim=rot, theta=1e6, eps=eps, q_norm=w, k_norm=w, q=(p, ld, d), k=(p + 2 * self.hq * d, ld, d),
+                    q_out=(self.q.data_ptr(), self.hq * d, d), k_out=(self.k.data_ptr(), d, d))
+
+    def want(self, rot, eps, pos):
+        with np.errstate(invalid="ignore", divide="ignore"):
+            return ref.norm_rope(ref.val(self.x)[:, :self.hq + 1], ref.val(self.w), pos, rot, 1e6, eps)
+
+
+def same(bits, want, size):
+    """NaN where the formula has NaN, and elsewhere the tolerance of the finite cases."""
+    got = ref.val(bits)
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    ok = ~np.isnan(want)
+    assert np.all(np.abs(got - want)[ok] <= (2.0 ** -8 * np.abs(want) + base.SLACK * size + 1e-37)[ok])
+
+
+@pytest.mark.parametrize("d,rot", [(256, 64), (128, 128), (64, 0), (128, 100)])
+def test_norm_rope_infinities(eng, d, rot):
+    """An infinity makes its own element NaN (inf * 0), and its partner in the rotation; the head's other
+    elements become 0. A NaN makes the whole head NaN."""
+    print(f"norm_rope infinities {d} {rot}", flush=True)
+    rng = np.random.default_rng(d + rot)
+    x = rng.standard_normal((6, 5, d))
+    x[0, 0, d - 1] = np.inf
+    x[1, 1, 3] = -np.inf
+    x[2, 3, 40], x[2, 3, 41] = np.inf, -np.inf
+    x[3, 2, 5] = np.nan
+    x[4, :, ::7] = np.inf
+    p = Plain(x, 3, d)
+    pos = np.arange(6) + 1000
+    eng.op_qk_norm_rope([1000], 6, 3, 1, d, **p.args(rot, 1e-6))
+    eng.sync()
+    want, size = p.want(rot, 1e-6, pos.astype(np.float64))
+    D = Dev()
+    same(D.bits(p.q), want[:, :3], size[:, :3])
+    same(D.bits(p.k), want[:, 3:], size[:, 3:])
+    assert np.isnan(want).any() and (want[4] == 0).any()
+
+
+def test_append_infinity_in_k(eng):
+    """Only the groups of k that hold a NaN after the norm are marked; the head's other groups are zeros."""
+    from qwen35 import KvCache4
+    d = 128
+    x = np.random.default_rng(2).standard_normal((3, 4, d))
+    x[1, 2, 70] = np.inf
+    p = Plain(x, 2, d)
+    c = KvCache4(eng, 1, 8, kv_heads=1, head_dim=d)
+    args = p.args(0, 1e-6)
+    args.update(v=(p.dx.data_ptr() + 2 * 3 * d, 4 * d, d), v_out=(p.v.data_ptr(), d, d))
+    eng.op_kv4_append(c, 0, [0], [0], 3, 2, **args)
+    eng.sync()
+    kc, ks, vc, vs = read_cache(eng, c, 0, 0, 1, 0, 3)
+    assert list(ks[0, 0, 1]) == [8, 8, 255, 8] and np.all(ks[0, 0, [0, 2]] < 200)
+    got = ref.values(kc[0, 0], ks[0, 0])
+    assert np.isnan(got[1, 64:96]).all() and np.all(np.delete(got[1], range(64, 96)) == 0)
+    assert np.isfinite(ref.values(vc, vs)).all()
+    c.close()
