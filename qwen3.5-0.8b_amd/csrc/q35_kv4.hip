@@ -413,8 +413,8 @@ struct Rows {
 // q: the rows' Q^T operands, [NQ][D / 32], in registers (NQ = 1) or, 16 rows more, in LDS with 64 lanes each
 // (the four waves of a block have the same rows). t's registers take the tile at next_p as soon as its K, then its
 // V, is used up. TIGHT: 32 rows of 256 dims leave no register for fragments made far ahead.
-// edge: some row may not see some slot.
-template <int D, int NQ, bool ONCE, bool TIGHT, class Q>
+// edge: some row may not see some slot. FAR: a score times scale2 is rounded before the reference is taken off.
+template <int D, int NQ, bool ONCE, bool TIGHT, bool FAR, class Q>
 __device__ __forceinline__ void tile_step(Tile<D>& t, const uint8_t* tile_p, const uint8_t* next_p, const Lanes& lo, int slot0,
                                           bool edge, const Q& q, const Sight* sight, float scale2, Rows<D, NQ>& st) {
     const int lane = threadIdx.x & 63, g = lane >> 4;
@@ -489,7 +489,10 @@ __device__ __forceinline__ void tile_step(Tile<D>& t, const uint8_t* tile_p, con
         const float ms = st.m[c] == -INFINITY ? 0.f : st.m[c];      // nothing seen so far: e^(-inf) stays 0
         float p[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][j >> 2][j & 3], scale2, -ms));
+        for (int j = 0; j < 8; ++j) {
+            const float x = s[c][j >> 2][j & 3];
+            p[j] = __builtin_amdgcn_exp2f(FAR ? x * scale2 - ms : __builtin_fmaf(x, scale2, -ms));
+        }
         // weights rounded to bf16 (2^-9) for the product; their sum is that of the rounded ones, a product with ones
         const f32x8 pw = {p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]};
         pf[c] = __builtin_convertvector(pw, q35_bf16x8);     // not f2bf2: the compiler must see what an MFMA is about to read
@@ -648,13 +651,16 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) attn_kv4_kernel(Kv4Attn
     auto at = [&](int i) { return i < tl.sink ? i : i - tl.sink + tl.main; };
     Tile<D> buf[kAhead];
     const auto tile_at = [&](int i) { return region + (size_t)at(i) * kv4_tile_bytes(D); };
-    if (t0 + wv < t1) {
+    const auto first_tiles = [&] {
+        if (t0 + wv < t1) {
 #pragma unroll
-        for (int b = 0; b < kAhead; ++b) {
-            load_k<D, kOnce>(buf[b], tile_at(min(t0 + wv + 4 * b, t1 - 1)), lo);
-            load_v<D, kOnce>(buf[b], tile_at(min(t0 + wv + 4 * b, t1 - 1)), lo);
+            for (int b = 0; b < kAhead; ++b) {
+                load_k<D, kOnce>(buf[b], tile_at(min(t0 + wv + 4 * b, t1 - 1)), lo);
+                load_v<D, kOnce>(buf[b], tile_at(min(t0 + wv + 4 * b, t1 - 1)), lo);
+            }
         }
-    }
+    };
+    first_tiles();
     q35_bf16x8 qf[NQ == 1 ? D / 32 : 1];
     q35_bf16x8* ql = (q35_bf16x8*)&os[0][0][0][0];
     if constexpr (NQ == 1) {
@@ -670,30 +676,47 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) attn_kv4_kernel(Kv4Attn
     int qlane = lane;
     const auto q = [&](int c, int k) { return NQ == 1 ? qf[k] : ql[(c * (D / 32) + k) * 64 + qlane]; };
     Sight sight[NQ];
-    Rows<D, NQ> st;
 #pragma unroll
     for (int c = 0; c < NQ; ++c) {
         const int p = pos + min(rho0 + c * 16 + nn, rows - 1) / group;
         sight[c] = {p, a.window > 0 ? p - a.window + 1 : 0, a.sinks};
-        st.m[c] = -INFINITY;
-        st.l[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-        st.bad[c] = 0;
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) st.o[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     // tiles whose every slot every row of the block sees: from the last row's window to the first row's slot
     const int full0 = a.window > 0 ? max(pos + rho1 / group - a.window + 1, 0) : 0, full1 = pos + rho0 / group;
-    for (int i0 = __builtin_amdgcn_readfirstlane(t0 + wv); i0 < t1; i0 += 4 * kAhead) {
+    Rows<D, NQ> st;
+    const auto walk = [&](auto far) {
 #pragma unroll
-        for (int b = 0; b < kAhead; ++b) {
-            const int i = i0 + 4 * b;
-            if (i >= t1) break;
-            if (NQ > 1) asm volatile("" : "+v"(qlane));     // or the compiler reads Q ahead of the loop, and spills it
-            const int tile = at(i);
-            const bool edge = tile * 32 < full0 || tile * 32 + 31 > full1;
-            tile_step<D, NQ, kOnce, kTight>(buf[b], tile_at(i), tile_at(min(i + 4 * kAhead, t1 - 1)), lo, tile * 32, edge, q,
-                                            sight, scale2, st);
+        for (int c = 0; c < NQ; ++c) {
+            st.m[c] = -INFINITY;
+            st.l[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+            st.bad[c] = 0;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) st.o[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
+        for (int i0 = __builtin_amdgcn_readfirstlane(t0 + wv); i0 < t1; i0 += 4 * kAhead) {
+#pragma unroll
+            for (int b = 0; b < kAhead; ++b) {
+                const int i = i0 + 4 * b;
+                if (i >= t1) break;
+                if (NQ > 1) asm volatile("" : "+v"(qlane));     // or the compiler reads Q ahead of the loop, and spills it
+                const int tile = at(i);
+                const bool edge = tile * 32 < full0 || tile * 32 + 31 > full1;
+                tile_step<D, NQ, kOnce, kTight, decltype(far)::value>(buf[b], tile_at(i), tile_at(min(i + 4 * kAhead, t1 - 1)), lo,
+                                                                      tile * 32, edge, q, sight, scale2, st);
+            }
+        }
+    };
+    walk(std::false_type{});
+    // References of 2^24 and more: there float32 numbers lie 2 and more apart, and the part of a product that its
+    // reference was rounded by, which a fused step keeps, is an exponent of its own (past 2^31 it can leave float32). The
+    // wave goes over its tiles again with products rounded as the reference is; the first way is the faster one (a
+    // 4096-row prompt 83.6 us a call, with a test of the reference in every tile 86.3).
+    bool far = false;
+#pragma unroll
+    for (int c = 0; c < NQ; ++c) far |= __any(fabsf(st.m[c]) >= 16777216.f && st.m[c] != -INFINITY);
+    if (far) {
+        first_tiles();
+        walk(std::true_type{});
     }
     // The four waves' states: wave w ends a quarter of the row's dims, which the others pass it through
     // LDS; a lane keeps its row, and its accumulators go as they are.

@@ -6,7 +6,7 @@ import pytest
 
 import kv4_ref as ref
 import test_gpu_kv4 as base
-from test_gpu_kv4 import Dev, read_cache
+from test_gpu_kv4 import Dev, Filled, read_cache, run_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -92,3 +92,29 @@ def test_append_infinity_in_k(eng):
     assert np.isnan(got[1, 64:96]).all() and np.all(np.delete(got[1], range(64, 96)) == 0)
     assert np.isfinite(ref.values(vc, vs)).all()
     c.close()
+
+
+# ------------------------------------------------------------------------------ attention
+@pytest.mark.parametrize("hq,kv,d,T,cap", [(4, 2, 128, 3, 500), (8, 2, 256, 1, 9000), (4, 1, 64, 20, 300)])
+def test_attention_scores_past_their_spacing(eng, hq, kv, d, T, cap):
+    """Scores so far from zero that float32 numbers lie further apart than 2^8 there: the largest one takes all the
+    weight, the row is its V exactly, and no row is NaN. Every row's largest score leads by more than
+    float32 sums of its products can be off."""
+    rng = np.random.default_rng(cap)
+    f = Filled(eng, rng, 1, cap, kv, d)
+    for scale in (3e8, -4e9, 1e12, 1e30):
+        print(f"attention far scores {hq} {kv} {d} {T} {cap} {scale}", flush=True)
+        got, q, _ = run_attention(eng, f, [0], [cap - T], T, hq, rng, scale=scale)
+        g, sure = ref.val(got), 0
+        assert np.isfinite(g).all()
+        for t in range(T):
+            for h in range(hq):
+                k, v = f.K[0][h // (hq // kv)][:cap - T + t + 1], f.V[0][h // (hq // kv)]
+                s = k @ q[t, h] * np.sign(scale)
+                off = (d + 4) * 2.0 ** -24 * (np.abs(k) @ np.abs(q[t, h])).max()
+                a = np.argsort(s)
+                if s[a[-1]] - s[a[-2]] > 4 * off and (s[a[-1]] - s[a[-2]]) * abs(scale) > 200:
+                    sure += 1
+                    assert np.array_equal(g[t, h], v[a[-1]]), (t, h)
+        assert sure >= T * hq // 2
+    f.c.close()
