@@ -413,7 +413,9 @@ struct Rows {
 // q: the rows' Q^T operands, [NQ][D / 32], in registers (NQ = 1) or, 16 rows more, in LDS with 64 lanes each
 // (the four waves of a block have the same rows). t's registers take the tile at next_p as soon as its K, then its
 // V, is used up. TIGHT: 32 rows of 256 dims leave no register for fragments made far ahead.
-// edge: some row may not see some slot. FAR: a score times scale2 is rounded before the reference is taken off.
+// edge: some row may not see some slot. FAR: a score times scale2 is rounded before the reference is taken off, and the
+// reference lies 28 above the maximum it was taken from, so that weights stay under 2^-20 and 2^18 slots' sum of
+// them times the largest V is still a float32.
 template <int D, int NQ, bool ONCE, bool TIGHT, bool FAR, class Q>
 __device__ __forceinline__ void tile_step(Tile<D>& t, const uint8_t* tile_p, const uint8_t* next_p, const Lanes& lo, int slot0,
                                           bool edge, const Q& q, const Sight* sight, float scale2, Rows<D, NQ>& st) {
@@ -477,9 +479,11 @@ __device__ __forceinline__ void tile_step(Tile<D>& t, const uint8_t* tile_p, con
         // the reference of the row's exponents follows its maximum only when that is past it by 2^8: weights
         // stay under 2^8 (as exact as under 1), and almost every tile goes without the four lanes' common
         // maximum and the rescale of O
-        if (__any(top * scale2 > st.m[c] + 8.f)) {
+        constexpr float kRoom = FAR ? 28.f : 0.f;
+        if (__any(top * scale2 > st.m[c] + (8.f - kRoom))) {
             top = fmaxf(top, xor16(top));
             top = fmaxf(top, xor32(top)) * scale2;
+            if (FAR) top += kRoom;
             const float mn = fmaxf(st.m[c], top), al = __builtin_amdgcn_exp2f(st.m[c] - (mn == -INFINITY ? 0.f : mn));
             st.l[c] *= al;
 #pragma unroll
@@ -707,13 +711,22 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) attn_kv4_kernel(Kv4Attn
         }
     };
     walk(std::false_type{});
-    // References of 2^24 and more: there float32 numbers lie 2 and more apart, and the part of a product that its
-    // reference was rounded by, which a fused step keeps, is an exponent of its own (past 2^31 it can leave float32). The
-    // wave goes over its tiles again with products rounded as the reference is; the first way is the faster one (a
-    // 4096-row prompt 83.6 us a call, with a test of the reference in every tile 86.3).
+    // Two kinds of rows want their tiles gone over again in the FAR form (the other one is the faster: a 4096-row
+    // prompt 83.6 us a call, with a test of the reference in every tile 86.3). References of 2^24 and more: there float32
+    // numbers lie 2 and more apart, and the part of a product that its reference was rounded by, which a fused step
+    // keeps, is an exponent of its own (past 2^31 it can leave float32). And sums of 2^100 and more, or none any longer:
+    // what the waves and the splits (2^10 at most) add up from smaller ones stays a float32.
     bool far = false;
+    float big = 0.f;                 // (a NaN anywhere makes it one)
 #pragma unroll
-    for (int c = 0; c < NQ; ++c) far |= __any(fabsf(st.m[c]) >= 16777216.f && st.m[c] != -INFINITY);
+    for (int c = 0; c < NQ; ++c) {
+        far |= __any(fabsf(st.m[c]) >= 16777216.f && st.m[c] != -INFINITY);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) big = __builtin_elementwise_maximum(big, fabsf(st.o[c][i][r]));
+    }
+    far |= __any(!(big < 0x1p100f));
     if (far) {
         first_tiles();
         walk(std::true_type{});

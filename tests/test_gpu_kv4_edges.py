@@ -6,7 +6,7 @@ import pytest
 
 import kv4_ref as ref
 import test_gpu_kv4 as base
-from test_gpu_kv4 import Dev, Filled, read_cache, run_attention
+from test_gpu_kv4 import Dev, Filled, check_attention, read_cache, run_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -95,6 +95,27 @@ def test_append_infinity_in_k(eng):
 
 
 # ------------------------------------------------------------------------------ attention
+def filled(eng, kc, ks, vc, vs):
+    """A cache of one layer with these codes and scale bytes [lanes][kv][cap][..], and its values."""
+    import torch
+    from qwen35 import KvCache4
+    lanes, kv, cap, half = kc.shape
+    f = Filled.__new__(Filled)
+    f.c = KvCache4(eng, lanes, cap, kv_heads=kv, head_dim=2 * half)
+    t = [torch.from_numpy(a).cuda() for a in (kc, ks, vc, vs)]
+    torch.cuda.synchronize()
+    f.c.write(0, 0, lanes, 0, cap, *[x.data_ptr() for x in t])
+    eng.sync()
+    f.K, f.V = ref.values(kc, ks), ref.values(vc, vs)
+    return f
+
+
+def random_rows(rng, lanes, kv, cap, d):
+    a = [rng.integers(0, 256, (lanes, kv, cap, d // 2)).astype(np.uint8) for _ in range(2)]
+    b = [rng.integers(124, 127, (lanes, kv, cap, d // 32)).astype(np.uint8) for _ in range(2)]
+    return a[0], b[0], a[1], b[1]
+
+
 @pytest.mark.parametrize("hq,kv,d,T,cap", [(4, 2, 128, 3, 500), (8, 2, 256, 1, 9000), (4, 1, 64, 20, 300)])
 def test_attention_scores_past_their_spacing(eng, hq, kv, d, T, cap):
     """Scores so far from zero that float32 numbers lie further apart than 2^8 there: the largest one takes all the
@@ -117,4 +138,23 @@ def test_attention_scores_past_their_spacing(eng, hq, kv, d, T, cap):
                     sure += 1
                     assert np.array_equal(g[t, h], v[a[-1]]), (t, h)
         assert sure >= T * hq // 2
+    f.c.close()
+
+
+@pytest.mark.parametrize("hq,kv,d,T,cap", [(4, 2, 128, 1, 500), (8, 2, 256, 1, 9000), (4, 1, 64, 20, 300)])
+def test_attention_largest_values(eng, hq, kv, d, T, cap):
+    """V at the largest numbers the format has: the sums before the division stay finite. A weight under 2^-126 is 0, and
+    the largest one is at least 2^-28 here, so each slot may lose 2^-98 of the largest V beyond attention_bound (at V
+    of 2^127 that is no longer under its 1e-30)."""
+    rng = np.random.default_rng(cap + 1)
+    kc, ks, vc, vs = random_rows(rng, 1, kv, cap, d)
+    vs[:], vc[:, :, :, : d // 4] = 252, 0x77
+    f = filled(eng, kc, ks, vc, vs)
+    for scale in (None, 1e-30, 5.0):
+        got, q, _ = run_attention(eng, f, [0], [cap - T], T, hq, rng, scale=scale)
+        g = ref.val(got)
+        out, pv, big = ref.attention(q, f.K[0], f.V[0], cap - T, 0, 0, d ** -0.5 if scale is None else scale)
+        want, e = ref.attention_bound(out, pv, big, cap, d)
+        assert np.isfinite(g).all() and np.all(np.abs(g - want) <= e + cap * 2.0 ** -98 * 6 * 2.0 ** 125)
+        assert (g[..., : d // 2] > 2.5e38).all()
     f.c.close()
