@@ -98,13 +98,12 @@ __device__ __forceinline__ double head_sum(double v) {
     return v;
 }
 constexpr int kAngles = 512;         // of a block's rows: kBlockRows x 128
-// 1 / sqrt(x) from the instruction's approximation by two Newton steps (float64 to its last bits); 0 of an infinity,
-// whose steps would be inf * 0
+// 1 / sqrt(x) from the instruction's approximation by two Newton steps (float64 to its last bits; NaN of an
+// infinity, whose steps are inf * 0)
 __device__ __forceinline__ double rsqrt_d(double x) {
     double y = __builtin_amdgcn_rsq(x);
     y = y * __builtin_fma(-0.5 * x * y, y, 1.5);
-    y = y * __builtin_fma(-0.5 * x * y, y, 1.5);
-    return x == INFINITY ? 0.0 : y;
+    return y * __builtin_fma(-0.5 * x * y, y, 1.5);
 }
 
 // A block takes `per_block` rows (of few rows with many heads: a part of one row's heads). Its work is the list of
@@ -114,13 +113,14 @@ __device__ __forceinline__ double rsqrt_d(double x) {
 // the first heads' loads in flight. What the kernel writes is decided by borders (a code's midpoints, a
 // scale's step), so every float32 operation is one rounding in the stated order, and the sum of
 // squares, the root and the angles are float64. QUADS: rot / 2 is a multiple of 4, so a lane's four dims lie
-// on one side of the pairs.
+// on one side of the pairs. TINY: eps is so small (under 2^-250) that a root may pass float32; without that form's care
+// 1999 rows as below take 0.4 us less.
 // Many rows: HBM and the instructions a head takes share the time (4096 rows of 8 + 2 heads of 256, 42 MB: 11.6 us;
 // 1999 rows of 32 + 2 x 8 heads of 128 with the append, 51 MB: 15.7 us, its codes in stores of 2 bytes a lane that the
 // cache's fragment order scatters); few rows: the chain of launch, loads and angles (1 row 3.7 us, 256 rows with
 // the append 5.4).
 constexpr int kBlockRows = 4;
-template <int D, bool QUADS>
+template <int D, bool QUADS, bool TINY>
 __global__ void __launch_bounds__(256) heads_kernel(HeadArgs a, int rows, int per_block, int parts, int some) {
     constexpr int C = D / 64;
     __shared__ float xs[4][4][D];
@@ -177,7 +177,15 @@ __global__ void __launch_bounds__(256) heads_kernel(HeadArgs a, int rows, int pe
             for (int c = 0; c < C; ++c)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) ss = __builtin_fma((double)x[c][e], (double)x[c][e], ss);
-            const float rs = (float)rsqrt_d(head_sum(ss) * (1.0 / D) + a.eps);
+            const double mean = head_sum(ss) * (1.0 / D) + a.eps, root = rsqrt_d(mean);
+            float rs = (float)root;
+            if (mean == INFINITY) rs = 0.f;
+            if (TINY) {                      // of subnormal numbers 2^64 of it go to x first, exactly
+                const bool past = rs == INFINITY;
+                if (past) rs = (float)(root * 0x1p-64);
+#pragma unroll
+                for (int c = 0; c < C; ++c) x[c] *= past ? 0x1p64f : 1.f;
+            }
             float* hx = xs[wv][j];
             wave_sync();
 #pragma unroll
@@ -263,9 +271,13 @@ hipError_t launch_heads(HeadArgs& a, int n, hipStream_t st) {
     a.q_inv = a.q_heads > 1 ? (uint32_t)(0x100000000ull / a.q_heads + 1) : 0;
     a.kv_inv = a.kv_heads > 1 ? (uint32_t)(0x100000000ull / a.kv_heads + 1) : 0;
     const bool quads = a.rot % 8 == 0;
-    auto k = a.D == 256 ? (quads ? heads_kernel<256, true> : heads_kernel<256, false>)
-           : a.D == 128 ? (quads ? heads_kernel<128, true> : heads_kernel<128, false>)
-                        : (quads ? heads_kernel<64, true> : heads_kernel<64, false>);
+    const auto pick = [&](auto tiny) {
+        constexpr bool t = decltype(tiny)::value;
+        return a.D == 256 ? (quads ? heads_kernel<256, true, t> : heads_kernel<256, false, t>)
+             : a.D == 128 ? (quads ? heads_kernel<128, true, t> : heads_kernel<128, false, t>)
+                          : (quads ? heads_kernel<64, true, t> : heads_kernel<64, false, t>);
+    };
+    const auto k = a.eps < 0x1p-250 ? pick(std::true_type{}) : pick(std::false_type{});
     hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(256), 0, st, a, rows, per_block, parts, some);
     return hipGetLastError();
 }

@@ -24,8 +24,9 @@ class Plain:
     """q, k, v rows of one kv head and `hq` q heads, dense, for heads of given values."""
 
     def __init__(self, x, hq, d):
-        D, R = Dev(), x.shape[0]
         import torch
+        D, R = Dev(), x.shape[0]
+        assert x.shape == (R, hq + 2, d)
         self.x, self.hq, self.d, self.R = ref.bf16_bits(x), hq, d, R          # [R][hq + 2][d]: q heads, k, v
         self.w = ref.bf16_bits(np.random.default_rng(d).standard_normal(d) * 0.1)
         self.dx, self.dw = D.up(self.x), D.up(self.w)
@@ -92,6 +93,29 @@ def test_append_infinity_in_k(eng):
     assert np.isnan(got[1, 64:96]).all() and np.all(np.delete(got[1], range(64, 96)) == 0)
     assert np.isfinite(ref.values(vc, vs)).all()
     c.close()
+
+
+@pytest.mark.parametrize("d,rot", [(256, 64), (64, 6)])
+def test_norm_rope_tiny_and_huge_heads(eng, d, rot):
+    """eps 0: heads of subnormal numbers, whose 1 / root is past float32, have the norm of any other head; so have
+    heads near bf16's largest number."""
+    print(f"norm_rope tiny and huge {d} {rot}", flush=True)
+    rng = np.random.default_rng(d)
+    x = rng.standard_normal((6, 4, d))
+    x[0] *= 2.0 ** -128
+    x[1] *= 2.0 ** -131
+    x[2] = 0
+    x[2, :, 17] = 2.0 ** -133
+    x[3] = np.clip(x[3], -1.5, 1.5) * 2.0 ** 127
+    x[4, :, ::2] *= 2.0 ** -130
+    p = Plain(x, 2, d)
+    eng.op_qk_norm_rope([77], 6, 2, 1, d, **p.args(rot, 0.0))
+    eng.sync()
+    want, size = p.want(rot, 0.0, 77.0 + np.arange(6))
+    assert np.isfinite(want).all() and np.abs(want[:3]).max() > 1
+    D = Dev()
+    same(D.bits(p.q), want[:, :2], size[:, :2])
+    same(D.bits(p.k), want[:, 2:], size[:, 2:])
 
 
 # ------------------------------------------------------------------------------ attention
