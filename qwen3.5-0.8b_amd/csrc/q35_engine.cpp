@@ -859,6 +859,8 @@ int q35::guard(const std::function<void()>& f) {
         f();
         return Q35_OK;
     } catch (const Q35Error& ex) {
+        // HIP keeps a failed call's error for the thread's next hipGetLastError(), which may be a later launch's
+        if (ex.code == Q35_ERR_HIP) (void)hipGetLastError();
         g_err = ex.what();
         return ex.code;
     } catch (const std::exception& ex) {

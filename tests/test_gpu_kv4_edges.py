@@ -182,3 +182,15 @@ def test_attention_largest_values(eng, hq, kv, d, T, cap):
         assert np.isfinite(g).all() and np.all(np.abs(g - want) <= e + cap * 2.0 ** -98 * 6 * 2.0 ** 125)
         assert (g[..., : d // 2] > 2.5e38).all()
     f.c.close()
+
+
+# ------------------------------------------------------------------------------ calls and their sizes
+def test_calls_after_a_refused_allocation(eng):
+    """A cache that no memory holds is refused, and the next call does not report that error again."""
+    from qwen35 import EngineError, KvCache4
+    with pytest.raises(EngineError):
+        KvCache4(eng, 65535, 40000, layers=64, kv_heads=1024, head_dim=256)
+    p = Plain(np.ones((1, 3, 64)), 1, 64)
+    eng.op_qk_norm_rope([0], 1, 1, 1, 64, **p.args(0, 0.0))
+    eng.sync()
+    assert Dev().bits(p.q).any()
