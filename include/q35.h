@@ -158,7 +158,9 @@ int q35_mtp_verify(q35_engine* e, q35_state* s, const int32_t* lanes, int n, con
  * and arguments of q35_mtp_verify, but the drafts are kept and the bonus drawn at `temperature` from the
  * random numbers u [n][k + 1] (host, in [0, 1)) by q35_op_draft_verify's rule with drafts that the drafter is
  * certain of, so every emitted token has the distribution softmax(logits / temperature); temperature 0 is
- * q35_mtp_verify. An accepted draft equal to `stop` ends the accepted prefix and is emitted pending. */
+ * q35_mtp_verify. An accepted draft equal to `stop` ends the accepted prefix and is emitted pending. A lane
+ * whose token would come from a row without a distribution (a NaN, a +inf or only -inf logits) emits nothing (n_emit 0),
+ * keeps its state and is left out of stats; the other lanes' rounds are not affected. */
 int q35_mtp_verify_sample(q35_engine* e, q35_state* s, const int32_t* lanes, int n, const int32_t* cur, int k,
                           const int32_t* drafts, double temperature, const float* u, int32_t stop, int32_t* emit,
                           int32_t* n_emit, int64_t* stats);

@@ -1591,7 +1591,9 @@ int q35_mtp_round(q35_engine* e, q35_state* s, const int32_t* lanes, int n, cons
 // over [cur, d1..dk] with per-row GDN factors, accept of the longest prefix the target rows
 // confirm (the stop cut applied), then the state, window and MTP cache kept for rows 0..a.
 // sampling (nullable): instead of the greedy accept, drafts kept and the bonus drawn at its temperature from
-// its random numbers u [n][k + 1] (q35_op_draft_verify's rule, the drafter taken as certain of its drafts).
+// its random numbers u [n][k + 1] (q35_op_draft_verify's rule, the drafter taken as certain of its drafts). A lane whose
+// token has no distribution to come from emits nothing and keeps its state: what the body left for it lies behind its
+// prefix and in its spare slots.
 struct Sampling { double temperature; const float* u; };
 static void mtp_verify_accept(q35_engine* e, q35_state* s, const std::vector<int>& ls, const std::vector<int>& P,
                    const int32_t* cur, int k, const std::vector<std::vector<int>>& drafts, int32_t stop,
@@ -1625,10 +1627,7 @@ static void mtp_verify_accept(q35_engine* e, q35_state* s, const std::vector<int
         HCK(hipMemcpyAsync(e->h_out, e->tok_dev, R * sizeof(int), hipMemcpyDeviceToHost, e->st));
     }
     HCK(hipStreamSynchronize(e->st));
-    if (sampling)
-        for (int i = 0; i < n; ++i)
-            REQ(tok[i * T + acc[i]] >= 0, Q35_ERR_STATE, "a verify row's logits have no distribution");
-    std::vector<int> rows(n);
+    std::vector<int> rows, kept;
     for (int i = 0; i < n; ++i) {
         const int* tgt = e->h_out + i * T;
         int a = 0;
@@ -1636,6 +1635,10 @@ static void mtp_verify_accept(q35_engine* e, q35_state* s, const std::vector<int
             while (a < acc[i] && drafts[i][a] != stop) ++a;
         else
             while (a < k && drafts[i][a] == tgt[a] && drafts[i][a] != stop) ++a;
+        if (sampling && a == acc[i] && tok[i * T + a] < 0) {
+            n_emit[i] = 0;
+            continue;
+        }
         int m = 0;
         for (int j = 0; j < a; ++j) emit[i * (k + 1) + m++] = drafts[i][j];
         // the token after the kept ones: with the stop cut in a sampled round, the kept stop draft itself
@@ -1650,10 +1653,11 @@ static void mtp_verify_accept(q35_engine* e, q35_state* s, const std::vector<int
         s->pset[l] ^= 1;
         s->wcur[l] = (s->wcur[l] + 1 + a) % s->nslots;
         if (a == k) s->mtp_len[l] += k;
-        rows[i] = i * T + a;
+        rows.push_back(i * T + a);
+        kept.push_back(l);
         if (stats) { stats[0] += k; stats[1] += a; stats[2] += 1; stats[3] += T; }
     }
-    save_hlast(e, s, rows, ls);
+    if (!kept.empty()) save_hlast(e, s, rows, kept);
     HCK(hipStreamSynchronize(e->st));
 }
 
@@ -1727,7 +1731,7 @@ int q35_mtp_verify_sample(q35_engine* e, q35_state* s, const int32_t* lanes, int
         for (long long i = 0; i < (long long)n * (k + 1); ++i)
             REQ(u[i] >= 0.f && u[i] < 1.f, Q35_ERR_ARG, "random numbers lie in [0, 1)");
         const Sampling smp{temperature, u};
-        mtp_verify(e, s, lanes, n, cur, k, drafts, stop, emit, n_emit, stats, &smp);
+        mtp_verify(e, s, lanes, n, cur, k, drafts, stop, emit, n_emit, stats, temperature == 0.0 ? nullptr : &smp);
     });
 }
 

@@ -510,7 +510,8 @@ class State:
     def mtp_verify_sample(self, cur, drafts, u, temperature: float, lanes=None, stats: np.ndarray | None = None,
                           stop: int = -1):
         """The verify half of a sampled round (q35_mtp_verify_sample): drafts [n][k] kept and the next token drawn at
-        `temperature` from the random numbers u [n][k + 1]; returns each lane's emitted tokens."""
+        `temperature` from the random numbers u [n][k + 1]; returns each lane's emitted tokens (none, its state
+        kept, for a lane whose logits have no distribution)."""
         c = _i32(cur)
         d = np.ascontiguousarray(np.asarray(drafts, np.int32).reshape(c.size, -1))
         n, k = d.shape
