@@ -293,8 +293,9 @@ int q35_op_attn_kv4(q35_engine* e, q35_kv4* c, int layer, const int32_t* lanes, 
         a.q_heads = q_heads; a.kv_heads = c->kv_heads; a.D = c->D; a.T = T;
         a.window = window; a.sinks = sinks; a.scale = scale; a.part = ev.kv4_part;
         OnDevice on(ev.device);
-        for (int i0 = 0; i0 < n; i0 += kSeqArgs) {
-            const int m = std::min(kSeqArgs, n - i0);
+        const int most = std::min(kSeqArgs, kLaunchBlocks / kv4_attn_items(q_heads, c->kv_heads, T));
+        for (int i0 = 0, m; i0 < n; i0 += m) {
+            m = std::min(most, n - i0);
             for (int i = 0; i < m; ++i) {
                 a.pos[i] = pos[i0 + i];
                 a.lane[i] = (uint16_t)(lanes ? lanes[i0 + i] : i0 + i);

@@ -49,6 +49,7 @@ __host__ __device__ inline int kv4_v_scale(int D, int tk, int blk) {
 struct HeadView { const uint16_t* p; long long row, head; };
 
 constexpr int kSeqArgs = 256;        // sequences of one launch (their positions travel as kernel arguments)
+constexpr int kLaunchBlocks = (1 << 24) - 1;   // blocks of 256 threads of one launch: HIP counts its threads in 32 bits
 struct HeadArgs {
     HeadView q, k, v, q_out, k_out, v_out;   // v, q_out, k_out, v_out: p null where not wanted
     const uint16_t *q_norm, *k_norm;
@@ -77,6 +78,11 @@ struct Kv4Attn {
     alignas(16) uint16_t lane[kSeqArgs];
     alignas(16) uint16_t first[kSeqArgs];   // first split of each sequence; 0xffff past the last
 };
+// Blocks of an unsplit sequence: for each kv head one for every 32 rows (T times its query heads), or for 16 rows or fewer.
+inline int kv4_attn_items(int q_heads, int kv_heads, int T) {
+    const long long rows = (long long)T * (q_heads / kv_heads), of = rows > 16 ? 32 : 16;
+    return (int)(kv_heads * ((rows + of - 1) / of));
+}
 size_t kv4_part_floats();
 hipError_t launch_attn_kv4(Kv4Attn& a, int n, hipStream_t st);
 

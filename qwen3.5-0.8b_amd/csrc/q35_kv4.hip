@@ -891,7 +891,7 @@ __global__ void __launch_bounds__(256) attn_kv4_join(Kv4Attn a, int row_tiles) {
 template <int D>
 static hipError_t launch_attn(Kv4Attn& a, int n, hipStream_t st) {
     const int group = a.q_heads / a.kv_heads, rows = a.T * group, nq = rows > 16 ? 2 : 1;
-    const int row_tiles = (rows + nq * 16 - 1) / (nq * 16), items = a.kv_heads * row_tiles;
+    const int row_tiles = (rows + nq * 16 - 1) / (nq * 16), items = kv4_attn_items(a.q_heads, a.kv_heads, a.T);
     // splits: a block a CU (two a CU: 64 lanes under a window 15.6 instead of 12.9 us with the join, 100 lanes x 4096
     // slots 50.6 instead of 45.7), each of its four waves with two tiles at least (four: 1 lane x 32768 slots
     // 14.7 instead of 13.6)
@@ -912,7 +912,7 @@ static hipError_t launch_attn(Kv4Attn& a, int n, hipStream_t st) {
     for (int i = n; i < kSeqArgs; ++i) a.first[i] = 0xffff;
     a.n = n;
     a.splits = z;
-    if (std::max<long long>((long long)z * items, (long long)n * a.kv_heads * rows * (D / 4)) > 0x7fffffffLL) return hipErrorInvalidValue;
+    if ((long long)z * items > kLaunchBlocks) return hipErrorInvalidValue;
     const unsigned blocks = (unsigned)z * items;
     if (nq == 1) hipLaunchKernelGGL((attn_kv4_kernel<D, 1>), dim3(blocks), dim3(256), 0, st, a, row_tiles);
     else hipLaunchKernelGGL((attn_kv4_kernel<D, 2>), dim3(blocks), dim3(256), 0, st, a, row_tiles);

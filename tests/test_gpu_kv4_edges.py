@@ -194,3 +194,24 @@ def test_calls_after_a_refused_allocation(eng):
     eng.op_qk_norm_rope([0], 1, 1, 1, 64, **p.args(0, 0.0))
     eng.sync()
     assert Dev().bits(p.q).any()
+
+
+def test_attention_of_many_rows(eng):
+    """2^27 rows of heads in one call (17 GB of output), more than a launch was once allowed: under a window of one slot
+    every row is its own slot's V."""
+    import torch
+    n, T, hq, d = 256, 8192, 64, 64
+    rng = np.random.default_rng(3)
+    f = filled(eng, *random_rows(rng, 1, 1, T, d))
+    q = Dev().up(base.bf16_randn(rng, d))
+    out = torch.empty(n * T, hq, d, dtype=torch.bfloat16, device="cuda")
+    v = torch.from_numpy(f.V[0][0]).to("cuda", torch.bfloat16)
+    torch.cuda.synchronize()
+    eng.op_attn_kv4(f.c, 0, [0] * n, [0] * n, T, hq, (q.data_ptr(), 0, 0), (out.data_ptr(), hq * d, d), window=1)
+    eng.sync()
+    out = out.view(n, T, hq, d)
+    for i in range(n):
+        assert torch.equal(out[i], v[:, None].expand(T, hq, d)), i
+    f.c.close()
+    del out
+    torch.cuda.empty_cache()
