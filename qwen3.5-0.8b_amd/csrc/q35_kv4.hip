@@ -286,9 +286,9 @@ hipError_t launch_heads(HeadArgs& a, int n, hipStream_t st) {
 // A thread per 8 dims of a (lane, kv head, slot): 4 bytes of codes, and a scale byte in one of four. Copies between
 // the fragment order and rows, for snapshots and checks: no step's path has it, so it is left simple.
 template <bool WRITE>
-__global__ void __launch_bounds__(256) kv4_copy_kernel(Kv4Copy a) {
+__global__ void __launch_bounds__(256) kv4_copy_kernel(Kv4Copy a, long long block0) {
     const int per = a.D / 8;
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long i = (block0 + blockIdx.x) * 256 + threadIdx.x;
     const long long rows = (long long)a.n_lanes * a.kv_heads * a.n_slots;
     const long long row = i / per;
     if (row >= rows) return;
@@ -316,10 +316,14 @@ __global__ void __launch_bounds__(256) kv4_copy_kernel(Kv4Copy a) {
 }
 hipError_t launch_kv4_copy(const Kv4Copy& a, bool write, hipStream_t st) {
     const long long n = (long long)a.n_lanes * a.kv_heads * a.n_slots * (a.D / 8), blocks = (n + 255) / 256;
-    if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
-    if (write) hipLaunchKernelGGL(kv4_copy_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(kv4_copy_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, st, a);
-    return hipGetLastError();
+    for (long long b = 0; b < blocks; b += kLaunchBlocks) {
+        const dim3 grid((unsigned)std::min<long long>(kLaunchBlocks, blocks - b));
+        if (write) hipLaunchKernelGGL(kv4_copy_kernel<true>, grid, dim3(256), 0, st, a, b);
+        else hipLaunchKernelGGL(kv4_copy_kernel<false>, grid, dim3(256), 0, st, a, b);
+        const hipError_t rc = hipGetLastError();
+        if (rc != hipSuccess) return rc;
+    }
+    return hipSuccess;
 }
 
 // ------------------------------------------------------------------ attention

@@ -215,3 +215,35 @@ def test_attention_of_many_rows(eng):
     f.c.close()
     del out
     torch.cuda.empty_cache()
+
+
+def test_cache_copies_past_one_launch(eng):
+    """Rows in and out of a 36 GB cache in one call: 2^32 threads' work, more than a launch can have."""
+    import torch
+    from qwen35 import KvCache4
+    lanes, kv, cap, d = 16, 1024, 32768, 64
+    c = KvCache4(eng, lanes, cap, kv_heads=kv, head_dim=d)
+    codes = torch.empty(lanes, kv, cap, d // 2, dtype=torch.uint8, device="cuda")
+    codes.view(torch.int64).random_()
+    scales = torch.randint(8, 250, (lanes, kv, cap, d // 32), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    c.write(0, 0, lanes, 0, cap, codes.data_ptr(), scales.data_ptr(), codes.data_ptr(), scales.data_ptr())
+    got = [torch.empty_like(x) for x in (codes, scales)]
+    torch.cuda.synchronize()
+    c.read(0, 0, lanes, 0, cap, got[0].data_ptr(), got[1].data_ptr(), got[0].data_ptr(), got[1].data_ptr())
+    eng.sync()
+    for i in range(lanes):
+        assert torch.equal(got[0][i], codes[i]) and torch.equal(got[1][i], scales[i]), i
+    # K and V of a few slots apart from each other, in every lane
+    k, v = (torch.empty(1, kv, 40, d // 2, dtype=torch.uint8, device="cuda") for _ in range(2))
+    ks, vs = (torch.empty(1, kv, 40, d // 32, dtype=torch.uint8, device="cuda") for _ in range(2))
+    for i in (0, 7, 8, 15):
+        for s in (0, cap - 40):
+            torch.cuda.synchronize()
+            c.read(0, i, 1, s, 40, k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr())
+            eng.sync()
+            assert torch.equal(k[0], codes[i, :, s:s + 40]) and torch.equal(v, k)
+            assert torch.equal(ks[0], scales[i, :, s:s + 40]) and torch.equal(vs, ks)
+    c.close()
+    del codes, scales, got
+    torch.cuda.empty_cache()
