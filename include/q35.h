@@ -288,7 +288,8 @@ typedef struct q35_view {
 /* q and k of a layer's rows (row i * T + t: sequence i's row at position pos[i] + t), and for an append v.
  * q and k: y = x * rsqrt(mean(x^2) + eps) * (1 + norm) per head (norm [head_dim] bf16), then dims
  * [0, rot_dim) rotated in pairs (d, d + rot_dim / 2) by position * theta^(-2 d / rot_dim); the sum, the
- * root and the angles in float64, the rest in float32, one rounding to bf16 at the end. */
+ * root and the angles in float64, the rest in float32, one rounding to bf16 at the end. A sequence has at most
+ * 2^26 - 4 rows, all together at most 2^31 - 1. */
 typedef struct q35_heads {
     int q_heads, rot_dim;
     double theta, eps;

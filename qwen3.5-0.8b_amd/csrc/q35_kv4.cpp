@@ -94,7 +94,7 @@ HeadArgs head_args(const q35_heads& s, int kv_heads, int D, int n, int T, bool c
     REQ(s.rot_dim >= 0 && s.rot_dim <= D && s.rot_dim % 2 == 0, Q35_ERR_ARG, "rot_dim is even and at most head_dim");
     REQ(s.rot_dim == 0 || (s.theta > 0.0 && std::isfinite(s.theta)), Q35_ERR_ARG, "theta must be positive");
     REQ(s.eps >= 0.0 && std::isfinite(s.eps), Q35_ERR_ARG, "eps must not be negative");
-    REQ(n > 0 && T > 0 && (long long)n * T <= INT32_MAX, Q35_ERR_ARG, "bad sequence or row count");
+    REQ(n > 0 && T > 0 && T <= kHeadRows && (long long)n * T <= INT32_MAX, Q35_ERR_ARG, "bad sequence or row count");
     REQ((s.q.ptr != nullptr) == (s.q_out.ptr != nullptr), Q35_ERR_ARG, "q and q_out go together");
     REQ(!s.q.ptr || s.q_heads > 0, Q35_ERR_ARG, "q without q_heads");
     REQ((!s.q.ptr || s.q_norm) && s.k_norm, Q35_ERR_ARG, "null norm weight");
@@ -121,11 +121,12 @@ HeadArgs head_args(const q35_heads& s, int kv_heads, int D, int n, int T, bool c
     return a;
 }
 
-// The launches of a call: kSeqArgs sequences each.
+// The launches of a call: at most kSeqArgs sequences and kHeadRows rows each.
 void run_heads(HeadArgs a, const int32_t* lanes, const int32_t* pos, int n, hipStream_t st) {
     const auto move = [](HeadView& v, long long rows) { if (v.p) v.p += rows * v.row; };
-    for (int i0 = 0; i0 < n; i0 += kSeqArgs) {
-        const int m = std::min(kSeqArgs, n - i0);
+    const int most = std::min(kSeqArgs, kHeadRows / a.T);
+    for (int i0 = 0, m; i0 < n; i0 += m) {
+        m = std::min(most, n - i0);
         for (int i = 0; i < m; ++i) {
             a.pos[i] = pos[i0 + i];
             a.lane[i] = (uint16_t)(lanes ? lanes[i0 + i] : i0 + i);

@@ -62,7 +62,8 @@ struct HeadArgs {
     uint16_t lane[kSeqArgs];
 };
 // q and k: RMS norm per head and rotation; with a.cache, k and v through 4 bits into the cache. n <= kSeqArgs
-// sequences of T rows.
+// sequences of T rows, n T <= kHeadRows.
+constexpr int kHeadRows = 4 * kLaunchBlocks;   // (a block takes four of many rows)
 hipError_t launch_heads(HeadArgs& a, int n, hipStream_t st);
 
 struct Kv4Attn {

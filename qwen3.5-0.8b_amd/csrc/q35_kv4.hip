@@ -267,7 +267,7 @@ hipError_t launch_heads(HeadArgs& a, int n, hipStream_t st) {
     const int items = ((a.q.p ? per_block * a.q_heads + 3 : 0) / 4) + kinds * ((per_block * a.kv_heads + 3) / 4);
     const int some = rows < 256 ? std::min(items, 4) : items, parts = (items + some - 1) / some;
     const long long blocks = (long long)((rows + per_block - 1) / per_block) * parts;
-    if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+    if (blocks > kLaunchBlocks) return hipErrorInvalidValue;
     a.q_inv = a.q_heads > 1 ? (uint32_t)(0x100000000ull / a.q_heads + 1) : 0;
     a.kv_inv = a.kv_heads > 1 ? (uint32_t)(0x100000000ull / a.kv_heads + 1) : 0;
     const bool quads = a.rot % 8 == 0;

@@ -247,3 +247,21 @@ def test_cache_copies_past_one_launch(eng):
     c.close()
     del codes, scales, got
     torch.cuda.empty_cache()
+
+
+def test_norm_rope_of_many_rows(eng):
+    """2^26 rows in one call, in two launches (8.6 GB of output): one input row, without a rotation."""
+    import torch
+    n, T, d = 2, 2 ** 25, 64
+    rng, D = np.random.default_rng(4), Dev()
+    k, w = D.up(base.bf16_randn(rng, d)), D.up(base.bf16_randn(rng, d, scale=0.1))
+    out = torch.zeros(n, T, d, dtype=torch.int16, device="cuda")
+    one = torch.zeros(1, d, dtype=torch.int16, device="cuda")
+    torch.cuda.synchronize()
+    args = dict(rot_dim=0, theta=1.0, eps=1e-6, q_norm=0, k_norm=w.data_ptr(), k=(k.data_ptr(), 0, 0))
+    eng.op_qk_norm_rope([0], 1, 0, 1, d, k_out=(one.data_ptr(), d, d), **args)
+    eng.op_qk_norm_rope([0, 0], T, 0, 1, d, k_out=(out.data_ptr(), d, d), **args)
+    eng.sync()
+    assert one.any() and all(torch.equal(out[i], one.expand(T, d)) for i in range(n))
+    del out
+    torch.cuda.empty_cache()
