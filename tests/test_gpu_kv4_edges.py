@@ -184,6 +184,101 @@ def test_attention_largest_values(eng, hq, kv, d, T, cap):
     f.c.close()
 
 
+class Pairs:
+    """A cache in which the slots of each pair hold the same K and other V, in every lane and head: a query along that K,
+    steep enough, takes half of each, so a row's answer shows a slot that is left out, counted twice or
+    seen wrongly."""
+
+    def __init__(self, eng, rng, lanes, cap, kv, d, pairs):
+        kc, ks, vc, vs = random_rows(rng, lanes, kv, cap, d)
+        for a, b in pairs:
+            kc[:, :, b], ks[:, :, b] = kc[:, :, a], ks[:, :, a]
+        self.f, self.pairs, self.d = filled(eng, kc, ks, vc, vs), pairs, d
+
+    def run(self, eng, lanes, pos, T, hq, probe, window=0, sinks=0):
+        """probe [n][T][hq]: the pair each row's head asks for."""
+        import torch
+        D, d, n, kv, K = Dev(), self.d, len(lanes), self.f.c.kv_heads, self.f.K
+        first = np.array([p[0] for p in self.pairs])[probe]
+        q = ref.bf16_bits(K[np.array(lanes)[:, None, None], (np.arange(hq) // (hq // kv))[None, None], first])
+        x, out = D.up(q.reshape(n * T, hq, d)), torch.zeros(n * T, hq, d, dtype=torch.int16, device="cuda")
+        torch.cuda.synchronize()
+        scale = 4 * d ** -0.5
+        eng.op_attn_kv4(self.f.c, 0, lanes, pos, T, hq, (x.data_ptr(), hq * d, d), (out.data_ptr(), hq * d, d), scale=scale,
+                        window=window, sinks=sinks)
+        eng.sync()
+        got, told = D.bits(out).reshape(n, T, hq, d), 0
+        for i, (l, p) in enumerate(zip(lanes, pos)):
+            r = ref.val(q[i])
+            o, pv, big = ref.attention(r, K[l], self.f.V[l], p, window, sinks, scale)
+            want, e = ref.attention_bound(o, pv, big, p + T, d)
+            assert np.all(np.abs(ref.val(got[i]) - want) <= e), (l, p)
+            # the reference itself, with the first slot of the last row's pairs left out and counted twice
+            for h in range(hq):
+                a, b = self.pairs[probe[i, T - 1, h]]
+                seen = lambda s: s <= p + T - 1 and (not window or s > p + T - 1 - window or s < sinks)  # noqa: E731
+                if seen(a) and seen(b):
+                    v = self.f.V[l][h // (hq // kv)]
+                    for wa in (0.0, 2.0):
+                        assert np.any(np.abs((wa * v[a] + v[b]) / (wa + 1) - want[T - 1, h]) > e[T - 1, h])
+                    told += 1
+        return told
+
+
+def tile_pairs(rng, tiles, cap):
+    """Every tile's first, last or another slot, paired with one of the tile half the length away."""
+    at = np.array([min(cap - 1, 32 * t + int(rng.choice([0, 31, rng.integers(1, 31)]))) for t in range(tiles)])
+    return [(int(at[i]), int(at[i + tiles // 2])) for i in range(tiles // 2)]
+
+
+@pytest.mark.parametrize("hq,kv,d", [(8, 2, 256), (4, 1, 128), (6, 2, 64)])
+def test_every_tile_of_a_long_context(eng, hq, kv, d):
+    """One lane of 9001 slots over up to 128 blocks (attn_kv4_join), a slot of each of its 282 tiles asked for."""
+    rng = np.random.default_rng(d + 1)
+    P = Pairs(eng, rng, 1, 9001, kv, d, tile_pairs(rng, 282, 9001))
+    told = 0
+    for i in range(0, 141, hq):
+        print(f"tiles {hq} {kv} {d}: pairs from {i}", flush=True)
+        told += P.run(eng, [0], [9000], 1, hq, np.minimum(i + np.arange(hq), 140)[None, None])
+    assert told >= 141
+    P.f.c.close()
+
+
+@pytest.mark.parametrize("hq,kv,d,T,lanes,cap", [(8, 2, 256, 1, 16, 2000), (8, 2, 256, 3, 4, 1100), (8, 2, 128, 9, 2, 1500),
+                                                 (8, 2, 128, 9, 2, 3000), (6, 1, 64, 12, 1, 5000), (8, 2, 256, 12, 1, 5000)])
+def test_tiles_of_split_rows(eng, hq, kv, d, T, lanes, cap):
+    """Ragged lanes of a few splits each (attn_kv4_join_few), and rows of 16 and 32 in more (attn_kv4_join)."""
+    rng = np.random.default_rng(cap + T)
+    tiles = (cap - T) // 32 - 1
+    P = Pairs(eng, rng, lanes, cap, kv, d, tile_pairs(rng, tiles, cap))
+    pos = np.array([cap - T - 37 * i for i in range(lanes)], np.int32)
+    for r in range(2):
+        print(f"split rows {hq} {kv} {d} {T} {lanes} {cap}: {r}", flush=True)
+        probe = rng.integers(0, len(P.pairs), (lanes, T, hq))
+        assert P.run(eng, np.arange(lanes), pos, T, hq, probe) > 0
+    P.f.c.close()
+
+
+@pytest.mark.parametrize("hq,kv,d,T", [(8, 2, 256, 1), (8, 1, 128, 1), (4, 2, 64, 40)])
+def test_slots_at_the_ends_of_a_window(eng, hq, kv, d, T):
+    """The last sink and the slot behind it, the window's first slot and the one before it, the row's own and the
+    next: each paired with a slot inside, in windows that end in and between tiles, over many splits and few."""
+    rng = np.random.default_rng(d + T)
+    cap, inside = 9001, 8900
+    for window, sinks in [(5000, 40), (4992, 32), (2049, 1), (300, 64), (4000, 0)]:
+        p = cap - 1 - T
+        low = p - window + 1
+        ends = {0, sinks - 1, sinks, low - 1, low, low + T - 1, low + T, p, p + T - 1, p + T}
+        ends = [s for s in sorted(ends) if 0 <= s < cap]
+        pairs = [(s, inside + i) for i, s in enumerate(ends)]
+        P = Pairs(eng, rng, 1, cap, kv, d, pairs)
+        print(f"window ends {hq} {kv} {d} {T}: {window} {sinks}", flush=True)
+        for i in range(0, len(pairs), hq):
+            probe = np.broadcast_to(np.minimum(i + np.arange(hq), len(pairs) - 1), (1, T, hq))
+            P.run(eng, [0], [p], T, hq, probe, window, sinks)
+        P.f.c.close()
+
+
 # ------------------------------------------------------------------------------ calls and their sizes
 def test_calls_after_a_refused_allocation(eng):
     """A cache that no memory holds is refused, and the next call does not report that error again."""
