@@ -118,6 +118,20 @@ def test_norm_rope_tiny_and_huge_heads(eng, d, rot):
     same(D.bits(p.k), want[:, 2:], size[:, 2:])
 
 
+@pytest.mark.parametrize("hq,kv,d,rot", [(5, 1, 128, 128), (3, 3, 128, 100), (14, 2, 64, 64), (8, 2, 256, 256), (2, 1, 256, 2)])
+@pytest.mark.parametrize("n,T", [(1, 1025), (205, 5), (1, 4099), (17, 241), (300, 15)])
+def test_norm_rope_rows_in_blocks(eng, hq, kv, d, rot, n, T):
+    """Two rows a block from 1024 rows on, four from 4096: waves that take heads of two rows, a short last block, the
+    whole table of angles, blocks over the border of two sequences."""
+    base.test_norm_rope(eng, hq, kv, d, rot, n, T)
+
+
+@pytest.mark.parametrize("hq,kv,d,rot", [(5, 1, 128, 128), (3, 3, 64, 6), (8, 2, 256, 256)])
+@pytest.mark.parametrize("n,T,pos0", [(1, 1025, 7), (41, 25, 3), (1, 4099, 30), (17, 241, 17)])
+def test_append_rows_in_blocks(eng, hq, kv, d, rot, n, T, pos0):
+    base.test_append(eng, hq, kv, d, rot, n, T, pos0)
+
+
 # ------------------------------------------------------------------------------ attention
 def filled(eng, kc, ks, vc, vs):
     """A cache of one layer with these codes and scale bytes [lanes][kv][cap][..], and its values."""
