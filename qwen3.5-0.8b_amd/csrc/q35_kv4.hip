@@ -14,7 +14,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((__vector_size__(8 * sizeof(float)))) float f32x8;
 
 // The pair of values in byte SEL of w, times the power of two in `scale`'s exponent: exact; NaN
-// where that exponent is 255 (all 256 bytes x 245 scales and 255 compared on MI355X).
+// where that exponent is 255 (all 256 bytes x scales 0 to 252 and 255 compared on MI355X).
 template <int SEL>
 __device__ __forceinline__ uint32_t two_values(uint32_t w, float scale) {
     const bf16x2 r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, SEL);

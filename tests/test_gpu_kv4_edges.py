@@ -198,6 +198,24 @@ def test_attention_largest_values(eng, hq, kv, d, T, cap):
     f.c.close()
 
 
+def test_attention_smallest_scales(eng):
+    """Scale bytes 0 to 8 with every pair of codes, written by the caller: a row that sees one slot gives its V exactly,
+    down to 2^-128; as K they give scores next to 0."""
+    rng, kv, d = np.random.default_rng(9), 2, 256
+    kc, ks, vc, vs = random_rows(rng, 1, kv, 9, d)
+    vs[0] = np.arange(9)[None, :, None]
+    vc[0] = np.arange(256).reshape(kv, 1, 128)
+    f = filled(eng, kc, ks, vc, vs)
+    got, q, g = run_attention(eng, f, [0], [0], 9, kv, rng, window=1)
+    assert np.array_equal(ref.val(got), f.V[0].transpose(1, 0, 2))
+    ks[0] = np.arange(9)[None, :, None]
+    f2 = filled(eng, kc, ks, *random_rows(rng, 1, kv, 9, d)[2:])
+    got, q, g = run_attention(eng, f2, [0], [8], 1, kv, rng)
+    check_attention(f2, [0], [8], 1, got, q, g)
+    f.c.close()
+    f2.c.close()
+
+
 class Pairs:
     """A cache in which the slots of each pair hold the same K and other V, in every lane and head: a query along that K,
     steep enough, takes half of each, so a row's answer shows a slot that is left out, counted twice or
