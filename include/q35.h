@@ -271,8 +271,8 @@ int q35_kv4_set_len(q35_engine* e, q35_kv4* c, const int32_t* lanes, const int32
 int q35_kv4_len(q35_engine* e, q35_kv4* c, int layer, int lane, int32_t* out);
 /* Slots [slot0, slot0 + n_slots) of lanes [lane0, lane0 + n_lanes) from / to device buffers in row order: codes
  * [n_lanes][kv_heads][n_slots][head_dim / 2], two codes a byte, the lower dim in the low nibble;
- * scales [n_lanes][kv_heads][n_slots][head_dim / 32] (a scale byte above 252 is stored as 255, NaN). A write
- * starts at most at a lane's length and raises it to slot0 + n_slots; a read stays below it. */
+ * scales [n_lanes][kv_heads][n_slots][head_dim / 32] (a scale byte above 252 is stored as 255, NaN; others as they
+ * are). A write starts at most at a lane's length and raises it to slot0 + n_slots; a read stays below it. */
 int q35_kv4_write(q35_engine* e, q35_kv4* c, int layer, int lane0, int n_lanes, int slot0, int n_slots,
                   const uint8_t* k_codes, const uint8_t* k_scales, const uint8_t* v_codes, const uint8_t* v_scales);
 int q35_kv4_read(q35_engine* e, q35_kv4* c, int layer, int lane0, int n_lanes, int slot0, int n_slots, uint8_t* k_codes,
@@ -309,7 +309,9 @@ int q35_op_kv4_append(q35_engine* e, q35_kv4* c, int layer, const int32_t* lanes
  * lanes[i], p = pos[i] + t; window 0: [0, p]. The lane must hold pos[i] + T slots, the rows' own included;
  * a lane may occur more than once; scale * log2(e) is finite in float32. out = softmax(scale * q K^T) V,
  * times sigmoid(gate) if gate is given, in float32 with the weights rounded to bf16 for the product with V,
- * and one rounding to bf16. A NaN in a slot reaches the rows that see it and no others. */
+ * and one rounding to bf16. A NaN in a slot reaches the rows that see it and no others. How a row's slots are
+ * split over the card depends on all the call's sequences, so its last bits may too (the same call gives the same
+ * bits); a sequence with pos[i] + T up to 256 stays in one piece. */
 int q35_op_attn_kv4(q35_engine* e, q35_kv4* c, int layer, const int32_t* lanes, const int32_t* pos, int n, int T,
                     int q_heads, const q35_view* q, const q35_view* gate, float scale, int window, int sinks,
                     const q35_view* out);

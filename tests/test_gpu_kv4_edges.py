@@ -311,6 +311,28 @@ def test_slots_at_the_ends_of_a_window(eng, hq, kv, d, T):
         P.f.c.close()
 
 
+def test_a_rows_bits_do_not_depend_on_the_others(eng):
+    """Lanes whose rows stay in one split give the same bits in another order, among fewer lanes, beside other rows and
+    on the other side of a launch's 256 sequences."""
+    import torch
+    rng, D, n, hq, d = np.random.default_rng(15), Dev(), 300, 8, 256
+    f = Filled(eng, rng, n, 64, 2, d)
+    pos, qb = rng.integers(0, 62, n).astype(np.int32), base.bf16_randn(rng, n, 2, hq, d)
+
+    def call(lanes):
+        q = D.up(qb[lanes].reshape(-1, hq, d))
+        out = torch.zeros_like(q)
+        torch.cuda.synchronize()
+        eng.op_attn_kv4(f.c, 0, lanes, pos[lanes], 2, hq, (q.data_ptr(), hq * d, d), (out.data_ptr(), hq * d, d))
+        eng.sync()
+        return D.bits(out).reshape(len(lanes), 2, hq, d)
+
+    whole = call(np.arange(n))
+    for lanes in (rng.permutation(n), rng.permutation(n)[:280], np.array([299]), np.array([7, 250, 7])):
+        assert np.array_equal(call(lanes), whole[lanes])
+    f.c.close()
+
+
 # ------------------------------------------------------------------------------ calls and their sizes
 def test_calls_after_a_refused_allocation(eng):
     """A cache that no memory holds is refused, and the next call does not report that error again."""
