@@ -443,6 +443,8 @@ void ensure_logits(q35_engine* e, int rows) {
         for (auto& kv : e->graphs) hipGraphExecDestroy(kv.second);
         e->graphs.clear();
         HCK(hipFree(e->logits_dev));
+        e->logits_dev = nullptr;         // the allocation below may fail
+        e->logits_rows = 0;
     }
     e->logits_dev = dalloc<float>((size_t)rows * kVocab);
     e->logits_rows = rows;
