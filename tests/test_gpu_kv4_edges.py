@@ -414,3 +414,31 @@ def test_norm_rope_of_many_rows(eng):
     assert one.any() and all(torch.equal(out[i], one.expand(T, d)) for i in range(n))
     del out
     torch.cuda.empty_cache()
+
+
+def test_lanes_past_32_bit_offsets(eng):
+    """Append, attention and read at the end of a lane, 6.8 GB into the cache."""
+    import torch
+    from qwen35 import KvCache4
+    rng, D, kv, d, cap, T = np.random.default_rng(16), Dev(), 1024, 64, 32768, 3
+    c = KvCache4(eng, 3, cap, kv_heads=kv, head_dim=d)
+    pos = cap - T
+    c.set_len([2], [pos])
+    x = base.bf16_randn(rng, T, 3 * kv, d)                   # q, k, v
+    w = D.up(np.zeros(d, np.uint16))
+    t, q = D.up(x), torch.zeros(T, kv, d, dtype=torch.int16, device="cuda")
+    out = torch.zeros_like(q)
+    torch.cuda.synchronize()
+    p, ld = t.data_ptr(), 3 * kv * d
+    eng.op_kv4_append(c, 0, [2], [pos], T, kv, rot_dim=0, theta=1.0, eps=1e-6, q_norm=w.data_ptr(), k_norm=w.data_ptr(),
+                      q=(p, ld, d), k=(p + 2 * kv * d, ld, d), v=(p + 4 * kv * d, ld, d), q_out=(q.data_ptr(), kv * d, d))
+    eng.op_attn_kv4(c, 0, [2], [pos], T, kv, (q.data_ptr(), kv * d, d), (out.data_ptr(), kv * d, d), window=2)
+    eng.sync()
+    kc, ks, vc, vs = read_cache(eng, c, 0, 2, 1, pos, T)
+    base.check_codes(ref.val(x[:, 2 * kv:]).transpose(1, 0, 2), vc[0], vs[0], 0.0)
+    K, V = ref.values(kc, ks)[0], ref.values(vc, vs)[0]
+    o, pv, big = ref.attention(ref.val(D.bits(q)), K, V, 0, 2, 0, d ** -0.5)
+    want, e = ref.attention_bound(o, pv, big, cap, d)
+    g = ref.val(D.bits(out))
+    assert np.all(np.abs(g - want)[1:] <= e[1:])             # (row 0 sees the slot before the appended ones, too)
+    c.close()
