@@ -115,10 +115,10 @@ __device__ __forceinline__ double rsqrt_d(double x) {
 // squares, the root and the angles are float64. QUADS: rot / 2 is a multiple of 4, so a lane's four dims lie
 // on one side of the pairs. TINY: eps is so small (under 2^-250) that a root may pass float32; without that form's care
 // 1999 rows as below take 0.4 us less.
-// Many rows: HBM and the instructions a head takes share the time (4096 rows of 8 + 2 heads of 256, 42 MB: 11.6 us;
-// 1999 rows of 32 + 2 x 8 heads of 128 with the append, 51 MB: 15.7 us, its codes in stores of 2 bytes a lane that the
-// cache's fragment order scatters); few rows: the chain of launch, loads and angles (1 row 3.7 us, 256 rows with
-// the append 5.4).
+// Many rows: memory and the instructions a head takes share the time (4096 rows of 8 + 2 heads of 256, 42 MB: 11.2 us,
+// the VALU at work in 65 % of the CUs' busy cycles; 1999 rows of 32 + 2 x 8 heads of 128 with the append, 51 MB:
+// 14.9 us, 75 %, its codes in stores of 2 bytes a lane that the cache's fragment order scatters); few rows: the chain
+// of launch, loads and angles (1 row 3.5 us, 256 rows with the append 5.5).
 constexpr int kBlockRows = 4;
 template <int D, bool QUADS, bool TINY>
 __global__ void __launch_bounds__(256) heads_kernel(HeadArgs a, int rows, int per_block, int parts, int some) {
@@ -260,9 +260,10 @@ __global__ void __launch_bounds__(256) heads_kernel(HeadArgs a, int rows, int pe
 
 hipError_t launch_heads(HeadArgs& a, int n, hipStream_t st) {
     const int rows = n * a.T, kinds = a.v.p ? 2 : 1;
-    // rows of a block: one while they are too few to give every CU two blocks of two, else up to four (1999 rows of 32 q
-    // heads by one 16.4 us, two 15.8, four 19.7; 4096 of 8 by one 17.1, two 14.2, four 12.1); of very few rows
-    // with many heads, four wave items (one a wave) in a block
+    // rows of a block: two when that leaves every CU two blocks or more, four when it leaves every CU four (1999 rows of
+    // 32 q heads by one 16.4 us, two 15.8, four 19.7; 4096 of 8 by one 17.1, two 14.2, four 12.1: both lines lie between
+    // these two shapes, and the number of heads is not in them); of very few rows with many heads, four wave
+    // items (one a wave) in a block
     const int per_block = rows >= 4096 ? kBlockRows : rows >= 1024 ? 2 : 1;
     const int items = ((a.q.p ? per_block * a.q_heads + 3 : 0) / 4) + kinds * ((per_block * a.kv_heads + 3) / 4);
     const int some = rows < 256 ? std::min(items, 4) : items, parts = (items + some - 1) / some;
@@ -334,8 +335,9 @@ hipError_t launch_kv4_copy(const Kv4Copy& a, bool write, hipStream_t st) {
 // Decode and verify rows are bound by the cache's bytes: 256 lanes x 4096 slots of 2 heads of 256 (574 MB) 88 us,
 // 6.5 TB/s; 128 lanes x 3 rows x up to 2000 slots (84 MB) 23 us and a join of 4, a block a CU or two for 40 tiles.
 // Prompts are bound by what the VALU issues beside the MFMAs, most of it making bf16 fragments of codes (192 of a
-// step's 293 instructions for 66 MFMAs of 32 rows): 4096 rows of 8 heads of 256 (69 GFLOP) 97 us, 8192 rows 323 (850
-// TFLOP/s; a library's 8192^3 product reaches 1191).
+// step's 293 instructions for 66 MFMAs of 32 rows): 4096 rows of 8 heads of 256 (69 GFLOP) 85 us, 8192 rows 279 (985
+// TFLOP/s; a library's 8192^3 product reaches 1191). These are launches back to back; the first ones after a card that
+// idled take 98 and 320.
 template <int D>
 struct Tile {
     u32x4 k[D / 64], v[D / 64];
@@ -513,7 +515,9 @@ __device__ __forceinline__ void tile_step(Tile<D>& t, const uint8_t* tile_p, con
             const float x = s[c][j >> 2][j & 3];
             p[j] = __builtin_amdgcn_exp2f(FAR ? x * scale2 - ms : __builtin_fmaf(x, scale2, -ms));
         }
-        // weights rounded to bf16 (2^-9) for the product; their sum is that of the rounded ones, a product with ones
+        // Weights rounded to bf16 (2^-8 at most) for the product, as V's values are bf16 and the MFMA takes one type: a
+        // float32 product has a sixteenth of its rate. Their sum is that of the rounded ones, a product with ones. Against 64
+        // bits outputs are off by 0.0021 to 0.0023 of their size, of which the last rounding alone makes 0.0017.
         const f32x8 pw = {p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]};
         pf[c] = __builtin_convertvector(pw, q35_bf16x8);     // not f2bf2: the compiler must see what an MFMA is about to read
         st.l[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_bf16x8, u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}),
@@ -630,9 +634,9 @@ __device__ __forceinline__ const float* part_of(const Kv4Attn& a, int row_tiles,
 // A block per (sequence, split of its tiles, kv head, NQ x 16 rows): its four waves take every fourth tile
 // with the next ones' loads in flight, and their states are joined through LDS. Under the causal mask the last
 // row tiles are the longest: they come first, so that the short ones fill the CUs' ends (4096 rows of 8 heads of
-// 256 in one prompt 96 us; each block with a long and a short tile in turn 100). One sequence of at most
-// two blocks a CU has them all at once: the second of a CU is then short where the first is long (2048 rows 35 us,
-// without 38, ascending 47).
+// 256 in one prompt 96 us, launched with waits between; each block with a long and a short tile in turn 100). One sequence
+// of at most two blocks a CU has them all at once: the second of a CU is then short where the first is long (2048
+// rows 35 us, without 38, ascending 47; back to back it takes 34).
 template <int D, int NQ>
 __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) attn_kv4_kernel(Kv4Attn a, int row_tiles) {
     constexpr int kQuarter = D / 64;         // of the D / 16 accumulators of 16 rows
@@ -851,7 +855,7 @@ __global__ void __launch_bounds__(256) attn_kv4_join_few(Kv4Attn a, int row_tile
 
 // The same for any number of splits: a block per (sequence, kv head, row, 64 dims). The splits' factors are
 // made once into LDS; 16 threads take a split's dims, 16 splits at a time, and their sums meet in LDS:
-// always in the same order. Latency here too: 8 rows of 128 splits 4.6 us.
+// always in the same order. Latency here too: 8 rows of 128 splits 4.5 us.
 template <int D, int NQ>
 __global__ void __launch_bounds__(256) attn_kv4_join(Kv4Attn a, int row_tiles) {
     __shared__ float fs[kSeqSplits];

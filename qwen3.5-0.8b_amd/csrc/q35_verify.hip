@@ -139,8 +139,8 @@ __device__ __forceinline__ Stat* stats_of(const VerifyArgs& a, int lane, int j) 
 }
 
 // A block per (chunk, row): the chunk in registers, its maximum, then its sum of exponentials. Bound by HBM: 256 lanes
-// x 3 rows of 248,320 float32 logits (763 MB) 142 to 154 us, 5.0 to 5.4 TB/s (with a ninth degree in place of the
-// table 174; chunks of 4096 instead of 8192 in turn 158 to 142).
+// x 3 rows of 248,320 float32 logits (763 MB) 132 us, 5.8 TB/s, launched back to back (with waits between 142 to 154, and
+// so measured: with a ninth degree in place of the table 174, chunks of 4096 instead of 8192 in turn 158 to 142).
 template <bool BF16, int LOADS>
 __global__ void __launch_bounds__(256) verify_stats(VerifyArgs a) {
     constexpr int N = BF16 ? 8 : 4;
@@ -354,7 +354,7 @@ struct Weights {
 
 // With a drafter's probabilities: the lanes' decisions, kept for verify_token, and the chunks' sums of max(p - q, 0)
 // for those that draw from it. A block per (chunk, lane); each block decides for itself, which costs less than another
-// launch would. 17 lanes x 4 drafts of 32,003 bfloat16 logits: 7.7 us, most of it the chain from the drafts to the
+// launch would. 17 lanes x 4 drafts of 32,003 bfloat16 logits: 7.4 us, most of it the chain from the drafts to the
 // decision to the row.
 template <bool BF16>
 __global__ void __launch_bounds__(256) verify_rest(VerifyArgs a, double* rest, Fate* fates) {
@@ -404,7 +404,7 @@ __device__ __forceinline__ int2 block_ends(int first, int last, int2* ends) {
     return make_int2(first, last);
 }
 
-// A block per lane: the decision, the chunk that holds the border, the token in it. One lane 7.0 us, 256 lanes 14.6: a
+// A block per lane: the decision, the chunk that holds the border, the token in it. One lane 7.0 us, 256 lanes 12.9: a
 // chain of four trips to memory and five block-wide sums. (Joined to verify_stats by its last blocks it would need a
 // device-wide release a block, which writes the caches back: 1256 us instead of 164 + 15; by relaxed counts 283.)
 template <bool BF16>
