@@ -442,3 +442,31 @@ def test_lanes_past_32_bit_offsets(eng):
     g = ref.val(D.bits(out))
     assert np.all(np.abs(g - want)[1:] <= e[1:])             # (row 0 sees the slot before the appended ones, too)
     c.close()
+
+
+def test_the_most_lanes_and_the_largest_windows(eng):
+    """A cache of 65,535 lanes, all of them in one append and one attention, the last lane first; windows and sinks of
+    2^31 - 1 see what no window sees."""
+    import torch
+    from qwen35 import KvCache4
+    rng, D, n, d, big = np.random.default_rng(17), Dev(), 65535, 64, 2 ** 31 - 1
+    c = KvCache4(eng, n, 3, kv_heads=1, head_dim=d)
+    lanes, pos = np.arange(n, dtype=np.int32)[::-1].copy(), np.zeros(n, np.int32)
+    x = base.bf16_randn(rng, n, 3, d)                        # q, k, v
+    w = D.up(np.zeros(d, np.uint16))
+    t, q, out = D.up(x), *(torch.zeros(n, d, dtype=torch.int16, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    p = t.data_ptr()
+    eng.op_kv4_append(c, 0, lanes, pos, 1, 1, rot_dim=0, theta=1.0, eps=1e-6, q_norm=w.data_ptr(), k_norm=w.data_ptr(),
+                      q=(p, 3 * d, d), k=(p + 2 * d, 3 * d, d), v=(p + 4 * d, 3 * d, d), q_out=(q.data_ptr(), d, d))
+    eng.op_attn_kv4(c, 0, lanes, pos, 1, 1, (q.data_ptr(), d, d), (out.data_ptr(), d, d))
+    eng.sync()
+    kc, ks, vc, vs = read_cache(eng, c, 0, 0, n, 0, 1)
+    base.check_codes(ref.val(x[:, 2]), vc[lanes, 0, 0], vs[lanes, 0, 0], 0.0)
+    assert np.array_equal(ref.val(D.bits(out)), ref.values(vc, vs)[lanes, 0, 0])      # one slot: its V
+    c.close()
+    f = Filled(eng, rng, 1, 400, 2, 128)
+    for window, sinks in [(big, 0), (big, big), (3, big)]:
+        got, q, g = run_attention(eng, f, [0], [380], 20, 4, rng, window, sinks)
+        check_attention(f, [0], [380], 20, got, q, g)
+    f.c.close()
