@@ -658,8 +658,8 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) attn_kv4_kernel(Kv4Attn
     const int seq = sq.i, splits = sq.splits, pos = sq.pos, group = a.q_heads / a.kv_heads, rows = a.T * group;
     const uint8_t* region = a.cache + sq.lane * a.lane_bytes + h * a.region;
     // positive, so that the largest product has the largest exponent and a dropped one's -inf stays it: a negative
-    // scale's sign goes to q, 0 becomes the smallest normal number
-    const float scale2 = fmaxf(fabsf(a.scale) * 1.44269504088896f, 1.17549435e-38f);
+    // scale's sign goes to q, 0 becomes the smallest number there is (the largest product then counts 5e-7)
+    const float scale2 = fmaxf(fabsf(a.scale) * 1.44269504088896f, 0x1p-149f);
     const Lanes lo = lane_offsets<D>();
     const int rho0 = rt * NQ * 16, rho1 = min(rho0 + NQ * 16, rows) - 1;
     const TileList tl = tile_list(pos + rho0 / group, pos + rho1 / group, a.window, a.sinks);

@@ -198,6 +198,22 @@ def test_attention_largest_values(eng, hq, kv, d, T, cap):
     f.c.close()
 
 
+@pytest.mark.parametrize("T", [1, 20])
+def test_attention_scale_of_zero_and_next_to_it(eng, T):
+    """Products near 10^38 times a scale of 0 or of a subnormal number: even weights, and those of the formula."""
+    import torch
+    rng, D, d, cap, hq = np.random.default_rng(18), Dev(), 128, 300, 4
+    f = Filled(eng, rng, 1, cap, 2, d)
+    qb = base.bf16_randn(rng, T, hq, d, scale=2e36)
+    q, out = D.up(qb), torch.zeros(T, hq, d, dtype=torch.int16, device="cuda")
+    torch.cuda.synchronize()
+    for scale in (0.0, 3e-38, 1e-39, -1e-39, 2e-41):
+        eng.op_attn_kv4(f.c, 0, [0], [cap - T], T, hq, (q.data_ptr(), hq * d, d), (out.data_ptr(), hq * d, d), scale=scale)
+        eng.sync()
+        check_attention(f, [0], [cap - T], T, D.bits(out), ref.val(qb), None, scale=float(np.float32(scale)))
+    f.c.close()
+
+
 def test_attention_smallest_scales(eng):
     """Scale bytes 0 to 8 with every pair of codes, written by the caller: a row that sees one slot gives its V exactly,
     down to 2^-128; as K they give scores next to 0."""
