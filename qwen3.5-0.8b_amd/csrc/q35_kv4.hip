@@ -433,7 +433,7 @@ struct Rows {
 // V, is used up. TIGHT: 32 rows of 256 dims leave no register for fragments made far ahead.
 // edge: some row may not see some slot. FAR: a score times scale2 is rounded before the reference is taken off, and the
 // reference lies 28 above the maximum it was taken from, so that weights stay under 2^-20 and 2^18 slots' sum of
-// them times the largest V is still a float32.
+// them times the largest V is still a float32 (from references of 2^29 on their spacing takes the 28 in).
 template <int D, int NQ, bool ONCE, bool TIGHT, bool FAR, class Q>
 __device__ __forceinline__ void tile_step(Tile<D>& t, const uint8_t* tile_p, const uint8_t* next_p, const Lanes& lo, int slot0,
                                           bool edge, const Q& q, const Sight* sight, float scale2, Rows<D, NQ>& st) {
