@@ -304,6 +304,19 @@ int q35_op_qk_norm_rope(q35_engine* e, const q35_heads* h, int kv_heads, int hea
  * pos[i] + T; no lane twice. k_out / v_out (nullable): the values that the new codes stand for. */
 int q35_op_kv4_append(q35_engine* e, q35_kv4* c, int layer, const int32_t* lanes, const int32_t* pos, int n, int T,
                       const q35_heads* h);
+/* The same two for rows at positions on up to four axes (a prompt with images: time, height, width), and with an append's
+ * slots apart from its positions (slots behind a prefix that other lanes share, or behind images, whose tokens
+ * outnumber their positions): pair d turns by the row's position on axis axis[d], times theta^(-2 d / rot_dim). axis: host
+ * memory, rot_dim / 2 bytes of 0 .. 3. Positions are device memory, any int32; pos and axis may be NULL with rot_dim 0. */
+typedef struct q35_positions {
+    const int32_t* pos;                  /* row r's position on axis a: pos[r * row_stride + a * axis_stride] */
+    int64_t row_stride, axis_stride;     /* in elements, not negative */
+} q35_positions;
+int q35_op_qk_norm_rope_axes(q35_engine* e, const q35_heads* h, int kv_heads, int head_dim, const q35_positions* at,
+                             const uint8_t* axis, int rows);
+/* Row i * T + t goes into slot slots[i] + t of lane lanes[i]; slots[i] is at most the lane's length. */
+int q35_op_kv4_append_axes(q35_engine* e, q35_kv4* c, int layer, const int32_t* lanes, const int32_t* slots, int n, int T,
+                           const q35_heads* h, const q35_positions* at, const uint8_t* axis);
 /* Attention over the cache: row i * T + t of q (normed and rotated, q_heads a multiple of kv_heads, query
  * head h on kv head h / (q_heads / kv_heads)) sees slots (p - window, p] and [0, sinks) of lane
  * lanes[i], p = pos[i] + t; window 0: [0, p]. The lane must hold pos[i] + T slots, the rows' own included;
@@ -315,6 +328,14 @@ int q35_op_kv4_append(q35_engine* e, q35_kv4* c, int layer, const int32_t* lanes
 int q35_op_attn_kv4(q35_engine* e, q35_kv4* c, int layer, const int32_t* lanes, const int32_t* pos, int n, int T,
                     int q_heads, const q35_view* q, const q35_view* gate, float scale, int window, int sinks,
                     const q35_view* out);
+/* The same for answers that share prompts: row i * T + t sees slots [0, prefix_lens[i]) of lane prefix_lanes[i] of
+ * `prefix` and slots [0, pos[i] + t] of lane lanes[i] of c, in one softmax. Both caches have the same heads, and each its
+ * own lanes and capacity; they may be the same one (a lane is not its own prefix). Sequences that name the same lane and length share
+ * the reading of it, in any order; prefix_lanes[i] < 0 or prefix_lens[i] 0: no prefix. Positions count c's slots: the keys'
+ * rotation is whatever they were appended with (q35_op_kv4_append_axes). Rounding, NaN and repetition as above. */
+int q35_op_attn_kv4_shared(q35_engine* e, q35_kv4* prefix, q35_kv4* c, int layer, const int32_t* prefix_lanes,
+                           const int32_t* prefix_lens, const int32_t* lanes, const int32_t* pos, int n, int T, int q_heads,
+                           const q35_view* q, const q35_view* gate, float scale, const q35_view* out);
 
 /* Sampled verification of drafted tokens from given random numbers (the reference verifies greedily,
  * engine/mtp_accept.h:248). Lane i has k <= 8 drafts, k + 1 rows of target logits, with p_j =
@@ -340,6 +361,27 @@ typedef struct q35_drafts {
     double temperature;              /* 0, or at least 0.001 */
 } q35_drafts;
 int q35_op_draft_verify(q35_engine* e, const q35_drafts* d, int n, int k, int vocab, int32_t* accepted, int32_t* tokens);
+/* How probable given tokens were: for each row of logits, with p = softmax(logits / temperature), log p of its target, the
+ * target's rank (the ids before it by falling logit, then by rising id: 0 is the argmax), the entropy -sum p log p,
+ * and the first `top` ids of that order with their log p (the reference hands a prompt's whole logits to its caller,
+ * engine/prefill.h:46-58). One pass over the logits; sums that end in float64, results rounded once to float32. A target
+ * that is no id (negative, or vocab or more) has log p NaN and rank -1; a row with a NaN, a +inf or only -inf logits has no
+ * distribution: NaN throughout, rank and ids -1. An id with logit -inf has log p -inf. Outputs that are NULL are
+ * left out. Any number of rows. Enqueued on the engine stream without waiting; its workspace is the engine's. */
+typedef struct q35_logprobs {
+    const void* logits;              /* device [rows][ld], ld at least vocab */
+    int64_t ld;
+    int dtype;                       /* 0 float32, 1 bfloat16 */
+    const int32_t* targets;          /* device [rows], or NULL: no log probabilities and ranks */
+    double temperature;              /* 0.001 .. 1000 */
+    int top;                         /* 0 .. 32, at most vocab */
+    float* logprobs;                 /* device [rows] */
+    int32_t* ranks;                  /* device [rows] */
+    float* entropy;                  /* device [rows] */
+    int32_t* top_ids;                /* device [rows][top] */
+    float* top_logprobs;             /* device [rows][top] */
+} q35_logprobs;
+int q35_op_token_logprobs(q35_engine* e, const q35_logprobs* d, int rows, int vocab);
 int q35_sync(q35_engine* e);
 /* Live per-kernel timing: with option "kprof" = family (1 projection/MLP GEMMs, 2 lm_head
  * GEMM, 3 GDN recurrence, 4 attention core, 0 off), each launch of that family is bracketed

@@ -27,7 +27,7 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-ffp-contract=o
 # MFMA accumulators in architectural VGPRs: without it the compiler keeps loop-carried
 # accumulators in AGPRs and copies them to VGPRs and back around every VALU touch of them
 # (the prompt attention's online-softmax rescale: ~190 v_accvgpr moves per K/V tile)
-FILE_FLAGS = {"q35_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"], "q35_kv4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+FILE_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("q35_attn.hip", "q35_kv4.hip", "q35_kv4_shared.hip")}
 
 
 def _compile(src: Path) -> Path:

@@ -18,6 +18,7 @@
 #include <vector>
 
 #include "../../include/q35.h"
+#include "q35_answers.h"
 #include "q35_common.h"
 #include "q35_host.h"
 #include "q35_kernels.h"
@@ -123,6 +124,7 @@ struct q35_engine {
     float* kpart;
     float* kv4_part = nullptr;       // the 4-bit cache's attention: partial results of split rows
     double* verify_ws = nullptr;     // draft verification: the rows' chunk statistics
+    char* logprob_ws = nullptr;      // token log probabilities: the rows' parts
     int *verify_io = nullptr, *h_verify_io = nullptr;   // sampled rounds: [drafts | u | accepted | tokens], R each
     uint16_t* prod;
     int *pidx, *tok_dev, *rlane, *rpos, *rslot, *rcur, *rwcur, *rpend, *ridx_src, *ridx_dst, *din = nullptr;
@@ -403,6 +405,7 @@ void alloc_scratch(q35_engine* e) {
     e->topv_dev = dalloc<float>(R);
     e->kv4_part = dalloc<float>(kv4_part_floats());
     e->verify_ws = dalloc<double>(verify_ws_doubles((int)R));
+    e->logprob_ws = dalloc<char>(logprob_ws_bytes());
     e->verify_io = dalloc<int>(4 * R);
     e->h_verify_io = halloc<int>(4 * R);
     e->gchunk = dalloc<float>(gdn_chunk_ws_floats(R));
@@ -871,7 +874,7 @@ int q35::guard(const std::function<void()>& f) {
     }
 }
 
-q35::EngineView q35::engine_view(q35_engine* e) { return {e->device, e->R, e->max_ctx, e->st, e->kv4_part, e->verify_ws}; }
+q35::EngineView q35::engine_view(q35_engine* e) { return {e->device, e->R, e->max_ctx, e->st, e->kv4_part, e->verify_ws, e->logprob_ws}; }
 
 // ====================================================================== C ABI
 extern "C" {
@@ -909,7 +912,8 @@ int q35_destroy(q35_engine* e) {
         e->graphs.clear();
         void* ds[] = {e->blob, e->x, e->h, e->delta, e->nrm, e->proj, e->gu, e->aout, e->cat, e->o, e->q,
                       e->sc, e->stats, e->part, e->pval, e->pidx, e->prod, e->din, e->inv_freq,
-                      e->logits_dev, e->kpart, e->gchunk, e->gcdec, e->topv_dev, e->kv4_part, e->verify_ws, e->verify_io};
+                      e->logits_dev, e->kpart, e->gchunk, e->gcdec, e->topv_dev, e->kv4_part, e->verify_ws, e->logprob_ws,
+                      e->verify_io};
         for (void* p : ds) if (p) hipFree(p);
         void* hs[] = {e->hin, e->h_out, e->h_verify_io};
         for (void* p : hs) if (p) hipHostFree(p);

@@ -24,6 +24,7 @@ struct EngineView {
     hipStream_t st;
     float* kv4_part;
     double* verify_ws;
+    char* logprob_ws;
 };
 EngineView engine_view(q35_engine* e);
 

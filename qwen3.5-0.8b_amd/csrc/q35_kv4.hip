@@ -1,26 +1,11 @@
 // Head norms with rotation, the 4-bit K/V cache, and the attention that reads it.
 #include <algorithm>
 #include <cstring>
+#include <type_traits>
 
-#include "q35_common.h"
-#include "q35_kv4.h"
+#include "q35_kv4_tile.h"
 
 namespace q35 {
-
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((__vector_size__(8 * sizeof(float)))) float f32x8;
-
-// The pair of values in byte SEL of w, times the power of two in `scale`'s exponent: exact; NaN
-// where that exponent is 255 (all 256 bytes x scales 0 to 252 and 255 compared on MI355X).
-template <int SEL>
-__device__ __forceinline__ uint32_t two_values(uint32_t w, float scale) {
-    const bf16x2 r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, SEL);
-    return __builtin_bit_cast(uint32_t, r);
-}
-__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
 
 __device__ __forceinline__ f32x4 wide(uint2 w) {          // four bf16
     return f32x4{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
@@ -82,6 +67,16 @@ __device__ __forceinline__ float2 turn(int pos, int i, double rate) {
     return k & 2 ? make_float2((float)-cc, (float)-ss) : make_float2((float)cc, (float)ss);
 }
 
+// The position of pair `i` of a row, on the pair's axis: all axes' are loaded with the map in flight, not behind it.
+__device__ __forceinline__ int axis_position(const AxisHeadArgs& a, int r, int i) {
+    const int32_t* p = a.axis_pos + r * a.row_step;
+    int at[kAxes];
+#pragma unroll
+    for (int x = 0; x < kAxes; ++x) at[x] = x < a.axes ? p[x * a.axis_step] : 0;
+    const uint32_t axis = (a.axis_of[i >> 4] >> 2 * (i & 15)) & 3u;
+    return axis == 0 ? at[0] : axis == 1 ? at[1] : axis == 2 ? at[2] : at[3];
+}
+
 // Sum over a head's 16 lanes in float64, by DPP moves.
 template <int CTRL>
 __device__ __forceinline__ double dpp_d(double v) {
@@ -120,8 +115,9 @@ __device__ __forceinline__ double rsqrt_d(double x) {
 // 14.9 us, 75 %, its codes in stores of 2 bytes a lane that the cache's fragment order scatters); few rows: the chain
 // of launch, loads and angles (1 row 3.5 us, 256 rows with the append 5.5).
 constexpr int kBlockRows = 4;
-template <int D, bool QUADS, bool TINY>
-__global__ void __launch_bounds__(256) heads_kernel(HeadArgs a, int rows, int per_block, int parts, int some) {
+template <int D, bool QUADS, bool TINY, class Args>
+__global__ void __launch_bounds__(256) heads_kernel(Args a, int rows, int per_block, int parts, int some) {
+    constexpr bool kOnAxes = std::is_same<Args, AxisHeadArgs>::value;
     constexpr int C = D / 64;
     __shared__ float xs[4][4][D];
     __shared__ float2 cs[kAngles];
@@ -152,7 +148,8 @@ __global__ void __launch_bounds__(256) heads_kernel(HeadArgs a, int rows, int pe
     fetch(now, raw);
     for (int i = tid; i < nr * half; i += 256) {
         const int rr = i / half, r = r0 + rr;
-        cs[i] = turn(a.pos[r / a.T] + r % a.T, i - rr * half, a.rate);
+        if constexpr (kOnAxes) cs[i] = turn(axis_position(a, r, i - rr * half), i - rr * half, a.rate);
+        else cs[i] = turn(a.pos[r / a.T] + r % a.T, i - rr * half, a.rate);
     }
     if (tid < nr) {
         const int r = r0 + tid, seq = r / a.T;
@@ -258,7 +255,8 @@ __global__ void __launch_bounds__(256) heads_kernel(HeadArgs a, int rows, int pe
     }
 }
 
-hipError_t launch_heads(HeadArgs& a, int n, hipStream_t st) {
+template <class Args>
+static hipError_t launch(Args& a, int n, hipStream_t st) {
     const int rows = n * a.T, kinds = a.v.p ? 2 : 1;
     // rows of a block: two when that leaves every CU two blocks or more, four when it leaves every CU four (1999 rows of
     // 32 q heads by one 16.4 us, two 15.8, four 19.7; 4096 of 8 by one 17.1, two 14.2, four 12.1: both lines lie between
@@ -274,14 +272,16 @@ hipError_t launch_heads(HeadArgs& a, int n, hipStream_t st) {
     const bool quads = a.rot % 8 == 0;
     const auto pick = [&](auto tiny) {
         constexpr bool t = decltype(tiny)::value;
-        return a.D == 256 ? (quads ? heads_kernel<256, true, t> : heads_kernel<256, false, t>)
-             : a.D == 128 ? (quads ? heads_kernel<128, true, t> : heads_kernel<128, false, t>)
-                          : (quads ? heads_kernel<64, true, t> : heads_kernel<64, false, t>);
+        return a.D == 256 ? (quads ? heads_kernel<256, true, t, Args> : heads_kernel<256, false, t, Args>)
+             : a.D == 128 ? (quads ? heads_kernel<128, true, t, Args> : heads_kernel<128, false, t, Args>)
+                          : (quads ? heads_kernel<64, true, t, Args> : heads_kernel<64, false, t, Args>);
     };
     const auto k = a.eps < 0x1p-250 ? pick(std::true_type{}) : pick(std::false_type{});
     hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(256), 0, st, a, rows, per_block, parts, some);
     return hipGetLastError();
 }
+hipError_t launch_heads(HeadArgs& a, int n, hipStream_t st) { return launch(a, n, st); }
+hipError_t launch_heads(AxisHeadArgs& a, int n, hipStream_t st) { return launch(a, n, st); }
 
 // ------------------------------------------------------------------ rows in and out of the cache
 // A thread per 8 dims of a (lane, kv head, slot): 4 bytes of codes, and a scale byte in one of four. Copies between
@@ -338,221 +338,6 @@ hipError_t launch_kv4_copy(const Kv4Copy& a, bool write, hipStream_t st) {
 // step's 293 instructions for 66 MFMAs of 32 rows): 4096 rows of 8 heads of 256 (69 GFLOP) 85 us, 8192 rows 279 (985
 // TFLOP/s; a library's 8192^3 product reaches 1191). These are launches back to back; the first ones after a card that
 // idled take 98 and 320.
-template <int D>
-struct Tile {
-    u32x4 k[D / 64], v[D / 64];
-    uint32_t ks;
-    u32x2 vs;
-};
-// A lane's places in a tile; with the tile's address in scalar registers (scalar_ptr) a load needs no other
-// vector register for its address.
-struct Lanes { uint32_t blob, ks, vs; };
-template <int D>
-__device__ __forceinline__ Lanes lane_offsets() {
-    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
-    return {(uint32_t)lane * 16, (uint32_t)(D == 256 ? lane * 4 : D == 64 ? ((g >> 1) * 16 + m) * 2 : lane * 2),
-            (uint32_t)(m * D / 512 * 32 + g * 8)};
-}
-typedef const __attribute__((address_space(1))) char* gptr;
-__device__ __forceinline__ gptr scalar_ptr(const uint8_t* p) {
-    const unsigned long long u = (unsigned long long)p;
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u), hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
-    return (gptr)(((unsigned long long)hi << 32) | lo);
-}
-template <class T, bool ONCE = false>
-__device__ __forceinline__ T load_at(gptr p, uint32_t off) {
-    const auto* w = (const __attribute__((address_space(1))) T*)(p + off);
-    if constexpr (ONCE) return __builtin_nontemporal_load(w);
-    else return *w;
-}
-// ONCE: the tile is read by one block only (nontemporal loads)
-template <int D, bool ONCE>
-__device__ __forceinline__ void load_k(Tile<D>& t, const uint8_t* tile, const Lanes& o) {
-    const gptr p = scalar_ptr(tile);
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) t.k[i] = load_at<u32x4, ONCE>(p, o.blob + i * 1024);
-    const gptr ps = scalar_ptr(tile + 32 * D);
-    t.ks = D == 256 ? load_at<uint32_t>(ps, o.ks) : load_at<uint16_t>(ps, o.ks);
-}
-template <int D, bool ONCE>
-__device__ __forceinline__ void load_v(Tile<D>& t, const uint8_t* tile, const Lanes& o) {
-    const gptr p = scalar_ptr(tile + 16 * D);
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) t.v[i] = load_at<u32x4, ONCE>(p, o.blob + i * 1024);
-    t.vs = load_at<u32x2>(scalar_ptr(tile + 33 * D), o.vs);
-}
-template <int D>
-__device__ __forceinline__ float k_scale(const Tile<D>& t, int half, int s) {
-    return scale_of((t.ks >> (D == 256 ? half * 16 + s / 4 * 8 : half * 8)) & 255u);
-}
-template <int D>
-__device__ __forceinline__ q35_bf16x8 k_frag(const Tile<D>& t, int half, int s) {
-    const int w = half * (D / 32) + s;
-    const uint32_t c = t.k[w / 4][w % 4];
-    const float sc = k_scale<D>(t, half, s);
-    const u32x4 r = {two_values<0>(c, sc), two_values<1>(c, sc), two_values<2>(c, sc), two_values<3>(c, sc)};
-    return __builtin_bit_cast(q35_bf16x8, r);
-}
-// The dims d and d + 1 (of the lane's D / 16; d even) of its 8 slots as the operands of two MFMAs.
-template <int D, int d>
-__device__ __forceinline__ void v_frags(const Tile<D>& t, const float* vs, q35_bf16x8& lo, q35_bf16x8& hi) {
-    u32x4 a, b;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        uint32_t w[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int byte = (2 * i + e) * (D / 32) + d / 2;
-            const uint32_t c = t.v[byte / 16][byte % 16 / 4];
-            const float sc = vs[2 * i + e];
-            w[e] = byte % 4 == 0 ? two_values<0>(c, sc) : byte % 4 == 1 ? two_values<1>(c, sc)
-                 : byte % 4 == 2 ? two_values<2>(c, sc) : two_values<3>(c, sc);
-        }
-        a[i] = __builtin_amdgcn_perm(w[1], w[0], 0x05040100u);
-        b[i] = __builtin_amdgcn_perm(w[1], w[0], 0x07060302u);
-    }
-    lo = __builtin_bit_cast(q35_bf16x8, a);
-    hi = __builtin_bit_cast(q35_bf16x8, b);
-}
-
-// Which slots a row sees: (pos - window, pos] and [0, sinks); window 0: [0, pos].
-struct Sight { int pos, low, sinks; };
-__device__ __forceinline__ bool sees(const Sight& s, int slot) { return (slot <= s.pos) & ((slot >= s.low) | (slot < s.sinks)); }
-
-// The running state of NQ x 16 rows over the tiles of one wave.
-template <int D, int NQ>
-struct Rows {
-    float m[NQ];                 // of row n: the reference of its exponents (log2 units)
-    f32x4 l[NQ];                 // its sum of weights, four times
-    uint32_t bad[NQ];            // groups of 32 dims whose V held a NaN at a slot the row sees
-    f32x4 o[NQ][D / 16];         // O^T: dims (4 g + r) D / 16 + i of row n in o[.][i][r]
-};
-
-// q: the rows' Q^T operands, [NQ][D / 32], in registers (NQ = 1) or, 16 rows more, in LDS with 64 lanes each
-// (the four waves of a block have the same rows). t's registers take the tile at next_p as soon as its K, then its
-// V, is used up. TIGHT: 32 rows of 256 dims leave no register for fragments made far ahead.
-// edge: some row may not see some slot. FAR: a score times scale2 is rounded before the reference is taken off, and the
-// reference lies 28 above the maximum it was taken from, so that weights stay under 2^-20 and 2^18 slots' sum of
-// them times the largest V is still a float32 (from references of 2^29 on their spacing takes the 28 in).
-template <int D, int NQ, bool ONCE, bool TIGHT, bool FAR, class Q>
-__device__ __forceinline__ void tile_step(Tile<D>& t, const uint8_t* tile_p, const uint8_t* next_p, const Lanes& lo, int slot0,
-                                          bool edge, const Q& q, const Sight* sight, float scale2, Rows<D, NQ>& st) {
-    const int lane = threadIdx.x & 63, g = lane >> 4;
-    f32x4 s[NQ][2];
-#pragma unroll
-    for (int c = 0; c < NQ; ++c) s[c][0] = s[c][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-    q35_bf16x8 qn[NQ];
-#pragma unroll
-    for (int c = 0; c < NQ; ++c) qn[c] = q(c, 0);
-#pragma unroll
-    for (int k = 0; k < D / 32; ++k) {
-        q35_bf16x8 qk[NQ];
-#pragma unroll
-        for (int c = 0; c < NQ; ++c) { qk[c] = qn[c]; if (k + 1 < D / 32) qn[c] = q(c, k + 1); }
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const q35_bf16x8 kf = k_frag<D>(t, half, k);
-#pragma unroll
-            for (int c = 0; c < NQ; ++c)
-                s[c][half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qk[c], s[c][half], 0, 0, 0);
-        }
-        if (TIGHT) __builtin_amdgcn_sched_barrier(0);
-    }
-    load_k<D, ONCE>(t, next_p, lo);
-    u32x2 vsb = t.vs;
-    // A slot some row may not see: its score is dropped, and a NaN group of V there must not meet the
-    // zero weight. Such a group is read as finite and noted for the rows that do see it.
-    if (edge) {
-        const auto has255 = [](uint32_t w) { return ((~w - 0x01010101u) & w & 0x80808080u) != 0; };
-        const bool nan = __any(has255(vsb.x) || has255(vsb.y));
-#pragma unroll
-        for (int c = 0; c < NQ; ++c) {
-            uint32_t seen = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const bool ok = sees(sight[c], slot0 + (j >> 2) * 16 + 4 * g + (j & 3));
-                if (!ok) s[c][j >> 2][j & 3] = -INFINITY;
-                seen |= (uint32_t)ok << j;
-            }
-            if (nan)
-                for (int b = 0; b < D / 32; ++b) {
-                    const uint8_t* p = tile_p + 33 * D + b * 32 + g * 8;
-                    for (int j = 0; j < 8; ++j)
-                        if (((seen >> j) & 1) && p[j] == 255) st.bad[c] |= 1u << b;
-                }
-        }
-        if (nan) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (((vsb.x >> 8 * j) & 255u) == 255u) vsb.x &= ~(128u << 8 * j);
-                if (((vsb.y >> 8 * j) & 255u) == 255u) vsb.y &= ~(128u << 8 * j);
-            }
-        }
-    }
-    q35_bf16x8 pf[NQ];
-#pragma unroll
-    for (int c = 0; c < NQ; ++c) {
-        float top = fmaxf(fmaxf(s[c][0][0], s[c][0][1]), fmaxf(s[c][0][2], s[c][0][3]));
-        top = fmaxf(top, fmaxf(fmaxf(s[c][1][0], s[c][1][1]), fmaxf(s[c][1][2], s[c][1][3])));
-        // the reference of the row's exponents follows its maximum only when that is past it by 2^8: weights
-        // stay under 2^8 (as exact as under 1), and almost every tile goes without the four lanes' common
-        // maximum and the rescale of O
-        constexpr float kRoom = FAR ? 28.f : 0.f;
-        if (__any(top * scale2 > st.m[c] + (8.f - kRoom))) {
-            top = fmaxf(top, xor16(top));
-            top = fmaxf(top, xor32(top)) * scale2;
-            if (FAR) top += kRoom;
-            const float mn = fmaxf(st.m[c], top), al = __builtin_amdgcn_exp2f(st.m[c] - (mn == -INFINITY ? 0.f : mn));
-            st.l[c] *= al;
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) st.o[c][i] *= al;
-            st.m[c] = mn;
-        }
-        const float ms = st.m[c] == -INFINITY ? 0.f : st.m[c];      // nothing seen so far: e^(-inf) stays 0
-        float p[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float x = s[c][j >> 2][j & 3];
-            p[j] = __builtin_amdgcn_exp2f(FAR ? x * scale2 - ms : __builtin_fmaf(x, scale2, -ms));
-        }
-        // Weights rounded to bf16 (2^-8 at most) for the product, as V's values are bf16 and the MFMA takes one type: a
-        // float32 product has a sixteenth of its rate. Their sum is that of the rounded ones, a product with ones. Against 64
-        // bits outputs are off by 0.0021 to 0.0023 of their size, of which the last rounding alone makes 0.0017.
-        const f32x8 pw = {p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]};
-        pf[c] = __builtin_convertvector(pw, q35_bf16x8);     // not f2bf2: the compiler must see what an MFMA is about to read
-        st.l[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_bf16x8, u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}),
-                                                          pf[c], st.l[c], 0, 0, 0);
-    }
-    float vs[8];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        vs[j] = scale_of((vsb.x >> 8 * j) & 255u);
-        vs[4 + j] = scale_of((vsb.y >> 8 * j) & 255u);
-    }
-    auto pv = [&](auto dc) {
-        constexpr int d = decltype(dc)::value;
-        if constexpr (d < D / 16) {
-            q35_bf16x8 lo, hi;
-            v_frags<D, d>(t, vs, lo, hi);
-#pragma unroll
-            for (int c = 0; c < NQ; ++c) {
-                st.o[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, pf[c], st.o[c][d], 0, 0, 0);
-                st.o[c][d + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, pf[c], st.o[c][d + 1], 0, 0, 0);
-            }
-            if (TIGHT) __builtin_amdgcn_sched_barrier(0);
-        }
-    };
-    pv(std::integral_constant<int, 0>{});
-    pv(std::integral_constant<int, 2>{});
-    pv(std::integral_constant<int, 4>{});
-    pv(std::integral_constant<int, 6>{});
-    pv(std::integral_constant<int, 8>{});
-    pv(std::integral_constant<int, 10>{});
-    pv(std::integral_constant<int, 12>{});
-    pv(std::integral_constant<int, 14>{});
-    load_v<D, ONCE>(t, next_p, lo);
-}
-
 // The tiles that rows at positions p0 .. p1 read: those of the sinks, then those from the first row's
 // window on. Tile i of the list is i (i < sink) or i - sink + main.
 struct TileList { int sink, main, count; };
@@ -576,10 +361,6 @@ size_t kv4_part_floats() { return (size_t)kMaxSplits * kSplitRows * (256 + 4); }
 // a wave loads all of them at once (four entries a lane) and finds the sequence by counting the entries of
 // first[] up to z, instead of bisecting them with a round trip to memory per step.
 struct Seq { int i, pos, lane, split, splits; };
-__device__ __forceinline__ int entry(uint32_t a, uint32_t b, uint32_t c, uint32_t d, int i) {
-    const uint32_t v = (i & 3) == 0 ? a : (i & 3) == 1 ? b : (i & 3) == 2 ? c : d;
-    return __builtin_amdgcn_readlane((int)v, i >> 2);
-}
 __device__ __forceinline__ Seq find_seq(const Kv4Attn& a, int z) {
     const int lane = threadIdx.x & 63;
     const uint2 f = ((const uint2*)a.first)[lane], l = ((const uint2*)a.lane)[lane];
@@ -597,34 +378,10 @@ __device__ __forceinline__ Seq find_seq(const Kv4Attn& a, int z) {
     return s;
 }
 
-// Where a row's dims go: normalised, gated, rounded. N dims (1, 2 or 4) from d on.
-struct Out {
-    const uint16_t* gate;
-    uint16_t* out;
-    __device__ __forceinline__ Out(const Kv4Attn& a, long long seq, int h, int rho) {
-        const int group = a.q_heads / a.kv_heads, t = rho / group, hq = h * group + rho - t * group;
-        const long long row = seq * a.T + t;
-        gate = a.gate.p + row * a.gate.row + hq * a.gate.head;
-        out = const_cast<uint16_t*>(a.out.p) + row * a.out.row + hq * a.out.head;
-    }
-    template <int N>
-    __device__ __forceinline__ void store(const Kv4Attn& a, float* x, float sum, int d) const {
-        const float inv = __builtin_amdgcn_rcpf(sum);
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] *= inv;
-        if (a.gate.p) {              // sigmoid by the instructions' 2^x and 1/x (a float32 ulp each)
-            uint16_t gt[N];
-            __builtin_memcpy(gt, gate + d, 2 * N);
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                x[i] *= __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(bf2f(gt[i]) * -1.44269504088896f));
-        }
-        uint16_t w[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) w[i] = f2bf(x[i]);
-        __builtin_memcpy(out + d, w, 2 * N);
-    }
-};
+__device__ __forceinline__ Out out_of(const Kv4Attn& a, long long seq, int h, int rho) {
+    const int group = a.q_heads / a.kv_heads, t = rho / group;
+    return Out(a, seq * a.T + t, h * group + rho - t * group);
+}
 // Partial result of (split z, kv head h, row rho): D sums, then the maximum and the sum of the weights.
 template <int D, int NQ>
 __device__ __forceinline__ const float* part_of(const Kv4Attn& a, int row_tiles, int z, int h, int rho) {
@@ -639,16 +396,10 @@ __device__ __forceinline__ const float* part_of(const Kv4Attn& a, int row_tiles,
 // rows 35 us, without 38, ascending 47; back to back it takes 34).
 template <int D, int NQ>
 __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) attn_kv4_kernel(Kv4Attn a, int row_tiles) {
-    constexpr int kQuarter = D / 64;         // of the D / 16 accumulators of 16 rows
-    __shared__ f32x4 os[4][4][kQuarter][64];
+    __shared__ f32x4 os[4][4][D / 64][64];
     __shared__ float ms[4][16], ls[4][16];
     __shared__ uint32_t bs[4][16];
     static_assert(NQ == 1 || sizeof(os) >= NQ * (D / 32) * 1024, "the Q operands lie where the waves' sums go at the end");
-    constexpr bool kOnce = NQ == 1, kTight = NQ == 2 && D == 256;
-    // tiles in registers: one of 256 dims (a second one's registers cost more than its loads in flight bring: 128
-    // lanes x 3 rows x 2000 slots 25.7 instead of 23.8 us), two smaller ones (64 lanes of 128 dims under a
-    // window 12.9 instead of 14.9 us)
-    constexpr int kAhead = D == 256 ? 1 : 2;
     const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63, nn = lane & 15, g = lane >> 4;
     const int per_split = row_tiles * a.kv_heads, z = blockIdx.x / per_split;
     int ix = blockIdx.x % per_split;
@@ -673,18 +424,9 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) attn_kv4_kernel(Kv4Attn
         return __builtin_bit_cast(q35_bf16x8, w);
     };
     auto at = [&](int i) { return i < tl.sink ? i : i - tl.sink + tl.main; };
-    Tile<D> buf[kAhead];
     const auto tile_at = [&](int i) { return region + (size_t)at(i) * kv4_tile_bytes(D); };
-    const auto first_tiles = [&] {
-        if (t0 + wv < t1) {
-#pragma unroll
-            for (int b = 0; b < kAhead; ++b) {
-                load_k<D, kOnce>(buf[b], tile_at(min(t0 + wv + 4 * b, t1 - 1)), lo);
-                load_v<D, kOnce>(buf[b], tile_at(min(t0 + wv + 4 * b, t1 - 1)), lo);
-            }
-        }
-    };
-    first_tiles();
+    Tile<D> buf[kAhead<D>];
+    first_tiles<D, NQ>(buf, t0, t1, tile_at, lo);
     q35_bf16x8 qf[NQ == 1 ? D / 32 : 1];
     q35_bf16x8* ql = (q35_bf16x8*)&os[0][0][0][0];
     if constexpr (NQ == 1) {
@@ -708,111 +450,20 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) attn_kv4_kernel(Kv4Attn
     // tiles whose every slot every row of the block sees: from the last row's window to the first row's slot
     const int full0 = a.window > 0 ? max(pos + rho1 / group - a.window + 1, 0) : 0, full1 = pos + rho0 / group;
     Rows<D, NQ> st;
-    const auto walk = [&](auto far) {
-#pragma unroll
-        for (int c = 0; c < NQ; ++c) {
-            st.m[c] = -INFINITY;
-            st.l[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-            st.bad[c] = 0;
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) st.o[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
-        for (int i0 = __builtin_amdgcn_readfirstlane(t0 + wv); i0 < t1; i0 += 4 * kAhead) {
-#pragma unroll
-            for (int b = 0; b < kAhead; ++b) {
-                const int i = i0 + 4 * b;
-                if (i >= t1) break;
-                if (NQ > 1) asm volatile("" : "+v"(qlane));     // or the compiler reads Q ahead of the loop, and spills it
-                const int tile = at(i);
-                const bool edge = tile * 32 < full0 || tile * 32 + 31 > full1;
-                tile_step<D, NQ, kOnce, kTight, decltype(far)::value>(buf[b], tile_at(i), tile_at(min(i + 4 * kAhead, t1 - 1)), lo,
-                                                                      tile * 32, edge, q, sight, scale2, st);
-            }
-        }
-    };
-    walk(std::false_type{});
-    // Two kinds of rows want their tiles gone over again in the FAR form (the other one is the faster: a 4096-row
-    // prompt 83.6 us a call, with a test of the reference in every tile 86.3). References of 2^24 and more: there float32
-    // numbers lie 2 and more apart, and the part of a product that its reference was rounded by, which a fused step
-    // keeps, is an exponent of its own (past 2^31 it can leave float32). And sums of 2^100 and more, or none any longer:
-    // what the waves and the splits (2^10 at most) add up from smaller ones stays a float32.
-    bool far = false;
-    float big = 0.f;                 // (a NaN anywhere makes it one)
-#pragma unroll
-    for (int c = 0; c < NQ; ++c) {
-        far |= __any(fabsf(st.m[c]) >= 16777216.f && st.m[c] != -INFINITY);
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) big = __builtin_elementwise_maximum(big, fabsf(st.o[c][i][r]));
-    }
-    far |= __any(!(big < 0x1p100f));
-    if (far) {
-        first_tiles();
-        walk(std::true_type{});
-    }
-    // The four waves' states: wave w ends a quarter of the row's dims, which the others pass it through
-    // LDS; a lane keeps its row, and its accumulators go as they are.
-#pragma unroll
-    for (int c = 0; c < NQ; ++c) {
-        if (rho0 + c * 16 >= rows) break;
-        if (NQ > 1 || c) __syncthreads();        // os was read: Q, or the 16 rows before these
-        uint32_t bad = st.bad[c];
-        bad |= (uint32_t)__shfl_xor((int)bad, 16);
-        bad |= (uint32_t)__shfl_xor((int)bad, 32);
-        if (g == 0) { ms[wv][nn] = st.m[c]; ls[wv][nn] = st.l[c][0]; bs[wv][nn] = bad; }
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-#pragma unroll
-            for (int i = 0; i < kQuarter; ++i)
-                if (w != wv) os[w][wv][i][lane] = st.o[c][w * kQuarter + i];
-        __syncthreads();
-        float m = st.m[c], sum = 0.f, f[4];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) m = fmaxf(m, ms[w][nn]);
-        bad = 0;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            f[w] = __builtin_amdgcn_exp2f(ms[w][nn] - (m == -INFINITY ? 0.f : m));
-            sum += f[w] * ls[w][nn];
-            bad |= bs[w][nn];
-        }
-        f32x4 o[kQuarter];
-#pragma unroll
-        for (int i = 0; i < kQuarter; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < 4; ++w)              // in the same order in every wave
-#pragma unroll
-            for (int i = 0; i < kQuarter; ++i) {
-                f32x4 x;
-                if (w == wv) {
-                    x = st.o[c][i];
-#pragma unroll
-                    for (int k = 1; k < 4; ++k) x = wv == k ? st.o[c][k * kQuarter + i] : x;
-                } else {
-                    x = os[wv][w][i][lane];
-                }
-                o[i] += f[w] * x;
-            }
-        const int rho = rho0 + c * 16 + nn;
-        if (rho >= rows) continue;
-        const Out to(a, seq, h, rho);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int d = (4 * g + r) * (D / 16) + wv * kQuarter;
-            float x[kQuarter];
-#pragma unroll
-            for (int i = 0; i < kQuarter; ++i) x[i] = (bad >> (d / 32)) & 1 ? __uint_as_float(0x7fc00000u) : o[i][r];
+    walk_tiles<D, NQ>(st, buf, t0, t1, at, tile_at, lo, q, qlane, sight, full0, full1, scale2);
+    join_waves<D, NQ>(st, rows - rho0, os, ms, ls, bs, [&](int c) {
+        const Out to = out_of(a, seq, h, rho0 + c * 16 + nn);
+        return [=, &a](float* x, int d, float m, float sum) {
             if (splits == 1) {
-                to.store<kQuarter>(a, x, sum, d);
+                to.store<D / 64>(a, x, sum, d);
             } else {
                 float* p = a.part + ((((size_t)z * a.kv_heads + h) * row_tiles + rt) * NQ + c) * kSplitRows * (D + 4) + nn * (D + 4);
 #pragma unroll
-                for (int i = 0; i < kQuarter; ++i) p[d + i] = x[i];
+                for (int i = 0; i < D / 64; ++i) p[d + i] = x[i];
                 if (d == 0) { p[D] = m; p[D + 1] = sum; }
             }
-        }
-    }
+        };
+    });
 }
 
 // Joins the splits of sequences that have few (up to 8): a thread per four dims of a row, all its
@@ -850,7 +501,7 @@ __global__ void __launch_bounds__(256) attn_kv4_join_few(Kv4Attn a, int row_tile
         sum += f * ml[s].y;
         x += f * o[s];
     }
-    Out(a, seq, h, rho).store<4>(a, (float*)&x, sum, d);
+    out_of(a, seq, h, rho).store<4>(a, (float*)&x, sum, d);
 }
 
 // The same for any number of splits: a block per (sequence, kv head, row, 64 dims). The splits' factors are
@@ -893,7 +544,7 @@ __global__ void __launch_bounds__(256) attn_kv4_join(Kv4Attn a, int row_tiles) {
     if (tid >= 16) return;
 #pragma unroll
     for (int i = 1; i < 16; ++i) o += os[i * 16 + tid];
-    Out(a, seq, h, rho).store<4>(a, (float*)&o, sum, d);
+    out_of(a, seq, h, rho).store<4>(a, (float*)&o, sum, d);
 }
 
 template <int D>

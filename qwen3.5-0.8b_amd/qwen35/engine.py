@@ -30,11 +30,12 @@ class _Config(C.Structure):
                 ("use_graph", C.c_int)]
 
 
-# q35_view, q35_heads and q35_drafts (include/q35.h), packed as bytes: a ctypes.Structure's fields cost a
+# q35_view, q35_heads, q35_positions, q35_drafts and q35_logprobs (include/q35.h), packed as bytes: a ctypes.Structure's fields cost a
 # call of a few microseconds more than its kernel takes.
 _VIEW = struct.Struct("@Pqq")
 _HEADS = struct.Struct("@iiddPP" + 6 * "Pqq")
 _DRAFTS = struct.Struct("@PqPqiPPd")
+_LOGPROBS = struct.Struct("@PqiPdiPPPPP")
 _NO_VIEW = (0, 0, 0)
 
 
@@ -103,6 +104,12 @@ _SIGS = {
     "q35_op_attn_kv4": ([C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int,
                          C.c_void_p, C.c_void_p, C.c_float, C.c_int, C.c_int, C.c_void_p], C.c_int),
     "q35_op_draft_verify": ([C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p], C.c_int),
+    "q35_op_qk_norm_rope_axes": ([C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_char_p, C.c_int], C.c_int),
+    "q35_op_kv4_append_axes": ([C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p,
+                                C.c_void_p, C.c_char_p], C.c_int),
+    "q35_op_attn_kv4_shared": ([C.c_void_p] * 3 + [C.c_int] + [C.c_void_p] * 4 + [C.c_int] * 3
+                               + [C.c_void_p, C.c_void_p, C.c_float, C.c_void_p], C.c_int),
+    "q35_op_token_logprobs": ([C.c_void_p, C.c_void_p, C.c_int, C.c_int], C.c_int),
     "q35_sync": ([C.c_void_p], C.c_int),
     "q35_kprof_read": ([C.c_void_p, C.POINTER(C.c_float), C.POINTER(C.c_int)], C.c_int),
     "q35_set_option": ([C.c_void_p, C.c_char_p, C.c_int], C.c_int),
@@ -162,6 +169,31 @@ def _lp(lanes: np.ndarray | None, pos: np.ndarray):
 def _heads(q_heads, rot_dim, theta, eps, q_norm, k_norm, q, k, v, q_out, k_out, v_out) -> bytes:
     return _HEADS.pack(q_heads, rot_dim, theta, eps, q_norm, k_norm, *(q or _NO_VIEW), *k, *(v or _NO_VIEW),
                        *(q_out or _NO_VIEW), *(k_out or _NO_VIEW), *(v_out or _NO_VIEW))
+
+
+def _axis(axis, rot_dim: int) -> bytes:
+    """The pairs' axes as bytes, one for each of the rot_dim / 2 pairs."""
+    if not isinstance(axis, bytes):
+        a = np.asarray(axis)
+        axis = a.tobytes() if a.dtype == np.uint8 else bytes(a.tolist())
+    if len(axis) != rot_dim // 2:
+        raise ValueError(f"{len(axis)} axes for {rot_dim // 2} pairs of dims")
+    return axis
+
+
+def pair_axes(sections, dealt: bool = False) -> bytes:
+    """The axis of each pair of rotated dims, sections[a] pairs on axis a: in sections one behind the other, or dealt out
+    to the axes in turn while each has pairs left."""
+    left = [int(n) for n in sections]
+    if not dealt:
+        return bytes(a for a, n in enumerate(left) for _ in range(n))
+    out = []
+    while any(left):
+        for a, n in enumerate(left):
+            if n:
+                out.append(a)
+                left[a] -= 1
+    return bytes(out)
 
 
 def safetensors_scan(data: bytes | np.ndarray) -> tuple[int, int]:
@@ -300,6 +332,23 @@ class Engine:
         h = _heads(q_heads, rot_dim, theta, eps, q_norm, k_norm, q, k, v, q_out, k_out, v_out)
         _ck(load_library().q35_op_kv4_append(self.h, cache.h, layer, _lp(la, p), _addr(p), p.size, T, h))
 
+    # the same with positions on several axes: `at` is (device pointer of int32, elements from row to row, elements from axis
+    # to axis), `axis` the axis of each of the rot_dim / 2 pairs (pair_axes)
+    def op_qk_norm_rope_axes(self, at, axis, rows: int, q_heads: int, kv_heads: int, head_dim: int, *, rot_dim: int,
+                             theta: float, eps: float, q_norm: int, k_norm: int, k, k_out, q=None, q_out=None):
+        """Norms of q and k per head and their rotation by the rows' positions (q35_op_qk_norm_rope_axes)."""
+        h = _heads(q_heads, rot_dim, theta, eps, q_norm, k_norm, q, k, None, q_out, k_out, None)
+        _ck(load_library().q35_op_qk_norm_rope_axes(self.h, h, kv_heads, head_dim, _VIEW.pack(*at), _axis(axis, rot_dim), rows))
+
+    def op_kv4_append_axes(self, cache: "KvCache4", layer: int, lanes, slots, T: int, q_heads: int, at, axis, *, rot_dim: int,
+                           theta: float, eps: float, q_norm: int, k_norm: int, k, v, q=None, q_out=None, k_out=None,
+                           v_out=None):
+        """The same with k and v appended to `cache` at slots[i] + t (q35_op_kv4_append_axes); lanes None: lane i."""
+        s, la = _i32(slots), None if lanes is None else _i32(lanes)
+        h = _heads(q_heads, rot_dim, theta, eps, q_norm, k_norm, q, k, v, q_out, k_out, v_out)
+        _ck(load_library().q35_op_kv4_append_axes(self.h, cache.h, layer, _lp(la, s), _addr(s), s.size, T, h,
+                                                  _VIEW.pack(*at), _axis(axis, rot_dim)))
+
     def op_attn_kv4(self, cache: "KvCache4", layer: int, lanes, pos, T: int, q_heads: int, q, out, *,
                     scale: float | None = None, window: int = 0, sinks: int = 0, gate=None):
         """Attention of T rows per sequence over `cache` (q35_op_attn_kv4): a row at p sees slots (p - window, p] and
@@ -310,6 +359,16 @@ class Engine:
                                            cache.head_dim ** -0.5 if scale is None else scale, window, sinks,
                                            _VIEW.pack(*out)))
 
+    def op_attn_kv4_shared(self, prefix: "KvCache4", cache: "KvCache4", layer: int, prefix_lanes, prefix_lens, lanes, pos, T: int,
+                           q_heads: int, q, out, *, scale: float | None = None, gate=None):
+        """Attention of T rows per sequence over the first prefix_lens[i] slots of lane prefix_lanes[i] of `prefix` (-1:
+        none) and the sequence's own of `cache` (q35_op_attn_kv4_shared): a prompt that sequences share is read once."""
+        p, pl, pn, la = _i32(pos), _i32(prefix_lanes), _i32(prefix_lens), None if lanes is None else _i32(lanes)
+        _ck(load_library().q35_op_attn_kv4_shared(self.h, prefix.h, cache.h, layer, _lp(pl, p), _lp(pn, p), _lp(la, p), _addr(p),
+                                                  p.size, T, q_heads, _VIEW.pack(*q),
+                                                  None if gate is None else _VIEW.pack(*gate),
+                                                  cache.head_dim ** -0.5 if scale is None else scale, _VIEW.pack(*out)))
+
     def op_draft_verify(self, n: int, k: int, vocab: int, logits: int, drafts: int, u: int, accepted: int, tokens: int, *,
                         temperature: float = 1.0, draft_logits: int = 0, bf16: bool = False, ld: int = 0,
                         draft_ld: int = 0):
@@ -317,6 +376,15 @@ class Engine:
         logits' row strides are vocab unless given."""
         d = _DRAFTS.pack(logits, ld or vocab, draft_logits, draft_ld or vocab, int(bf16), drafts, u, temperature)
         _ck(load_library().q35_op_draft_verify(self.h, d, n, k, vocab, accepted, tokens))
+
+    def op_token_logprobs(self, rows: int, vocab: int, logits: int, *, targets: int = 0, logprobs: int = 0, ranks: int = 0,
+                          entropy: int = 0, top: int = 0, top_ids: int = 0, top_logprobs: int = 0,
+                          temperature: float = 1.0, bf16: bool = False, ld: int = 0):
+        """Log probabilities and ranks of the rows' targets, entropy, and the `top` most likely ids with theirs
+        (q35_op_token_logprobs); the logits' row stride is vocab unless given."""
+        d = _LOGPROBS.pack(logits, ld or vocab, int(bf16), targets, temperature, top, logprobs, ranks, entropy, top_ids,
+                           top_logprobs)
+        _ck(load_library().q35_op_token_logprobs(self.h, d, rows, vocab))
 
     def timer_begin(self):
         _ck(load_library().q35_timer_begin(self.h))
