@@ -4,9 +4,10 @@
 //   log p_i = z_i - log S,   entropy = log S - A / S,   rank of t = #{x_i > x_t} + #{x_i = x_t, i < t},
 // and the most likely tokens are the first of the order (x falling, i rising). Both sums move with m by a
 // factor (and A by a multiple of S), so every wave keeps its own m and the states are joined at the end.
-// A token that is all but certain has log p ~ -(S - 1): the term 1 of the maximum itself goes into a float64
+// A token that is all but certain has log p ~ -(S - 1): there the term 1 of the maximum itself goes into a float64
 // sum by itself, so that S - 1 keeps float32's relative accuracy and does not end at 2^-24.
 #include <algorithm>
+#include <type_traits>
 
 #include "q35_answers.h"
 #include "q35_common.h"
@@ -42,62 +43,28 @@ __device__ __forceinline__ double wave_sum_d(double v) {
     return v;
 }
 __device__ __forceinline__ bool before(float a, int ia, float b, int ib) { return (a > b) | ((a == b) & (ia < ib)); }
+__device__ __forceinline__ bool before(float2 a, float2 b) { return before(a.x, __float_as_int(a.y), b.x, __float_as_int(b.y)); }
+__device__ __forceinline__ float2 nobody() { return make_float2(-INFINITY, __int_as_float(0x7fffffff)); }
+// How many of list[0 .. n) come before mine. Eight at a time, past n too: there lie nobody()s.
+constexpr int kPad = 8;
+__device__ __forceinline__ int rank_in(const float2* list, int n, float2 mine) {
+    int r = 0;
+    for (int k = 0; k < n; k += kPad) {
+        float2 o[kPad];
+#pragma unroll
+        for (int i = 0; i < kPad; ++i) o[i] = list[k + i];
+#pragma unroll
+        for (int i = 0; i < kPad; ++i) r += before(o[i], mine);
+    }
+    return r;
+}
 
-// The best tokens of a wave so far: a list of (logit, id) in LDS that holds every token it has met that may be among
-// the row's `top` first, and at most kTight of them after each step. floor: what a token's logit must reach
-// (strict: exceed, since `top` tokens of lower ids reach it) to get in.
-constexpr int kTight = 64, kStep = 512, kList = kTight + kStep;
-struct Best {
-    float2* list;                    // [kList]: logit, id as bits
-    float2* sorted;                  // [kTopMost]
-    float floor;
-    bool strict;
-    int count, top;
-};
-__device__ __forceinline__ bool gets_in(const Best& b, float x) { return b.strict ? x > b.floor : x >= b.floor; }
-// Keeps the list's first `top` in order.
-__device__ __forceinline__ void tighten(Best& b) {
-    const int lane = threadIdx.x & 63;
-    wave_sync();
-    for (int c = lane; c < b.count; c += 64) {
-        const float2 mine = b.list[c];
-        int r = 0;
-        for (int k = 0; k < b.count; ++k) {
-            const float2 o = b.list[k];
-            r += before(o.x, __float_as_int(o.y), mine.x, __float_as_int(mine.y));
-        }
-        if (r < b.top) b.sorted[r] = mine;
-    }
-    wave_sync();
-    b.count = min(b.count, b.top);
-    if (lane < b.count) b.list[lane] = b.sorted[lane];
-    wave_sync();
-    if (b.count == b.top) {
-        b.floor = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__float_as_int(b.sorted[b.top - 1].x)));
-        b.strict = true;
-    }
-}
-// One element a lane.
-__device__ __forceinline__ void push(Best& b, float x, int id, bool on) {
-    const bool in = on && gets_in(b, x);
-    const unsigned long long mask = __ballot(in);
-    if (!mask) return;
-    if (in) b.list[b.count + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0))] =
-        make_float2(x, __int_as_float(id));
-    b.count += __popcll(mask);
-}
-// The `top`-th largest of the lanes' maxima: a floor that `top` tokens reach at least.
+// A floor that at least `top` of the lanes' numbers reach: the smallest that fewer than `top` exceed.
 __device__ __forceinline__ float floor_of(float x, int top) {
-    const int lane = threadIdx.x & 63;
     int r = 0;
 #pragma unroll
-    for (int i = 0; i < 64; ++i) {
-        const float o = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__float_as_int(x), i));
-        r += before(o, i, x, lane);
-    }
-    const unsigned long long at = __ballot(r == top - 1);
-    if (!at) return -INFINITY;       // (a NaN among them)
-    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__float_as_int(x), __ffsll((long long)at) - 1));
+    for (int i = 0; i < 64; ++i) r += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__float_as_int(x), i)) > x;
+    return -wave_max(r < top ? -x : -INFINITY);
 }
 
 // The running sums of a wave's lanes, all against the same m.
@@ -111,7 +78,42 @@ __device__ __forceinline__ void raise(Sums& u, float m, float c) {     // m > u.
     u.m = m;
 }
 
-constexpr int kLoads = 8;            // 16-byte loads of a lane's tile
+// A row's results but its best tokens.
+__device__ __forceinline__ void finish(const LogprobArgs& a, int row, const LpPart& p, bool bad, double lse) {
+    const int t = a.targets ? a.targets[row] : -1;
+    const bool on = !bad && t >= 0 && t < a.vocab;
+    if (a.logprobs) {
+        double v = NAN;
+        if (on) {
+            const long long i = row * a.ld + t;
+            const float x = a.bf16 ? bf2f(((const uint16_t*)a.logits)[i]) : ((const float*)a.logits)[i];
+            v = (((double)x - p.m) * a.c - lse) * 0.69314718055994530942;
+        }
+        a.logprobs[row] = (float)v;
+    }
+    if (a.ranks) a.ranks[row] = on ? p.above : -1;
+    if (a.entropy) a.entropy[row] = bad ? NAN : (float)((lse - p.a / p.s) * 0.69314718055994530942);
+}
+__device__ __forceinline__ bool no_distribution(const LpPart& p) { return !(p.s > 0.0) || !(p.s < INFINITY) || !(p.m < INFINITY); }
+__device__ __forceinline__ void store_top(const LogprobArgs& a, int row, int r, float2 token, bool bad, float m, double lse) {
+    const long long o = (long long)row * a.top + r;
+    if (a.top_ids) a.top_ids[o] = bad ? -1 : __float_as_int(token.y);
+    if (a.top_logprobs)
+        a.top_logprobs[o] = bad ? NAN : (float)((((double)token.x - m) * a.c - lse) * 0.69314718055994530942);
+}
+// A part's state against the common m.
+__device__ __forceinline__ void against(const LpPart& q, float m, double c, double& s, double& a) {
+    s = a = 0.0;
+    if (q.m == -INFINITY && q.s == 0.0) return;
+    const double z = q.m == m ? 0.0 : ((double)q.m - m) * c, f = exp2(z);
+    s = f * q.s;
+    a = f > 0.0 ? f * (q.a + z * q.s) : 0.0;
+}
+
+__device__ __forceinline__ float eight(const float* w) {
+    return ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+}
+constexpr int kEach = 32;            // elements of a lane's tile
 template <bool BF16>
 __device__ __forceinline__ float element(const u32x4* w, int i) {
     if (BF16) {
@@ -121,27 +123,93 @@ __device__ __forceinline__ float element(const u32x4* w, int i) {
     return __uint_as_float(w[i / 4][i % 4]);
 }
 
-// A block per (row, part of it). The row's 16-byte pieces go to waves in tiles of 64 x kLoads, the next tile's loads in
-// flight; the up to 14 elements in front of its first whole piece and behind its last are the first part's first wave's.
-template <bool BF16, bool TOP>
-__global__ void __launch_bounds__(256) logprobs_kernel(LogprobArgs a, int row0) {
-    constexpr int V = BF16 ? 8 : 4, E = kLoads * V;
-    __shared__ float2 lists[TOP ? 4 : 1][TOP ? kList : 1], sorts[TOP ? 4 : 1][TOP ? kTopMost : 1];
-    __shared__ LpPart waves[4];
-    __shared__ int counts[4];
+// The best tokens of a wave: a list of (logit, id) in LDS that holds every token it has met that may be among
+// the row's `top` first, and at most kTight of them after each step. floor: what a token's logit must reach
+// (strict: exceed, since `top` tokens of lower ids reach it) to get in.
+constexpr int kTight = 64, kStep = 512, kList = kTight + kStep;
+struct Best {
+    float2* list;                    // [kList + kPad]: logit, id as bits
+    float2* sorted;                  // [kTopMost]
+    float floor;
+    bool strict;
+    int count, top;
+};
+// Keeps the list's first `top` in order.
+__device__ __forceinline__ void tighten(Best& b) {
+    const int lane = threadIdx.x & 63;
+    if (lane < kPad) b.list[b.count + lane] = nobody();
+    wave_sync();
+    for (int c = lane; c < b.count; c += 64) {
+        const float2 mine = b.list[c];
+        const int r = rank_in(b.list, b.count, mine);
+        if (r < b.top) b.sorted[r] = mine;
+    }
+    wave_sync();
+    b.count = min(b.count, b.top);
+    if (lane < b.count) b.list[lane] = b.sorted[lane];
+    wave_sync();
+    if (b.count == b.top) {
+        b.floor = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__float_as_int(b.sorted[b.top - 1].x)));
+        b.strict = true;
+    }
+}
+// One element a lane.
+__device__ __forceinline__ void push(Best& b, float x, int id, bool on) {
+    const bool in = on && (b.strict ? x > b.floor : x >= b.floor);
+    const unsigned long long mask = __ballot(in);
+    if (!mask) return;
+    if (in) b.list[b.count + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0))] =
+        make_float2(x, __int_as_float(id));
+    b.count += __popcll(mask);
+}
+
+// A block per (row, part of it). The row's 16-byte pieces go to waves in tiles of kEach elements a lane; the up to 14
+// elements in front of its first whole piece and behind its last (edges) are the first part's first wave's. A row of one
+// part is finished here, others by logprobs_join.
+// The best tokens: while the sums are made, a lane keeps the largest of its elements of each run of tiles. Of those
+// lanes the same ones of the waves make 64 groups; `top` groups reach the top-th largest of their
+// maxima (floor), so the row's best do, and only the pieces of the lanes and runs that reach it are read
+// again: some 25 of them for 20 tokens, of any number of elements. If ties or infinities bring more candidates than there is
+// room for, the part is gone over in order with a list a wave (Best).
+// float32: bound by memory, 256 rows of 248,320 with 5 tokens each (254 MB) 45.8 us, 5.6 TB/s (without tokens 42.2, with 32
+// 50.2). bfloat16: by memory and the 8 instructions an element takes, 1999 rows of 32,003 with 20 tokens (128 MB) 37.7 us,
+// 3.4 TB/s (without 31.8). One row of 248,320: a chain of loads and barriers, 8.8 us and the join's 3.8.
+constexpr int kRuns = 16;            // of a part's tiles a wave
+constexpr int kRoom = 256;           // candidates, and lanes' runs that may hold some
+template <bool BF16, bool TOP, int W>
+__global__ void __launch_bounds__(64 * W, 5) logprobs_kernel(LogprobArgs a, int row0) {
+    constexpr int V = BF16 ? 8 : 4, L = kEach / V;
+    struct Lists { float2 list[W][kList + kPad], sorted[W][kTopMost]; };
+    union Store {
+        float runs[kRuns][64 * W];
+        Lists lists;
+    };
+    __shared__ __align__(16) char store[TOP ? sizeof(Store) : 16];
+    Store* st = (Store*)store;
+    __shared__ float2 flat[TOP ? kRoom + kPad : 1];
+    __shared__ uint16_t held[TOP ? kRoom : 1];
+    __shared__ LpPart waves[W];
+    __shared__ int counts[W], n_held, n_flat;
+    __shared__ double row_lse;
+    __shared__ float row_m, row_floor;
     const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63;
     const int part = blockIdx.x % a.parts, row = row0 + blockIdx.x / a.parts;
     const char* base = (const char*)a.logits + row * a.ld * (BF16 ? 2 : 4);
     const int head = min((int)((16 - ((uintptr_t)base & 15)) & 15) / (BF16 ? 2 : 4), a.vocab);
-    const int pieces = (a.vocab - head) / V, tiles = (pieces + 64 * kLoads - 1) / (64 * kLoads);
+    const int pieces = (a.vocab - head) / V, tiles = (pieces + 64 * L - 1) / (64 * L);
     const int t0 = (int)((long long)tiles * part / a.parts), t1 = (int)((long long)tiles * (part + 1) / a.parts);
     const char* body = base + head * (BF16 ? 2 : 4);
     const uint32_t none = BF16 ? 0xff80ff80u : 0xff800000u;
-    u32x4 buf[kLoads];
-    const auto fetch = [&](int t) {
+    const auto fetch = [&](u32x4* buf, int t) {
+        if ((t + 1) * L * 64 <= pieces) {
+            const char* from = body + (size_t)t * (L * 1024);
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int p = (t * kLoads + i) * 64 + lane;
+            for (int i = 0; i < L; ++i) buf[i] = *(const u32x4*)(from + lane * 16 + i * 1024);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            const int p = (t * L + i) * 64 + lane;
             buf[i] = u32x4{none, none, none, none};
             if (p < pieces) buf[i] = *(const u32x4*)(body + (size_t)p * 16);
         }
@@ -150,7 +218,8 @@ __global__ void __launch_bounds__(256) logprobs_kernel(LogprobArgs a, int row0) 
         return BF16 ? __uint_as_float((uint32_t)((const uint16_t*)base)[i] << 16) : ((const float*)base)[i];
     };
     int target = a.targets ? a.targets[row] : -1;
-    if (t0 + wv < t1) fetch(t0 + wv);
+    u32x4 buf[L];
+    if (t0 + wv < t1) fetch(buf, t0 + wv);
     if (target >= a.vocab) target = -1;
     // Tokens before the target: of the pieces before its own those that reach x_t, of the others those that reach the
     // next float32 above it, and in its own piece (tp) the lower ids with x_t as well.
@@ -161,197 +230,281 @@ __global__ void __launch_bounds__(256) logprobs_kernel(LogprobArgs a, int row0) 
     const float c = (float)a.c;
     Sums u = {-INFINITY, 0.0, 0.0};
     int above = 0;
-    Best best = {lists[TOP ? wv : 0], sorts[TOP ? wv : 0], -INFINITY, false, 0, a.top};
-    // elements in front (the first step) and behind
-    const bool edges = part == 0 && wv == 0;
-    const auto single = [&](int id, bool on) {
-        const float x = on ? at(id) : -INFINITY;
-        const float top = wave_max(x);
+    // the edges: an element a lane
+    const int tail = head + pieces * V, edge = lane < head ? lane : tail + lane - head;
+    const bool edges = part == 0 && wv == 0, on_edge = edges && edge < a.vocab;
+    const float x_edge = on_edge ? at(edge) : -INFINITY;
+    if (edges) {
+        const float top = wave_max(x_edge);
         if (top > u.m) raise(u, top, c);
-        const float z = on ? (x - (u.m == -INFINITY ? 0.f : u.m)) * c : -INFINITY, w = __builtin_amdgcn_exp2f(z);
+        const float z = on_edge ? (x_edge - (u.m == -INFINITY ? 0.f : u.m)) * c : -INFINITY, w = __builtin_amdgcn_exp2f(z);
         u.s += w;
         u.a += w * __builtin_elementwise_maximum(z, -200.f);
-        above += __popcll(__ballot(on && before(x, id, xt, target)));
-        if (TOP) push(best, x, id, on);
-    };
-    if (edges && head) single(lane, lane < head);
-    if (edges && tp >= 0 && tp < pieces) {
-        const int id = head + tp * V + lane;
-        above += __popcll(__ballot(id < target && at(min(id, target)) == xt));
+        above += __popcll(__ballot(on_edge && before(x_edge, edge, xt, target)));
+        if (tp >= 0 && tp < pieces) {
+            const int id = head + tp * V + lane;
+            above += __popcll(__ballot(id < target && at(min(id, target)) == xt));
+        }
     }
-    bool first = true;
-    for (int t = t0 + wv; t < t1; t += 4) {
-        float x[E];
+    const int each = (t1 - t0 + W * kRuns - 1) / (W * kRuns);       // tiles of a run
+    float run = -INFINITY;
+    int n_run = 0, i_run = 0, t_max = -1;
+    for (int t = t0 + wv; t < t1; t += W) {
+        float x[kEach];
 #pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = element<BF16>(buf, i);
-        if (t + 4 < t1) fetch(t + 4);
+        for (int i = 0; i < kEach; ++i) x[i] = element<BF16>(buf, i);
         float top = x[0];
 #pragma unroll
-        for (int i = 1; i < E; ++i) top = fmaxf(top, x[i]);
-        if (__any(top > u.m)) raise(u, wave_max(fmaxf(top, u.m)), c);
-        const float m = u.m == -INFINITY ? 0.f : u.m;
-        float as = 0.f;
-        double ss = 0.0;
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const float z = (x[i] - m) * c, w = __builtin_amdgcn_exp2f(z);
-            ss += w;
-            as = __builtin_fmaf(w, __builtin_elementwise_maximum(z, -200.f), as);
+        for (int i = 1; i < kEach; ++i) top = fmaxf(top, x[i]);
+        if (__any(top > u.m)) {
+            raise(u, wave_max(fmaxf(top, u.m)), c);
+            t_max = t;
         }
-        u.s += ss;
+        const float m = u.m == -INFINITY ? 0.f : u.m;
+        // float32 sums of eight terms by halves, then of the four eights: 5 roundings each
+        float ss = 0.f, as = 0.f;
+#pragma unroll
+        for (int i = 0; i < kEach; i += 8) {
+            float w[8], z[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                z[k] = (x[i + k] - m) * c;
+                w[k] = __builtin_amdgcn_exp2f(z[k]);
+                as = __builtin_fmaf(w[k], __builtin_elementwise_maximum(z[k], -200.f), as);
+            }
+            ss += eight(w);
+            asm volatile("" : "+v"(as), "+v"(ss));   // now: or all 32 terms wait for a later place, in 64 registers
+        }
         u.a += as;
-        const int id0 = head + (t * kLoads * 64 + lane) * V;
-        if (a.targets) {
+        u.s += ss;
+        if (__any(top >= xt)) {
             int n = 0;
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                const float reach = (t * kLoads + i) * 64 + lane < tp ? xt : over;
+            for (int i = 0; i < L; ++i) {
+                const float reach = (t * L + i) * 64 + lane < tp ? xt : over;
 #pragma unroll
                 for (int k = 0; k < V; ++k) n += __popcll(__ballot(x[i * V + k] >= reach));
             }
             above += n;
         }
         if (TOP) {
-            if (first) best.floor = fmaxf(best.floor, floor_of(top, a.top));
-            first = false;
-            if (__any(gets_in(best, top))) {
-#pragma unroll
-                for (int i = 0; i < kLoads; ++i) {
-                    if (best.count > kTight) tighten(best);
-                    const bool on = (t * kLoads + i) * 64 + lane < pieces;
-#pragma unroll
-                    for (int k = 0; k < V; ++k) push(best, x[i * V + k], id0 + i * 64 * V + k, on);
-                }
-                if (best.count > kTight) tighten(best);
+            run = fmaxf(run, top);
+            if (++n_run == each) {
+                st[0].runs[i_run++][tid] = run;
+                run = -INFINITY;
+                n_run = 0;
             }
         }
+        if (t + W < t1) fetch(buf, t + W);
     }
-    const int tail = head + pieces * V;
-    if (edges && tail < a.vocab) {
-        single(tail + lane, tail + lane < a.vocab);
-        if (TOP && best.count > kTight) tighten(best);
+    double s = wave_sum_d(u.s);
+    if (t_max >= 0 && s < 2.0 && u.m < INFINITY) {
+        // the maximum all but alone: its tile's float32 sums again, with its 1 apart from the rest
+        fetch(buf, t_max);
+        float ss = 0.f, rest = 0.f;
+        int ones = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; i += 8) {
+            float w[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k] = __builtin_amdgcn_exp2f((element<BF16>(buf, i + k) - u.m) * c);
+            ss += eight(w);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (element<BF16>(buf, i + k) == u.m) { ++ones; w[k] = 0.f; }
+            rest += eight(w);
+        }
+        s = wave_sum_d(u.s - ss + rest + ones);
     }
-    u.s = wave_sum_d(u.s);
+    u.s = s;
     u.a = wave_sum_d(u.a);
-    if (lane == 0) {
-        waves[wv] = {u.s, u.a, u.m, above};
-        counts[wv] = best.count;
+    if (lane == 0) waves[wv] = {u.s, u.a, u.m, above};
+    if (TOP) {
+        for (; i_run < kRuns; ++i_run, run = -INFINITY) st[0].runs[i_run][tid] = run;
+        if (tid == 0) n_held = n_flat = 0;
     }
     __syncthreads();
     const size_t room = blockIdx.x;
-    LpPart* parts = (LpPart*)a.ws;
-    float2* tops = (float2*)(a.ws + kPartRooms * sizeof(LpPart)) + room * kTopMost;
-    if (tid == 0) {
-        LpPart p = waves[0];
-        for (int w = 1; w < 4; ++w) p.m = fmaxf(p.m, waves[w].m);
-        p.s = p.a = 0.0;
-        p.above = 0;
-        for (int w = 0; w < 4; ++w) {
-            const LpPart& q = waves[w];
-            p.above += q.above;
-            if (q.m == -INFINITY && q.s == 0.0) continue;
-            const double z = q.m == p.m ? 0.0 : ((double)q.m - p.m) * a.c, f = exp2(z);
-            p.s += f * q.s;
-            p.a += f > 0.0 ? f * (q.a + z * q.s) : 0.0;
-        }
-        parts[room] = p;
-    }
-    if (TOP) {
-        const bool on = lane < counts[wv];
-        const float2 mine = on ? lists[wv][lane] : make_float2(-INFINITY, 0.f);
-        int r = 0;
-        for (int w = 0; w < 4; ++w)
-            for (int k = 0; k < counts[w]; ++k) {
-                const float2 o = lists[w][k];
-                r += before(o.x, __float_as_int(o.y), mine.x, __float_as_int(mine.y));
-            }
-        if (on && r < a.top) tops[r] = mine;
-        int all = 0;
-        for (int w = 0; w < 4; ++w) all += counts[w];
-        if (tid >= all && tid < a.top) tops[tid] = make_float2(-INFINITY, __int_as_float(0x7fffffff));
-    }
-}
-
-// Joins a row's parts: a block a row.
-template <bool TOP>
-__global__ void __launch_bounds__(256) logprobs_join(LogprobArgs a, int row0) {
-    __shared__ float2 c[TOP ? kParts * kTopMost : 1];
-    __shared__ int kept;
-    __shared__ double lse;
-    __shared__ float mx;
-    const int tid = threadIdx.x, row = row0 + blockIdx.x;
-    const LpPart* parts = (const LpPart*)a.ws + (size_t)blockIdx.x * a.parts;
-    const float2* tops = (const float2*)(a.ws + kPartRooms * sizeof(LpPart)) + (size_t)blockIdx.x * a.parts * kTopMost;
-    if (tid < 64) {
-        LpPart p = tid < a.parts ? parts[tid] : LpPart{0.0, 0.0, -INFINITY, 0};
+    if (wv == W - 1) {
+        LpPart p = lane < W ? waves[lane] : LpPart{0.0, 0.0, -INFINITY, 0};
         const float m = wave_max(p.m);
-        double s = 0.0, e = 0.0;
-        if (tid < a.parts && !(p.m == -INFINITY && p.s == 0.0)) {
-            const double z = p.m == m ? 0.0 : ((double)p.m - m) * a.c, f = exp2(z);
-            s = f * p.s;
-            e = f > 0.0 ? f * (p.a + z * p.s) : 0.0;
-        }
-        s = wave_sum_d(s);
-        e = wave_sum_d(e);
-        int above = p.above;
-        for (int k = 32; k; k >>= 1) above += __shfl_xor(above, k);
-        if (tid == 0) {
-            const bool bad = !(s > 0.0) || !(s < INFINITY) || !(m < INFINITY);
-            const double l = bad ? (double)NAN : log2(s);
-            lse = l;
-            mx = m;
-            kept = 0;
-            const int t = a.targets ? a.targets[row] : -1;
-            const bool on = !bad && t >= 0 && t < a.vocab;
-            if (a.logprobs) {
-                double v = NAN;
-                if (on) {
-                    const long long i = row * a.ld + t;
-                    const float x = a.bf16 ? bf2f(((const uint16_t*)a.logits)[i]) : ((const float*)a.logits)[i];
-                    v = (((double)x - m) * a.c - l) * 0.69314718055994530942;
-                }
-                a.logprobs[row] = (float)v;
+        double s, e;
+        against(p, m, a.c, s, e);
+        p = {wave_sum_d(s), wave_sum_d(e), m, (int)wave_sum_d(p.above)};
+        if (lane == 0) {
+            if (a.parts == 1) {
+                const bool bad = no_distribution(p);
+                const double l = bad ? (double)NAN : log2(p.s);
+                row_lse = l;
+                row_m = m;
+                finish(a, row, p, bad, l);
+            } else {
+                ((LpPart*)a.ws)[room] = p;
             }
-            if (a.ranks) a.ranks[row] = on ? above : -1;
-            if (a.entropy) a.entropy[row] = (float)((l - e / s) * 0.69314718055994530942);
         }
     }
     if (!TOP) return;
-    const int n = a.parts * a.top;
-    for (int i = tid; i < n; i += 256) c[i] = tops[i / a.top * kTopMost + i % a.top];
+    if (wv == 0) {
+        float most = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < kRuns; ++r)
+#pragma unroll
+            for (int w = 0; w < W; ++w) most = fmaxf(most, st[0].runs[r][w * 64 + lane]);
+        const float f = floor_of(most, a.top);
+        if (lane == 0) row_floor = f;
+    }
     __syncthreads();
-    const long long o = (long long)row * a.top;
-    if (!(lse == lse)) {
-        if (tid < a.top) {
-            if (a.top_ids) a.top_ids[o + tid] = -1;
-            if (a.top_logprobs) a.top_logprobs[o + tid] = NAN;
+    const float floor = row_floor;
+    for (int r = 0; r < kRuns; ++r) {
+        const int t = t0 + wv + W * r * each;        // the run's first tile
+        if (t < t1 && t * L * 64 + lane < pieces && st[0].runs[r][tid] >= floor) {
+            const int k = atomicAdd(&n_held, 1);
+            if (k < kRoom) held[k] = (uint16_t)(r * 64 * W + tid);
         }
+    }
+    __syncthreads();
+    const int runs = n_held;
+    if (runs <= kRoom) {
+        const auto keep = [&](float x, int id) {
+            if (!(x >= floor)) return;
+            const int k = atomicAdd(&n_flat, 1);
+            if (k < kRoom) flat[k] = make_float2(x, __int_as_float(id));
+        };
+        if (on_edge) keep(x_edge, edge);
+        for (int i = tid; i < runs * each * L; i += 64 * W) {
+            const int h = held[i / (each * L)], k = i % (each * L);
+            const int t = t0 + h / 64 % W + W * (h / (64 * W) * each + k / L), p = (t * L + k % L) * 64 + h % 64;
+            if (t >= t1 || p >= pieces) continue;
+            const u32x4 w = *(const u32x4*)(body + (size_t)p * 16);
+#pragma unroll
+            for (int e = 0; e < V; ++e) keep(element<BF16>(&w, e), head + p * V + e);
+        }
+    }
+    __syncthreads();
+    int all = n_flat;
+    if (runs > kRoom || all > kRoom) {       // in order, a list a wave
+        __syncthreads();                     // (st was read as runs, n_flat by all)
+        Best best = {st[0].lists.list[wv], st[0].lists.sorted[wv], floor, false, 0, a.top};
+        if (edges) push(best, x_edge, edge, on_edge && lane < head);
+        for (int t = t0 + wv; t < t1; t += W) {
+            fetch(buf, t);
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                const int p = (t * L + i) * 64 + lane;
+#pragma unroll
+                for (int k = 0; k < V; ++k) push(best, element<BF16>(buf, i * V + k), head + p * V + k, p < pieces);
+                if (best.count > kTight) tighten(best);
+            }
+        }
+        if (edges) push(best, x_edge, edge, on_edge && lane >= head);
+        if (best.count > kTight) tighten(best);
+        if (lane == 0) counts[wv] = best.count;
+        __syncthreads();
+        int from = 0;
+        all = 0;
+        for (int w = 0; w < W; ++w) {
+            if (w < wv) from += counts[w];
+            all += counts[w];
+        }
+        if (lane < best.count) flat[from + lane] = best.list[lane];
+    }
+    if (tid < kPad) flat[all + tid] = nobody();
+    __syncthreads();
+    float2* tops = (float2*)(a.ws + kPartRooms * sizeof(LpPart)) + room * kTopMost;
+    const bool bad = a.parts == 1 && row_lse != row_lse;
+    for (int i = tid; i < all && !bad; i += 64 * W) {
+        const int r = rank_in(flat, all, flat[i]);
+        if (r >= a.top) continue;
+        if (a.parts > 1) tops[r] = flat[i];
+        else store_top(a, row, r, flat[i], false, row_m, row_lse);
+    }
+    if (a.parts > 1 && tid >= all && tid < a.top) tops[tid] = nobody();
+    if (bad && tid < a.top) store_top(a, row, tid, nobody(), true, 0.f, 0.0);
+}
+
+// Joins a row's parts: a block a row. Of the parts' sorted lists only what may be among the first `top` of all is ranked:
+// what reaches the top-th largest of 64 of them, the parts' firsts, seconds and so on.
+template <bool TOP>
+__global__ void __launch_bounds__(256) logprobs_join(LogprobArgs a, int row0) {
+    __shared__ float2 kept[TOP ? kParts * kTopMost + kPad : 1];
+    __shared__ int count;
+    __shared__ double lse;
+    __shared__ float mx, least;
+    const int tid = threadIdx.x, row = row0 + blockIdx.x;
+    const LpPart* parts = (const LpPart*)a.ws + (size_t)blockIdx.x * a.parts;
+    const float2* tops = (const float2*)(a.ws + kPartRooms * sizeof(LpPart)) + (size_t)blockIdx.x * a.parts * kTopMost;
+    const int n = TOP ? a.parts * a.top : 0;
+    float2 mine[kParts * kTopMost / 256];
+    if (TOP) {
+#pragma unroll
+        for (int i = 0; i < kParts * kTopMost / 256; ++i) {
+            const int k = tid + 256 * i;
+            mine[i] = k < n ? tops[k / a.top * kTopMost + k % a.top] : nobody();
+        }
+    }
+    if (tid < 64) {
+        LpPart p = tid < a.parts ? parts[tid] : LpPart{0.0, 0.0, -INFINITY, 0};
+        const float m = wave_max(p.m);
+        double s, e;
+        against(p, m, a.c, s, e);
+        int above = p.above;
+        for (int k = 32; k; k >>= 1) above += __shfl_xor(above, k);
+        p = {wave_sum_d(s), wave_sum_d(e), m, above};
+        if (tid == 0) {
+            const bool bad = no_distribution(p);
+            const double l = bad ? (double)NAN : log2(p.s);
+            lse = l;
+            mx = m;
+            count = 0;
+            finish(a, row, p, bad, l);
+        }
+    } else if (TOP && tid < 128) {
+        const int i = tid - 64, depth = i / a.parts;
+        const bool on = depth < min(64 / a.parts, a.top);
+        const float f = floor_of(on ? tops[i % a.parts * kTopMost + depth].x : -INFINITY, a.top);
+        if (tid == 64) least = f;
+    }
+    if (!TOP) return;
+    __syncthreads();
+    if (lse != lse) {
+        if (tid < a.top) store_top(a, row, tid, nobody(), true, 0.f, 0.0);
         return;
     }
-    for (int i = tid; i < n; i += 256) {
-        const float2 mine = c[i];
-        int r = 0;
-        for (int k = 0; k < n; ++k) r += before(c[k].x, __float_as_int(c[k].y), mine.x, __float_as_int(mine.y));
-        if (r < a.top && __float_as_int(mine.y) < a.vocab) {
-            if (a.top_ids) a.top_ids[o + r] = __float_as_int(mine.y);
-            if (a.top_logprobs)
-                a.top_logprobs[o + r] = (float)((((double)mine.x - mx) * a.c - lse) * 0.69314718055994530942);
-        }
+#pragma unroll
+    for (int i = 0; i < kParts * kTopMost / 256; ++i)
+        if (mine[i].x >= least && __float_as_int(mine[i].y) < a.vocab) kept[atomicAdd(&count, 1)] = mine[i];
+    __syncthreads();
+    const int all = count;
+    if (tid < kPad) kept[all + tid] = nobody();
+    __syncthreads();
+    for (int k = tid; k < all; k += 256) {
+        const int r = rank_in(kept, all, kept[k]);
+        if (r < a.top) store_top(a, row, r, kept[k], false, mx, lse);
     }
 }
 
 hipError_t launch_logprobs(LogprobArgs a, hipStream_t st) {
-    const int el = a.bf16 ? 8 : 4, tiles = (a.vocab / el + 64 * kLoads - 1) / (64 * kLoads);
-    a.parts = std::max(1, std::min({kParts, (tiles + 3) / 4, (2048 + a.rows - 1) / a.rows}));
+    const int el = a.bf16 ? 8 : 4, tiles = (a.vocab / el + 64 * kEach / el - 1) / (64 * kEach / el);
+    // Blocks of four waves, as many of a row as give every CU four, each wave with a tile at least. The card holds about
+    // 1280 of them: of more rows a block has two waves, whose ends fill the CUs better (1999 rows of 32,003 bf16 42.3 ->
+    // 37.6 us; with fewer rows the candidates' steps of twice the blocks cost more: 256 rows of 248,320 float32 and 32
+    // tokens 50.1 -> 55.2).
+    const bool pairs = a.rows > 1280;
+    a.parts = std::max(1, std::min({kParts, (tiles + 3) / 4, 1024 / a.rows}));
     const int most = kPartRooms / a.parts;
+    const auto pick = [&](auto bf16, auto top) {
+        constexpr bool b = decltype(bf16)::value, t = decltype(top)::value;
+        return pairs ? logprobs_kernel<b, t, 2> : logprobs_kernel<b, t, 4>;
+    };
+    using Yes = std::true_type;
+    using No = std::false_type;
+    const auto k = a.bf16 ? (a.top ? pick(Yes{}, Yes{}) : pick(Yes{}, No{})) : (a.top ? pick(No{}, Yes{}) : pick(No{}, No{}));
     for (int r = 0, m; r < a.rows; r += m) {
         m = std::min(most, a.rows - r);
-        const dim3 grid((unsigned)(m * a.parts));
-        const auto k = a.bf16 ? (a.top ? logprobs_kernel<true, true> : logprobs_kernel<true, false>)
-                              : (a.top ? logprobs_kernel<false, true> : logprobs_kernel<false, false>);
-        hipLaunchKernelGGL(k, grid, dim3(256), 0, st, a, r);
+        hipLaunchKernelGGL(k, dim3((unsigned)(m * a.parts)), dim3(pairs ? 128 : 256), 0, st, a, r);
         hipError_t rc = hipGetLastError();
         if (rc != hipSuccess) return rc;
+        if (a.parts == 1) continue;
         hipLaunchKernelGGL(a.top ? logprobs_join<true> : logprobs_join<false>, dim3(m), dim3(256), 0, st, a, r);
         rc = hipGetLastError();
         if (rc != hipSuccess) return rc;

@@ -2,8 +2,11 @@
 they can go wrong.
 
 Tolerances, in units of e = 2^-24. z = (x - m) c is off by three roundings, 3 e |z|, so a term w = 2^z by 3 e |z| ln 2
-and the instruction's 2 e; the term of the maximum itself is exact, and sums end in float64. With gap = sum w |z| ln 2 /
-S and r rescalings of a wave (one a tile at most, each another 2 e), log S is off by (8 + 3 gap + 2 r) e (S - 1) / S.
+and the instruction's 2 e, and a float32 sum of 32 terms by eights by its 3 + 3 roundings, 6 e; the sums end in float64.
+The term of the maximum itself, 1, is exact; it lies in one such sum of a wave, whose 6 roundings may then be e
+each, unless the wave's S is under 2, where that sum is made without it: 6 e at S - 1 >= 1, so 6 e (S - 1) at most.
+With gap = sum w |z| ln 2 / S and r rescalings of a wave (one a tile at most, each another 2 e), log S is off by
+(14 + 3 gap + 2 r) e (S - 1) / S.
 The entropy log S + gap adds gap's own error: up to 64 terms of a lane in float32, (64 + 8 + 2 r) e gap + 3 e gap2,
 gap2 = sum w z^2 / S, and log S's relative one. Each result is rounded once, e |result|. Ranks and ids are exact."""
 import numpy as np
@@ -72,7 +75,7 @@ def check(got, x, targets, top, temperature=1.0, skip=()):
         zz = np.where(w > 0, z, 0)
         gap, gap2 = (w * -zz).sum() / s, (w * zz * zz).sum() / s
         lse = np.log1p(w[np.arange(v) != row.argmax()].sum())
-        e_lse = (8 + 3 * gap + 2 * tiles) * E * (1 - 1 / s) + 1e-15
+        e_lse = (14 + 3 * gap + 2 * tiles) * E * (1 - 1 / s) + 1e-15
         e_ent = (72 + 2 * tiles) * E * gap + 3 * E * gap2 + e_lse * (1 + gap)
         order = np.lexsort((np.arange(v), -row))
         if 0 <= t < v:
