@@ -88,9 +88,8 @@ int q35_op_attn_kv4_shared(q35_engine* e, q35_kv4* prefix, q35_kv4* c, int layer
         a.q_heads = q_heads; a.kv_heads = c->kv_heads; a.D = c->D; a.TT = T; a.scale = scale; a.part = ev.kv4_part;
         OnDevice on(ev.device);
         // A launch takes sequences out of kSeqArgs neighbours, as many of their rows as the partial results have room for.
-        const long long room = kv4_shared_room(c->D);
-        const int rows = (int)std::min<long long>(T, room / kv4_shared_need(q_heads));
-        const int most = (int)std::min<long long>(kSeqArgs, room / kv4_shared_need((long long)rows * q_heads));
+        const long long room = kv4_shared_room(c->D) / c->kv_heads;
+        const int group = q_heads / c->kv_heads, rows = (int)std::min<long long>({T, std::max(room / 2 * 16 / group, 1LL), 32768 / group});
         std::vector<int> order;
         for (int i0 = 0; i0 < n; i0 += kSeqArgs) {
             order.resize(std::min(kSeqArgs, n - i0));
@@ -105,19 +104,22 @@ int q35_op_attn_kv4_shared(q35_engine* e, q35_kv4* prefix, q35_kv4* c, int layer
                 const auto moved = [&](HeadView v) { return HeadView{v.p ? v.p + ((long long)i0 * T + t0) * v.row : nullptr, v.row, v.head}; };
                 a.q = moved(qv); a.gate = moved(gv); a.out = moved(ov);
                 for (size_t k = 0; k < order.size();) {
-                    a.n = a.groups = 0;
-                    for (; k < order.size() && a.n < most; ++k) {
-                        const int i = order[k];
-                        if (a.n == 0 || less(order[k - 1], i)) {
-                            if (a.groups == kGroupArgs) break;
-                            a.gstart[a.groups] = (uint16_t)a.n;
-                            a.glane[a.groups] = (uint16_t)(has(i) ? prefix_lanes[i] : 0);
-                            a.glen[a.groups++] = has(i) ? prefix_lens[i] : 0;
+                    a.n = a.entries = 0;
+                    long long used = 0;
+                    for (; k < order.size(); ++k) {
+                        const int i = order[k], next = a.n == 0 || less(order[k - 1], i), per = a.T * group;
+                        const long long with = next ? 0 : a.n - a.gstart[a.entries - 1];
+                        const long long more = kv4_tiles(per) + kv4_tiles((with + 1) * per) - kv4_tiles(with * per);
+                        if (a.n && (a.entries + next > kEntryArgs || used + more > room)) break;
+                        used += more;
+                        if (next) {
+                            a.gstart[a.entries] = (uint16_t)a.n;
+                            a.glane[a.entries] = (uint16_t)(has(i) ? prefix_lanes[i] : 0);
+                            a.glen[a.entries++] = has(i) ? prefix_lens[i] : 0;
                         }
                         a.pos[a.n] = pos[i] + t0;
                         a.lane[a.n] = (uint16_t)(lanes ? lanes[i] : i);
-                        a.seq[a.n] = (uint8_t)(i - i0);
-                        a.group[a.n++] = (uint8_t)(a.groups - 1);
+                        a.seq[a.n++] = (uint8_t)(i - i0);
                     }
                     HCK(launch_attn_kv4_shared(a, ev.st));
                 }

@@ -8,9 +8,9 @@
 
 namespace q35 {
 
-// Attention of answers that share prompts. The launch's sequences are sorted by prompt; group j's are gstart[j] ..
-// gstart[j + 1] - 1 (those without a prompt the last group, of length 0). Each block leaves a partial result of its rows.
-constexpr int kGroupArgs = 64;       // prompts of one launch
+// Attention of answers that share prompts. The launch's sequences are sorted by prompt; entry j is the prompt of gcount
+// sequences from gstart on (those without one are the last entry, of length 0). Each block leaves partial results.
+constexpr int kEntryArgs = 64;       // prompts of one launch
 struct Kv4Shared {
     const uint8_t *prefix, *cache;                       // layer bases
     size_t prefix_lane, prefix_region, lane_bytes, region;
@@ -18,19 +18,20 @@ struct Kv4Shared {
     int q_heads, kv_heads, D, T, TT;                     // T of a sequence's TT rows are this launch's
     float scale;
     float* part;
-    int n, groups;
-    int prefix_blocks, own_splits;                       // (set by the launcher, as all below but pos, lane, seq, glen, glane, gstart)
-    long long own_part;                                  // first partial row of the sequences' own slots
+    int n, entries;
+    int prompt_blocks, own_splits, own_units, own_part;  // (set by the launcher, as all below but pos, lane, seq, glen, glane, gstart)
+    uint32_t per_inv, group_inv, kv_inv;                 // reciprocals of T x group, group and kv_heads
     alignas(16) int pos[kSeqArgs];
     alignas(16) uint16_t lane[kSeqArgs];
     alignas(16) uint16_t first[kSeqArgs];                // first split of each sequence's own slots; 0xffff past the last
-    alignas(16) uint8_t seq[kSeqArgs], group[kSeqArgs];  // which row block of the views it is; its prompt
-    alignas(16) int gfirst[kGroupArgs], gpart[kGroupArgs], glen[kGroupArgs];   // first block, first partial row, slots
-    alignas(16) uint16_t glane[kGroupArgs], gstart[kGroupArgs], gsplits[kGroupArgs];
+    alignas(16) uint8_t seq[kSeqArgs];                   // its row block in the views
+    alignas(16) int gfirst[kEntryArgs], gpart[kEntryArgs], glen[kEntryArgs], gtile[kEntryArgs];   // first block, first partial tile, slots, first tile to join
+    alignas(16) uint16_t glane[kEntryArgs], gstart[kEntryArgs], gcount[kEntryArgs], gsplits[kEntryArgs];
 };
 static_assert(sizeof(Kv4Shared) <= 4096, "kernel arguments");
-// Partial rows that a launch of `rows` rows (sequences x T x query heads) needs at least, and has.
-inline long long kv4_shared_need(long long rows) { return 2 * rows; }
+// Partial results lie in tiles of 16 rows: a launch needs at least kv_heads times kv4_tiles of each prompt's rows and of each
+// sequence's (T x group), and has room for so many.
+inline long long kv4_tiles(long long rows) { return (rows + 15) / 16; }
 long long kv4_shared_room(int D);
 hipError_t launch_attn_kv4_shared(Kv4Shared& a, hipStream_t st);
 

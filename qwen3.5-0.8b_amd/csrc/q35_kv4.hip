@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) attn_kv4_kernel(Kv4Attn
     auto at = [&](int i) { return i < tl.sink ? i : i - tl.sink + tl.main; };
     const auto tile_at = [&](int i) { return region + (size_t)at(i) * kv4_tile_bytes(D); };
     Tile<D> buf[kAhead<D>];
-    first_tiles<D, NQ>(buf, t0, t1, tile_at, lo);
+    first_tiles<D, NQ, 4>(buf, t0, t1, tile_at, lo);
     q35_bf16x8 qf[NQ == 1 ? D / 32 : 1];
     q35_bf16x8* ql = (q35_bf16x8*)&os[0][0][0][0];
     if constexpr (NQ == 1) {
@@ -450,17 +450,21 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) attn_kv4_kernel(Kv4Attn
     // tiles whose every slot every row of the block sees: from the last row's window to the first row's slot
     const int full0 = a.window > 0 ? max(pos + rho1 / group - a.window + 1, 0) : 0, full1 = pos + rho0 / group;
     Rows<D, NQ> st;
-    walk_tiles<D, NQ>(st, buf, t0, t1, at, tile_at, lo, q, qlane, sight, full0, full1, scale2);
-    join_waves<D, NQ>(st, rows - rho0, os, ms, ls, bs, [&](int c) {
+    walk_tiles<D, NQ, 4>(st, buf, t0, t1, at, tile_at, lo, q, qlane, sight, full0, full1, scale2);
+    join_waves<D, NQ, 4>(st, rows - rho0, os, ms, ls, bs, [&](int c) {
         const Out to = out_of(a, seq, h, rho0 + c * 16 + nn);
-        return [=, &a](float* x, int d, float m, float sum) {
-            if (splits == 1) {
-                to.store<D / 64>(a, x, sum, d);
-            } else {
-                float* p = a.part + ((((size_t)z * a.kv_heads + h) * row_tiles + rt) * NQ + c) * kSplitRows * (D + 4) + nn * (D + 4);
+        return [=, &a](float (*x)[D / 64], float m, float sum) {
 #pragma unroll
-                for (int i = 0; i < D / 64; ++i) p[d + i] = x[i];
-                if (d == 0) { p[D] = m; p[D + 1] = sum; }
+            for (int r = 0; r < 4; ++r) {
+                const int d = first_dim<D, 4>(r);
+                if (splits == 1) {
+                    to.store<D / 64>(a, x[r], sum, d);
+                } else {
+                    float* p = a.part + ((((size_t)z * a.kv_heads + h) * row_tiles + rt) * NQ + c) * kSplitRows * (D + 4) + nn * (D + 4);
+#pragma unroll
+                    for (int i = 0; i < D / 64; ++i) p[d + i] = x[r][i];
+                    if (d == 0) { p[D] = m; p[D + 1] = sum; }
+                }
             }
         };
     });

@@ -5,8 +5,7 @@
 // l_p and sums o_p, out = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p. A prompt's part has the rows of all its answers
 // (answers x T x query heads of a kv head) in the MFMAs' N dimension, so a tile of slots is fetched and turned
 // into bf16 once for 32 rows instead of once for each answer's 4 or 16; the answers' own slots are short lists, as in
-// the attention of single lanes. Both kinds are blocks of one launch, split so that all take about as long; a second launch
-// joins the parts.
+// the attention of single lanes. Both kinds are blocks of one launch, and a second launch joins the parts.
 #include <algorithm>
 #include <climits>
 
@@ -15,81 +14,52 @@
 
 namespace q35 {
 
-long long kv4_shared_room(int D) { return (long long)(kv4_part_floats() / (D + 4)); }
+// A partial result of 16 rows, as the waves that end it hold it, so that stores and loads are whole runs (rows of dims in
+// order, in pieces of 16 bytes from 64 lanes, took 5 us of 256 blocks' 17): row n's kRun dims from (4 g + r) D / 16 + w kRun on
+// at kRun (64 (4 w + r) + 16 g + n), g, r, w < 4; then the rows' references and sums of weights.
+template <int D>
+constexpr int kRun = D / 64;
+__host__ __device__ constexpr int tile_floats(int D) { return 16 * D + 32; }
+long long kv4_shared_room(int D) { return (long long)(kv4_part_floats() / tile_floats(D)); }
 
-// What a block works on: rows rho0 .. of the `rows` rows of the sorted sequences from `start` on, over tiles t0 .. t1 - 1.
+// x / d for x d < 2^32, by d's reciprocal 2^32 / d + 1 (0 stands for d = 1): what the product has too much is under
+// x / 2^32 < 1 / d. A launch's rows are at most 16 of the partial results' tiles, 129,072 of 64 dims, its T x group at most
+// 32,768, its kv_heads and group 1024.
+static uint32_t reciprocal(int d) { return d > 1 ? (uint32_t)(0x100000000ull / d + 1) : 0; }
+__device__ __forceinline__ int over(int x, uint32_t inv) { return inv ? (int)__umulhi((uint32_t)x, inv) : x; }
+
+// Rows rho0 .. of the `rows` rows of the sorted sequences from `start` on, over tiles t0 .. t1 - 1 of a region.
 struct Part {
     const uint8_t* region;
     int start, rows, rho0, h, t0, t1;
-    int last;                        // a prompt's last slot; -1: a row sees up to its own position
-    int pos;                         // of the sequence's row 0 (own slots)
-    long long row0;                  // where the part's rows go in the partial results
+    int last;                        // the last slot of all rows, or -1: a row's own position, from pos on
+    int pos;
+    int tile;                        // where its rows go: tiles of partial results from here on
 };
 
-__device__ __forceinline__ Part prompt_part(const Kv4Shared& a, int per, int tile_rows) {
-    const int b = blockIdx.x, lane = threadIdx.x & 63;
-    const int f = a.gfirst[lane], pt = a.gpart[lane], ln = a.glen[lane], gl = a.glane[lane], gs = a.gstart[lane], sp = a.gsplits[lane];
-    const int j = __popcll(__ballot(f <= b)) - 1;
-    const auto of = [&](int v, int i) { return __builtin_amdgcn_readlane(v, i); };
-    const int end = j + 1 < a.groups ? of(gs, j + 1) : a.n, splits = of(sp, j), tiles = (of(ln, j) + 31) >> 5;
-    // splits vary fastest: the blocks of one split, which read the same tiles, lie on one XCD where the
-    // splits are a multiple of 8
-    const int ix = b - of(f, j), split = ix % splits, item = ix / splits;
-    Part p;
-    p.start = of(gs, j);
-    p.rows = (end - p.start) * per;
-    p.h = item % a.kv_heads;
-    p.rho0 = item / a.kv_heads * tile_rows;
-    p.t0 = (int)((long long)tiles * split / splits);
-    p.t1 = (int)((long long)tiles * (split + 1) / splits);
-    p.region = a.prefix + of(gl, j) * a.prefix_lane + p.h * a.prefix_region;
-    p.last = of(ln, j) - 1;
-    p.pos = 0;
-    p.row0 = of(pt, j) + (long long)(split * a.kv_heads + p.h) * p.rows;
-    return p;
-}
-__device__ __forceinline__ Part own_part(const Kv4Shared& a, int per, int tile_rows) {
-    const int row_tiles = (per + tile_rows - 1) / tile_rows, lane = threadIdx.x & 63;
-    const int b = blockIdx.x - a.prefix_blocks, z = b / (row_tiles * a.kv_heads), ix = b % (row_tiles * a.kv_heads);
-    const uint2 f = ((const uint2*)a.first)[lane], l = ((const uint2*)a.lane)[lane];
-    const uint4 ps = ((const uint4*)a.pos)[lane];
-    const uint32_t f0 = f.x & 0xffffu, f1 = f.x >> 16, f2 = f.y & 0xffffu, f3 = f.y >> 16, zz = (uint32_t)z;
-    const int i = __popcll(__ballot(f0 <= zz)) + __popcll(__ballot(f1 <= zz)) + __popcll(__ballot(f2 <= zz)) +
-                  __popcll(__ballot(f3 <= zz)) - 1;
-    const int first = entry(f0, f1, f2, f3, i), splits = (i + 1 < a.n ? entry(f0, f1, f2, f3, i + 1) : a.own_splits) - first;
-    Part p;
-    p.start = i;
-    p.rows = per;
-    p.h = ix % a.kv_heads;
-    p.rho0 = ix / a.kv_heads * tile_rows;
-    p.pos = entry(ps.x, ps.y, ps.z, ps.w, i);
-    const int tiles = ((p.pos + (min(p.rho0 + tile_rows, per) - 1) / (per / a.T)) >> 5) + 1;
-    p.t0 = (int)((long long)tiles * (z - first) / splits);
-    p.t1 = (int)((long long)tiles * (z - first + 1) / splits);
-    p.region = a.cache + entry(l.x & 0xffffu, l.x >> 16, l.y & 0xffffu, l.y >> 16, i) * a.lane_bytes + p.h * a.region;
-    p.last = -1;
-    p.row0 = a.own_part + (long long)(z * a.kv_heads + p.h) * per;
-    return p;
-}
-
-// A block's part: its four waves take every fourth tile, their states are joined through LDS.
-template <int D, int NQ>
-__device__ __forceinline__ void part_rows(const Kv4Shared& a, const Part& p, f32x4 (*os)[4][D / 64][64], float (*ms)[16],
-                                          float (*ls)[16], uint32_t (*bs)[16]) {
-    const int tid = threadIdx.x, lane = tid & 63, nn = lane & 15, g = lane >> 4;
-    const int group = a.q_heads / a.kv_heads, per = a.T * group;
+// A part: by a block's four waves, each every fourth tile, their states joined through LDS (W 4), or by a wave (1).
+template <int D>
+struct Exchange {                    // between a block's waves
+    f32x4 os[4][4][D / 64][64];
+    float ms[4][16], ls[4][16];
+    uint32_t bs[4][16];
+};
+template <int D, int NQ, int W>
+__device__ __forceinline__ void part_rows(const Kv4Shared& a, const Part& p, uint32_t seqs, Exchange<D>& ex) {
+    const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63, nn = lane & 15, g = lane >> 4, group = a.q_heads / a.kv_heads;
     const float scale2 = fmaxf(fabsf(a.scale) * 1.44269504088896f, 0x1p-149f);      // (as in the attention of single lanes)
     const Lanes lo = lane_offsets<D>();
     const auto at = [&](int i) { return i; };
     const auto tile_at = [&](int i) { return p.region + (size_t)i * kv4_tile_bytes(D); };
     Tile<D> buf[kAhead<D>];
-    first_tiles<D, NQ>(buf, p.t0, p.t1, tile_at, lo);
+    first_tiles<D, NQ, W>(buf, p.t0, p.t1, tile_at, lo);
     const uint16_t* qrow[NQ];
     Sight sight[NQ];
 #pragma unroll
     for (int c = 0; c < NQ; ++c) {
-        const int rho = min(p.rho0 + c * 16 + nn, p.rows - 1), i = rho / per, r = rho - i * per, t = r / group;
-        qrow[c] = a.q.p + ((long long)a.seq[p.start + i] * a.TT + t) * a.q.row + (p.h * group + r - t * group) * a.q.head;
+        const int rho = min(p.rho0 + c * 16 + nn, p.rows - 1), i = over(rho, a.per_inv), r = rho - i * a.T * group;
+        const int t = over(r, a.group_inv), s = p.start + i, seq = __shfl((int)seqs, s >> 2) >> 8 * (s & 3) & 255;
+        qrow[c] = a.q.p + ((long long)seq * a.TT + t) * a.q.row + (p.h * group + r - t * group) * a.q.head;
         sight[c] = {p.last >= 0 ? p.last : p.pos + t, 0, 0};
     }
     const auto q_at = [&](int c, int gg, int k) {
@@ -98,150 +68,256 @@ __device__ __forceinline__ void part_rows(const Kv4Shared& a, const Part& p, f32
         return __builtin_bit_cast(q35_bf16x8, w);
     };
     q35_bf16x8 qf[NQ == 1 ? D / 32 : 1];
-    q35_bf16x8* ql = (q35_bf16x8*)&os[0][0][0][0];
+    q35_bf16x8* ql = (q35_bf16x8*)&ex.os[0][0][0][0] + (W == 1 ? wv * NQ * (D / 32) * 64 : 0);
     if constexpr (NQ == 1) {
 #pragma unroll
         for (int k = 0; k < D / 32; ++k) qf[k] = q_at(0, g, k);
     } else {
-        // wave w fetches every fourth step's operands
 #pragma unroll
         for (int c = 0; c < NQ; ++c)
-            for (int k = tid >> 6; k < D / 32; k += 4) ql[(c * (D / 32) + k) * 64 + lane] = q_at(c, g, k);
-        lds_barrier();
+#pragma unroll
+            for (int k = 0; k < (D / 32 + W - 1) / W; ++k) {
+                const int kk = W == 1 ? k : k * W + wv;
+                if (kk < D / 32) ql[(c * (D / 32) + kk) * 64 + lane] = q_at(c, g, kk);
+            }
+        if (W > 1) lds_barrier();
+        else wave_sync();
     }
     int qlane = lane;
     const auto q = [&](int c, int k) { return NQ == 1 ? qf[k] : ql[(c * (D / 32) + k) * 64 + qlane]; };
-    const int full1 = p.last >= 0 ? p.last : p.pos + p.rho0 / group;
+    const int full1 = p.last >= 0 ? p.last : p.pos + over(p.rho0, a.group_inv);
     Rows<D, NQ> st;
-    walk_tiles<D, NQ>(st, buf, p.t0, p.t1, at, tile_at, lo, q, qlane, sight, 0, full1, scale2);
-    join_waves<D, NQ>(st, p.rows - p.rho0, os, ms, ls, bs, [&](int c) {
-        float* to = a.part + (p.row0 + p.rho0 + c * 16 + nn) * (D + 4);
-        return [=](float* x, int d, float m, float sum) {
+    walk_tiles<D, NQ, W>(st, buf, p.t0, p.t1, at, tile_at, lo, q, qlane, sight, 0, full1, scale2);
+    if constexpr (W > 1) {
+        join_waves<D, NQ, W>(st, p.rows - p.rho0, ex.os, ex.ms, ex.ls, ex.bs, [&](int c) {
+            float* to = a.part + (size_t)(p.tile + c) * tile_floats(D);
+            return [=](float (*x)[kRun<D>], float m, float sum) {
 #pragma unroll
-            for (int i = 0; i < D / 64; ++i) to[d + i] = x[i];
-            if (d == 0) { to[D] = m; to[D + 1] = sum; }
-        };
-    });
-}
-
-// NQP, NQO: 16 rows a block takes of a prompt's and of an answer's own.
-template <int D, int NQP, int NQO>
-__global__ void __launch_bounds__(256, D == 256 ? 2 : 1) shared_kernel(Kv4Shared a) {
-    __shared__ f32x4 os[4][4][D / 64][64];
-    __shared__ float ms[4][16], ls[4][16];
-    __shared__ uint32_t bs[4][16];
-    static_assert(NQP == 1 || sizeof(os) >= NQP * (D / 32) * 1024, "the Q operands lie where the waves' sums go at the end");
-    const int per = a.T * (a.q_heads / a.kv_heads);
-    const bool prompt = (int)blockIdx.x < a.prefix_blocks;
-    if constexpr (NQP == NQO) {
-        const Part p = prompt ? prompt_part(a, per, NQP * 16) : own_part(a, per, NQP * 16);
-        part_rows<D, NQP>(a, p, os, ms, ls, bs);
-    } else if (prompt) {
-        part_rows<D, NQP>(a, prompt_part(a, per, NQP * 16), os, ms, ls, bs);
+                for (int r = 0; r < 4; ++r) __builtin_memcpy(to + (64 * (4 * wv + r) + lane) * kRun<D>, x[r], 4 * kRun<D>);
+                if (wv == 0 && g == 0) *(float2*)(to + 16 * D + 2 * nn) = make_float2(m, sum);
+            };
+        });
     } else {
-        part_rows<D, NQO>(a, own_part(a, per, NQO * 16), os, ms, ls, bs);
+#pragma unroll
+        for (int c = 0; c < NQ; ++c) {
+            uint32_t bad = st.bad[c];
+            bad |= (uint32_t)__shfl_xor((int)bad, 16);
+            bad |= (uint32_t)__shfl_xor((int)bad, 32);
+            if (p.rho0 + c * 16 + nn >= p.rows) continue;
+            float* to = a.part + (size_t)(p.tile + c) * tile_floats(D);
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float x[kRun<D>];
+#pragma unroll
+                    for (int i = 0; i < kRun<D>; ++i)
+                        x[i] = (bad >> ((4 * g + r) * (D / 16) + w * kRun<D>) / 32) & 1 ? __uint_as_float(0x7fc00000u) : st.o[c][w * kRun<D> + i][r];
+                    __builtin_memcpy(to + (64 * (4 * w + r) + lane) * kRun<D>, x, 4 * kRun<D>);
+                }
+            if (g == 0) *(float2*)(to + 16 * D + 2 * nn) = make_float2(st.m[c], st.l[c][0]);
+        }
     }
 }
 
-// Joins the parts: D / 4 threads a row, a thread four dims, kJoin parts' loads in flight.
-constexpr int kJoin = 8;
+// The launch's entries and sequences as a wave holds them, an entry and four sequences a lane: the arrays are kernel
+// arguments, cold in every cache at a launch, so all are fetched at once and picked from by lane. (Indexing them
+// costs a trip to memory for each that depends on another, and was compiled wrongly: an int array's scalar load from an
+// address that shares the index of a 16-bit one, whose low bit the hardware drops.)
+struct Entries {
+    int first, part, len, tile, lane, start, count, splits;
+    __device__ __forceinline__ Entries(const Kv4Shared& a) {
+        const int l = threadIdx.x & 63;
+        first = a.gfirst[l]; part = a.gpart[l]; len = a.glen[l]; tile = a.gtile[l];
+        lane = a.glane[l]; start = a.gstart[l]; count = a.gcount[l]; splits = a.gsplits[l];
+    }
+};
+__device__ __forceinline__ int pick(int v, int j) { return __builtin_amdgcn_readlane(v, j); }
+__device__ __forceinline__ int low16(uint2 v, int i) { return entry(v.x & 0xffffu, v.x >> 16, v.y & 0xffffu, v.y >> 16, i); }
+
+// NQP, NQO: 16 rows a block takes of a prompt's and a wave of an answer's own.
+template <int D, int NQP, int NQO>
+__global__ void __launch_bounds__(256, D == 256 ? 2 : 1) shared_kernel(Kv4Shared a) {
+    __shared__ Exchange<D> ex;
+    static_assert(NQO == 1 || sizeof(ex.os) >= 4 * NQO * (D / 32) * 1024, "the waves' Q operands lie where their sums go at the end");
+    const int per = a.T * (a.q_heads / a.kv_heads), lane = threadIdx.x & 63;
+    const uint32_t seqs = ((const uint32_t*)a.seq)[lane];
+    Part p;
+    if ((int)blockIdx.x < a.prompt_blocks) {
+        const Entries en(a);
+        const int j = __popcll(__ballot(en.first <= (int)blockIdx.x)) - 1;
+        const int len = pick(en.len, j), splits = pick(en.splits, j), tiles = (len + 31) >> 5;
+        // splits vary fastest: the blocks of one split of a prompt, which read the same tiles, lie on one XCD where the
+        // splits are a multiple of 8
+        const uint32_t ix = blockIdx.x - pick(en.first, j), item = ix / (uint32_t)splits, split = ix - item * splits;
+        const int each = (uint32_t)tiles / (uint32_t)splits, more = tiles - each * splits, rt = over(item, a.kv_inv);
+        p.start = pick(en.start, j);
+        p.rows = pick(en.count, j) * per;
+        p.h = item - rt * a.kv_heads;
+        p.rho0 = rt * NQP * 16;
+        p.t0 = split * each + min((int)split, more);
+        p.t1 = p.t0 + each + ((int)split < more);
+        p.region = a.prefix + pick(en.lane, j) * a.prefix_lane + p.h * a.prefix_region;
+        p.last = len - 1;
+        p.pos = 0;
+        p.tile = pick(en.part, j) + (split * a.kv_heads + p.h) * ((p.rows + 15) >> 4) + rt * NQP;
+        part_rows<D, NQP, 4>(a, p, seqs, ex);
+        return;
+    }
+    // Of a sequence's own slots a wave has a part to itself: the lists are short, and four waves of a block on one of them
+    // took longer to join than to walk it.
+    const int unit = __builtin_amdgcn_readfirstlane((blockIdx.x - a.prompt_blocks) * 4 + (threadIdx.x >> 6));
+    if (unit >= a.own_units) return;
+    const uint2 f = ((const uint2*)a.first)[lane], lanes = ((const uint2*)a.lane)[lane];
+    const uint4 ps = ((const uint4*)a.pos)[lane];
+    const int row_tiles = (per + NQO * 16 - 1) / (NQO * 16), zr = over(unit, a.kv_inv), z = (uint32_t)zr / (uint32_t)row_tiles, rt = zr - z * row_tiles;
+    const uint32_t zz = (uint32_t)z;
+    const int i = __popcll(__ballot((f.x & 0xffffu) <= zz)) + __popcll(__ballot((f.x >> 16) <= zz)) +
+                  __popcll(__ballot((f.y & 0xffffu) <= zz)) + __popcll(__ballot((f.y >> 16) <= zz)) - 1;
+    const int first = low16(f, i), splits = (i + 1 < a.n ? low16(f, i + 1) : a.own_splits) - first, split = z - first;
+    p.start = i;
+    p.rows = per;
+    p.h = unit - zr * a.kv_heads;
+    p.rho0 = rt * NQO * 16;
+    p.pos = entry(ps.x, ps.y, ps.z, ps.w, i);
+    const int tiles = ((p.pos + over(min(p.rho0 + NQO * 16, per) - 1, a.group_inv)) >> 5) + 1;
+    const int each = (uint32_t)tiles / (uint32_t)splits, more = tiles - each * splits;
+    p.t0 = split * each + min(split, more);
+    p.t1 = p.t0 + each + (split < more);
+    p.region = a.cache + low16(lanes, i) * a.lane_bytes + p.h * a.region;
+    p.last = -1;
+    p.tile = a.own_part + (z * a.kv_heads + p.h) * ((per + 15) >> 4) + rt * NQO;
+    part_rows<D, NQO, 1>(a, p, seqs, ex);
+}
+
+// Joins the parts of 16 rows of an entry: a wave one of a lane's runs of 4 dims (256 dims, so that there are waves enough)
+// or its four of 1 or 2 (8192 rows of 128 dims: 9.8 us by 2 dims a lane, 7.3 by 8), some parts in flight.
+template <int D>
+constexpr int kJoinBlocks = D == 256 ? 4 : 1;    // of four waves, for 16 rows
 template <int D>
 __global__ void __launch_bounds__(256) shared_join(Kv4Shared a) {
-    const int group = a.q_heads / a.kv_heads, per = a.T * group, d = threadIdx.x % (D / 4) * 4;
-    const long long e = ((long long)blockIdx.x * 256 + threadIdx.x) / (D / 4);
-    const int r = (int)(e % per), h = (int)(e / per % a.kv_heads);
-    const long long i = e / ((long long)per * a.kv_heads);
-    if (i >= a.n) return;
-    const int j = a.group[i];
-    const int end = j + 1 < a.groups ? a.gstart[j + 1] : a.n, start = a.gstart[j], prompt = a.glen[j] ? a.gsplits[j] : 0;
-    const int first = a.first[i], own = (i + 1 < a.n ? a.first[i + 1] : a.own_splits) - first;
-    const long long step = (long long)a.kv_heads * (end - start) * per, own_step = (long long)a.kv_heads * per;
-    const long long p0 = a.gpart[j] + ((long long)h * (end - start) + (i - start)) * per + r;
-    const long long o0 = a.own_part + ((long long)first * a.kv_heads + h) * per + r;
+    constexpr int N = kRun<D>, B = kJoinBlocks<D>, R = 4 / B, kJoin = B == 1 ? 4 : 8;
+    const int group = a.q_heads / a.kv_heads, per = a.T * group, lane = threadIdx.x & 63, g = lane >> 4;
+    const uint32_t seqs = ((const uint32_t*)a.seq)[lane];
+    const uint2 f = ((const uint2*)a.first)[lane];
+    const Entries en(a);
+    const int wv = threadIdx.x >> 6, r = B == 1 ? wv : blockIdx.x & 3, w0 = B == 1 ? 0 : wv, ix = blockIdx.x / B, j = __popcll(__ballot(en.tile <= ix)) - 1;
+    const int start = pick(en.start, j), rows = pick(en.count, j) * per, tiles = (rows + 15) >> 4, part = pick(en.part, j);
+    const int prompt = pick(en.len, j) ? pick(en.splits, j) : 0;
+    const uint32_t it = ix - pick(en.tile, j);
+    const int rt = over(it, a.kv_inv), h = it - rt * a.kv_heads, rho = rt * 16 + (lane & 15);
+    // this lane's row: of sequence i its row s
+    const int i0 = over(min(rho, rows - 1), a.per_inv), s = min(rho, rows - 1) - i0 * per, i = start + i0, t = over(s, a.group_inv);
+    const int seq = __shfl((int)seqs, i >> 2) >> 8 * (i & 3) & 255;
+    const auto first_of = [&](int k) {
+        const int x = __shfl((int)f.x, k >> 2), y = __shfl((int)f.y, k >> 2), v = k & 2 ? y : x;
+        return (k & 1 ? v >> 16 : v) & 0xffff;
+    };
+    const int first = first_of(i), next = first_of(min(i + 1, kSeqArgs - 1));
+    const int own = (i + 1 < a.n ? next : a.own_splits) - first, own_tiles = (per + 15) >> 4;
+    if (rho >= rows) return;
+    const int at = (64 * (4 * w0 + r) + 16 * g) * N;
+    const float* pp = a.part + (size_t)(part + h * tiles + rt) * tile_floats(D);
+    const float* po = a.part + (size_t)(a.own_part + (first * a.kv_heads + h) * own_tiles + (s >> 4)) * tile_floats(D);
+    const size_t step = (size_t)a.kv_heads * tiles * tile_floats(D), own_step = (size_t)a.kv_heads * own_tiles * tile_floats(D);
     const int parts = prompt + own;
-    f32x4 x = {0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, sum = 0.f;
-    for (int s0 = 0; s0 < parts; s0 += kJoin) {
-        f32x4 o[kJoin];
+    float x[R * N], m = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < R * N; ++e) x[e] = 0.f;
+    for (int k0 = 0; k0 < parts; k0 += kJoin) {
+        float o[kJoin][R * N];
         float2 ml[kJoin];
 #pragma unroll
-        for (int s = 0; s < kJoin; ++s) {
-            const int k = s0 + s;
-            const float* p = a.part + (k < prompt ? p0 + k * step : o0 + (k - prompt) * own_step) * (D + 4);
-            const bool in = k < parts;
-            o[s] = in ? *(const f32x4*)(p + d) : f32x4{0.f, 0.f, 0.f, 0.f};
-            ml[s] = in ? *(const float2*)(p + D) : make_float2(-INFINITY, 0.f);
+        for (int k = 0; k < kJoin; ++k) {
+            const int kk = min(k0 + k, parts - 1), n = kk < prompt ? lane & 15 : s & 15;
+            const float* from = kk < prompt ? pp + kk * step : po + (kk - prompt) * own_step;
+#pragma unroll
+            for (int w = 0; w < R; ++w) __builtin_memcpy(&o[k][w * N], from + at + (256 * w + n) * N, 4 * N);
+            ml[k] = *(const float2*)(from + 16 * D + 2 * n);
         }
         float mn = m;
 #pragma unroll
-        for (int s = 0; s < kJoin; ++s) mn = fmaxf(mn, ml[s].x);
+        for (int k = 0; k < kJoin; ++k) mn = fmaxf(mn, ml[k].x);
         const float mz = mn == -INFINITY ? 0.f : mn, al = __builtin_amdgcn_exp2f(m - mz);
-        x *= al;
-        sum *= al;
         m = mn;
+        sum *= al;
 #pragma unroll
-        for (int s = 0; s < kJoin; ++s) {
-            const float f = __builtin_amdgcn_exp2f(ml[s].x - mz);
-            sum += f * ml[s].y;
-            x += f * o[s];
+        for (int e = 0; e < R * N; ++e) x[e] *= al;
+#pragma unroll
+        for (int k = 0; k < kJoin; ++k) {
+            if (k0 + k >= parts) break;
+            const float c = __builtin_amdgcn_exp2f(ml[k].x - mz);
+            sum += c * ml[k].y;
+#pragma unroll
+            for (int e = 0; e < R * N; ++e) x[e] += c * o[k][e];
         }
     }
-    const int t = r / group;
-    Out(a, (long long)a.seq[i] * a.TT + t, h * group + r - t * group).template store<4>(a, (float*)&x, sum, d);
+    Out(a, (long long)seq * a.TT + t, h * group + s - t * group).template store<R * N>(a, x, sum, (4 * g + r) * (D / 16) + w0 * N);
 }
 
-constexpr int kPromptSplits = 128, kOwnSplits = 128;
+constexpr int kPromptSplits = 64, kOwnSplits = 64;
 template <int D>
 static hipError_t launch(Kv4Shared& a, hipStream_t st) {
-    const int group = a.q_heads / a.kv_heads, per = a.T * group;
-    const auto members = [&](int j) { return (j + 1 < a.groups ? a.gstart[j + 1] : a.n) - a.gstart[j]; };
+    const int group = a.q_heads / a.kv_heads, per = a.T * group, nqo = per > 16 ? 2 : 1;
     int most = 0;
-    for (int j = 0; j < a.groups; ++j)
-        if (a.glen[j]) most = std::max(most, members(j) * per);
-    const int nqp = most > 16 ? 2 : 1, nqo = per > 16 ? 2 : 1;
-    const auto row_tiles = [](int rows, int nq) { return (rows + nq * 16 - 1) / (nq * 16); };
+    for (int j = 0; j < a.entries; ++j) {
+        a.gcount[j] = (uint16_t)((j + 1 < a.entries ? a.gstart[j + 1] : a.n) - a.gstart[j]);
+        if (a.glen[j]) most = std::max(most, a.gcount[j] * per);
+    }
+    const int nqp = most > 16 ? 2 : 1;
+    const auto items = [&](int j) { return a.kv_heads * ((kv4_tiles(a.gcount[j] * per) + nqp - 1) / nqp); };
+    const auto prompt_tiles = [&](int j) { return (a.glen[j] + 31) >> 5; };
     const auto own_tiles = [&](int i) { return ((a.pos[i] + a.T - 1) >> 5) + 1; };
-    long long work = 0;                                  // tiles of all blocks
-    for (int j = 0; j < a.groups; ++j)
-        work += (long long)((a.glen[j] + 31) >> 5) * a.kv_heads * row_tiles(members(j) * per, nqp);
-    for (int i = 0; i < a.n; ++i) work += (long long)own_tiles(i) * a.kv_heads * row_tiles(per, nqo);
-    long long rows = 0, blocks = 0;
-    for (int tiles = (int)std::max<long long>(8, (work + 511) / 512);; tiles *= 2) {
-        rows = blocks = 0;
+    const long long own_items = a.kv_heads * ((kv4_tiles(per) + nqo - 1) / nqo);
+    long long work = 0, own = 0, part = 0, blocks = 0, joins = 0;
+    for (int j = 0; j < a.entries; ++j) work += prompt_tiles(j) * items(j);
+    for (int i = 0; i < a.n; ++i) own += own_tiles(i) * own_items;
+    // One block a CU, or two where each has 128 tiles or more: a second wave on a SIMD fills the waits of the first (512
+    // tiles of 256 dims: 97.8 -> 83.3 us; about 160 of 128: 51.1 -> 45.4), but twice the partial results take their time to write
+    // and to join (64 tiles of 256 dims: 23.8 + 5.7 -> 29.7 + 7.8).
+    long long tiles = std::max<long long>(8, (work + 255) / 256);
+    if (tiles >= 128) tiles = (tiles + 1) / 2;
+    long long own_per = std::max<long long>(8, (own + 2047) / 2048);
+    for (;; tiles *= 2, own_per *= 2) {
+        part = blocks = joins = 0;
         bool least = true;
-        for (int j = 0; j < a.groups; ++j) {
-            const int len = (a.glen[j] + 31) >> 5, s = std::min(kPromptSplits, (len + tiles - 1) / tiles);
+        for (int j = 0; j < a.entries; ++j) {
+            const int s = (int)std::min<long long>(kPromptSplits, (prompt_tiles(j) + tiles - 1) / tiles);
             least &= s <= 1;
             a.gfirst[j] = (int)blocks;
-            a.gpart[j] = (int)rows;
+            a.gpart[j] = (int)part;
+            a.gtile[j] = (int)joins;
             a.gsplits[j] = (uint16_t)std::max(1, s);
-            blocks += (long long)s * a.kv_heads * row_tiles(members(j) * per, nqp);
-            rows += (long long)s * a.kv_heads * members(j) * per;
+            blocks += s * items(j);
+            part += s * a.kv_heads * kv4_tiles(a.gcount[j] * per);
+            joins += a.kv_heads * kv4_tiles(a.gcount[j] * per);
         }
-        a.prefix_blocks = (int)blocks;
-        a.own_part = rows;
+        a.prompt_blocks = (int)blocks;
+        a.own_part = (int)part;
         int z = 0;
         for (int i = 0; i < a.n; ++i) {
-            const int s = std::min(kOwnSplits, (own_tiles(i) + tiles - 1) / tiles);
+            const int s = (int)std::min<long long>(kOwnSplits, (own_tiles(i) + own_per - 1) / own_per);
             least &= s == 1;
             a.first[i] = (uint16_t)z;
             z += s;
         }
         a.own_splits = z;
-        rows += (long long)z * a.kv_heads * per;
-        blocks += (long long)z * a.kv_heads * row_tiles(per, nqo);
-        if (rows <= kv4_shared_room(D)) break;
-        if (least) return hipErrorInvalidValue;
+        a.own_units = (int)(z * own_items);
+        part += z * a.kv_heads * kv4_tiles(per);
+        blocks += (a.own_units + 3) / 4;
+        if (part <= kv4_shared_room(D) || least) break;
     }
-    for (int j = a.groups; j < kGroupArgs; ++j) a.gfirst[j] = INT_MAX;
+    for (int j = a.entries; j < kEntryArgs; ++j) a.gfirst[j] = a.gtile[j] = INT_MAX;
     for (int i = a.n; i < kSeqArgs; ++i) a.first[i] = 0xffff;
-    if (blocks > kLaunchBlocks) return hipErrorInvalidValue;
+    if (part > kv4_shared_room(D) || blocks > kLaunchBlocks || joins * 4 > kLaunchBlocks) return hipErrorInvalidValue;
+    a.per_inv = reciprocal(per);
+    a.group_inv = reciprocal(group);
+    a.kv_inv = reciprocal(a.kv_heads);
     const auto k = nqp == 1 ? shared_kernel<D, 1, 1> : nqo == 1 ? shared_kernel<D, 2, 1> : shared_kernel<D, 2, 2>;
     hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(256), 0, st, a);
     const hipError_t rc = hipGetLastError();
     if (rc != hipSuccess) return rc;
-    const long long threads = (long long)a.n * a.kv_heads * per * (D / 4);
-    hipLaunchKernelGGL(shared_join<D>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(shared_join<D>, dim3((unsigned)joins * kJoinBlocks<D>), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 hipError_t launch_attn_kv4_shared(Kv4Shared& a, hipStream_t st) {

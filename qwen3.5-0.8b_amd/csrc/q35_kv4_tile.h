@@ -247,23 +247,23 @@ __device__ __forceinline__ void tile_step(Tile<D>& t, const uint8_t* tile_p, con
 // window 12.9 instead of 14.9 us).
 template <int D>
 constexpr int kAhead = D == 256 ? 1 : 2;
-// A block's four waves take every fourth of its tiles t0 .. t1 - 1: the loads of a wave's first ones.
-template <int D, int NQ, class TileAt>
+// W waves take every W-th of the tiles t0 .. t1 - 1 (a block's waves; 1: a wave for itself): the loads of a wave's first ones.
+template <int D, int NQ, int W, class TileAt>
 __device__ __forceinline__ void first_tiles(Tile<D>* buf, int t0, int t1, const TileAt& tile_at, const Lanes& lo) {
-    const int wv = threadIdx.x >> 6;
+    const int wv = W > 1 ? threadIdx.x >> 6 : 0;
     if (t0 + wv < t1) {
 #pragma unroll
         for (int b = 0; b < kAhead<D>; ++b) {
-            load_k<D, NQ == 1>(buf[b], tile_at(min(t0 + wv + 4 * b, t1 - 1)), lo);
-            load_v<D, NQ == 1>(buf[b], tile_at(min(t0 + wv + 4 * b, t1 - 1)), lo);
+            load_k<D, NQ == 1>(buf[b], tile_at(min(t0 + wv + W * b, t1 - 1)), lo);
+            load_v<D, NQ == 1>(buf[b], tile_at(min(t0 + wv + W * b, t1 - 1)), lo);
         }
     }
 }
-template <int D, int NQ, bool FAR, class At, class TileAt, class Q>
+template <int D, int NQ, int W, bool FAR, class At, class TileAt, class Q>
 __device__ __forceinline__ void walk_once(Rows<D, NQ>& st, Tile<D>* buf, int t0, int t1, const At& at, const TileAt& tile_at,
                                           const Lanes& lo, const Q& q, int& qlane, const Sight* sight, int full0, int full1,
                                           float scale2) {
-    const int wv = threadIdx.x >> 6;
+    const int wv = W > 1 ? threadIdx.x >> 6 : 0;
 #pragma unroll
     for (int c = 0; c < NQ; ++c) {
         st.m[c] = -INFINITY;
@@ -272,26 +272,26 @@ __device__ __forceinline__ void walk_once(Rows<D, NQ>& st, Tile<D>* buf, int t0,
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) st.o[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    for (int i0 = __builtin_amdgcn_readfirstlane(t0 + wv); i0 < t1; i0 += 4 * kAhead<D>) {
+    for (int i0 = __builtin_amdgcn_readfirstlane(t0 + wv); i0 < t1; i0 += W * kAhead<D>) {
 #pragma unroll
         for (int b = 0; b < kAhead<D>; ++b) {
-            const int i = i0 + 4 * b;
+            const int i = i0 + W * b;
             if (i >= t1) break;
             if (NQ > 1) asm volatile("" : "+v"(qlane));     // or the compiler reads Q ahead of the loop, and spills it
             const int tile = at(i);
             const bool edge = tile * 32 < full0 || tile * 32 + 31 > full1;
-            tile_step<D, NQ, NQ == 1, NQ == 2 && D == 256, FAR>(buf[b], tile_at(i), tile_at(min(i + 4 * kAhead<D>, t1 - 1)), lo,
+            tile_step<D, NQ, NQ == 1, NQ == 2 && D == 256, FAR>(buf[b], tile_at(i), tile_at(min(i + W * kAhead<D>, t1 - 1)), lo,
                                                                 tile * 32, edge, q, sight, scale2, st);
         }
     }
 }
 // A wave's state over its tiles. at(i): the number of the i-th tile (slots 32 at(i) .. + 31), tile_at(i): its address; every
 // row sees every slot of the tiles within full0 .. full1.
-template <int D, int NQ, class At, class TileAt, class Q>
+template <int D, int NQ, int W, class At, class TileAt, class Q>
 __device__ __forceinline__ void walk_tiles(Rows<D, NQ>& st, Tile<D>* buf, int t0, int t1, const At& at, const TileAt& tile_at,
                                            const Lanes& lo, const Q& q, int& qlane, const Sight* sight, int full0, int full1,
                                            float scale2) {
-    walk_once<D, NQ, false>(st, buf, t0, t1, at, tile_at, lo, q, qlane, sight, full0, full1, scale2);
+    walk_once<D, NQ, W, false>(st, buf, t0, t1, at, tile_at, lo, q, qlane, sight, full0, full1, scale2);
     // Two kinds of rows want their tiles gone over again in the FAR form (the other one is the faster: a 4096-row
     // prompt 83.6 us a call, with a test of the reference in every tile 86.3). References of 2^24 and more: there float32
     // numbers lie 2 and more apart, and the part of a product that its reference was rounded by, which a fused step
@@ -309,69 +309,61 @@ __device__ __forceinline__ void walk_tiles(Rows<D, NQ>& st, Tile<D>* buf, int t0
     }
     far |= __any(!(big < 0x1p100f));
     if (far) {
-        first_tiles<D, NQ>(buf, t0, t1, tile_at, lo);
-        walk_once<D, NQ, true>(st, buf, t0, t1, at, tile_at, lo, q, qlane, sight, full0, full1, scale2);
+        first_tiles<D, NQ, W>(buf, t0, t1, tile_at, lo);
+        walk_once<D, NQ, W, true>(st, buf, t0, t1, at, tile_at, lo, q, qlane, sight, full0, full1, scale2);
     }
 }
-// The four waves' states of `rows` rows: wave w ends a quarter of the row's dims, which the others pass it through LDS; a
-// lane keeps its row, and its accumulators go as they are. place(c) gives where row 16 c + lane % 16 goes: a function of
-// (D / 64 sums from dim d on, d, the reference, the sum of weights).
-template <int D, int NQ, class Place>
-__device__ __forceinline__ void join_waves(Rows<D, NQ>& st, int rows, f32x4 (*os)[4][D / 64][64], float (*ms)[16],
+// The W waves' states of `rows` rows: wave w ends a W-th of the row's dims, which all pass it through LDS (its own part too:
+// picking it out of the registers by the wave's number took longer); a lane keeps its row, and its accumulators go as they
+// are. place(c) gives where row 16 c + lane % 16 goes: a function of (sums x[r][i] of dim first_dim(r) + i, r < 4, i < D / 16 /
+// W; the reference; the sum of weights).
+template <int D, int W>
+__device__ __forceinline__ int first_dim(int r) {
+    return (4 * ((threadIdx.x & 63) >> 4) + r) * (D / 16) + (threadIdx.x >> 6) * (D / 16 / W);
+}
+template <int D, int NQ, int W, class Place>
+__device__ __forceinline__ void join_waves(Rows<D, NQ>& st, int rows, f32x4 (*os)[W][D / 16 / W][64], float (*ms)[16],
                                            float (*ls)[16], uint32_t (*bs)[16], const Place& place) {
-    constexpr int kQuarter = D / 64;         // of the D / 16 accumulators of 16 rows
+    constexpr int kPart = D / 16 / W;        // of the D / 16 accumulators of 16 rows
     const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63, nn = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int c = 0; c < NQ; ++c) {
         if (c * 16 >= rows) break;
-        if (NQ > 1 || c) __syncthreads();        // os was read: Q, or the 16 rows before these
+        if (NQ > 1 || c) lds_barrier();          // os was read: Q, or the 16 rows before these
         uint32_t bad = st.bad[c];
         bad |= (uint32_t)__shfl_xor((int)bad, 16);
         bad |= (uint32_t)__shfl_xor((int)bad, 32);
         if (g == 0) { ms[wv][nn] = st.m[c]; ls[wv][nn] = st.l[c][0]; bs[wv][nn] = bad; }
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
+        for (int w = 0; w < W; ++w)
 #pragma unroll
-            for (int i = 0; i < kQuarter; ++i)
-                if (w != wv) os[w][wv][i][lane] = st.o[c][w * kQuarter + i];
-        __syncthreads();
-        float m = st.m[c], sum = 0.f, f[4];
+            for (int i = 0; i < kPart; ++i) os[w][wv][i][lane] = st.o[c][w * kPart + i];
+        lds_barrier();
+        float m = st.m[c], sum = 0.f, f[W];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) m = fmaxf(m, ms[w][nn]);
+        for (int w = 0; w < W; ++w) m = fmaxf(m, ms[w][nn]);
         bad = 0;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < W; ++w) {
             f[w] = __builtin_amdgcn_exp2f(ms[w][nn] - (m == -INFINITY ? 0.f : m));
             sum += f[w] * ls[w][nn];
             bad |= bs[w][nn];
         }
-        f32x4 o[kQuarter];
+        f32x4 o[kPart];
 #pragma unroll
-        for (int i = 0; i < kQuarter; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < kPart; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < 4; ++w)              // in the same order in every wave
+        for (int w = 0; w < W; ++w)              // in the same order in every wave
 #pragma unroll
-            for (int i = 0; i < kQuarter; ++i) {
-                f32x4 x;
-                if (w == wv) {
-                    x = st.o[c][i];
-#pragma unroll
-                    for (int k = 1; k < 4; ++k) x = wv == k ? st.o[c][k * kQuarter + i] : x;
-                } else {
-                    x = os[wv][w][i][lane];
-                }
-                o[i] += f[w] * x;
-            }
+            for (int i = 0; i < kPart; ++i) o[i] += f[w] * os[wv][w][i][lane];
         if (c * 16 + nn >= rows) continue;
-        const auto to = place(c);
+        float x[4][kPart];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int d = (4 * g + r) * (D / 16) + wv * kQuarter;
-            float x[kQuarter];
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int i = 0; i < kQuarter; ++i) x[i] = (bad >> (d / 32)) & 1 ? __uint_as_float(0x7fc00000u) : o[i][r];
-            to(x, d, m, sum);
-        }
+            for (int i = 0; i < kPart; ++i)
+                x[r][i] = (bad >> (first_dim<D, W>(r) / 32)) & 1 ? __uint_as_float(0x7fc00000u) : o[i][r];
+        place(c)(x, m, sum);
     }
 }
 

@@ -15,7 +15,7 @@ hipError_t launch_heads(AxisHeadArgs& a, int n, hipStream_t) {
     return count();
 }
 hipError_t launch_logprobs(LogprobArgs, hipStream_t) { return count(); }
-long long kv4_shared_room(int) { return g_room ? g_room : 32768; }
+long long kv4_shared_room(int) { return g_room ? g_room : 2064; }
 hipError_t launch_attn_kv4_shared(Kv4Shared& a, hipStream_t) {
     g_shared = a;
     g_rows += (long long)a.n * a.T;
@@ -31,10 +31,11 @@ int stub_axes() { return g_axes.axes; }
 // What the last launch of shared attention took: sequences, prompts, T; then per sequence its row block, prompt and position.
 void stub_shared(int32_t* out) {
     *out++ = g_shared.n;
-    *out++ = g_shared.groups;
+    *out++ = g_shared.entries;
     *out++ = g_shared.T;
     for (int i = 0; i < g_shared.n; ++i) {
-        const int j = g_shared.group[i];
+        int j = 0;
+        while (j + 1 < g_shared.entries && g_shared.gstart[j + 1] <= i) ++j;
         *out++ = g_shared.seq[i];
         *out++ = g_shared.glen[j] ? g_shared.glane[j] : -1;
         *out++ = g_shared.glen[j];

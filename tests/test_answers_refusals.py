@@ -186,10 +186,11 @@ def test_shared_in_launches(lib):
 
     assert launches(256, 1, 8) == 1 and launches(257, 1, 8) == 2 and launches(1000, 1, 8) == 4
     assert launches(128, 1, 8, 64) == 1 and launches(130, 1, 8, 65) == 2 and launches(256, 1, 8, 100) == 2
-    assert launches(256, 8, 8) == 1 and launches(256, 9, 8) == 2          # 2 x 16,384 rows of 32,768
-    assert launches(1, 2048, 8) == 1 and launches(1, 2049, 8) == 2 and launches(3, 2048, 8) == 3
-    assert launches(1, 4096, 1024) == 256
-    lib.stub_room(2048)
+    # room for 2064 tiles of 16 rows, 1032 a kv head: T / 4 of each sequence (4 rows a query row), and as much of its prompt's
+    assert launches(256, 8, 8) == 1 and launches(256, 9, 8) == 2 and launches(128, 16, 8, 64) == 1 and launches(128, 17, 8, 64) == 2
+    assert launches(1, 2064, 8) == 1 and launches(1, 2065, 8) == 2 and launches(3, 4096, 8) == 6
+    assert launches(1, 4096, 1024) == 256      # 512 query heads each: 16 rows of T in 512 tiles
+    lib.stub_room(68)
     assert launches(5, 3, 1024) == 15
     lib.stub_room(0)
 
