@@ -382,6 +382,14 @@ typedef struct q35_logprobs {
     float* top_logprobs;             /* device [rows][top] */
 } q35_logprobs;
 int q35_op_token_logprobs(q35_engine* e, const q35_logprobs* d, int rows, int vocab);
+/* The same on the model's own rows, d's arrays host memory here and d->logits NULL (ld and dtype unread): a prompt as
+ * q35_prefill_all takes it, every row of it, where targets NULL stands for the prompt's own next tokens (the last row, which has
+ * none, gets log p NaN and rank -1); and a step of q35_decode_step, where targets NULL stands for the greedy ids. The state
+ * advances and sampled / out_tok come out as there; the logits stay on the device. Waits for the results. */
+int q35_prefill_logprobs(q35_engine* e, q35_state* s, int lane, const int32_t* ids, int n, int32_t* sampled,
+                         const q35_logprobs* d);
+int q35_decode_step_logprobs(q35_engine* e, q35_state* s, const int32_t* lanes, int n, const int32_t* tokens,
+                             int32_t* out_tok, const q35_logprobs* d);
 int q35_sync(q35_engine* e);
 /* Live per-kernel timing: with option "kprof" = family (1 projection/MLP GEMMs, 2 lm_head
  * GEMM, 3 GDN recurrence, 4 attention core, 0 off), each launch of that family is bracketed

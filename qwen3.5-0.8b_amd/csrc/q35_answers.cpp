@@ -26,6 +26,21 @@ static AxisHeadArgs axis_args(const HeadArgs& h, const q35_positions& at, const 
     return a;
 }
 
+LogprobArgs q35::logprob_args(const q35_logprobs& d, int rows, int vocab) {
+    REQ(rows > 0, Q35_ERR_ARG, "bad row count");
+    REQ(vocab >= 1 && vocab <= 1 << 20, Q35_ERR_ARG, "vocab is 1 .. 1048576");
+    REQ(d.temperature >= 1e-3 && d.temperature <= 1e3, Q35_ERR_ARG, "temperature is 0.001 .. 1000");
+    REQ(d.top >= 0 && d.top <= std::min(kTopMost, vocab), Q35_ERR_ARG, "top is 0 .. 32, at most vocab");
+    REQ(d.targets || (!d.logprobs && !d.ranks), Q35_ERR_ARG, "log probabilities and ranks need targets");
+    LogprobArgs a{};
+    a.rows = rows; a.vocab = vocab;
+    a.top = d.top_ids || d.top_logprobs ? d.top : 0;
+    a.c = 1.4426950408889634074 / d.temperature;
+    a.targets = d.targets; a.logprobs = d.logprobs; a.ranks = d.ranks; a.entropy = d.entropy;
+    a.top_ids = d.top_ids; a.top_logprobs = d.top_logprobs;
+    return a;
+}
+
 extern "C" {
 
 int q35_op_qk_norm_rope_axes(q35_engine* e, const q35_heads* h, int kv_heads, int head_dim, const q35_positions* at,
@@ -131,20 +146,11 @@ int q35_op_attn_kv4_shared(q35_engine* e, q35_kv4* prefix, q35_kv4* c, int layer
 int q35_op_token_logprobs(q35_engine* e, const q35_logprobs* d, int rows, int vocab) {
     return guard([&] {
         REQ(e && d && d->logits, Q35_ERR_ARG, "null argument");
-        REQ(rows > 0, Q35_ERR_ARG, "bad row count");
-        REQ(vocab >= 1 && vocab <= 1 << 20, Q35_ERR_ARG, "vocab is 1 .. 1048576");
+        LogprobArgs a = logprob_args(*d, rows, vocab);
         REQ(d->ld >= vocab, Q35_ERR_ARG, "row stride below vocab");
         REQ(d->dtype == 0 || d->dtype == 1, Q35_ERR_ARG, "dtype is 0 (float32) or 1 (bfloat16)");
         REQ((uintptr_t)d->logits % (d->dtype ? 2 : 4) == 0, Q35_ERR_ARG, "misaligned logits");
-        REQ(d->temperature >= 1e-3 && d->temperature <= 1e3, Q35_ERR_ARG, "temperature is 0.001 .. 1000");
-        REQ(d->top >= 0 && d->top <= std::min(kTopMost, vocab), Q35_ERR_ARG, "top is 0 .. 32, at most vocab");
-        REQ(d->targets || (!d->logprobs && !d->ranks), Q35_ERR_ARG, "log probabilities and ranks need targets");
-        LogprobArgs a{};
-        a.logits = d->logits; a.ld = d->ld; a.bf16 = d->dtype; a.rows = rows; a.vocab = vocab;
-        a.top = d->top_ids || d->top_logprobs ? d->top : 0;
-        a.c = 1.4426950408889634074 / d->temperature;
-        a.targets = d->targets; a.logprobs = d->logprobs; a.ranks = d->ranks; a.entropy = d->entropy;
-        a.top_ids = d->top_ids; a.top_logprobs = d->top_logprobs;
+        a.logits = d->logits; a.ld = d->ld; a.bf16 = d->dtype;
         const EngineView ev = engine_view(e);
         a.ws = ev.logprob_ws;
         OnDevice on(ev.device);

@@ -6,6 +6,8 @@
 
 #include "q35_kv4.h"
 
+struct q35_logprobs;
+
 namespace q35 {
 
 // Attention of answers that share prompts. The launch's sequences are sorted by prompt; entry j is the prompt of gcount
@@ -48,6 +50,8 @@ struct LogprobArgs {
     int parts;                       // blocks of a row (set by the launcher)
 };
 size_t logprob_ws_bytes();
+// A caller's wishes, looked over, but for logits, ld, dtype and the workspace.
+LogprobArgs logprob_args(const q35_logprobs& d, int rows, int vocab);
 hipError_t launch_logprobs(LogprobArgs a, hipStream_t st);
 
 }  // namespace q35

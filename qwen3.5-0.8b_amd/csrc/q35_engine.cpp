@@ -125,6 +125,7 @@ struct q35_engine {
     float* kv4_part = nullptr;       // the 4-bit cache's attention: partial results of split rows
     double* verify_ws = nullptr;     // draft verification: the rows' chunk statistics
     char* logprob_ws = nullptr;      // token log probabilities: the rows' parts
+    int *logprob_io = nullptr, *h_logprob_io = nullptr;   // and what a row has on the device and comes back: target, log p, entropy, rank, top ids, top log p
     int *verify_io = nullptr, *h_verify_io = nullptr;   // sampled rounds: [drafts | u | accepted | tokens], R each
     uint16_t* prod;
     int *pidx, *tok_dev, *rlane, *rpos, *rslot, *rcur, *rwcur, *rpend, *ridx_src, *ridx_dst, *din = nullptr;
@@ -406,6 +407,8 @@ void alloc_scratch(q35_engine* e) {
     e->kv4_part = dalloc<float>(kv4_part_floats());
     e->verify_ws = dalloc<double>(verify_ws_doubles((int)R));
     e->logprob_ws = dalloc<char>(logprob_ws_bytes());
+    e->logprob_io = dalloc<int>((4 + 2 * kTopMost) * R);
+    e->h_logprob_io = halloc<int>((4 + 2 * kTopMost) * R);
     e->verify_io = dalloc<int>(4 * R);
     e->h_verify_io = halloc<int>(4 * R);
     e->gchunk = dalloc<float>(gdn_chunk_ws_floats(R));
@@ -797,6 +800,42 @@ void lm_head(q35_engine* e, int row0, int M, bool want_logits, const uint16_t* n
     HCK(launch_argmax(e->pval, e->pidx, kVocab / 16, gemm_argmax_partials(a), M, e->tok_dev, top_val, e->st));
 }
 
+// A caller's wishes for rows of the model, looked over (without targets, the call gives them).
+LogprobArgs check_scores(const q35_logprobs& d, int rows) {
+    REQ(!d.logits, Q35_ERR_ARG, "logits are the model's own here");
+    q35_logprobs w = d;
+    static const int32_t some = 0;
+    w.targets = &some;
+    return logprob_args(w, rows, kVocab);
+}
+// Log probabilities of the first M rows of logits_dev, to row `at` on of d's arrays. next: host targets; null: tok_dev.
+void score_rows(q35_engine* e, const LogprobArgs& want, const q35_logprobs& d, int M, int at, const int32_t* next) {
+    LogprobArgs a = want;
+    int *io = e->logprob_io, *h = e->h_logprob_io;
+    a.logits = e->logits_dev; a.ld = kVocab; a.rows = M; a.ws = e->logprob_ws;
+    a.targets = e->tok_dev;
+    if (next) {
+        std::copy(next, next + M, h);
+        HCK(hipMemcpyAsync(io, h, M * sizeof(int), hipMemcpyHostToDevice, e->st));
+        a.targets = io;
+    }
+    const size_t tops = (size_t)M * a.top;
+    a.logprobs = d.logprobs ? (float*)(io + M) : nullptr;
+    a.entropy = d.entropy ? (float*)(io + 2 * M) : nullptr;
+    a.ranks = d.ranks ? io + 3 * M : nullptr;
+    a.top_ids = a.top && d.top_ids ? io + 4 * M : nullptr;
+    a.top_logprobs = a.top && d.top_logprobs ? (float*)(io + 4 * M + tops) : nullptr;
+    HCK(launch_logprobs(a, e->st));
+    HCK(hipMemcpyAsync(h + M, io + M, (3 * M + 2 * tops) * sizeof(int), hipMemcpyDeviceToHost, e->st));
+    HCK(hipStreamSynchronize(e->st));
+    const auto give = [&](void* to, const int* from, size_t first, size_t n) { if (to) std::memcpy((int*)to + first, from, n * sizeof(int)); };
+    give(d.logprobs, h + M, at, M);
+    give(d.entropy, h + 2 * M, at, M);
+    give(d.ranks, h + 3 * M, at, M);
+    give(d.top_ids, h + 4 * M, (size_t)at * a.top, tops);
+    give(d.top_logprobs, h + 4 * M + tops, (size_t)at * a.top, tops);
+}
+
 void save_hlast(q35_engine* e, q35_state* s, const std::vector<int>& src_rows, const std::vector<int>& lanes) {
     const int n = (int)src_rows.size();
     HCK(hipStreamSynchronize(e->st));
@@ -913,9 +952,9 @@ int q35_destroy(q35_engine* e) {
         void* ds[] = {e->blob, e->x, e->h, e->delta, e->nrm, e->proj, e->gu, e->aout, e->cat, e->o, e->q,
                       e->sc, e->stats, e->part, e->pval, e->pidx, e->prod, e->din, e->inv_freq,
                       e->logits_dev, e->kpart, e->gchunk, e->gcdec, e->topv_dev, e->kv4_part, e->verify_ws, e->logprob_ws,
-                      e->verify_io};
+                      e->verify_io, e->logprob_io};
         for (void* p : ds) if (p) hipFree(p);
-        void* hs[] = {e->hin, e->h_out, e->h_verify_io};
+        void* hs[] = {e->hin, e->h_out, e->h_verify_io, e->h_logprob_io};
         for (void* p : hs) if (p) hipHostFree(p);
         noalloc_release(e->device, e);
         hipEventDestroy(e->ev0);
@@ -1329,12 +1368,19 @@ int q35_state_write(q35_engine* e, q35_state* s, int lane, int which, int n_slot
 // kAllChunk rows; otherwise only the prompt's last row (*sampled, logits nullable).
 constexpr int kAllChunk = 256;
 void prefill_waves(q35_engine* e, q35_state* s, int lane, const int32_t* ids, int n, bool all_rows,
-                   int32_t* sampled, float* top, float* logits) {
+                   int32_t* sampled, float* top, float* logits, const q35_logprobs* scores = nullptr) {
     REQ(e && s && ids && sampled, Q35_ERR_ARG, "null argument");
     REQ(n > 0, Q35_ERR_ARG, "empty prompt");
     check_lane(s, lane);
     REQ(s->prefix[lane] + n <= s->cap, Q35_ERR_CAP, "prompt exceeds the lane's cache capacity");
     for (int i = 0; i < n; ++i) check_tok(ids[i]);
+    LogprobArgs want{};
+    std::vector<int32_t> next;               // the rows' targets
+    if (scores) {
+        want = check_scores(*scores, n);
+        if (scores->targets) next.assign(scores->targets, scores->targets + n);
+        else { next.assign(ids + 1, ids + n); next.push_back(-1); }
+    }
     int done = 0;
     while (done < n) {
         const int T = std::min(e->R, n - done);
@@ -1353,12 +1399,13 @@ void prefill_waves(q35_engine* e, q35_state* s, int lane, const int32_t* ids, in
             // the body's tokens are consumed: lm_head leaves row r0 + i's id in tok_dev[i]
             for (int r0 = 0; r0 < T; r0 += kAllChunk) {
                 const int M = std::min(kAllChunk, T - r0);
-                lm_head(e, r0, M, logits != nullptr, normw, e->topv_dev);
+                lm_head(e, r0, M, logits || scores, normw, e->topv_dev);
                 HCK(hipMemcpyAsync(sampled + done + r0, e->tok_dev, M * sizeof(int), hipMemcpyDeviceToHost, e->st));
                 if (top) HCK(hipMemcpyAsync(top + done + r0, e->topv_dev, M * sizeof(float), hipMemcpyDeviceToHost, e->st));
                 if (logits)
                     HCK(hipMemcpyAsync(logits + (size_t)(done + r0) * kVocab, e->logits_dev, (size_t)M * kVocab * 4,
                                        hipMemcpyDeviceToHost, e->st));
+                if (scores) score_rows(e, want, *scores, M, done + r0, next.data() + done + r0);
                 HCK(hipStreamSynchronize(e->st));
             }
         }
@@ -1469,11 +1516,22 @@ int q35_prefill_all(q35_engine* e, q35_state* s, int lane, const int32_t* ids, i
     return guard([&] { prefill_waves(e, s, lane, ids, n, true, sampled, top_logit, logits); });
 }
 
-int q35_decode_step(q35_engine* e, q35_state* s, const int32_t* lanes, int n, const int32_t* tokens,
-                    int32_t* out_tok, float* out_logits) {
+int q35_prefill_logprobs(q35_engine* e, q35_state* s, int lane, const int32_t* ids, int n, int32_t* sampled,
+                         const q35_logprobs* d) {
     return guard([&] {
+        REQ(d, Q35_ERR_ARG, "null argument");
+        prefill_waves(e, s, lane, ids, n, true, sampled, nullptr, nullptr, d);
+    });
+}
+
+static int decode_step(q35_engine* e, q35_state* s, const int32_t* lanes, int n, const int32_t* tokens, int32_t* out_tok,
+                       float* out_logits, bool scored, const q35_logprobs* scores) {
+    return guard([&] {
+        REQ(!scored || scores, Q35_ERR_ARG, "null argument");
         REQ(e && s && tokens && out_tok, Q35_ERR_ARG, "null argument");
         REQ(n > 0 && n <= e->R, Q35_ERR_CAP, "lane count exceeds max_rows");
+        const LogprobArgs want = scores ? check_scores(*scores, n) : LogprobArgs{};
+        const bool logits = out_logits || scores;
         HCK(hipStreamSynchronize(e->st));
         std::vector<int> ls(n);
         for (int i = 0; i < n; ++i) {
@@ -1500,14 +1558,14 @@ int q35_decode_step(q35_engine* e, q35_state* s, const int32_t* lanes, int n, co
         const int defer = step_defer(e);
         auto step = [&] {
             body_kernels(e, s, n, 1, false, defer);
-            lm_head(e, 0, n, out_logits != nullptr, !body_final_normed(e, n, 1, false) ? e->final_norm : nullptr);
+            lm_head(e, 0, n, logits, !body_final_normed(e, n, 1, false) ? e->final_norm : nullptr);
             HCK(launch_copy_rows_advance(e->nrm, e->ridx_src, s->hlast, e->ridx_dst, n, kHidden, e->rpos, e->rslot,
                                          e->rcur, e->rwcur, e->rpend, s->nslots, defer, e->st));
         };
         if (e->use_graph && e->kprof == 0) {
-            if (out_logits) ensure_logits(e, n);
+            if (logits) ensure_logits(e, n);
             char key[128];
-            std::snprintf(key, sizeof key, "dec:%p:%d:%d:%d:%d", (void*)s, n, out_logits ? 1 : 0, e->n_layers, defer);
+            std::snprintf(key, sizeof key, "dec:%p:%d:%d:%d:%d", (void*)s, n, logits ? 1 : 0, e->n_layers, defer);
             auto it = e->graphs.find(key);
             if (it == e->graphs.end()) {
                 hipGraph_t g;
@@ -1534,6 +1592,7 @@ int q35_decode_step(q35_engine* e, q35_state* s, const int32_t* lanes, int n, co
         }
         HCK(hipMemcpyAsync(e->h_out, e->tok_dev, n * sizeof(int), hipMemcpyDeviceToHost, e->st));
         if (out_logits) HCK(hipMemcpyAsync(out_logits, e->logits_dev, (size_t)n * kVocab * 4, hipMemcpyDeviceToHost, e->st));
+        if (scores) score_rows(e, want, *scores, n, 0, scores->targets);
         HCK(hipStreamSynchronize(e->st));
         for (int i = 0; i < n; ++i) out_tok[i] = e->h_out[i];
         e->fast_lanes.assign(ls.begin(), ls.begin() + n);
@@ -1549,6 +1608,16 @@ int q35_decode_step(q35_engine* e, q35_state* s, const int32_t* lanes, int n, co
         e->fast_epoch = e->meta_epoch;
         e->fast_s = s;
     });
+}
+
+int q35_decode_step(q35_engine* e, q35_state* s, const int32_t* lanes, int n, const int32_t* tokens,
+                    int32_t* out_tok, float* out_logits) {
+    return decode_step(e, s, lanes, n, tokens, out_tok, out_logits, false, nullptr);
+}
+
+int q35_decode_step_logprobs(q35_engine* e, q35_state* s, const int32_t* lanes, int n, const int32_t* tokens,
+                             int32_t* out_tok, const q35_logprobs* d) {
+    return decode_step(e, s, lanes, n, tokens, out_tok, nullptr, true, d);
 }
 
 int q35_mtp_draft(q35_engine* e, q35_state* s, const int32_t* lanes, int n, const int32_t* y,

@@ -4,6 +4,7 @@ from __future__ import annotations
 import ctypes as C
 import struct
 from pathlib import Path
+from typing import NamedTuple
 
 import numpy as np
 
@@ -110,6 +111,8 @@ _SIGS = {
     "q35_op_attn_kv4_shared": ([C.c_void_p] * 3 + [C.c_int] + [C.c_void_p] * 4 + [C.c_int] * 3
                                + [C.c_void_p, C.c_void_p, C.c_float, C.c_void_p], C.c_int),
     "q35_op_token_logprobs": ([C.c_void_p, C.c_void_p, C.c_int, C.c_int], C.c_int),
+    "q35_prefill_logprobs": ([C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p], C.c_int),
+    "q35_decode_step_logprobs": ([C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p], C.c_int),
     "q35_sync": ([C.c_void_p], C.c_int),
     "q35_kprof_read": ([C.c_void_p, C.POINTER(C.c_float), C.POINTER(C.c_int)], C.c_int),
     "q35_set_option": ([C.c_void_p, C.c_char_p, C.c_int], C.c_int),
@@ -437,6 +440,27 @@ class MtpPolicy:
             pass
 
 
+class TokenLogprobs(NamedTuple):
+    """Of rows' next tokens: their log probabilities, ranks (0: the argmax), the rows' entropy, and the first ids by falling
+    logit with their log probabilities [rows][top]."""
+    logprobs: np.ndarray
+    ranks: np.ndarray
+    entropy: np.ndarray
+    top_ids: np.ndarray
+    top_logprobs: np.ndarray
+
+
+def _scores(rows: int, targets, top: int, temperature: float):
+    out = TokenLogprobs(np.empty(rows, np.float32), np.empty(rows, np.int32), np.empty(rows, np.float32),
+                        np.empty((rows, max(top, 0)), np.int32), np.empty((rows, max(top, 0)), np.float32))
+    t = _i32(targets) if targets is not None else None
+    if t is not None and t.shape != (rows,):
+        raise ValueError(f"{rows} targets wanted")
+    d = _LOGPROBS.pack(0, 0, 0, t.ctypes.data if t is not None else 0, temperature, top,
+                       *(x.ctypes.data for x in (out.logprobs, out.ranks, out.entropy, out.top_ids, out.top_logprobs)))
+    return out, d, t
+
+
 class State:
     """`lanes` independent requests (RequestState, engine/state.h:83-116)."""
 
@@ -549,6 +573,25 @@ class State:
         _ck(load_library().q35_decode_step(self.eng.h, self.h, _p(ln) if ln is not None else None, n,
                                            _p(t), _p(out), _p(lg) if logits else None))
         return (out, lg) if logits else out
+
+    def prefill_logprobs(self, lane: int, ids, targets=None, top: int = 0, temperature: float = 1.0):
+        """The prompt with each row's greedy id and the log probabilities of the token after it (q35_prefill_logprobs): the
+        prompt's own next ones unless targets gives others, NaN in the last row then. Returns the ids and a TokenLogprobs."""
+        ids = _i32(ids)
+        samp = np.empty(ids.size, np.int32)
+        out, d, _targets = _scores(ids.size, targets, top, temperature)
+        _ck(load_library().q35_prefill_logprobs(self.eng.h, self.h, lane, _p(ids), ids.size, _p(samp), d))
+        return samp, out
+
+    def decode_step_logprobs(self, tokens, lanes=None, targets=None, top: int = 0, temperature: float = 1.0):
+        """decode_step, and the log probabilities of the greedy ids or of given targets (q35_decode_step_logprobs)."""
+        t = _i32(tokens)
+        ln = _i32(lanes) if lanes is not None else None
+        ids = np.empty(t.size, np.int32)
+        out, d, _targets = _scores(t.size, targets, top, temperature)
+        _ck(load_library().q35_decode_step_logprobs(self.eng.h, self.h, _p(ln) if ln is not None else None, t.size, _p(t),
+                                                    _p(ids), d))
+        return ids, out
 
     def mtp_draft(self, y, pos, step: int, lanes=None, logits: bool = False):
         y, pos = _i32(y), _i32(pos)
