@@ -274,9 +274,17 @@ static hipError_t launch(Kv4Shared& a, hipStream_t st) {
     for (int i = 0; i < a.n; ++i) own += own_tiles(i) * own_items;
     // One block a CU, or two where each has 128 tiles or more: a second wave on a SIMD fills the waits of the first (512
     // tiles of 256 dims: 97.8 -> 83.3 us; about 160 of 128: 51.1 -> 45.4), but twice the partial results take their time to write
-    // and to join (64 tiles of 256 dims: 23.8 + 5.7 -> 29.7 + 7.8).
-    long long tiles = std::max<long long>(8, (work + 255) / 256);
-    if (tiles >= 128) tiles = (tiles + 1) / 2;
+    // and to join (64 tiles of 256 dims: 23.8 + 5.7 -> 29.7 + 7.8). No block more than that, which would run behind them,
+    // and 16 tiles at least (64 answers x 3 rows x 2000 slots, 48 items of 63 tiles: 12 tiles in 288 blocks 19.6 + 5.8, 16
+    // in 192 16.2 + 5.1).
+    const auto prompt_blocks = [&](long long tiles) {
+        long long s = 0;
+        for (int j = 0; j < a.entries; ++j) s += (prompt_tiles(j) + tiles - 1) / tiles * items(j);
+        return s;
+    };
+    const long long most_blocks = (work + 255) / 256 < 128 ? 256 : 512;
+    long long tiles = std::max<long long>(16, (work + most_blocks - 1) / most_blocks), least_blocks = prompt_blocks(INT_MAX);
+    while (prompt_blocks(tiles) > std::max(most_blocks, least_blocks)) tiles += (tiles + 7) / 8;
     long long own_per = std::max<long long>(8, (own + 2047) / 2048);
     for (;; tiles *= 2, own_per *= 2) {
         part = blocks = joins = 0;
