@@ -1,4 +1,4 @@
-// What the entry points over the 4-bit cache share (q35_kv4.cpp, q35_kv4_shared.cpp): the cache's handle and the
+// What the entry points over the 4-bit cache share (q35_kv4.cpp, q35_answers.cpp): the cache's handle and the
 // checks of arguments.
 #pragma once
 #include <algorithm>

@@ -259,7 +259,7 @@ constexpr int kPromptSplits = 64, kOwnSplits = 64;
 template <int D>
 static hipError_t launch(Kv4Shared& a, hipStream_t st) {
     const int group = a.q_heads / a.kv_heads, per = a.T * group, nqo = per > 16 ? 2 : 1;
-    int most = 0;
+    int most = per;
     for (int j = 0; j < a.entries; ++j) {
         a.gcount[j] = (uint16_t)((j + 1 < a.entries ? a.gstart[j + 1] : a.n) - a.gstart[j]);
         if (a.glen[j]) most = std::max(most, a.gcount[j] * per);

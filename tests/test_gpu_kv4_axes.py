@@ -145,3 +145,29 @@ def test_append_axes(eng, hq, kv, d, rot, axes, dealt, n, T, slot0):
         assert np.array_equal(a, b)
     assert not any(z.any() for z in read_cache(eng, c, 0, 0, n + 1, 0, cap))
     c.close()
+
+
+def test_positions_far_apart(eng):
+    """Rows' and axes' positions more than 2^32 bytes apart."""
+    import torch
+    rng, D = np.random.default_rng(8), Dev()
+    h = Heads(rng, 3, 4, 2, 128)
+    axis, step = a_map(64, 2, True), 2 ** 30 + 3
+    at = rng.integers(-1000, 100000, (3, 2)).astype(np.int32)
+    x, qn, kn = D.up(h.x), D.up(h.qn), D.up(h.kn)
+    for rows, axes in ((step, 1), (1, step)):
+        t = torch.zeros(2 * step + 8, dtype=torch.int32, device="cuda")
+        for r in range(3):
+            for a in range(2):
+                t[r * rows + a * axes] = int(at[r, a])
+        qo, ko = (torch.zeros(3, m, 128, dtype=torch.int16, device="cuda") for m in (4, 2))
+        torch.cuda.synchronize()
+        v, _ = h.views(x.data_ptr())
+        eng.op_qk_norm_rope_axes((t.data_ptr(), rows, axes), axis, 3, 4, 2, 128, rot_dim=64, theta=1e6, eps=1e-6, q_norm=qn.data_ptr(),
+                                 k_norm=kn.data_ptr(), q_out=(qo.data_ptr(), 512, 128), k_out=(ko.data_ptr(), 256, 128), **v)
+        eng.sync()
+        q, k, _ = h.parts()
+        close(D.bits(qo), *turned(q, h.qn, at, axis, 64, 1e6, 1e-6))
+        close(D.bits(ko), *turned(k, h.kn, at, axis, 64, 1e6, 1e-6))
+        del t
+    torch.cuda.empty_cache()

@@ -113,6 +113,19 @@ def test_no_prompt_is_the_attention(eng):
     own.c.close()
 
 
+@pytest.mark.parametrize("hq,kv,d", [(8, 2, 256), (4, 1, 128), (6, 6, 64)])
+@pytest.mark.parametrize("T", [4, 5, 17, 40])
+def test_no_prompt_many_rows(eng, hq, kv, d, T):
+    """Launches without any prompt, of fewer and more rows a kv head than one tile has."""
+    rng = np.random.default_rng(T + d)
+    own = Filled(eng, rng, 3, 300, kv, d)
+    lanes, pos = np.array([2, 0, 1], np.int32), np.array([300 - T, 0, 100], np.int32)
+    none = np.full(3, -1, np.int32)
+    got, q, g = run(eng, own, own, none, none + 1, lanes, pos, T, hq, rng, True)
+    check(own, own, none, none + 1, lanes, pos, T, got, q, g)
+    own.c.close()
+
+
 def test_many(eng):
     """More sequences and prompts than a launch takes, and more rows than the partial results have room for."""
     rng = np.random.default_rng(5)

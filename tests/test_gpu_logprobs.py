@@ -224,3 +224,30 @@ def test_row_is_its_own(eng):
     one = call(eng, x[32:], t[32:], 20, True)
     assert all(np.array_equal(a[k], b[k]) for k in a)
     assert np.array_equal(a["top_ids"][32:], one["top_ids"]) and a["ranks"][32] == one["ranks"][0]
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_many_rows_and_far_ones(eng, bf16):
+    """More rows than a launch takes, and rows more than 2^32 bytes apart."""
+    import torch
+    rng = np.random.default_rng(6)
+    x = values(rng, 20000, 33, bf16)
+    t = rng.integers(-1, 34, 20000)
+    pick = np.r_[0, 8191, 8192, 16383, 16384, 19999, rng.integers(0, 20000, 30)]
+    got = call(eng, x, t, 4, bf16)
+    check({k: v[pick] for k, v in got.items()}, x[pick], t[pick], 4)
+    v, ld = 70001, 2 ** 31 + 5
+    far = torch.zeros(2 * ld + v, dtype=torch.bfloat16 if bf16 else torch.float32, device="cuda")
+    x, t = values(rng, 3, v, bf16), rng.integers(0, v, 3)
+    for i in range(3):
+        far[i * ld:i * ld + v] = torch.from_numpy(x[i]).cuda().to(far.dtype)
+    tg = torch.from_numpy(t.astype(np.int32)).cuda()
+    out = {k: torch.zeros(3, *s, dtype=d, device="cuda") for k, s, d in
+           [("logprobs", (), torch.float32), ("ranks", (), torch.int32), ("entropy", (), torch.float32), ("top_ids", (9,), torch.int32),
+            ("top_logprobs", (9,), torch.float32)]}
+    torch.cuda.synchronize()
+    eng.op_token_logprobs(3, v, far.data_ptr(), targets=tg.data_ptr(), top=9, bf16=bf16, ld=ld, **{k: o.data_ptr() for k, o in out.items()})
+    eng.sync()
+    check({k: o.cpu().numpy() for k, o in out.items()}, x, t, 9)
+    del far
+    torch.cuda.empty_cache()
