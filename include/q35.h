@@ -332,7 +332,8 @@ int q35_op_attn_kv4(q35_engine* e, q35_kv4* c, int layer, const int32_t* lanes, 
  * `prefix` and slots [0, pos[i] + t] of lane lanes[i] of c, in one softmax. Both caches have the same heads, and each its
  * own lanes and capacity; they may be the same one (a lane is not its own prefix). Sequences that name the same lane and length share
  * the reading of it, in any order; prefix_lanes[i] < 0 or prefix_lens[i] 0: no prefix. Positions count c's slots: the keys'
- * rotation is whatever they were appended with (q35_op_kv4_append_axes). Rounding, NaN and repetition as above. */
+ * rotation is whatever they were appended with (q35_op_kv4_append_axes). Rounding and NaN as above; the same call gives the
+ * same bits, and other sequences beside a row may change its last ones at any length. */
 int q35_op_attn_kv4_shared(q35_engine* e, q35_kv4* prefix, q35_kv4* c, int layer, const int32_t* prefix_lanes,
                            const int32_t* prefix_lens, const int32_t* lanes, const int32_t* pos, int n, int T, int q_heads,
                            const q35_view* q, const q35_view* gate, float scale, const q35_view* out);
