@@ -171,23 +171,25 @@ __device__ __forceinline__ void push(Best& b, float x, int id, bool on) {
 // maxima (floor), so the row's best do, and only the pieces of the lanes and runs that reach it are read
 // again: some 25 of them for 20 tokens, of any number of elements. If ties or infinities bring more candidates than there is
 // room for, the part is gone over in order with a list a wave (Best).
-// float32: bound by memory, 256 rows of 248,320 with 5 tokens each (254 MB) 45.8 us, 5.6 TB/s (without tokens 42.2, with 32
-// 50.2). bfloat16: by memory and the 8 instructions an element takes, 1999 rows of 32,003 with 20 tokens (128 MB) 37.7 us,
-// 3.4 TB/s (without 31.8). One row of 248,320: a chain of loads and barriers, 8.8 us and the join's 3.8.
-constexpr int kRuns = 16;            // of a part's tiles a wave
-constexpr int kRoom = 256;           // candidates, and lanes' runs that may hold some
+// float32: bound by memory, 256 rows of 248,320 with 5 tokens each (254 MB) 45.0 us, 5.6 TB/s. bfloat16: by memory and the 8
+// instructions an element takes, 1999 rows of 32,003 with 20 tokens (128 MB) 37.4 us, 3.4 TB/s (without 31.8). One row of
+// 248,320: a chain of loads and barriers, 8.8 us and the join's 3.8.
+template <int W>
+constexpr int kRuns = W > 4 ? 64 / W : 16;       // of a part's tiles a wave
+template <int W>
+constexpr int kRoom = W > 4 ? 64 * W : 256;      // candidates, and lanes' runs that may hold some; a list of kTight a wave
 template <bool BF16, bool TOP, int W>
-__global__ void __launch_bounds__(64 * W, 5) logprobs_kernel(LogprobArgs a, int row0) {
+__global__ void __launch_bounds__(64 * W, W > 4 ? 4 : 5) logprobs_kernel(LogprobArgs a, int row0) {
     constexpr int V = BF16 ? 8 : 4, L = kEach / V;
     struct Lists { float2 list[W][kList + kPad], sorted[W][kTopMost]; };
     union Store {
-        float runs[kRuns][64 * W];
+        float runs[kRuns<W>][64 * W];
         Lists lists;
     };
     __shared__ __align__(16) char store[TOP ? sizeof(Store) : 16];
     Store* st = (Store*)store;
-    __shared__ float2 flat[TOP ? kRoom + kPad : 1];
-    __shared__ uint16_t held[TOP ? kRoom : 1];
+    __shared__ float2 flat[TOP ? kRoom<W> + kPad : 1];
+    __shared__ uint16_t held[TOP ? kRoom<W> : 1];
     __shared__ LpPart waves[W];
     __shared__ int counts[W], n_held, n_flat;
     __shared__ double row_lse;
@@ -246,7 +248,7 @@ __global__ void __launch_bounds__(64 * W, 5) logprobs_kernel(LogprobArgs a, int 
             above += __popcll(__ballot(id < target && at(min(id, target)) == xt));
         }
     }
-    const int each = (t1 - t0 + W * kRuns - 1) / (W * kRuns);       // tiles of a run
+    const int each = (t1 - t0 + W * kRuns<W> - 1) / (W * kRuns<W>);       // tiles of a run
     float run = -INFINITY;
     int n_run = 0, i_run = 0, t_max = -1;
     for (int t = t0 + wv; t < t1; t += W) {
@@ -320,7 +322,7 @@ __global__ void __launch_bounds__(64 * W, 5) logprobs_kernel(LogprobArgs a, int 
     u.a = wave_sum_d(u.a);
     if (lane == 0) waves[wv] = {u.s, u.a, u.m, above};
     if (TOP) {
-        for (; i_run < kRuns; ++i_run, run = -INFINITY) st[0].runs[i_run][tid] = run;
+        for (; i_run < kRuns<W>; ++i_run, run = -INFINITY) st[0].runs[i_run][tid] = run;
         if (tid == 0) n_held = n_flat = 0;
     }
     __syncthreads();
@@ -347,7 +349,7 @@ __global__ void __launch_bounds__(64 * W, 5) logprobs_kernel(LogprobArgs a, int 
     if (wv == 0) {
         float most = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < kRuns; ++r)
+        for (int r = 0; r < kRuns<W>; ++r)
 #pragma unroll
             for (int w = 0; w < W; ++w) most = fmaxf(most, st[0].runs[r][w * 64 + lane]);
         const float f = floor_of(most, a.top);
@@ -355,20 +357,20 @@ __global__ void __launch_bounds__(64 * W, 5) logprobs_kernel(LogprobArgs a, int 
     }
     __syncthreads();
     const float floor = row_floor;
-    for (int r = 0; r < kRuns; ++r) {
+    for (int r = 0; r < kRuns<W>; ++r) {
         const int t = t0 + wv + W * r * each;        // the run's first tile
         if (t < t1 && t * L * 64 + lane < pieces && st[0].runs[r][tid] >= floor) {
             const int k = atomicAdd(&n_held, 1);
-            if (k < kRoom) held[k] = (uint16_t)(r * 64 * W + tid);
+            if (k < kRoom<W>) held[k] = (uint16_t)(r * 64 * W + tid);
         }
     }
     __syncthreads();
     const int runs = n_held;
-    if (runs <= kRoom) {
+    if (runs <= kRoom<W>) {
         const auto keep = [&](float x, int id) {
             if (!(x >= floor)) return;
             const int k = atomicAdd(&n_flat, 1);
-            if (k < kRoom) flat[k] = make_float2(x, __int_as_float(id));
+            if (k < kRoom<W>) flat[k] = make_float2(x, __int_as_float(id));
         };
         if (on_edge) keep(x_edge, edge);
         for (int i = tid; i < runs * each * L; i += 64 * W) {
@@ -382,7 +384,7 @@ __global__ void __launch_bounds__(64 * W, 5) logprobs_kernel(LogprobArgs a, int 
     }
     __syncthreads();
     int all = n_flat;
-    if (runs > kRoom || all > kRoom) {       // in order, a list a wave
+    if (runs > kRoom<W> || all > kRoom<W>) {       // in order, a list a wave
         __syncthreads();                     // (st was read as runs, n_flat by all)
         Best best = {st[0].lists.list[wv], st[0].lists.sorted[wv], floor, false, 0, a.top};
         if (edges) push(best, x_edge, edge, on_edge && lane < head);
@@ -485,23 +487,27 @@ __global__ void __launch_bounds__(256) logprobs_join(LogprobArgs a, int row0) {
 
 hipError_t launch_logprobs(LogprobArgs a, hipStream_t st) {
     const int el = a.bf16 ? 8 : 4, tiles = (a.vocab / el + 64 * kEach / el - 1) / (64 * kEach / el);
-    // Blocks of four waves, as many of a row as give every CU four, each wave with a tile at least. The card holds about
-    // 1280 of them: of more rows a block has two waves, whose ends fill the CUs better (1999 rows of 32,003 bf16 42.3 ->
-    // 37.6 us; with fewer rows the candidates' steps of twice the blocks cost more: 256 rows of 248,320 float32 and 32
-    // tokens 50.1 -> 55.2).
-    const bool pairs = a.rows > 1280;
-    a.parts = std::max(1, std::min({kParts, (tiles + 3) / 4, 1024 / a.rows}));
+    // A row is one block's where 512 rows or fewer have as many as tiles (of 2048 elements) at least: 16 waves up to 256
+    // rows, a block a CU, and 8 above, two. Without a second launch and its join 256 rows of 248,320 float32 and 5 tokens take
+    // 45.0 instead of 47.3 + 4.7 us, 16 of 32,003 bfloat16 and 20 tokens 11.6 for 9.5 + 4.5, 448 17 for 18 + 5; where rows
+    // are fewer than tiles a CU takes too long for one (64 of 248,320 26.1 for 18.2 + 4.0; 75 of 151,936 even).
+    // Otherwise blocks of four waves, as many of a row as give every CU four, each wave with a tile at least. The card holds
+    // about 1280 of them: of more rows a block has two waves, whose ends fill the CUs better (1999 rows of 32,003 bf16 42.3 ->
+    // 37.6 us).
+    const bool whole = tiles > 4 && a.rows >= tiles && a.rows <= 512;
+    const int waves = whole ? a.rows > 256 ? 8 : 16 : a.rows > 1280 ? 2 : 4;
+    a.parts = whole ? 1 : std::max(1, std::min({kParts, (tiles + 3) / 4, 1024 / a.rows}));
     const int most = kPartRooms / a.parts;
     const auto pick = [&](auto bf16, auto top) {
         constexpr bool b = decltype(bf16)::value, t = decltype(top)::value;
-        return pairs ? logprobs_kernel<b, t, 2> : logprobs_kernel<b, t, 4>;
+        return waves == 16 ? logprobs_kernel<b, t, 16> : waves == 8 ? logprobs_kernel<b, t, 8> : waves == 4 ? logprobs_kernel<b, t, 4> : logprobs_kernel<b, t, 2>;
     };
     using Yes = std::true_type;
     using No = std::false_type;
     const auto k = a.bf16 ? (a.top ? pick(Yes{}, Yes{}) : pick(Yes{}, No{})) : (a.top ? pick(No{}, Yes{}) : pick(No{}, No{}));
     for (int r = 0, m; r < a.rows; r += m) {
         m = std::min(most, a.rows - r);
-        hipLaunchKernelGGL(k, dim3((unsigned)(m * a.parts)), dim3(pairs ? 128 : 256), 0, st, a, r);
+        hipLaunchKernelGGL(k, dim3((unsigned)(m * a.parts)), dim3(64 * waves), 0, st, a, r);
         hipError_t rc = hipGetLastError();
         if (rc != hipSuccess) return rc;
         if (a.parts == 1) continue;

@@ -178,6 +178,25 @@ def test_orders_and_masks(eng, order, bf16):
 
 
 @pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("order", list(ORDERS))
+def test_orders_in_a_wide_block(eng, order, bf16):
+    """The same in rows that a block of 16 or 8 waves has to itself, and of lengths that leave some of its waves without a tile."""
+    rng = np.random.default_rng(8)
+    for v, n, shift in [(40001, 30, 3), (10300, 6, 1), (40001, 300, 0), (70003, 257, 5)]:
+        x = np.stack([ORDERS[order](rng, v) for _ in range(3)]).astype(np.float32)
+        x = ref.val(ref.bf16_bits(x)).astype(np.float32) if bf16 else x
+        x = np.ascontiguousarray(np.resize(x, (n, v)))
+        t = rng.integers(0, v, n)
+        t[0] = np.flatnonzero(x[0] == x[0].max())[-1]
+        t[1] = x[1].argmin()
+        for top, temp in [(20, 1.0), (32, 0.01), (0, 3.0)]:
+            print(f"logprobs {order} bf16={bf16} v={v} n={n} top={top}", flush=True)
+            got = call(eng, x, t, top, bf16, temp, shift=shift)
+            pick = np.array([0, 1, 2, n - 1])
+            check({k: a[pick] for k, a in got.items()}, x[pick], t[pick], top, temp)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
 def test_rows_without_a_distribution(eng, bf16):
     """A NaN, a +inf or nothing but -inf anywhere in a row: NaN and -1 there, the rows beside it untouched."""
     rng = np.random.default_rng(3)
