@@ -141,8 +141,10 @@ __device__ __forceinline__ int low16(uint2 v, int i) { return entry(v.x & 0xffff
 // of the busy cycles and the MFMA pipes work in 43 %. Without turning codes into bf16 it takes 8 us less; from which
 // level of the memory the tiles come makes no difference, nor do loads further ahead. Shorter ones are bound by what surrounds the
 // walk: over 4,096 slots 23.5 us, of which 11 are launch, Q, a first tile and the waves' join, 3.5 the partial results' stores.
+// 128 dims: in the registers of three waves a SIMD, so that answers' blocks run beside two prompts' of a CU (8 x 32 answers over 8192
+// slots 45.4 -> 42.5 us, a few registers spilled).
 template <int D, int NQP, int NQO>
-__global__ void __launch_bounds__(256, D == 256 ? 2 : 1) shared_kernel(Kv4Shared a) {
+__global__ void __launch_bounds__(256, D == 256 ? 2 : 3) shared_kernel(Kv4Shared a) {
     __shared__ Exchange<D> ex;
     static_assert(NQO == 1 || sizeof(ex.os) >= 4 * NQO * (D / 32) * 1024, "the waves' Q operands lie where their sums go at the end");
     const int per = a.T * (a.q_heads / a.kv_heads), lane = threadIdx.x & 63;
