@@ -280,7 +280,7 @@ static hipError_t launch(Kv4Shared& a, hipStream_t st) {
     for (int j = 0; j < a.entries; ++j) work += prompt_tiles(j) * items(j);
     for (int i = 0; i < a.n; ++i) own += own_tiles(i) * own_items;
     // One block a CU, or two where each has 128 tiles or more: a second wave on a SIMD fills the waits of the first (512
-    // tiles of 256 dims: 97.8 -> 83.3 us; about 160 of 128: 51.1 -> 45.4), but twice the partial results take their time to write
+    // tiles of 256 dims: 97.8 -> 83.3 us; about 160 of 128: 56.6 -> 42.5), but twice the partial results take their time to write
     // and to join (64 tiles of 256 dims: 23.8 + 5.7 -> 29.7 + 7.8). No block more than that, which would run behind them,
     // and 16 tiles at least (64 answers x 3 rows x 2000 slots, 48 items of 63 tiles: 12 tiles in 288 blocks 19.6 + 5.8, 16
     // in 192 16.2 + 5.1).
