@@ -5,7 +5,8 @@
 // l_p and sums o_p, out = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p. A prompt's part has the rows of all its answers
 // (answers x T x query heads of a kv head) in the MFMAs' N dimension, so a tile of slots is fetched and turned
 // into bf16 once for 32 rows instead of once for each answer's 4 or 16; the answers' own slots are short lists, as in
-// the attention of single lanes. Both kinds are blocks of one launch, and a second launch joins the parts.
+// the attention of single lanes. Both kinds are blocks of one launch, and a second launch joins the parts. Where the lists are
+// short, that costs more than it saves, and each answer's rows walk their prompt's tiles and their own in one launch.
 #include <algorithm>
 #include <climits>
 
@@ -35,6 +36,8 @@ struct Part {
     int last;                        // the last slot of all rows, or -1: a row's own position, from pos on
     int pos;
     int tile;                        // where its rows go: tiles of partial results from here on
+    const uint8_t* prefix;           // (both lists at once) the prompt's region, its slots and tiles: the list's first
+    int len, ahead;
 };
 
 // A part: by a block's four waves, each every fourth tile, their states joined through LDS (W 4), or by a wave (1).
@@ -44,13 +47,19 @@ struct Exchange {                    // between a block's waves
     float ms[4][16], ls[4][16];
     uint32_t bs[4][16];
 };
-template <int D, int NQ, int W>
+// BOTH: not a part, but all that the rows see, the prompt's tiles and then their own, and the end of it. The prompt's last
+// tile comes first, as a few sinks before a window: the only one of the prompt's that may hold more than they see.
+template <int D, int NQ, int W, bool BOTH = false>
 __device__ __forceinline__ void part_rows(const Kv4Shared& a, const Part& p, uint32_t seqs, Exchange<D>& ex) {
     const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63, nn = lane & 15, g = lane >> 4, group = a.q_heads / a.kv_heads;
     const float scale2 = fmaxf(fabsf(a.scale) * 1.44269504088896f, 0x1p-149f);      // (as in the attention of single lanes)
     const Lanes lo = lane_offsets<D>();
     const auto at = [&](int i) { return i; };
-    const auto tile_at = [&](int i) { return p.region + (size_t)i * kv4_tile_bytes(D); };
+    const auto tile_at = [&](int i) {
+        if (!BOTH) return p.region + (size_t)i * kv4_tile_bytes(D);
+        return i < p.ahead ? p.prefix + (size_t)(i ? i - 1 : p.ahead - 1) * kv4_tile_bytes(D)
+                           : p.region + (size_t)(i - p.ahead) * kv4_tile_bytes(D);
+    };
     Tile<D> buf[kAhead<D>];
     first_tiles<D, NQ, W>(buf, p.t0, p.t1, tile_at, lo);
     const uint16_t* qrow[NQ];
@@ -60,7 +69,8 @@ __device__ __forceinline__ void part_rows(const Kv4Shared& a, const Part& p, uin
         const int rho = min(p.rho0 + c * 16 + nn, p.rows - 1), i = over(rho, a.per_inv), r = rho - i * a.T * group;
         const int t = over(r, a.group_inv), s = p.start + i, seq = __shfl((int)seqs, s >> 2) >> 8 * (s & 3) & 255;
         qrow[c] = a.q.p + ((long long)seq * a.TT + t) * a.q.row + (p.h * group + r - t * group) * a.q.head;
-        sight[c] = {p.last >= 0 ? p.last : p.pos + t, 0, 0};
+        if (BOTH) sight[c] = {32 * p.ahead + p.pos + t, p.len & 31 ? 32 : 0, p.len & 31};
+        else sight[c] = {p.last >= 0 ? p.last : p.pos + t, 0, 0};
     }
     const auto q_at = [&](int c, int gg, int k) {
         u32x4 w = *(const u32x4*)(qrow[c] + gg * (D / 4) + 8 * k);
@@ -85,10 +95,21 @@ __device__ __forceinline__ void part_rows(const Kv4Shared& a, const Part& p, uin
     }
     int qlane = lane;
     const auto q = [&](int c, int k) { return NQ == 1 ? qf[k] : ql[(c * (D / 32) + k) * 64 + qlane]; };
-    const int full1 = p.last >= 0 ? p.last : p.pos + over(p.rho0, a.group_inv);
+    const int full0 = BOTH && p.len & 31 ? 32 : 0;
+    const int full1 = BOTH ? 32 * p.ahead + p.pos + over(p.rho0, a.group_inv) : p.last >= 0 ? p.last : p.pos + over(p.rho0, a.group_inv);
     Rows<D, NQ> st;
-    walk_tiles<D, NQ, W>(st, buf, p.t0, p.t1, at, tile_at, lo, q, qlane, sight, 0, full1, scale2);
-    if constexpr (W > 1) {
+    walk_tiles<D, NQ, W>(st, buf, p.t0, p.t1, at, tile_at, lo, q, qlane, sight, full0, full1, scale2);
+    if constexpr (BOTH) {
+        join_waves<D, NQ, W>(st, p.rows - p.rho0, ex.os, ex.ms, ex.ls, ex.bs, [&](int c) {
+            const int rho = min(p.rho0 + c * 16 + nn, p.rows - 1), t = over(rho, a.group_inv);
+            const int seq = __builtin_amdgcn_readlane((int)seqs, p.start >> 2) >> 8 * (p.start & 3) & 255;
+            const Out to(a, (long long)seq * a.TT + t, p.h * group + rho - t * group);
+            return [=, &a](float (*x)[kRun<D>], float m, float sum) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) to.store<kRun<D>>(a, x[r], sum, first_dim<D, W>(r));
+            };
+        });
+    } else if constexpr (W > 1) {
         join_waves<D, NQ, W>(st, p.rows - p.rho0, ex.os, ex.ms, ex.ls, ex.bs, [&](int c) {
             float* to = a.part + (size_t)(p.tile + c) * tile_floats(D);
             return [=](float (*x)[kRun<D>], float m, float sum) {
@@ -197,6 +218,34 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 3) shared_kernel(Kv4Shared
     part_rows<D, NQO, 1>(a, p, seqs, ex);
 }
 
+// Answers with prompts too short to share: a block takes all that 16 or 32 rows of one see, and ends it.
+template <int D, int NQ>
+__global__ void __launch_bounds__(256, D == 256 ? 2 : 3) whole_kernel(Kv4Shared a) {
+    __shared__ Exchange<D> ex;
+    const int per = a.T * (a.q_heads / a.kv_heads), lane = threadIdx.x & 63;
+    const uint32_t seqs = ((const uint32_t*)a.seq)[lane];
+    const uint2 lanes = ((const uint2*)a.lane)[lane];
+    const uint4 ps = ((const uint4*)a.pos)[lane];
+    const Entries en(a);
+    const int row_tiles = (per + NQ * 16 - 1) / (NQ * 16), zr = over(blockIdx.x, a.kv_inv), i = (uint32_t)zr / (uint32_t)row_tiles;
+    const int j = __popcll(__ballot(en.start <= i)) - 1;
+    Part p;
+    p.start = i;
+    p.rows = per;
+    p.h = blockIdx.x - zr * a.kv_heads;
+    p.rho0 = (zr - i * row_tiles) * NQ * 16;
+    p.len = pick(en.len, j);
+    p.ahead = (p.len + 31) >> 5;
+    p.prefix = a.prefix + pick(en.lane, j) * a.prefix_lane + p.h * a.prefix_region;
+    p.region = a.cache + low16(lanes, i) * a.lane_bytes + p.h * a.region;
+    p.last = -1;
+    p.pos = entry(ps.x, ps.y, ps.z, ps.w, i);
+    p.t0 = 0;
+    p.t1 = p.ahead + ((p.pos + over(min(p.rho0 + NQ * 16, per) - 1, a.group_inv)) >> 5) + 1;
+    p.tile = 0;
+    part_rows<D, NQ, 4, true>(a, p, seqs, ex);
+}
+
 // Joins the parts of 16 rows of an entry: a wave one of a lane's runs of 4 dims (256 dims, so that there are waves enough)
 // or its four of 1 or 2 (8192 rows of 128 dims: 9.8 us by 2 dims a lane, 7.3 by 8), some parts in flight.
 template <int D>
@@ -266,19 +315,45 @@ constexpr int kPromptSplits = 64, kOwnSplits = 64;
 template <int D>
 static hipError_t launch(Kv4Shared& a, hipStream_t st) {
     const int group = a.q_heads / a.kv_heads, per = a.T * group, nqo = per > 16 ? 2 : 1;
-    int most = per;
+    int widest = per;
     for (int j = 0; j < a.entries; ++j) {
         a.gcount[j] = (uint16_t)((j + 1 < a.entries ? a.gstart[j + 1] : a.n) - a.gstart[j]);
-        if (a.glen[j]) most = std::max(most, a.gcount[j] * per);
+        if (a.glen[j]) widest = std::max(widest, a.gcount[j] * per);
     }
-    const int nqp = most > 16 ? 2 : 1;
+    const int nqp = widest > 16 ? 2 : 1;
     const auto items = [&](int j) { return a.kv_heads * ((kv4_tiles(a.gcount[j] * per) + nqp - 1) / nqp); };
     const auto prompt_tiles = [&](int j) { return (a.glen[j] + 31) >> 5; };
     const auto own_tiles = [&](int i) { return ((a.pos[i] + a.T - 1) >> 5) + 1; };
     const long long own_items = a.kv_heads * ((kv4_tiles(per) + nqo - 1) / nqo);
-    long long work = 0, own = 0, part = 0, blocks = 0, joins = 0;
-    for (int j = 0; j < a.entries; ++j) work += prompt_tiles(j) * items(j);
-    for (int i = 0; i < a.n; ++i) own += own_tiles(i) * own_items;
+    a.per_inv = reciprocal(per);
+    a.group_inv = reciprocal(group);
+    a.kv_inv = reciprocal(a.kv_heads);
+    for (int j = a.entries; j < kEntryArgs; ++j) {
+        a.gfirst[j] = a.gtile[j] = INT_MAX;
+        a.gstart[j] = 0xffff;
+    }
+    long long work = 0, own = 0, steps = 0, longest = 0, part = 0, blocks = 0, joins = 0;
+    for (int j = 0; j < a.entries; ++j) {
+        work += prompt_tiles(j) * items(j);
+        for (int i = a.gstart[j]; i < a.gstart[j] + a.gcount[j]; ++i) {
+            own += own_tiles(i) * own_items;
+            steps += (prompt_tiles(j) + own_tiles(i)) * own_items;
+            longest = std::max<long long>(longest, prompt_tiles(j) + own_tiles(i));
+        }
+    }
+    // Short lists are walked whole, without parts and their join, some 4 us less: while a wave's quarter of the longest takes
+    // no more than 7 us (a tile 0.7, 0.4 and 0.33 us of 256, 128 and 64 dims, half as much again for 32 rows), and all
+    // of them not much more than with the prompts shared (4 us are 13,000 tiles on the card); longer ones where sharing saves
+    // little, and there are so many that the longest one's end does not matter. Calls, us, in parts and whole: 12.9 and 8.5 for 6
+    // answers to 4 slots, 15.7 and 11.9 for 143 to 246, 18.5 and 10.9 for 2 x 29 x 2 rows to 234 with 615 of their own, 101 and 68
+    // for 6 x 27 x 3 rows to 1281 with 505 of their own; 12.9 and 16.6 for 2 x 11 to 2091, 20.5 and 35.6 for 135 x 3 rows to 1400.
+    const long long shared = work + own, most = (long long)(28 / (0.2 + D / 512.0) / (nqo == 2 ? 1.5 : 1.0));
+    const bool whole = longest < 1 << 25 &&         // (their slots are numbered in one row)
+                       ((longest <= most && steps <= 2 * shared + 13000) || (steps * 5 <= shared * 7 && longest * 300 <= steps));
+    if (whole) {
+        hipLaunchKernelGGL((nqo == 1 ? whole_kernel<D, 1> : whole_kernel<D, 2>), dim3((unsigned)(a.n * own_items)), dim3(256), 0, st, a);
+        return hipGetLastError();
+    }
     // One block a CU, or two where each has 128 tiles or more: a second wave on a SIMD fills the waits of the first (512
     // tiles of 256 dims: 97.8 -> 83.3 us; about 160 of 128: 56.6 -> 42.5), but twice the partial results take their time to write
     // and to join (64 tiles of 256 dims: 23.8 + 5.7 -> 29.7 + 7.8). No block more than that, which would run behind them,
@@ -322,12 +397,8 @@ static hipError_t launch(Kv4Shared& a, hipStream_t st) {
         blocks += (a.own_units + 3) / 4;
         if (part <= kv4_shared_room(D) || least) break;
     }
-    for (int j = a.entries; j < kEntryArgs; ++j) a.gfirst[j] = a.gtile[j] = INT_MAX;
     for (int i = a.n; i < kSeqArgs; ++i) a.first[i] = 0xffff;
     if (part > kv4_shared_room(D) || blocks > kLaunchBlocks || joins * 4 > kLaunchBlocks) return hipErrorInvalidValue;
-    a.per_inv = reciprocal(per);
-    a.group_inv = reciprocal(group);
-    a.kv_inv = reciprocal(a.kv_heads);
     const auto k = nqp == 1 ? shared_kernel<D, 1, 1> : nqo == 1 ? shared_kernel<D, 2, 1> : shared_kernel<D, 2, 2>;
     hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(256), 0, st, a);
     const hipError_t rc = hipGetLastError();

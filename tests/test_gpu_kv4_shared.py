@@ -77,6 +77,25 @@ def test_groups(eng, hq, kv, d, T):
     own.c.close()
 
 
+@pytest.mark.parametrize("hq,kv,d", [(8, 2, 256), (32, 8, 128), (14, 2, 64), (5, 1, 128), (48, 3, 256)])
+@pytest.mark.parametrize("T", [1, 5])
+def test_long_groups(eng, hq, kv, d, T):
+    """The same with prompts long enough to be read in parts for many answers, some beside short ones and none."""
+    rng = np.random.default_rng(hq + d + T)
+    pre, own = Filled(eng, rng, 4, 4300, kv, d), Filled(eng, rng, 9, 100, kv, d)
+    plane = np.array([0, 1, 1, 2, -1, 2, 2, 3, 0, 3, 3, 1, 2, 2, 1], np.int32)
+    plen = np.array([4300, 4031, 4031, 4064, 7, 4064, 4063, 1, 4300, 33, 0, 4032, 4064, 4064, 4031], np.int32)
+    lanes = rng.integers(0, 9, plane.size).astype(np.int32)
+    pos = rng.integers(0, 101 - T, plane.size).astype(np.int32)
+    pos[:4] = [0, 100 - T, 31, 32]
+    for gated in (False, True):
+        print(f"shared long groups {hq} {kv} {d} T={T} gated={gated}", flush=True)
+        got, q, g = run(eng, pre, own, plane, plen, lanes, pos, T, hq, rng, gated, spread=8)
+        check(pre, own, plane, plen, lanes, pos, T, got, q, g, pick=None if not gated else [0, 3, 4, 7, 10])
+    pre.c.close()
+    own.c.close()
+
+
 @pytest.mark.parametrize("hq,kv,d,n,P,T", [(8, 2, 256, 64, 3000, 1), (8, 2, 256, 2, 9000, 1), (32, 4, 128, 40, 2500, 1),
                                            (4, 4, 64, 100, 1500, 3), (8, 2, 256, 20, 1111, 3), (48, 3, 256, 9, 700, 5)])
 def test_long_prompt(eng, hq, kv, d, n, P, T):
@@ -157,15 +176,16 @@ def test_many(eng):
 
 
 @pytest.mark.parametrize("hq,kv,d", [(8, 2, 256), (4, 1, 128), (2, 2, 64)])
-@pytest.mark.parametrize("T", [1, 3, 40])
-def test_nan_slots(eng, hq, kv, d, T):
+@pytest.mark.parametrize("T,far", [(1, 0), (3, 0), (40, 0), (1, 6000), (3, 6000), (9, 6016)])
+def test_nan_slots(eng, hq, kv, d, T, far):
     """A NaN group of a prompt's K or V reaches the answers that name it with that length, in V its dims only; one behind
-    the prefix's length, or in an answer's later slots, nobody."""
+    the prefix's length, or in an answer's later slots, nobody. In prompts of up to 100 slots, and of 6000 more."""
     rng = np.random.default_rng(d + T)
-    pre = Filled(eng, rng, 3, 100, kv, d, [("v", 0, 0, 70, 0), ("v", 0, kv - 1, 75, d // 32 - 1), ("k", 1, 0, 60, 0), ("v", 2, 0, 99, 1)])
+    pre = Filled(eng, rng, 3, far + 100, kv, d, [("v", 0, 0, far + 70, 0), ("v", 0, kv - 1, far + 75, d // 32 - 1),
+                                                     ("k", 1, 0, far + 60, 0), ("v", 2, 0, far + 99, 1)])
     own = Filled(eng, rng, 4, 60, kv, d, [("v", 0, 0, 59, 0), ("k", 1, 0, 45, 1), ("v", 2, kv - 1, 41, 1)])
     plane = np.array([0, 0, 1, 1, 2, 2, 0, -1], np.int32)
-    plen = np.array([70, 76, 60, 61, 99, 100, 76, 0], np.int32)
+    plen = np.array([70, 76, 60, 61, 99, 100, 76, -far], np.int32) + far
     lanes = np.array([0, 0, 1, 2, 2, 3, 3, 1], np.int32)
     pos = np.array([60 - T, 0, 5, 10, 41 if T < 3 else 20, 3, 60 - T, 2], np.int32)
     got, q, _ = run(eng, pre, own, plane, plen, lanes, pos, T, hq, rng)
