@@ -246,18 +246,23 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 3) whole_kernel(Kv4Shared 
     part_rows<D, NQ, 4, true>(a, p, seqs, ex);
 }
 
-// Joins the parts of 16 rows of an entry: a wave one of a lane's runs of 4 dims (256 dims, so that there are waves enough)
-// or its four of 1 or 2 (8192 rows of 128 dims: 9.8 us by 2 dims a lane, 7.3 by 8), some parts in flight.
-template <int D>
-constexpr int kJoinBlocks = D == 256 ? 4 : 1;    // of four waves, for 16 rows
-template <int D>
-__global__ void __launch_bounds__(256) shared_join(Kv4Shared a) {
-    constexpr int N = kRun<D>, B = kJoinBlocks<D>, R = 4 / B, kJoin = B == 1 ? 4 : 8;
+// Joins the parts of 16 rows of an entry. A wave takes one of a lane's runs of 4 dims (256 dims, so that there are waves enough)
+// or its four of 1 or 2 (8192 rows of 128 dims: 9.8 us by 2 dims a lane, 7.3 by 8), some parts in flight. FEW rows of many
+// parts: a block's eight waves take a run's parts in turn, and the first ends it (4 rows' 53 parts of 128 dims 22.6 -> 4.4 us;
+// 1024 rows' 4 of 256 5.9 -> 15.2).
+template <int D, bool FEW>
+constexpr int kJoinBlocks = FEW ? 16 : D == 256 ? 4 : 1;     // for 16 rows
+template <bool FEW>
+constexpr int kJoinWaves = FEW ? 8 : 4;
+template <int D, bool FEW>
+__global__ void __launch_bounds__(64 * kJoinWaves<FEW>) shared_join(Kv4Shared a) {
+    constexpr int N = kRun<D>, B = kJoinBlocks<D, FEW>, R = B == 1 ? 4 : 1, kJoin = B == 1 ? 4 : 8, W = FEW ? 8 : 1;
+    __shared__ float states[FEW ? W : 1][R * N + 2][64];
     const int group = a.q_heads / a.kv_heads, per = a.T * group, lane = threadIdx.x & 63, g = lane >> 4;
     const uint32_t seqs = ((const uint32_t*)a.seq)[lane];
     const uint2 f = ((const uint2*)a.first)[lane];
     const Entries en(a);
-    const int wv = threadIdx.x >> 6, r = B == 1 ? wv : blockIdx.x & 3, w0 = B == 1 ? 0 : wv, ix = blockIdx.x / B, j = __popcll(__ballot(en.tile <= ix)) - 1;
+    const int wv = threadIdx.x >> 6, r = B == 1 ? wv : blockIdx.x & 3, w0 = FEW ? blockIdx.x >> 2 & 3 : B == 1 ? 0 : wv, ix = blockIdx.x / B, j = __popcll(__ballot(en.tile <= ix)) - 1;
     const int start = pick(en.start, j), rows = pick(en.count, j) * per, tiles = (rows + 15) >> 4, part = pick(en.part, j);
     const int prompt = pick(en.len, j) ? pick(en.splits, j) : 0;
     const uint32_t it = ix - pick(en.tile, j);
@@ -271,7 +276,7 @@ __global__ void __launch_bounds__(256) shared_join(Kv4Shared a) {
     };
     const int first = first_of(i), next = first_of(min(i + 1, kSeqArgs - 1));
     const int own = (i + 1 < a.n ? next : a.own_splits) - first, own_tiles = (per + 15) >> 4;
-    if (rho >= rows) return;
+    if (!FEW && rho >= rows) return;
     const int at = (64 * (4 * w0 + r) + 16 * g) * N;
     const float* pp = a.part + (size_t)(part + h * tiles + rt) * tile_floats(D);
     const float* po = a.part + (size_t)(a.own_part + (first * a.kv_heads + h) * own_tiles + (s >> 4)) * tile_floats(D);
@@ -280,12 +285,12 @@ __global__ void __launch_bounds__(256) shared_join(Kv4Shared a) {
     float x[R * N], m = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int e = 0; e < R * N; ++e) x[e] = 0.f;
-    for (int k0 = 0; k0 < parts; k0 += kJoin) {
+    for (int k0 = FEW ? wv : 0; k0 < parts; k0 += W * kJoin) {
         float o[kJoin][R * N];
         float2 ml[kJoin];
 #pragma unroll
         for (int k = 0; k < kJoin; ++k) {
-            const int kk = min(k0 + k, parts - 1), n = kk < prompt ? lane & 15 : s & 15;
+            const int kk = min(k0 + W * k, parts - 1), n = kk < prompt ? lane & 15 : s & 15;
             const float* from = kk < prompt ? pp + kk * step : po + (kk - prompt) * own_step;
 #pragma unroll
             for (int w = 0; w < R; ++w) __builtin_memcpy(&o[k][w * N], from + at + (256 * w + n) * N, 4 * N);
@@ -301,11 +306,32 @@ __global__ void __launch_bounds__(256) shared_join(Kv4Shared a) {
         for (int e = 0; e < R * N; ++e) x[e] *= al;
 #pragma unroll
         for (int k = 0; k < kJoin; ++k) {
-            if (k0 + k >= parts) break;
+            if (k0 + W * k >= parts) break;
             const float c = __builtin_amdgcn_exp2f(ml[k].x - mz);
             sum += c * ml[k].y;
 #pragma unroll
             for (int e = 0; e < R * N; ++e) x[e] += c * o[k][e];
+        }
+    }
+    if constexpr (FEW) {
+        states[wv][R * N][lane] = m;
+        states[wv][R * N + 1][lane] = sum;
+#pragma unroll
+        for (int e = 0; e < R * N; ++e) states[wv][e][lane] = x[e];
+        __syncthreads();
+        if (wv || rho >= rows) return;
+        float mn = m, f[W];
+#pragma unroll
+        for (int w = 1; w < W; ++w) mn = fmaxf(mn, states[w][R * N][lane]);
+        sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < R * N; ++e) x[e] = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            f[w] = __builtin_amdgcn_exp2f(states[w][R * N][lane] - (mn == -INFINITY ? 0.f : mn));
+            sum += f[w] * states[w][R * N + 1][lane];
+#pragma unroll
+            for (int e = 0; e < R * N; ++e) x[e] += f[w] * states[w][e][lane];
         }
     }
     Out(a, (long long)seq * a.TT + t, h * group + s - t * group).template store<R * N>(a, x, sum, (4 * g + r) * (D / 16) + w0 * N);
@@ -335,6 +361,8 @@ static hipError_t launch(Kv4Shared& a, hipStream_t st) {
     long long work = 0, own = 0, steps = 0, longest = 0, part = 0, blocks = 0, joins = 0;
     for (int j = 0; j < a.entries; ++j) {
         work += prompt_tiles(j) * items(j);
+        a.gtile[j] = (int)joins;
+        joins += a.kv_heads * kv4_tiles(a.gcount[j] * per);
         for (int i = a.gstart[j]; i < a.gstart[j] + a.gcount[j]; ++i) {
             own += own_tiles(i) * own_items;
             steps += (prompt_tiles(j) + own_tiles(i)) * own_items;
@@ -365,22 +393,28 @@ static hipError_t launch(Kv4Shared& a, hipStream_t st) {
         return s;
     };
     const long long most_blocks = (work + 255) / 256 < 128 ? 256 : 512;
-    long long tiles = std::max<long long>(16, (work + most_blocks - 1) / most_blocks), least_blocks = prompt_blocks(INT_MAX);
+    // Few rows, whose parts' join takes them by eight waves: down to 4 tiles in no more than 128 blocks (8 answers to 3000 slots
+    // of 256 dims 12.1 -> 8.7 us, 32 to 8000 in 256 blocks of 8 tiles 16.0, in 128 of 16 14.1), an answer's own by 4 (one
+    // of 7000 11.4 -> 8.1).
+    const bool few = joins <= 32, short_blocks = few && work < 128 * 16;
+    long long tiles = short_blocks ? std::max<long long>(4, (work + 127) / 128) : std::max<long long>(16, (work + most_blocks - 1) / most_blocks);
+    const long long least_blocks = prompt_blocks(INT_MAX);
     while (prompt_blocks(tiles) > std::max(most_blocks, least_blocks)) tiles += (tiles + 7) / 8;
-    long long own_per = std::max<long long>(8, (own + 2047) / 2048);
+    int parts = 0;                   // of a row, at most
+    long long own_per = std::max<long long>(few ? 4 : 8, (own + 2047) / 2048);
     for (;; tiles *= 2, own_per *= 2) {
-        part = blocks = joins = 0;
+        part = blocks = 0;
+        int from_prompt = 0, from_own = 0;
         bool least = true;
         for (int j = 0; j < a.entries; ++j) {
             const int s = (int)std::min<long long>(kPromptSplits, (prompt_tiles(j) + tiles - 1) / tiles);
             least &= s <= 1;
             a.gfirst[j] = (int)blocks;
             a.gpart[j] = (int)part;
-            a.gtile[j] = (int)joins;
             a.gsplits[j] = (uint16_t)std::max(1, s);
             blocks += s * items(j);
+            from_prompt = std::max(from_prompt, s);
             part += s * a.kv_heads * kv4_tiles(a.gcount[j] * per);
-            joins += a.kv_heads * kv4_tiles(a.gcount[j] * per);
         }
         a.prompt_blocks = (int)blocks;
         a.own_part = (int)part;
@@ -390,20 +424,25 @@ static hipError_t launch(Kv4Shared& a, hipStream_t st) {
             least &= s == 1;
             a.first[i] = (uint16_t)z;
             z += s;
+            from_own = std::max(from_own, s);
         }
         a.own_splits = z;
         a.own_units = (int)(z * own_items);
         part += z * a.kv_heads * kv4_tiles(per);
         blocks += (a.own_units + 3) / 4;
+        parts = from_prompt + from_own;
         if (part <= kv4_shared_room(D) || least) break;
     }
     for (int i = a.n; i < kSeqArgs; ++i) a.first[i] = 0xffff;
-    if (part > kv4_shared_room(D) || blocks > kLaunchBlocks || joins * 4 > kLaunchBlocks) return hipErrorInvalidValue;
+    if (part > kv4_shared_room(D) || blocks > kLaunchBlocks || joins * 16 > kLaunchBlocks) return hipErrorInvalidValue;
     const auto k = nqp == 1 ? shared_kernel<D, 1, 1> : nqo == 1 ? shared_kernel<D, 2, 1> : shared_kernel<D, 2, 2>;
     hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(256), 0, st, a);
     const hipError_t rc = hipGetLastError();
     if (rc != hipSuccess) return rc;
-    hipLaunchKernelGGL(shared_join<D>, dim3((unsigned)joins * kJoinBlocks<D>), dim3(256), 0, st, a);
+    if (joins <= std::max(32, 2 * parts))          // (288 rows' 8 parts, 36 of these, 5.7 -> 7.7)
+        hipLaunchKernelGGL((shared_join<D, true>), dim3((unsigned)joins * kJoinBlocks<D, true>), dim3(64 * kJoinWaves<true>), 0, st, a);
+    else
+        hipLaunchKernelGGL((shared_join<D, false>), dim3((unsigned)joins * kJoinBlocks<D, false>), dim3(64 * kJoinWaves<false>), 0, st, a);
     return hipGetLastError();
 }
 hipError_t launch_attn_kv4_shared(Kv4Shared& a, hipStream_t st) {
