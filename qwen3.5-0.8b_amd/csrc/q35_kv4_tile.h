@@ -313,10 +313,10 @@ __device__ __forceinline__ void walk_tiles(Rows<D, NQ>& st, Tile<D>* buf, int t0
         walk_once<D, NQ, W, true>(st, buf, t0, t1, at, tile_at, lo, q, qlane, sight, full0, full1, scale2);
     }
 }
-// The W waves' states of `rows` rows: wave w ends a W-th of the row's dims, which all pass it through LDS (its own part too:
-// picking it out of the registers by the wave's number took longer); a lane keeps its row, and its accumulators go as they
-// are. place(c) gives where row 16 c + lane % 16 goes: a function of (sums x[r][i] of dim first_dim(r) + i, r < 4, i < D / 16 /
-// W; the reference; the sum of weights).
+// The W waves' states of `rows` rows: wave w ends a W-th of the row's dims, which the others pass it through LDS (its own part
+// too, instead of picking it out of the registers: a prompt of 4096 rows 84.2 for 83.4 us, 256 answers to 32,768 slots 86.3 for
+// 84.9); a lane keeps its row, and its accumulators go as they are. place(c) gives where row 16 c + lane % 16 goes: a function of
+// (sums x[r][i] of dim first_dim(r) + i, r < 4, i < D / 16 / W; the reference; the sum of weights).
 template <int D, int W>
 __device__ __forceinline__ int first_dim(int r) {
     return (4 * ((threadIdx.x & 63) >> 4) + r) * (D / 16) + (threadIdx.x >> 6) * (D / 16 / W);
@@ -337,7 +337,8 @@ __device__ __forceinline__ void join_waves(Rows<D, NQ>& st, int rows, f32x4 (*os
 #pragma unroll
         for (int w = 0; w < W; ++w)
 #pragma unroll
-            for (int i = 0; i < kPart; ++i) os[w][wv][i][lane] = st.o[c][w * kPart + i];
+            for (int i = 0; i < kPart; ++i)
+                if (w != wv) os[w][wv][i][lane] = st.o[c][w * kPart + i];
         lds_barrier();
         float m = st.m[c], sum = 0.f, f[W];
 #pragma unroll
@@ -355,7 +356,17 @@ __device__ __forceinline__ void join_waves(Rows<D, NQ>& st, int rows, f32x4 (*os
 #pragma unroll
         for (int w = 0; w < W; ++w)              // in the same order in every wave
 #pragma unroll
-            for (int i = 0; i < kPart; ++i) o[i] += f[w] * os[wv][w][i][lane];
+            for (int i = 0; i < kPart; ++i) {
+                f32x4 v;
+                if (w == wv) {
+                    v = st.o[c][i];
+#pragma unroll
+                    for (int k = 1; k < W; ++k) v = wv == k ? st.o[c][k * kPart + i] : v;
+                } else {
+                    v = os[wv][w][i][lane];
+                }
+                o[i] += f[w] * v;
+            }
         if (c * 16 + nn >= rows) continue;
         float x[4][kPart];
 #pragma unroll
