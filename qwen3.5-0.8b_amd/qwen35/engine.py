@@ -188,6 +188,8 @@ def pair_axes(sections, dealt: bool = False) -> bytes:
     """The axis of each pair of rotated dims, sections[a] pairs on axis a: in sections one behind the other, or dealt out
     to the axes in turn while each has pairs left."""
     left = [int(n) for n in sections]
+    if any(n < 0 for n in left):
+        raise ValueError("a section's number of pairs must not be negative")
     if not dealt:
         return bytes(a for a, n in enumerate(left) for _ in range(n))
     out = []
