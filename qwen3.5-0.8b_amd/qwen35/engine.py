@@ -178,6 +178,8 @@ def _axis(axis, rot_dim: int) -> bytes:
     """The pairs' axes as bytes, one for each of the rot_dim / 2 pairs."""
     if not isinstance(axis, bytes):
         a = np.asarray(axis)
+        if a.ndim == 0:
+            raise ValueError("axes are a list of one for each of the pairs")
         axis = a.tobytes() if a.dtype == np.uint8 else bytes(a.tolist())
     if len(axis) != rot_dim // 2:
         raise ValueError(f"{len(axis)} axes for {rot_dim // 2} pairs of dims")

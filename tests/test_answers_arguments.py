@@ -1,4 +1,5 @@
 """Arguments of the answers' operators that the Python side looks over itself, on the CPU."""
+import numpy as np
 import pytest
 
 
@@ -9,3 +10,12 @@ def test_pair_axes_of_negative_sections(sections, dealt):
     from qwen35 import pair_axes
     with pytest.raises(ValueError, match="negative"):
         pair_axes(sections, dealt)
+
+
+@pytest.mark.parametrize("axis", [0, 1, 32, np.int64(32), np.uint8(7)])
+@pytest.mark.parametrize("rot_dim", [0, 2, 64])
+def test_one_number_is_no_list_of_axes(axis, rot_dim):
+    """bytes(32) is 32 zero bytes: every pair on axis 0."""
+    from qwen35.engine import _axis
+    with pytest.raises(ValueError, match="pairs"):
+        _axis(axis, rot_dim)
