@@ -591,6 +591,8 @@ class State:
         """decode_step, and the log probabilities of the greedy ids or of given targets (q35_decode_step_logprobs)."""
         t = _i32(tokens)
         ln = _i32(lanes) if lanes is not None else None
+        if ln is not None and ln.size != t.size:
+            raise ValueError(f"{ln.size} lanes and {t.size} tokens")
         ids = np.empty(t.size, np.int32)
         out, d, _targets = _scores(t.size, targets, top, temperature)
         _ck(load_library().q35_decode_step_logprobs(self.eng.h, self.h, _p(ln) if ln is not None else None, t.size, _p(t),

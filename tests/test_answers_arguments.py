@@ -19,3 +19,14 @@ def test_one_number_is_no_list_of_axes(axis, rot_dim):
     from qwen35.engine import _axis
     with pytest.raises(ValueError, match="pairs"):
         _axis(axis, rot_dim)
+
+
+@pytest.mark.parametrize("lanes", [[], [0], [0, 1, 2], np.zeros(7, np.int32)])
+def test_scored_step_with_other_lanes_than_tokens(lanes):
+    """The library reads a lane for each token: of a shorter list it would read what lies behind it."""
+    from types import SimpleNamespace
+    from qwen35 import State
+    s = object.__new__(State)
+    s.eng, s.h = SimpleNamespace(h=None), None
+    with pytest.raises(ValueError, match="lanes"):
+        s.decode_step_logprobs([5, 6], lanes)
