@@ -309,7 +309,8 @@ int q35_op_kv4_append(q35_engine* e, q35_kv4* c, int layer, const int32_t* lanes
  * outnumber their positions): pair d turns by the row's position on axis axis[d], times theta^(-2 d / rot_dim). axis: host
  * memory, rot_dim / 2 bytes of 0 .. 3. Positions are device memory, any int32; pos and axis may be NULL with rot_dim 0. */
 typedef struct q35_positions {
-    const int32_t* pos;                  /* row r's position on axis a: pos[r * row_stride + a * axis_stride] */
+    const int32_t* pos;                  /* row r's position on axis a: pos[r * row_stride + a * axis_stride]; no other
+                                          * axes' are read than pairs have */
     int64_t row_stride, axis_stride;     /* in elements, not negative */
 } q35_positions;
 int q35_op_qk_norm_rope_axes(q35_engine* e, const q35_heads* h, int kv_heads, int head_dim, const q35_positions* at,

@@ -17,12 +17,14 @@ static AxisHeadArgs axis_args(const HeadArgs& h, const q35_positions& at, const 
     REQ(at.row_stride >= 0 && at.axis_stride >= 0, Q35_ERR_ARG, "positions: negative stride");
     a.axis_pos = at.pos;
     a.row_step = at.row_stride;
-    a.axis_step = at.axis_stride;
+    bool named[kAxes] = {};
     for (int i = 0; i < h.rot / 2; ++i) {
         REQ(axis[i] < kAxes, Q35_ERR_ARG, "a pair's axis is 0 .. 3");
+        named[axis[i]] = true;
         a.axes = std::max(a.axes, axis[i] + 1);
         a.axis_of[i >> 4] |= (uint32_t)axis[i] << 2 * (i & 15);
     }
+    for (int x = 0; x < a.axes; ++x) a.axis_at[x] = (named[x] ? x : a.axes - 1) * at.axis_stride;
     return a;
 }
 

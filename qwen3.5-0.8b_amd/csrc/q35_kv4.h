@@ -65,13 +65,14 @@ struct HeadArgs {
 // sequences of T rows, n T <= kHeadRows.
 constexpr int kHeadRows = 4 * kLaunchBlocks;   // (a block takes four of many rows)
 hipError_t launch_heads(HeadArgs& a, int n, hipStream_t st);
-// The same with rows at positions on up to four axes: pair d turns by axis_pos[row * row_step + axis * axis_step] of its
-// axis (two bits a pair in axis_of); pos holds the slots of an append then.
+// The same with rows at positions on up to four axes: pair d turns by axis_pos[row * row_step + axis_at[axis]] of its
+// axis (two bits a pair in axis_of); pos holds the slots of an append then. The first `axes` are read, and an axis
+// that no pair has is read at another one's place: the caller need not have positions on it.
 constexpr int kAxes = 4;
 struct AxisHeadArgs : HeadArgs {
     const int32_t* axis_pos;
-    long long row_step, axis_step;
-    int axes;
+    long long row_step, axis_at[kAxes];
+    int axes;                    // the largest that a pair has, and one
     uint32_t axis_of[8];
 };
 hipError_t launch_heads(AxisHeadArgs& a, int n, hipStream_t st);

@@ -72,7 +72,7 @@ __device__ __forceinline__ int axis_position(const AxisHeadArgs& a, int r, int i
     const int32_t* p = a.axis_pos + r * a.row_step;
     int at[kAxes];
 #pragma unroll
-    for (int x = 0; x < kAxes; ++x) at[x] = x < a.axes ? p[x * a.axis_step] : 0;
+    for (int x = 0; x < kAxes; ++x) at[x] = x < a.axes ? p[a.axis_at[x]] : 0;
     const uint32_t axis = (a.axis_of[i >> 4] >> 2 * (i & 15)) & 3u;
     return axis == 0 ? at[0] : axis == 1 ? at[1] : axis == 2 ? at[2] : at[3];
 }
