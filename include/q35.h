@@ -331,8 +331,9 @@ int q35_op_attn_kv4(q35_engine* e, q35_kv4* c, int layer, const int32_t* lanes, 
                     const q35_view* out);
 /* The same for answers that share prompts: row i * T + t sees slots [0, prefix_lens[i]) of lane prefix_lanes[i] of
  * `prefix` and slots [0, pos[i] + t] of lane lanes[i] of c, in one softmax. Both caches have the same heads, and each its
- * own lanes and capacity; they may be the same one (a lane is not its own prefix). Sequences that name the same lane and length share
- * the reading of it, in any order; prefix_lanes[i] < 0 or prefix_lens[i] 0: no prefix. Positions count c's slots: the keys'
+ * own lanes and capacity; they may be the same one (a lane is not its own prefix). Of 256 neighbouring sequences those that name the
+ * same lane and length share the reading of it, in any order (other lengths of a lane are read apart, and a launch has room
+ * for 64 prompts); prefix_lanes[i] < 0 or prefix_lens[i] 0: no prefix. Positions count c's slots: the keys'
  * rotation is whatever they were appended with (q35_op_kv4_append_axes). Rounding and NaN as above; the same call gives the
  * same bits, and other sequences beside a row may change its last ones at any length. */
 int q35_op_attn_kv4_shared(q35_engine* e, q35_kv4* prefix, q35_kv4* c, int layer, const int32_t* prefix_lanes,
@@ -366,7 +367,8 @@ int q35_op_draft_verify(q35_engine* e, const q35_drafts* d, int n, int k, int vo
 /* How probable given tokens were: for each row of logits, with p = softmax(logits / temperature), log p of its target, the
  * target's rank (the ids before it by falling logit, then by rising id: 0 is the argmax), the entropy -sum p log p,
  * and the first `top` ids of that order with their log p (the reference hands a prompt's whole logits to its caller,
- * engine/prefill.h:46-58). One pass over the logits; sums that end in float64, results rounded once to float32. A target
+ * engine/prefill.h:46-58). The logits are read once, and again where ties or masks leave too many that may be among the
+ * first. Sums that end in float64, results rounded once to float32. A target
  * that is no id (negative, or vocab or more) has log p NaN and rank -1; a row with a NaN, a +inf or only -inf logits has no
  * distribution: NaN throughout, rank and ids -1. An id with logit -inf has log p -inf. Outputs that are NULL are
  * left out. Any number of rows. Enqueued on the engine stream without waiting; its workspace is the engine's. */

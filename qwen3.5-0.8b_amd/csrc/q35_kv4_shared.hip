@@ -7,6 +7,9 @@
 // into bf16 once for 32 rows instead of once for each answer's 4 or 16; the answers' own slots are short lists, as in
 // the attention of single lanes. Both kinds are blocks of one launch, and a second launch joins the parts. Where the lists are
 // short, that costs more than it saves, and each answer's rows walk their prompt's tiles and their own in one launch.
+//
+// Times below of a kernel alone are a tracer's. Under it calls of two launches take up to 10 us longer than without (256 answers
+// to 32,768 slots 91 for 81.5), so the two do not add up to the call's.
 #include <algorithm>
 #include <climits>
 
@@ -157,8 +160,8 @@ __device__ __forceinline__ int pick(int v, int j) { return __builtin_amdgcn_read
 __device__ __forceinline__ int low16(uint2 v, int i) { return entry(v.x & 0xffffu, v.x >> 16, v.y & 0xffffu, v.y >> 16, i); }
 
 // NQP, NQO: 16 rows a block takes of a prompt's and a wave of an answer's own.
-// Long prompts are bound by instructions: 256 answers x 8 heads over 32,768 slots of 256 dims (69 GFLOP) 82.7 us, 0.83
-// PFLOP/s; an MFMA has 5 other vector instructions beside it (codes and weights into bf16, exponentials), the SIMDs issue in 68 %
+// Long prompts are bound by instructions: 256 answers x 8 heads over 32,768 slots of 256 dims (69 GFLOP) 81.5 us a call with its
+// join, 0.85 PFLOP/s; an MFMA has 5 other vector instructions beside it (codes and weights into bf16, exponentials), the SIMDs issue in 68 %
 // of the busy cycles and the MFMA pipes work in 43 %. Without turning codes into bf16 it takes 8 us less; from which
 // level of the memory the tiles come makes no difference, nor do loads further ahead. Shorter ones are bound by what surrounds the
 // walk: over 4,096 slots 23.5 us, of which 11 are launch, Q, a first tile and the waves' join, 3.5 the partial results' stores.
@@ -337,6 +340,9 @@ __global__ void __launch_bounds__(64 * kJoinWaves<FEW>) shared_join(Kv4Shared a)
     Out(a, (long long)seq * a.TT + t, h * group + s - t * group).template store<R * N>(a, x, sum, (4 * g + r) * (D / 16) + w0 * N);
 }
 
+// Of one list, after the rules below: few sequences with few kv heads leave most CUs idle over a long one. An answer of 5 heads
+// over one kv head to 32,768 slots has 64 blocks and takes 12.8 us; over as many slots of its own it has 64 waves, 17.3 us, where
+// the attention of single lanes takes 12.3 (2 kv heads of 256 dims 21.7 and 14.1).
 constexpr int kPromptSplits = 64, kOwnSplits = 64;
 template <int D>
 static hipError_t launch(Kv4Shared& a, hipStream_t st) {
@@ -375,6 +381,9 @@ static hipError_t launch(Kv4Shared& a, hipStream_t st) {
     // little, and there are so many that the longest one's end does not matter. Calls, us, in parts and whole: 12.9 and 8.5 for 6
     // answers to 4 slots, 15.7 and 11.9 for 143 to 246, 18.5 and 10.9 for 2 x 29 x 2 rows to 234 with 615 of their own, 101 and 68
     // for 6 x 27 x 3 rows to 1281 with 505 of their own; 12.9 and 16.6 for 2 x 11 to 2091, 20.5 and 35.6 for 135 x 3 rows to 1400.
+    // Over 390 drawn cases the geometric mean is within 1 % of the better form's; seven cases miss it by more than a tenth, six
+    // lists of 47 to 107 tiles in parts (41 x 3 rows to 1175 with 506 of their own, 48 / 3 heads of 256: 34.5 for 25.7) and one
+    // of 96 whole (8 to 3019, 16 heads of 64: 16.2 for 12.7).
     const long long shared = work + own, most = (long long)(28 / (0.2 + D / 512.0) / (nqo == 2 ? 1.5 : 1.0));
     const bool whole = longest < 1 << 25 &&         // (their slots are numbered in one row)
                        ((longest <= most && steps <= 2 * shared + 13000) || (steps * 5 <= shared * 7 && longest * 300 <= steps));

@@ -313,9 +313,10 @@ __device__ __forceinline__ void walk_tiles(Rows<D, NQ>& st, Tile<D>* buf, int t0
         walk_once<D, NQ, W, true>(st, buf, t0, t1, at, tile_at, lo, q, qlane, sight, full0, full1, scale2);
     }
 }
-// The W waves' states of `rows` rows: wave w ends a W-th of the row's dims, which the others pass it through LDS (its own part
-// too, instead of picking it out of the registers: a prompt of 4096 rows 84.2 for 83.4 us, 256 answers to 32,768 slots 86.3 for
-// 84.9); a lane keeps its row, and its accumulators go as they are. place(c) gives where row 16 c + lane % 16 goes: a function of
+// The W waves' states of `rows` rows: wave w ends a W-th of the row's dims, which the others pass it through LDS, and picks its
+// own part out of its registers (through LDS too that was slower: a prompt of 4096 rows 84.2 for 83.4 us, 256 answers to
+// 32,768 slots 86.3 for 84.9); a lane keeps its row, and its accumulators go as they are. place(c) gives where row
+// 16 c + lane % 16 goes: a function of
 // (sums x[r][i] of dim first_dim(r) + i, r < 4, i < D / 16 / W; the reference; the sum of weights).
 template <int D, int W>
 __device__ __forceinline__ int first_dim(int r) {
@@ -378,7 +379,7 @@ __device__ __forceinline__ void join_waves(Rows<D, NQ>& st, int rows, f32x4 (*os
     }
 }
 
-// Where a row's dims go: normalised, gated, rounded. N dims (1, 2 or 4) from d on.
+// Where a row's dims go: normalised, gated, rounded. N dims (1, 2, 4 or 8) from d on.
 struct Out {
     const uint16_t* gate;
     uint16_t* out;

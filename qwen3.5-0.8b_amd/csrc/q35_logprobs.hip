@@ -1,4 +1,5 @@
-// Log probabilities of given tokens, their ranks, the rows' entropy and most likely tokens, in one pass over the logits.
+// Log probabilities of given tokens, their ranks, the rows' entropy and most likely tokens, in one pass over the logits
+// (in two where ties or masks leave too many tokens that may be among the most likely).
 //
 // With z_i = (x_i - m) / T, m = max x, S = sum e^z_i, A = sum z_i e^z_i of a row:
 //   log p_i = z_i - log S,   entropy = log S - A / S,   rank of t = #{x_i > x_t} + #{x_i = x_t, i < t},
@@ -170,10 +171,14 @@ __device__ __forceinline__ void push(Best& b, float x, int id, bool on) {
 // lanes the same ones of the waves make 64 groups; `top` groups reach the top-th largest of their
 // maxima (floor), so the row's best do, and only the pieces of the lanes and runs that reach it are read
 // again: some 25 of them for 20 tokens, of any number of elements. If ties or infinities bring more candidates than there is
-// room for, the part is gone over in order with a list a wave (Best).
-// float32: bound by memory, 256 rows of 248,320 with 5 tokens each (254 MB) 45.0 us, 5.6 TB/s. bfloat16: by memory and the 8
-// instructions an element takes, 1999 rows of 32,003 with 20 tokens (128 MB) 37.4 us, 3.4 TB/s (without 31.8). One row of
-// 248,320: a chain of loads and barriers, 8.8 us and the join's 3.8.
+// room for, the part is gone over in order with a list a wave (Best). Fewer than `top` groups with a finite logit have no
+// floor, and every element is a candidate: masks that leave 10 tokens of a row take 1999 rows of 32,003 with 20 tokens
+// from 52 to 128 us in float32 and from 35 to 236 in bfloat16, one row of 248,320 from 12.6 to 96 and from 12.9 to 176
+// (256 rows of 248,320 with 5 tokens, fewer than those 10, take what they took).
+// float32: bound by memory, 256 rows of 248,320 with 5 tokens each (254 MB) 51 us over buffers in turn, 5.0 TB/s (one buffer over
+// and over, which the last cache nearly holds, 44 us). bfloat16: by memory and the 8 instructions an element takes here (the
+// entropy's among them, also where it is not wanted), 1999 rows of 32,003 with 20 tokens (128 MB) 37 us, 3.5 TB/s (without
+// tokens 31.8 of 37.4 on one buffer). One row of 248,320: a chain of loads and barriers, 8.8 us and the join's 3.8.
 template <int W>
 constexpr int kRuns = W > 4 ? 64 / W : 16;       // of a part's tiles a wave
 template <int W>
@@ -489,7 +494,7 @@ hipError_t launch_logprobs(LogprobArgs a, hipStream_t st) {
     const int el = a.bf16 ? 8 : 4, tiles = (a.vocab / el + 64 * kEach / el - 1) / (64 * kEach / el);
     // A row is one block's where 512 rows or fewer have as many as tiles (of 2048 elements) at least: 16 waves up to 256
     // rows, a block a CU, and 8 above, two. Without a second launch and its join 256 rows of 248,320 float32 and 5 tokens take
-    // 45.0 instead of 47.3 + 4.7 us, 16 of 32,003 bfloat16 and 20 tokens 11.6 for 9.5 + 4.5, 448 17 for 18 + 5; where rows
+    // 45.0 instead of 47.3 + 4.7 us (one buffer over and over), 16 of 32,003 bfloat16 and 20 tokens 11.6 for 9.5 + 4.5, 448 17 for 18 + 5; where rows
     // are fewer than tiles a CU takes too long for one (64 of 248,320 26.1 for 18.2 + 4.0; 75 of 151,936 even).
     // Otherwise blocks of four waves, as many of a row as give every CU four, each wave with a tile at least. The card holds
     // about 1280 of them: of more rows a block has two waves, whose ends fill the CUs better (1999 rows of 32,003 bf16 42.3 ->
